@@ -336,6 +336,80 @@ int qmk_static_set_timeout_cycles(int device, int64_t cycles);
 int qmk_static_set_wait_first_dependency(int device, int32_t on);
 const char* qmk_static_last_cuda_error(void);
 
+/*
+ * Paged KV cache.  The pool of a layer is [num_pages, page_size, NKV, HD] bf16; a block table names, per request, the page
+ * of every page_size positions.  Requests that start with the same tokens name the same pages for them (a shared prefix,
+ * whole pages), so those rows are stored once and the attention below reads them once for all requests.  The reference
+ * keeps one contiguous cache per sequence (decode_schedule/globs.py:27-28) and has no counterpart.  The three entry
+ * points take no handle and own no memory: they launch on `cuda_stream` of `device` (any current device; it is left as
+ * it was) and return at once.  page_size: 16, 32, 64, 128 or 256.  A refused call launches nothing.
+ */
+
+/* Block tables of a batch from the lengths its requests have to have room for (prefix included).  Row s gets
+ * n_s = min(ceil(lengths[s] / page_size), max_pages) entries: the first prefix_pages are prefix_table's, the others come
+ * from free_pages, in order, behind those of the rows before; entries from n_s on, and entries for which free_pages has run
+ * out, are -1.  A length of zero or less is an empty row. */
+typedef struct qmk_block_tables_args {
+  const int32_t* lengths;      /* [seqs]                                                                     */
+  const int32_t* free_pages;   /* [num_free] (may be NULL when num_free is 0)                                */
+  const int32_t* prefix_table; /* [prefix_pages] (may be NULL when prefix_pages is 0)                        */
+  int32_t* tables;             /* out [seqs, max_pages]                                                      */
+  int32_t* used;               /* out [2]: pages taken from free_pages (more than num_free: it ran out); rows
+                                  that would have needed more than max_pages                                 */
+  int32_t seqs, num_free, prefix_pages, page_size, max_pages;
+} qmk_block_tables_args;
+int qmk_build_block_tables(const qmk_block_tables_args* args, int device, void* cuda_stream);
+
+/* Where the K and V rows of a step's new tokens go.  Request s holds kv_lengths[s] tokens and appends new_lengths[s]
+ * (values below zero count as zero); the tokens of the step are numbered request by request, cut off at `tokens`.  Token t
+ * of request s: position = kv_lengths[s] + (t - cu_tokens[s]), slot = page * page_size + position % page_size, or -1 where
+ * the table has no page.  Entries behind the last token: slot -1, position 0, seq_id -1, active 0. */
+typedef struct qmk_slot_map_args {
+  const int32_t* block_tables;   /* [seqs, max_pages]                                  */
+  const int32_t* kv_lengths;     /* [seqs]                                             */
+  const int32_t* new_lengths;    /* [seqs]                                             */
+  int64_t* slots;                /* out [tokens]                                       */
+  int32_t* positions;            /* out [tokens]                                       */
+  int32_t* seq_ids;              /* out [tokens]                                       */
+  uint8_t* active;               /* out [tokens]: 1 where slots[t] >= 0                */
+  int32_t* cu_tokens;            /* out [seqs + 1]: first token of every request       */
+  int32_t* kv_lengths_out;       /* out [seqs]: tokens in the cache after the step; not kv_lengths itself */
+  int32_t seqs, tokens, page_size, max_pages;
+} qmk_slot_map_args;
+int qmk_build_slot_map(const qmk_slot_map_args* args, int device, void* cuda_stream);
+
+/* Attention of a step's query rows over the paged cache, the shared prefix computed once for all of them.
+ * Request s has the rows cu_tokens[s] .. cu_tokens[s + 1] - 1 and kv_lengths[s] tokens in the cache, the step's own
+ * included (their K and V are there).  Its row i sees the positions below kv_lengths[s] - rows + i + 1: those below
+ * prefix_len through prefix_table, the others through its block table (whose entries below prefix_len are not read).
+ * A row that sees nothing gets zeros and an lse of minus infinity; rows from cu_tokens[seqs] on are left as they were.
+ * A page index outside the pool reads as keys and values of zero.  What lies behind a request's last token in its last
+ * page is never used, whatever it holds.  bf16, fp32 accumulation; head_dim 64 or 128, 1..16 query heads per KV head. */
+typedef struct qmk_prefix_attention_args {
+  const void* q;               /* [tokens, num_heads, head_dim], q_token_stride elements from token to token */
+  void* out;                   /* the same, out_token_stride (strides: multiples of 8; 16-byte aligned)      */
+  float* lse;                  /* optional [tokens, num_heads]: natural log of the sum of exponentials       */
+  const void* k_pages;         /* [num_pages, page_size, num_kv_heads, head_dim]                             */
+  const void* v_pages;
+  const int32_t* block_tables; /* [seqs, max_pages]                                                          */
+  const int32_t* kv_lengths;   /* [seqs]                                                                     */
+  const int32_t* cu_tokens;    /* [seqs + 1], ascending from 0                                               */
+  const int32_t* prefix_table; /* [prefix_len / page_size] (may be NULL when prefix_len is 0)                */
+  int64_t q_token_stride, out_token_stride;
+  int32_t tokens, seqs, num_heads, num_kv_heads, head_dim, page_size, num_pages, max_pages;
+  int32_t prefix_len;          /* positions every request shares; a multiple of page_size                    */
+  float scale;
+  void* workspace;             /* qmk_prefix_attention_workspace bytes, 256-byte aligned; its contents need not be kept,
+                                  but two calls that may run at the same time need one each */
+  int64_t workspace_bytes;
+} qmk_prefix_attention_args;
+int64_t qmk_prefix_attention_workspace(int32_t tokens, int32_t seqs, int32_t num_heads, int32_t num_kv_heads,
+                                       int32_t head_dim, int32_t prefix_len, int device);
+int qmk_prefix_attention(const qmk_prefix_attention_args* args, int device, void* cuda_stream);
+
+/* Text behind the last QMK_ERR_CUDA that one of these three returned to the calling thread. */
+const char* qmk_paged_last_cuda_error(void);
+
 void qmk_destroy(qmk_handle* h);
 const char* qmk_strerror(int code);
 const char* qmk_last_cuda_error(const qmk_handle* h);

@@ -54,6 +54,26 @@ class Status(C.Structure):
                 ("seen", C.c_uint32), ("expected", C.c_uint32), ("detail", C.c_int32), ("reserved", C.c_int32)]
 
 
+class BlockTablesArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("lengths", "free_pages", "prefix_table", "tables", "used")] + \
+               [(n, C.c_int32) for n in ("seqs", "num_free", "prefix_pages", "page_size", "max_pages")]
+
+
+class SlotMapArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("block_tables", "kv_lengths", "new_lengths", "slots", "positions", "seq_ids",
+                                          "active", "cu_tokens", "kv_lengths_out")] + \
+               [(n, C.c_int32) for n in ("seqs", "tokens", "page_size", "max_pages")]
+
+
+class PrefixAttentionArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out", "lse", "k_pages", "v_pages", "block_tables", "kv_lengths",
+                                          "cu_tokens", "prefix_table")] + \
+               [("q_token_stride", C.c_int64), ("out_token_stride", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("tokens", "seqs", "num_heads", "num_kv_heads", "head_dim", "page_size", "num_pages",
+                                         "max_pages", "prefix_len")] + \
+               [("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 # Every symbol include/qmk_b200.h declares: (name, restype, argtypes).
 SYMBOLS = [
     ("qmk_create", C.c_int, [C.POINTER(ModelDesc), C.POINTER(WeightPtrs), C.c_int, C.POINTER(C.c_void_p)]),
@@ -84,6 +104,11 @@ SYMBOLS = [
     ("qmk_static_set_wait_first_dependency", C.c_int, [C.c_int, C.c_int32]),
     ("qmk_generate_device", C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]),
     ("qmk_static_last_cuda_error", C.c_char_p, []),
+    ("qmk_build_block_tables", C.c_int, [C.POINTER(BlockTablesArgs), C.c_int, C.c_void_p]),
+    ("qmk_build_slot_map", C.c_int, [C.POINTER(SlotMapArgs), C.c_int, C.c_void_p]),
+    ("qmk_prefix_attention_workspace", C.c_int64, [C.c_int32] * 6 + [C.c_int]),
+    ("qmk_prefix_attention", C.c_int, [C.POINTER(PrefixAttentionArgs), C.c_int, C.c_void_p]),
+    ("qmk_paged_last_cuda_error", C.c_char_p, []),
     ("qmk_destroy", None, [C.c_void_p]),
     ("qmk_strerror", C.c_char_p, [C.c_int]),
     ("qmk_last_cuda_error", C.c_char_p, [C.c_void_p]),

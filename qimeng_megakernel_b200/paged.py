@@ -1,0 +1,279 @@
+"""Paged KV cache whose sequences share a prefix: block tables, slot maps and the attention that reads it.
+
+The pool of one layer is `[num_pages, page_size, NKV, HD]` bf16.  A sequence's block table names the page of every
+`page_size` positions; sequences that start with the same tokens name the same pages for them, so a shared prompt is
+stored once and `prefix_attention` reads it once for the whole batch:
+
+    tables = build_block_tables(lengths, free_pages, page_size=64, max_pages=40, prefix_table=prefix_pages)
+    step   = build_slot_map(tables.tables, kv_lengths, new_lengths, page_size=64, tokens=T)
+    # K and V rows of the step's tokens go to step.slots (row page * page_size + offset of the pool) ...
+    out    = prefix_attention(q, k_pages, v_pages, tables.tables, step.kv_lengths, step.cu_tokens,
+                              prefix_table=prefix_pages, prefix_len=len(prefix_pages) * 64)
+
+All three are one call into libqmk_b200.so on the current stream of the tensors' device; nothing is copied to the host,
+so a step can be captured into a CUDA graph.  CUDA tensors only: there is no CPU path.  `run_prefill_synthetic(...,
+shared_prefix=n)` sets up a decode state on this cache, which `decode()` then runs.
+
+The reference keeps one contiguous cache per sequence (qimeng_megakernel/models/LLM/llama/llama3_2__1b/A100/
+multi_batch/decode_schedule/globs.py:27-28); this module has no counterpart there.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+HEAD_DIMS = (64, 128)
+MAX_GROUP = 16            # query heads per KV head
+
+
+@dataclass
+class BlockTables:
+    tables: torch.Tensor       # int32 [seqs, max_pages], -1 where there is no page
+    used: torch.Tensor         # int32 [2]: pages taken from the free list, rows cut off at max_pages
+
+    @classmethod
+    def empty(cls, seqs: int, max_pages: int, device) -> "BlockTables":
+        return cls(torch.empty(seqs, max_pages, dtype=torch.int32, device=device),
+                   torch.empty(2, dtype=torch.int32, device=device))
+
+
+@dataclass
+class SlotMap:
+    slots: torch.Tensor        # int64 [tokens]: row of the pool, -1 where there is none
+    positions: torch.Tensor    # int32 [tokens]
+    seq_ids: torch.Tensor      # int32 [tokens], -1 behind the last token
+    active: torch.Tensor       # uint8 [tokens]: 1 where the token has a slot
+    cu_tokens: torch.Tensor    # int32 [seqs + 1]: first token of every request
+    kv_lengths: torch.Tensor   # int32 [seqs]: tokens in the cache after the step
+
+    @classmethod
+    def empty(cls, seqs: int, tokens: int, device) -> "SlotMap":
+        i32 = lambda n: torch.empty(n, dtype=torch.int32, device=device)
+        return cls(torch.empty(tokens, dtype=torch.int64, device=device), i32(tokens), i32(tokens),
+                   torch.empty(tokens, dtype=torch.uint8, device=device), i32(seqs + 1), i32(seqs))
+
+
+def _check(name: str, t, dtype: torch.dtype, dim: int) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.dim() != dim:
+        raise ValueError(f"{name}: expected {dim} dimensions, got shape {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _on(device: torch.device, **tensors) -> None:
+    """Every tensor of the call is on one CUDA device (the last check: what it says is about a call that is right otherwise)."""
+    if device.type != "cuda":
+        raise ValueError(f"the tensors must be CUDA tensors (there is no CPU path), got {device}")
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _page_size(page_size: int) -> int:
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size {page_size}: expected one of {PAGE_SIZES}")
+    return int(page_size)
+
+
+def _call(fn, args, device: torch.device) -> None:
+    code = fn(C.byref(args), device.index, torch.cuda.current_stream(device).cuda_stream)
+    if code != 0:
+        raise _lib.QmkError(code, _lib.load().qmk_paged_last_cuda_error().decode() if code == -3 else "")
+
+
+def build_block_tables(lengths: torch.Tensor, free_pages: torch.Tensor, *, page_size: int, max_pages: int,
+                       prefix_table: torch.Tensor | None = None, out: BlockTables | None = None) -> BlockTables:
+    """Block tables for requests that need room for `lengths` tokens each (int32 [seqs], the shared prefix included).
+
+    Row s gets min(ceil(lengths[s] / page_size), max_pages) pages: first those of `prefix_table` (int32), then pages of
+    `free_pages` (int32) in order, behind those of the rows before it; the rest of the row is -1.  `used` holds the
+    pages taken from `free_pages` (more than there are when it ran out: the entries it could not give are -1) and the
+    number of rows cut off at `max_pages`."""
+    _check("lengths", lengths, torch.int32, 1)
+    device = lengths.device
+    _check("free_pages", free_pages, torch.int32, 1)
+    seqs, max_pages, shared, page_size = lengths.shape[0], int(max_pages), 0, _page_size(page_size)
+    if prefix_table is not None:
+        _check("prefix_table", prefix_table, torch.int32, 1)
+        shared = prefix_table.shape[0]
+    if seqs < 1:
+        raise ValueError("lengths: no requests")
+    if not 1 <= max_pages < 2 ** 31:
+        raise ValueError(f"max_pages {max_pages}: expected at least 1")
+    if shared > max_pages:
+        raise ValueError(f"prefix_table has {shared} pages, more than max_pages = {max_pages}")
+    if out is None:
+        out = BlockTables.empty(seqs, max_pages, device)
+    else:
+        _check("out.tables", out.tables, torch.int32, 2)
+        _check("out.used", out.used, torch.int32, 1)
+        if out.tables.shape != (seqs, max_pages) or out.used.shape != (2,):
+            raise ValueError(f"out: expected tables {(seqs, max_pages)} and used (2,), got {tuple(out.tables.shape)} "
+                             f"and {tuple(out.used.shape)}")
+    _on(device, free_pages=free_pages, prefix_table=prefix_table, out=out.tables, used=out.used)
+    args = _lib.BlockTablesArgs(lengths.data_ptr(), free_pages.data_ptr(),
+                                prefix_table.data_ptr() if shared else None, out.tables.data_ptr(), out.used.data_ptr(),
+                                seqs, free_pages.shape[0], shared, page_size, max_pages)
+    _call(_lib.load().qmk_build_block_tables, args, device)
+    return out
+
+
+def build_slot_map(block_tables: torch.Tensor, kv_lengths: torch.Tensor, new_lengths: torch.Tensor, *, page_size: int,
+                   tokens: int, out: SlotMap | None = None) -> SlotMap:
+    """Where the K and V rows of a step's new tokens go: request s holds `kv_lengths[s]` tokens and appends
+    `new_lengths[s]` (both int32 [seqs]).  The step's tokens are numbered request by request; `tokens` is the room of the
+    outputs: what does not fit is cut off (the request that straddles it appends fewer), what is left over is filled
+    with slot -1, position 0, request -1, inactive.  `out.kv_lengths` may not be `kv_lengths` itself."""
+    _check("block_tables", block_tables, torch.int32, 2)
+    device = block_tables.device
+    _check("kv_lengths", kv_lengths, torch.int32, 1)
+    _check("new_lengths", new_lengths, torch.int32, 1)
+    seqs, max_pages = block_tables.shape
+    tokens, page_size = int(tokens), _page_size(page_size)
+    if seqs < 1 or max_pages < 1:
+        raise ValueError(f"block_tables: empty shape {tuple(block_tables.shape)}")
+    if kv_lengths.shape[0] != seqs or new_lengths.shape[0] != seqs:
+        raise ValueError(f"kv_lengths and new_lengths: expected {seqs} requests, got {kv_lengths.shape[0]} and "
+                         f"{new_lengths.shape[0]}")
+    if not 1 <= tokens < 2 ** 31:
+        raise ValueError(f"tokens {tokens}: expected at least 1")
+    if out is None:
+        out = SlotMap.empty(seqs, tokens, device)
+    else:
+        for name, dtype, n in (("slots", torch.int64, tokens), ("positions", torch.int32, tokens),
+                               ("seq_ids", torch.int32, tokens), ("active", torch.uint8, tokens),
+                               ("cu_tokens", torch.int32, seqs + 1), ("kv_lengths", torch.int32, seqs)):
+            t = getattr(out, name)
+            _check(f"out.{name}", t, dtype, 1)
+            if t.shape[0] != n:
+                raise ValueError(f"out.{name}: expected {n} entries, got {t.shape[0]}")
+        if out.kv_lengths.data_ptr() == kv_lengths.data_ptr():
+            raise ValueError("out.kv_lengths must not be kv_lengths itself")
+    _on(device, kv_lengths=kv_lengths, new_lengths=new_lengths, slots=out.slots, positions=out.positions,
+        seq_ids=out.seq_ids, active=out.active, cu_tokens=out.cu_tokens, out=out.kv_lengths)
+    args = _lib.SlotMapArgs(block_tables.data_ptr(), kv_lengths.data_ptr(), new_lengths.data_ptr(), out.slots.data_ptr(),
+                            out.positions.data_ptr(), out.seq_ids.data_ptr(), out.active.data_ptr(),
+                            out.cu_tokens.data_ptr(), out.kv_lengths.data_ptr(), seqs, tokens, page_size, max_pages)
+    _call(_lib.load().qmk_build_slot_map, args, device)
+    return out
+
+
+def _rows(name: str, t) -> None:
+    """[tokens, heads, head_dim] bf16 whose tokens may be any distance apart (a slice of a wider row)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: expected {torch.bfloat16}, got {t.dtype}")
+    if t.dim() != 3:
+        raise ValueError(f"{name}: expected [tokens, heads, head_dim], got shape {tuple(t.shape)}")
+    tokens, heads, size = t.shape
+    stride = t.stride()
+    if (stride[2] != 1 or (heads > 1 and stride[1] != size) or
+            (tokens > 1 and (stride[0] % 8 != 0 or stride[0] < heads * size)) or t.data_ptr() % 16 != 0):
+        raise ValueError(f"{name}: heads and dimensions must be contiguous, tokens a multiple of 8 elements apart and the "
+                         f"data 16-byte aligned; got strides {stride}")
+
+
+def attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, seqs: int, *, prefix_len: int = 0) -> torch.Tensor:
+    """The workspace of `prefix_attention` for calls with these shapes: a program that keeps it saves the allocation.  Calls
+    that may run at the same time (two streams, two captured graphs) need one each."""
+    n = _lib.load().qmk_prefix_attention_workspace(q.shape[0], seqs, q.shape[1], k_pages.shape[2], q.shape[2], prefix_len,
+                                                   q.device.index)
+    if n < 0:
+        raise _lib.QmkError(int(n))
+    return torch.empty(n, dtype=torch.uint8, device=q.device)
+
+
+def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables: torch.Tensor,
+                     kv_lengths: torch.Tensor, cu_tokens: torch.Tensor, *, prefix_table: torch.Tensor | None = None,
+                     prefix_len: int = 0, scale: float | None = None, out: torch.Tensor | None = None,
+                     lse: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a step's rows `q` [tokens, NH, HD] over the paged cache, causal inside a request.
+
+    Request s has the rows cu_tokens[s] .. cu_tokens[s + 1] - 1 and `kv_lengths[s]` tokens in the cache, its rows'
+    included; its row i sees the positions below kv_lengths[s] - rows + i + 1.  Positions below `prefix_len` (a multiple
+    of the page size) are read through `prefix_table`, once for all requests; the others through `block_tables`, whose
+    entries below prefix_len are not read.  A row that sees nothing gets zeros (lse: minus infinity).  Rows from
+    cu_tokens[seqs] on are left as they were in `out` and `lse` (a new `out` holds zeros there).  A page index outside the
+    pool reads as zeros.  What the last page holds behind a request's last token is never used; a non-finite V row
+    inside a request may reach every row of its step.
+
+    scale: 1 / sqrt(HD) by default.  lse: optional float32 [tokens, NH], receives the natural logarithm of the sum of
+    exponentials.  Sums are held in 32 bits; probabilities are rounded to bf16 before they meet V.  Inference only."""
+    _rows("q", q)
+    device = q.device
+    _check("k_pages", k_pages, torch.bfloat16, 4)
+    _check("v_pages", v_pages, torch.bfloat16, 4)
+    _check("block_tables", block_tables, torch.int32, 2)
+    _check("kv_lengths", kv_lengths, torch.int32, 1)
+    _check("cu_tokens", cu_tokens, torch.int32, 1)
+    tokens, heads, size = q.shape
+    num_pages, page_size, kv_heads, kv_size = k_pages.shape
+    seqs, max_pages = block_tables.shape
+    prefix_len = int(prefix_len)
+    if k_pages.shape != v_pages.shape:
+        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} differ")
+    if size not in HEAD_DIMS or kv_size != size:
+        raise ValueError(f"head_dim {size} (cache {kv_size}): expected one of {HEAD_DIMS}")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads != 0 or heads // kv_heads > MAX_GROUP:
+        raise ValueError(f"{heads} query heads over {kv_heads} KV heads: expected 1..{MAX_GROUP} per KV head")
+    if seqs < 1 or max_pages < 1 or num_pages < 1:
+        raise ValueError("block_tables and pages must not be empty")
+    if kv_lengths.shape[0] != seqs or cu_tokens.shape[0] != seqs + 1:
+        raise ValueError(f"expected kv_lengths [{seqs}] and cu_tokens [{seqs + 1}], got {kv_lengths.shape[0]} and "
+                         f"{cu_tokens.shape[0]}")
+    if prefix_len < 0 or prefix_len % _page_size(page_size) != 0:
+        raise ValueError(f"prefix_len {prefix_len}: expected whole pages of {page_size}")
+    if prefix_len:
+        if prefix_table is None:
+            raise ValueError("prefix_len needs a prefix_table")
+        _check("prefix_table", prefix_table, torch.int32, 1)
+        if prefix_table.shape[0] * page_size < prefix_len:
+            raise ValueError(f"prefix_table has {prefix_table.shape[0]} pages, prefix_len needs {prefix_len // page_size}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(size)
+    elif not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"scale {scale}: expected a positive number")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("prefix_attention has no gradient: call it under torch.inference_mode() or torch.no_grad()")
+    if out is None:
+        out = torch.zeros(tokens, heads, size, dtype=torch.bfloat16, device=device)
+    else:
+        _rows("out", out)
+        if out.shape != q.shape:
+            raise ValueError(f"out: expected shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    if workspace is not None:
+        _check("workspace", workspace, torch.uint8, 1)
+    if lse is not None:
+        _check("lse", lse, torch.float32, 2)
+        if lse.shape != (tokens, heads):
+            raise ValueError(f"lse: expected shape {(tokens, heads)}, got {tuple(lse.shape)}")
+    _on(device, k_pages=k_pages, v_pages=v_pages, block_tables=block_tables, kv_lengths=kv_lengths, cu_tokens=cu_tokens,
+        prefix_table=prefix_table if prefix_len else None, out=out, lse=lse, workspace=workspace)
+    if tokens == 0:
+        return out
+    lib = _lib.load()
+    need = lib.qmk_prefix_attention_workspace(tokens, seqs, heads, kv_heads, size, prefix_len, device.index)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    else:
+        if workspace.shape[0] < need:
+            raise ValueError(f"workspace has {workspace.shape[0]} bytes, the call needs {need}")
+    args = _lib.PrefixAttentionArgs(q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
+                                    k_pages.data_ptr(), v_pages.data_ptr(), block_tables.data_ptr(), kv_lengths.data_ptr(),
+                                    cu_tokens.data_ptr(), prefix_table.data_ptr() if prefix_len else None,
+                                    q.stride(0) if tokens > 1 else heads * size, out.stride(0) if tokens > 1 else heads * size,
+                                    tokens, seqs, heads, kv_heads, size, page_size, num_pages, max_pages, prefix_len, scale,
+                                    workspace.data_ptr(), workspace.shape[0])
+    _call(lib.qmk_prefix_attention, args, device)
+    return out

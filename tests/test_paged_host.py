@@ -1,0 +1,143 @@
+"""Paged KV cache without a GPU: what the entry points refuse, from Python and through the C ABI (a refused call launches
+nothing, so no device is needed)."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def paged():
+    from qimeng_megakernel_b200 import _build
+    _build.build()
+    from qimeng_megakernel_b200 import paged
+    return paged
+
+
+i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
+bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+
+
+def refused(exc, text, fn, *args, **kw):
+    with pytest.raises(exc, match=text):
+        fn(*args, **kw)
+
+
+def test_block_tables_refusals(paged):
+    f = paged.build_block_tables
+    ok = dict(page_size=16, max_pages=4)
+    refused(TypeError, "lengths must be a tensor", f, [1], i32(3), **ok)
+    refused(TypeError, "lengths: expected torch.int32", f, i32(3).long(), i32(3), **ok)
+    refused(ValueError, "lengths: expected 1 dim", f, i32(3, 1), i32(3), **ok)
+    refused(ValueError, "lengths must be contiguous", f, i32(6)[::2], i32(3), **ok)
+    refused(ValueError, "no requests", f, i32(0), i32(3), **ok)
+    refused(ValueError, "page_size 24", f, i32(3), i32(3), page_size=24, max_pages=4)
+    refused(ValueError, "max_pages 0", f, i32(3), i32(3), page_size=16, max_pages=0)
+    refused(ValueError, "more than max_pages", f, i32(3), i32(3), prefix_table=i32(5), **ok)
+    refused(ValueError, "out: expected", f, i32(3), i32(3), out=paged.BlockTables(i32(3, 5), i32(2)), **ok)
+    refused(TypeError, "out.tables", f, i32(3), i32(3), out=paged.BlockTables(i32(3, 4).long(), i32(2)), **ok)
+    refused(ValueError, "no CPU path", f, i32(3), i32(3), **ok)
+
+
+def test_slot_map_refusals(paged):
+    f = paged.build_slot_map
+    ok = dict(page_size=16, tokens=4)
+    refused(TypeError, "block_tables: expected", f, i32(3, 2).long(), i32(3), i32(3), **ok)
+    refused(ValueError, "empty shape", f, i32(3, 0), i32(3), i32(3), **ok)
+    refused(ValueError, "expected 3 requests", f, i32(3, 2), i32(2), i32(3), **ok)
+    refused(ValueError, "expected 3 requests", f, i32(3, 2), i32(3), i32(4), **ok)
+    refused(ValueError, "tokens 0", f, i32(3, 2), i32(3), i32(3), page_size=16, tokens=0)
+    refused(ValueError, "page_size 8", f, i32(3, 2), i32(3), i32(3), page_size=8, tokens=4)
+    out = paged.SlotMap.empty(3, 4, "cpu")
+    refused(ValueError, "out.slots: expected 5", f, i32(3, 2), i32(3), i32(3), page_size=16, tokens=5, out=out)
+    refused(ValueError, "not be kv_lengths itself", f, i32(3, 2), out.kv_lengths, i32(3), out=out, **ok)
+    refused(ValueError, "no CPU path", f, i32(3, 2), i32(3), i32(3), out=out, **ok)
+
+
+def attention(paged, T=3, H=8, HK=2, D=64, pages=6, page=16, seqs=2, room=4, prefix=32, **more):
+    a = dict(q=bf(T, H, D), k=bf(pages, page, HK, D), v=bf(pages, page, HK, D), tables=i32(seqs, room), kv=i32(seqs),
+             cu=i32(seqs + 1), prefix_table=i32(prefix // 16 if prefix >= 0 else 0), prefix_len=prefix)
+    a.update(more)
+    args = [a.pop(n) for n in ("q", "k", "v", "tables", "kv", "cu")]
+    return paged.prefix_attention(*args, **a)
+
+
+def test_attention_refusals(paged):
+    f = lambda **kw: attention(paged, **kw)
+    refused(TypeError, "q: expected torch.bfloat16", f, q=torch.zeros(3, 8, 64))
+    refused(TypeError, "k_pages: expected torch.bfloat16", f, k=torch.zeros(6, 16, 2, 64).half())
+    refused(ValueError, "q: expected .tokens, heads", f, q=bf(3, 512))
+    refused(ValueError, "q: heads and dimensions", f, q=bf(3, 64, 8).transpose(1, 2))
+    refused(ValueError, "16-byte aligned", f, q=bf(3 * 512 + 4)[4:].view(3, 8, 64))
+    refused(ValueError, "head_dim 96", f, D=96)
+    refused(ValueError, "head_dim 64 .cache 128", f, k=bf(6, 16, 2, 128), v=bf(6, 16, 2, 128))
+    refused(ValueError, "k_pages .* differ", f, v=bf(5, 16, 2, 64))
+    refused(ValueError, "query heads over", f, H=8, HK=3)
+    refused(ValueError, "query heads over", f, H=17, HK=1)
+    refused(ValueError, "k_pages must be contiguous", f, k=bf(6, 16, 4, 64)[:, :, :2])
+    refused(ValueError, "page_size 48", f, page=48, prefix=48)
+    refused(ValueError, "whole pages", f, prefix=24)
+    refused(ValueError, "whole pages", f, prefix=-16)
+    refused(ValueError, "prefix_table has 1 pages", f, prefix_table=i32(1))
+    refused(ValueError, "needs a prefix_table", f, prefix_table=None)
+    refused(ValueError, "expected kv_lengths", f, kv=i32(3))
+    refused(ValueError, "expected kv_lengths", f, cu=i32(2))
+    refused(ValueError, "scale 0", f, scale=0.0)
+    refused(ValueError, "scale nan", f, scale=float("nan"))
+    refused(ValueError, "scale inf", f, scale=float("inf"))
+    refused(ValueError, "out: expected shape", f, out=bf(2, 8, 64))
+    refused(ValueError, "lse: expected shape", f, lse=torch.zeros(3, 7))
+    refused(TypeError, "lse: expected torch.float32", f, lse=bf(3, 8))
+    refused(TypeError, "workspace: expected torch.uint8", f, workspace=torch.zeros(3))
+    refused(RuntimeError, "no gradient", f, q=bf(3, 8, 64).requires_grad_())
+    refused(ValueError, "no CPU path", f)
+
+
+def test_c_entries_refuse_before_they_launch(paged):
+    from qimeng_megakernel_b200 import _lib
+    lib = _lib.load()
+    assert lib.qmk_build_block_tables(None, 0, None) == -1
+    assert lib.qmk_build_slot_map(None, 0, None) == -1
+    assert lib.qmk_prefix_attention(None, 0, None) == -1
+    P = 4096                                                       # an aligned address that nothing may touch
+
+    def tables(**kw):
+        a = dict(lengths=P, free_pages=P, prefix_table=P, tables=P, used=P, seqs=2, num_free=3, prefix_pages=1, page_size=16,
+                 max_pages=4)
+        a.update(kw)
+        return lib.qmk_build_block_tables(C.byref(_lib.BlockTablesArgs(**a)), 0, None)
+
+    for kw in (dict(lengths=None), dict(tables=None), dict(used=None), dict(free_pages=None), dict(prefix_table=None),
+               dict(seqs=0), dict(num_free=-1), dict(prefix_pages=-1), dict(page_size=0), dict(page_size=512),
+               dict(page_size=17), dict(max_pages=0), dict(prefix_pages=5)):
+        assert tables(**kw) == -1, kw
+
+    def slots(**kw):
+        a = dict(block_tables=P, kv_lengths=P, new_lengths=P, slots=P, positions=P, seq_ids=P, active=P, cu_tokens=P,
+                 kv_lengths_out=2 * P, seqs=2, tokens=3, page_size=16, max_pages=4)
+        a.update(kw)
+        return lib.qmk_build_slot_map(C.byref(_lib.SlotMapArgs(**a)), 0, None)
+
+    for name in ("block_tables", "kv_lengths", "new_lengths", "slots", "positions", "seq_ids", "active", "cu_tokens",
+                 "kv_lengths_out"):
+        assert slots(**{name: None}) == -1, name
+    for kw in (dict(seqs=0), dict(tokens=0), dict(page_size=1), dict(max_pages=0), dict(kv_lengths_out=P)):
+        assert slots(**kw) == -1, kw
+
+    need = lib.qmk_prefix_attention_workspace(3, 2, 8, 2, 64, 32, 0)
+
+    def attn(**kw):
+        a = dict(q=P, out=P, lse=None, k_pages=P, v_pages=P, block_tables=P, kv_lengths=P, cu_tokens=P, prefix_table=P,
+                 q_token_stride=512, out_token_stride=512, tokens=3, seqs=2, num_heads=8, num_kv_heads=2, head_dim=64,
+                 page_size=16, num_pages=6, max_pages=4, prefix_len=32, scale=0.125, workspace=P,
+                 workspace_bytes=max(need, 1 << 30))
+        a.update(kw)
+        return lib.qmk_prefix_attention(C.byref(_lib.PrefixAttentionArgs(**a)), 0, None)
+
+    for name in ("q", "out", "k_pages", "v_pages", "block_tables", "kv_lengths", "cu_tokens", "prefix_table"):
+        assert attn(**{name: None}) == -1, name
+    for kw in (dict(q=P + 8), dict(out=P + 2), dict(k_pages=P + 8), dict(v_pages=P + 8), dict(q_token_stride=508),
+               dict(out_token_stride=516), dict(tokens=0), dict(seqs=0), dict(num_heads=9), dict(num_kv_heads=0),
+               dict(num_heads=34), dict(head_dim=80), dict(page_size=48), dict(num_pages=0), dict(max_pages=0),
+               dict(prefix_len=33), dict(prefix_len=-16), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf"))):
+        assert attn(**kw) == -1, kw
