@@ -1,9 +1,12 @@
 // C entry points of the paged KV cache: block tables, slot maps, attention with a shared prefix.
 // Plain launches on the caller's stream; no handle, no library-owned memory.
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdio.h>
 #include <string.h>
+
+#include <atomic>
 
 #include "../../include/qmk_b200.h"
 #include "qmk_paged_tables.cuh"
@@ -84,28 +87,133 @@ extern "C" int qmk_build_slot_map(const qmk_slot_map_args* a, int device, void* 
   return e == cudaSuccess ? QMK_OK : paged_fail(e, "slot_map_kernel");
 }
 
+// ------------------------------------------------------------------------------------------------ attention
+static int sm_count(int device) {
+  static std::atomic<int> known[64];
+  if (device < 0) return 0;
+  int n = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (device < 64) known[device].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+static PlanDims plan_dims(int tokens, int seqs, int num_heads, int num_kv_heads, int prefix_len, int ctas) {
+  PlanDims d;
+  d.tokens = tokens; d.seqs = seqs; d.G = num_heads / num_kv_heads; d.NKV = num_kv_heads; d.prefix_len = prefix_len;
+  d.ctas = ctas; d.room = prefix_len;
+  return d;
+}
+
+// Regions of the workspace; every one starts on a 256-byte boundary.
+struct WorkspaceLayout { long long dense_ml, dense_o, item_ml, item_o, dense_desc, item_desc, total; };
+static WorkspaceLayout workspace_layout(const PlanDims& d, int head_dim) {
+  WorkspaceLayout w;
+  long long at = 0;
+  auto take = [&](long long bytes) { const long long here = at; at += (bytes + 255) / 256 * 256; return here; };
+  const long long records = max_dense_records(d), items = max_items(d);
+  w.dense_ml = take(records * kUnitRows * 8);
+  w.item_ml = take(items * kItemRows * 8);
+  w.dense_desc = take((long long)d.tokens * d.NKV * 8);
+  w.item_desc = take((long long)d.tokens * d.NKV * 8);
+  w.dense_o = take(records * kUnitRows * head_dim * 4);
+  w.item_o = take(items * kItemRows * head_dim * 4);
+  w.total = at;
+  return w;
+}
+
+static bool attention_sizes_ok(int tokens, int seqs, int num_heads, int num_kv_heads, int head_dim, int prefix_len) {
+  return tokens >= 1 && tokens <= (1 << 20) && seqs >= 1 && seqs <= kMaxSeqs && (head_dim == 64 || head_dim == 128) &&
+         num_kv_heads >= 1 && num_heads >= 1 && num_heads <= 1024 && num_heads % num_kv_heads == 0 &&
+         num_heads / num_kv_heads <= kItemRows && prefix_len >= 0;
+}
+
 extern "C" int64_t qmk_prefix_attention_workspace(int32_t tokens, int32_t seqs, int32_t num_heads, int32_t num_kv_heads,
                                                   int32_t head_dim, int32_t prefix_len, int device) {
-  (void)tokens; (void)seqs; (void)num_heads; (void)num_kv_heads; (void)head_dim; (void)prefix_len; (void)device;
-  return 0;
+  if (!attention_sizes_ok(tokens, seqs, num_heads, num_kv_heads, head_dim, prefix_len)) return QMK_ERR_INVALID_ARG;
+  const int ctas = sm_count(device);
+  if (ctas < 1) return QMK_ERR_DEVICE;
+  return workspace_layout(plan_dims(tokens, seqs, num_heads, num_kv_heads, prefix_len, ctas), head_dim).total;
 }
 
 static int attention_args(const qmk_prefix_attention_args* a) {
   if (!a) return QMK_ERR_INVALID_ARG;
-  if (a->tokens < 1 || a->seqs < 1 || a->max_pages < 1 || a->num_pages < 1 || a->prefix_len < 0) return QMK_ERR_INVALID_ARG;
-  if (a->head_dim != 64 && a->head_dim != 128) return QMK_ERR_INVALID_ARG;
-  if (a->num_kv_heads < 1 || a->num_heads < 1 || a->num_heads % a->num_kv_heads != 0 || a->num_heads / a->num_kv_heads > 16)
-    return QMK_ERR_INVALID_ARG;
+  if (!attention_sizes_ok(a->tokens, a->seqs, a->num_heads, a->num_kv_heads, a->head_dim, a->prefix_len)) return QMK_ERR_INVALID_ARG;
+  if (a->max_pages < 1 || a->num_pages < 1) return QMK_ERR_INVALID_ARG;
   if (page_shift_of(a->page_size) < 0 || a->prefix_len % a->page_size != 0) return QMK_ERR_INVALID_ARG;
+  // positions and rows of the pool are 32-bit coordinates
+  if ((long long)a->max_pages * a->page_size > (1ll << 30) || a->prefix_len > (1 << 30) ||
+      (long long)a->num_pages * a->page_size > (1ll << 31) - 1024)
+    return QMK_ERR_INVALID_ARG;
   if (a->prefix_len > 0 && !a->prefix_table) return QMK_ERR_INVALID_ARG;
-  if (!a->block_tables || !a->kv_lengths || !a->cu_tokens || !a->q || !a->out || !a->k_pages || !a->v_pages) return QMK_ERR_INVALID_ARG;
+  if (!a->block_tables || !a->kv_lengths || !a->cu_tokens || !a->q || !a->out || !a->k_pages || !a->v_pages || !a->workspace)
+    return QMK_ERR_INVALID_ARG;
   const long long row = (long long)a->num_heads * a->head_dim;
   if (a->q_token_stride < row || a->out_token_stride < row || a->q_token_stride % 8 != 0 || a->out_token_stride % 8 != 0)
     return QMK_ERR_INVALID_ARG;
-  if (!aligned_to(a->q, 16) || !aligned_to(a->out, 16) || !aligned_to(a->k_pages, 16) || !aligned_to(a->v_pages, 16))
+  if (!aligned_to(a->q, 16) || !aligned_to(a->out, 16) || !aligned_to(a->k_pages, 16) || !aligned_to(a->v_pages, 16) ||
+      !aligned_to(a->workspace, 256))
     return QMK_ERR_INVALID_ARG;
   if (!(a->scale > 0.f) || isinf(a->scale)) return QMK_ERR_INVALID_ARG;
   return QMK_OK;
+}
+
+typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static encode_fn tensor_map_encoder() {
+  static std::atomic<void*> known{nullptr};
+  void* fn = known.load(std::memory_order_relaxed);
+  if (fn) return (encode_fn)fn;
+  cudaDriverEntryPointQueryResult q;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn ||
+      q != cudaDriverEntryPointSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  known.store(fn, std::memory_order_relaxed);
+  return (encode_fn)fn;
+}
+// The pool as {HD, NKV, rows}; boxes of 64 dimensions of one head, `box_rows` rows.  Rows outside read as zeros.
+static bool pool_map(encode_fn enc, CUtensorMap* m, const void* base, const qmk_prefix_attention_args* a, int box_rows) {
+  const cuuint64_t dims[3] = {(cuuint64_t)a->head_dim, (cuuint64_t)a->num_kv_heads, (cuuint64_t)a->num_pages * a->page_size};
+  const cuuint64_t strides[2] = {(cuuint64_t)a->head_dim * 2, (cuuint64_t)a->head_dim * 2 * a->num_kv_heads};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, es[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD>
+static int launch_attention(const qmk_prefix_attention_args* a, const AttnParams& p, const AttnMaps& maps, int device,
+                            cudaStream_t stream) {
+  using S = AttnSmem<HD>;
+  static std::atomic<unsigned long long> ready{0};                  // devices whose kernel may use its shared memory
+  cudaError_t e;
+  const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(prefix_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::total(kMaxSeqs));
+    if (e != cudaSuccess) return paged_fail(e, "cudaFuncSetAttribute");
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  prefix_attention_kernel<HD><<<(unsigned)p.d.ctas, kAttnThreads, S::total(p.d.seqs), stream>>>(p, maps);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return paged_fail(e, "prefix_attention_kernel");
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)(((long long)a->tokens * a->num_heads + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // (the kernel waits for its predecessor itself)
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, merge_kernel<HD>, p);
+  return e == cudaSuccess ? QMK_OK : paged_fail(e, "merge_kernel");
 }
 
 extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int device, void* cuda_stream) {
@@ -113,17 +221,38 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
   if (rc) return rc;
   DeviceScope scope(device);
   if (scope.err != cudaSuccess) return paged_fail(scope.err, "cudaSetDevice");
+  const int ctas = sm_count(device);
+  if (ctas < 1) return QMK_ERR_DEVICE;
   AttnParams p;
+  memset(&p, 0, sizeof(p));
+  p.d = plan_dims(a->tokens, a->seqs, a->num_heads, a->num_kv_heads, a->prefix_len, ctas);
+  const long long room = (long long)a->max_pages * a->page_size;
+  p.d.room = (int)(room > a->prefix_len ? room : a->prefix_len);
+  // 32-bit counts on the device: blocks of a KV head, items
+  if (max_units(p.d) * (p.d.room / kBlockKeys + 1) > 0x7fffffffll || max_items(p.d) > 0x7fffffffll) return QMK_ERR_INVALID_ARG;
+  const WorkspaceLayout w = workspace_layout(p.d, a->head_dim);
+  if (a->workspace_bytes < w.total) return QMK_ERR_INVALID_ARG;
   p.q = (const uint16_t*)a->q; p.out = (uint16_t*)a->out; p.lse = a->lse;
-  p.k_pages = (const uint16_t*)a->k_pages; p.v_pages = (const uint16_t*)a->v_pages;
   p.tables = a->block_tables; p.kv_lengths = a->kv_lengths; p.cu_tokens = a->cu_tokens; p.prefix_table = a->prefix_table;
   p.q_stride = a->q_token_stride; p.out_stride = a->out_token_stride;
-  p.tokens = a->tokens; p.seqs = a->seqs; p.NH = a->num_heads; p.NKV = a->num_kv_heads;
-  p.page_shift = page_shift_of(a->page_size); p.num_pages = a->num_pages; p.max_pages = a->max_pages; p.prefix_len = a->prefix_len;
+  p.NH = a->num_heads; p.page_shift = page_shift_of(a->page_size); p.num_pages = a->num_pages; p.max_pages = a->max_pages;
   p.scale_log2e = a->scale * 1.4426950408889634f;
-  const unsigned grid = (unsigned)(((long long)a->tokens * a->num_heads + 3) / 4);
-  if (a->head_dim == 64) prefix_attention_simple<64><<<grid, 128, 0, (cudaStream_t)cuda_stream>>>(p);
-  else prefix_attention_simple<128><<<grid, 128, 0, (cudaStream_t)cuda_stream>>>(p);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? QMK_OK : paged_fail(e, "prefix_attention_simple");
+  unsigned char* ws = (unsigned char*)a->workspace;
+  p.dense_ml = (float2*)(ws + w.dense_ml); p.dense_o = (float*)(ws + w.dense_o);
+  p.item_ml = (float2*)(ws + w.item_ml); p.item_o = (float*)(ws + w.item_o);
+  p.dense_desc = (int2*)(ws + w.dense_desc); p.item_desc = (int2*)(ws + w.item_desc);
+  encode_fn enc = tensor_map_encoder();
+  if (!enc) {
+    snprintf(g_paged_err, sizeof(g_paged_err), "cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)");
+    return QMK_ERR_CUDA;
+  }
+  AttnMaps maps;
+  const int box = a->page_size < kBlockKeys ? a->page_size : kBlockKeys;
+  if (!pool_map(enc, &maps.k, a->k_pages, a, box) || !pool_map(enc, &maps.v, a->v_pages, a, box) ||
+      !pool_map(enc, &maps.k16, a->k_pages, a, 16) || !pool_map(enc, &maps.v16, a->v_pages, a, 16)) {
+    snprintf(g_paged_err, sizeof(g_paged_err), "cuTensorMapEncodeTiled failed");
+    return QMK_ERR_CUDA;
+  }
+  return a->head_dim == 64 ? launch_attention<64>(a, p, maps, device, (cudaStream_t)cuda_stream)
+                           : launch_attention<128>(a, p, maps, device, (cudaStream_t)cuda_stream);
 }

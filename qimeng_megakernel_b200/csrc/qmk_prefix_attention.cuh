@@ -3,80 +3,1015 @@
 //   row i of request s (n_s rows this step, kv_s tokens in the cache with them):  lim = kv_s - n_s + i + 1
 //   o = sum_{j < lim} softmax_j(scale * q . k_j) v_j,    lse = log sum_{j < lim} exp(scale * q . k_j)
 //   position j lies in page prefix_table[j / page] for j < prefix_len and in block_tables[s][j / page] behind it
+//
+// One persistent CTA per SM works through its share of the plan (qmk_prefix_plan.h) in two parts.
+//
+// Blocks.  Up to 256 rows against 128 keys at a time with tcgen05.mma, in the manner of a running softmax: S = Q K^T into
+// tensor memory, a group of four warps (one thread per row) turns S into P = exp2(S - m), rounded to bf16 and put over S, and
+// O += P V.  Two groups alternate, so that the tensor pipe works for one while the other does its exponentials: each has
+// a tile of 128 rows, or, where a unit has only one tile, they share it and take alternate blocks.  m is raised (and O
+// rescaled) only when a row's maximum grows by more than 2^8; P then stays below 2^8, which costs no accuracy.
+//   tensor memory: S0 | S1 (128 columns each, P over S), O0 | O1 (HD columns each)
+//   warps 0-3, 4-7 softmax groups; 8 loads K and V blocks (one TMA box per page and 64 dimensions); 9 issues the products;
+//   10 clears the V rows behind the last key of a block that ends inside it
+//
+// Items.  What a short request holds behind the prefix: a warp per item, up to 16 rows x ck keys, mma.sync on 16-row tiles,
+// K and V through a ring of its own in shared memory (the ring of the blocks, free by then).
+//
+// Both parts leave partial results (m, l, unnormalised O, all in 32 bits) unless a row is complete; merge_kernel adds them
+// up in a fixed order, so a call gives the same bits every time.  Nothing is kept between calls.
+//
+// Every wait is bounded: one that expires raises the CTA's abort word, all waits then return, and the CTA's rows are NaN.
 #pragma once
+#include <cuda.h>
 #include <stdint.h>
 
 #include "qmk_device.cuh"
+#include "qmk_prefix_plan.h"
 
 namespace qmkp {
+
+using namespace qmk;
 
 struct AttnParams {
   const uint16_t* q;           // [tokens, NH, HD], q_stride elements from token to token
   uint16_t* out;               // [tokens, NH, HD], out_stride elements from token to token
   float* lse;                  // [tokens, NH] or null
-  const uint16_t* k_pages;     // [num_pages, page, NKV, HD]
-  const uint16_t* v_pages;
   const int* tables;           // [seqs, max_pages]
   const int* kv_lengths;       // [seqs]
   const int* cu_tokens;        // [seqs + 1]
   const int* prefix_table;     // [prefix_len / page]
   long long q_stride, out_stride;
-  int tokens, seqs, NH, NKV, page_shift, num_pages, max_pages, prefix_len;
+  PlanDims d;
+  int NH, page_shift, num_pages, max_pages;
   float scale_log2e;
+  // workspace
+  float* dense_o;              // [records, 256, HD]
+  float2* dense_ml;            // [records, 256]   (m in log2 units, l)
+  float* item_o;               // [items, 16, HD]
+  float2* item_ml;             // [items, 16]
+  int2* dense_desc;            // [tokens, NKV]    {first record, records | dual << 15 | row << 16}; records 0: none
+  int2* item_desc;             // [tokens, NKV]    {first record, records | row << 16}
+};
+struct AttnMaps {
+  CUtensorMap k, v;            // {HD, NKV, slots}, box {64, 1, min(page, 128)}
+  CUtensorMap k16, v16;        // the same, box {64, 1, 16}
 };
 
-// Request of a token: the last s with cu[s] <= token (empty requests before it share its start).
-__device__ __forceinline__ int request_of(const int* cu, int seqs, int token) {
-  int lo = 0, hi = seqs;
+constexpr int kAttnThreads = 384;
+constexpr int kProducerWarp = 8, kIssueWarp = 9, kClearWarp = 10;
+constexpr long long kWaitCycles = 4000000000ll;      // about two seconds
+
+template <int HD>
+struct AttnSmem {
+  static constexpr int kHalves = HD / 64;
+  static constexpr int kTileBytes = 128 * HD * 2;               // a 128-row Q tile, or a K or V block
+  static constexpr int kStages = HD == 64 ? 4 : 2;
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = 2 * kTileBytes;
+  static constexpr int kOffV = kOffK + kStages * kTileBytes;
+  static constexpr int kRing = kOffV + kStages * kTileBytes;
+  // items: per warp a ring of kItemStages stages of 8 KiB
+  static constexpr int kItemStages = 3, kItemStageBytes = 8192;
+  static constexpr int kItemKeys = HD == 64 ? 32 : 16;          // keys of a stage
+  static constexpr int kItemRing = kItemWarps * kItemStages * kItemStageBytes;
+  static constexpr int kOffBars = kRing > kItemRing ? kRing : kItemRing;
+  static constexpr int kNumBars = 4 * kStages + 1 + 2 + 2 + 2 + 2 + kItemWarps * kItemStages;
+  static constexpr int kOffCtl = kOffBars + kNumBars * 8;       // words: 0 abort, 1 tensor memory base
+  static constexpr int kOffRed = (kOffCtl + 16 + 7) / 8 * 8;    // long long [4][16] scratch of the scans
+  static constexpr int kOffTot = kOffRed + 4 * 16 * 8;          // Totals, Plan
+  static constexpr int kOffScan = (kOffTot + 128 + 15) / 16 * 16;   // int [4][seqs + 1]
+  static __host__ __device__ constexpr int total(int seqs) { return kOffScan + 4 * (seqs + 1) * 4; }
+};
+
+// ------------------------------------------------------------------------------------------------ primitives
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Operand in shared memory, 128-byte swizzle.  K-major (Q, K): 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | (1ull << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// V as the N x K operand, N (the dimensions) contiguous: 64-dimension atoms `half_bytes` apart, groups of 8 keys 1024 bytes.
+__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr, uint32_t half_bytes) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(half_bytes >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit_to(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(float* r, uint32_t addr) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+        "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
+        "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
+        "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+      "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]),
+      "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]),
+      "r"(u[31])
+      : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {   // 2^x, 2 ulp; results below 2^-126 are zero
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t u;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
+  return u;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Bounded wait on a phase of a barrier; false once the CTA has been aborted.
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile unsigned* ctl) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (ctl[0] != 0u) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      ctl[0] = 1u;
+      return false;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ plan
+struct Scans {                 // prefix sums over the requests, in shared memory, seqs + 1 entries each
+  int* long_blocks;
+  int* long_units;
+  int* short_tokens;
+  int* items;                  // row blocks x chunks (one KV head)
+};
+__device__ __forceinline__ Req load_request(const AttnParams& p, int s) {
+  return request(p.d, p.cu_tokens[s], p.cu_tokens[s + 1], p.kv_lengths[s]);
+}
+// The last entry of a[0 .. n] that is at most v (a[0] = 0 <= v < a[n]).
+__device__ __forceinline__ int find_last(const int* a, int n, int v) {
+  int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= token) lo = mid; else hi = mid;
+    if (a[mid] <= v) lo = mid; else hi = mid;
   }
   return lo;
 }
+// Exclusive prefix sums of up to four values over the CTA's threads; the totals come back too.
+template <int N>
+__device__ __forceinline__ void scan_values(long long (&v)[N], long long (&total)[N], long long* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int W = kAttnThreads / 32;
+  long long incl[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    long long x = v[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(kFullMask, x, o);
+      if (lane >= o) x += u;
+    }
+    incl[k] = x;
+    if (lane == 31) red[k * 16 + warp] = x;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const long long x = red[k * 16 + w];
+      before += w < warp ? x : 0;
+      all += x;
+    }
+    v[k] = before + incl[k] - v[k];
+    total[k] = all;
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc, long long* red, Totals& t, Plan& plan,
+                                           long long& items) {
+  const int seqs = p.d.seqs;
+  long long base[4] = {0, 0, 0, 0};
+  for (int s0 = 0; s0 < seqs; s0 += kAttnThreads) {
+    const int s = s0 + (int)threadIdx.x;
+    long long v[4] = {0, 0, 0, 0}, tot[4];
+    if (s < seqs) {
+      const Req r = load_request(p, s);
+      if (is_long(p.d, r)) {
+        const int n = units_of(p.d, r);
+        for (int u = 0; u < n; ++u) v[0] += unit_blocks(p.d, r, u);
+        v[1] = n;
+      } else {
+        v[2] = r.n;
+        v[3] = (long long)own_keys(p.d, r) * item_rows_blocks(p.d, r);
+      }
+    }
+    scan_values<4>(v, tot, red);
+    if (s < seqs) {
+      sc.long_blocks[s] = (int)(base[0] + v[0]);
+      sc.long_units[s] = (int)(base[1] + v[1]);
+      sc.short_tokens[s] = (int)(base[2] + v[2]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) base[k] += tot[k];
+  }
+  if (threadIdx.x == 0) {
+    sc.long_blocks[seqs] = (int)base[0];
+    sc.long_units[seqs] = (int)base[1];
+    sc.short_tokens[seqs] = (int)base[2];
+  }
+  t.long_blocks = base[0]; t.long_units = (int)base[1]; t.short_tokens = (int)base[2]; t.item_keys = base[3];
+  plan = make_plan(p.d, t);
+  long long at = 0;
+  for (int s0 = 0; s0 < seqs; s0 += kAttnThreads) {
+    const int s = s0 + (int)threadIdx.x;
+    long long v[1] = {0}, tot[1];
+    if (s < seqs) {
+      const Req r = load_request(p, s);
+      if (!is_long(p.d, r)) v[0] = (long long)item_rows_blocks(p.d, r) * item_chunks(own_keys(p.d, r), plan.ck);
+    }
+    scan_values<1>(v, tot, red);
+    if (s < seqs) sc.items[s] = (int)(at + v[0]);
+    at += tot[0];
+  }
+  if (threadIdx.x == 0) sc.items[seqs] = (int)at;
+  items = at * p.d.NKV;
+  __syncthreads();
+}
 
-// One warp per (token, query head): lanes share the head's dimensions, the keys are walked one by one with the running
-// maximum and sum of the softmax.
+// A unit of one KV head.
+struct Unit {
+  int kvh, index;       // index among the KV head's units
+  int s, u;             // long: request and unit inside it; short: s = -1, u = unit among the short ones
+  int blocks, limit;    // 128-key blocks; keys the unit's rows can see
+  int rows;             // packed rows that exist
+  Req r;
+};
+__device__ __forceinline__ Unit unit_at(const AttnParams& p, const Scans& sc, const Totals& t, const Plan& plan, long long b,
+                                        int& block) {
+  Unit x;
+  x.kvh = (int)(b / plan.blocks);
+  long long rest = b - (long long)x.kvh * plan.blocks;
+  if (rest < t.long_blocks) {
+    int lo = find_last(sc.long_blocks, p.d.seqs, (int)rest);
+    rest -= sc.long_blocks[lo];
+    x.s = lo;
+    x.r = load_request(p, lo);
+    x.u = 0;
+    for (;; ++x.u) {
+      x.blocks = unit_blocks(p.d, x.r, x.u);
+      if (rest < x.blocks) break;
+      rest -= x.blocks;
+    }
+    x.index = sc.long_units[lo] + x.u;
+    x.limit = unit_limit(p.d, x.r, x.u);
+    x.rows = min(p.d.unit_tokens(), x.r.n - x.u * p.d.unit_tokens()) * p.d.G;
+  } else {
+    rest -= t.long_blocks;
+    x.s = -1;
+    x.blocks = p.d.prefix_blocks();
+    x.u = (int)(rest / x.blocks);
+    rest -= (long long)x.u * x.blocks;
+    x.index = t.long_units + x.u;
+    x.limit = p.d.prefix_len;
+    x.rows = min(p.d.unit_tokens(), t.short_tokens - x.u * p.d.unit_tokens()) * p.d.G;
+    x.r = Req{0, 0, 0};
+  }
+  block = (int)rest;
+  return x;
+}
+// The row `row` of a unit: token (-1: none) and the keys it sees of the unit's.
+__device__ __forceinline__ int row_token(const AttnParams& p, const Scans& sc, const Unit& x, int row, int& lim) {
+  lim = 0x7fffffff;
+  if (row >= x.rows) return -1;
+  const int i = row / p.d.G;
+  if (x.s >= 0) {
+    const int t = x.u * p.d.unit_tokens() + i;
+    lim = limit_of(p.d, x.r, t);
+    return x.r.first + t;
+  }
+  const int at = x.u * p.d.unit_tokens() + i;
+  const int s = find_last(sc.short_tokens, p.d.seqs, at);
+  const Req r = load_request(p, s);
+  const int t = at - sc.short_tokens[s];
+  lim = min(limit_of(p.d, r, t), p.d.prefix_len);
+  return r.first + t;
+}
+
+// ------------------------------------------------------------------------------------------------ blocks
 template <int HD>
-__global__ void __launch_bounds__(128) prefix_attention_simple(const AttnParams p) {
-  constexpr int PER = HD / 32;
+struct Dense {
+  using S = AttnSmem<HD>;
+  const AttnParams& p;
+  const AttnMaps& maps;
+  unsigned char* smem;
+  uint32_t base;               // shared address of smem
+  volatile unsigned* ctl;
+  Scans sc;
+  Totals t;
+  Plan plan;
+  long long lo, hi;            // blocks of this CTA
+  uint32_t tmem;
+  int warp, lane;
+
+  __device__ __forceinline__ uint32_t bar(int i) const { return base + S::kOffBars + i * 8; }
+  __device__ __forceinline__ uint32_t k_full(int s) const { return bar(s); }
+  __device__ __forceinline__ uint32_t k_empty(int s) const { return bar(S::kStages + s); }
+  __device__ __forceinline__ uint32_t v_full(int s) const { return bar(2 * S::kStages + s); }
+  __device__ __forceinline__ uint32_t v_empty(int s) const { return bar(3 * S::kStages + s); }
+  __device__ __forceinline__ uint32_t q_full() const { return bar(4 * S::kStages); }
+  __device__ __forceinline__ uint32_t s_full(int g) const { return bar(4 * S::kStages + 1 + g); }
+  __device__ __forceinline__ uint32_t p_full(int g) const { return bar(4 * S::kStages + 3 + g); }
+  __device__ __forceinline__ uint32_t o_full(int g) const { return bar(4 * S::kStages + 5 + g); }
+  __device__ __forceinline__ uint32_t c_ask() const { return bar(4 * S::kStages + 7); }     // issuer -> warp 10: clear this block's V
+  __device__ __forceinline__ uint32_t c_done() const { return bar(4 * S::kStages + 8); }    // and back
+
+  // keys of block b of a unit that rows can see, and whether the V rows behind them have to be cleared
+  __device__ __forceinline__ static int valid_keys(const Unit& x, int b) { return max(0, min(kBlockKeys, x.limit - b * kBlockKeys)); }
+
+  __device__ __forceinline__ int page_of(const Unit& x, int key) const {
+    int id;
+    if (key < p.d.prefix_len) id = p.prefix_table[key >> p.page_shift];
+    else id = x.s >= 0 ? p.tables[(size_t)x.s * p.max_pages + (key >> p.page_shift)] : -1;
+    return id;
+  }
+  // K and V of the CTA's blocks: lane l loads box l of a block (a page, or 128 rows of one, of 64 dimensions).
+  __device__ __forceinline__ unsigned produce() {
+    const int box_rows = min(1 << p.page_shift, kBlockKeys);
+    const int key_of_lane = (lane / S::kHalves) * box_rows, half = lane % S::kHalves;
+    const int boxes = kBlockKeys / box_rows * S::kHalves;
+    const int oob = p.num_pages << p.page_shift;             // behind the last row: reads as zeros
+    unsigned n = 0;
+    for (long long b = lo; b < hi;) {
+      int b0;
+      const Unit x = unit_at(p, sc, t, plan, b, b0);
+      const int b1 = (int)min((long long)x.blocks, b0 + (hi - b));
+      auto row_of = [&](int blk) {                           // row of the pool that this lane's box starts at, -1: no box
+        const int key = blk * kBlockKeys + key_of_lane;
+        if (lane >= boxes || key >= x.limit) return -1;
+        const int id = page_of(x, key);
+        if (id < 0 || id >= p.num_pages) return oob;
+        return (id << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+      };
+      int row = row_of(b0);
+      for (int blk = b0; blk < b1; ++blk, ++n) {
+        const int st = n % S::kStages;
+        const uint32_t par = ((n / S::kStages) & 1u) ^ 1u;
+        const unsigned issue = __ballot_sync(kFullMask, row >= 0);
+        const uint32_t bytes = (uint32_t)__popc(issue) * (uint32_t)(box_rows * 128);
+        const uint32_t dst = (uint32_t)(half * kBlockKeys * 128 + key_of_lane * 128);
+        const int next = blk + 1 < b1 ? row_of(blk + 1) : -1;
+        if (!wait_bar(k_empty(st), par, ctl)) return n;
+        if (lane == 0) mbar_expect_tx(k_full(st), bytes);
+        __syncwarp();
+        if (row >= 0) tma_box(base + S::kOffK + st * S::kTileBytes + dst, &maps.k, half * 64, x.kvh, row, k_full(st));
+        if (!wait_bar(v_empty(st), par, ctl)) {
+          wait_bar(k_full(st), par ^ 1u, ctl);
+          return n;
+        }
+        if (lane == 0) mbar_expect_tx(v_full(st), bytes);
+        __syncwarp();
+        if (row >= 0) tma_box(base + S::kOffV + st * S::kTileBytes + dst, &maps.v, half * 64, x.kvh, row, v_full(st));
+        row = next;
+      }
+      b += b1 - b0;
+    }
+    return n;
+  }
+
+  // S = Q K^T and O += P V for the CTA's blocks (one lane).
+  __device__ __forceinline__ void issue() {
+    constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)HD >> 3) << 17) | ((128u >> 4) << 24);
+    const uint32_t s_col[2] = {tmem, tmem + 128}, o_col[2] = {tmem + 256, tmem + 384};
+    unsigned n = 0, segs = 0, p_par[2] = {0, 0}, clears = 0;
+    auto score = [&](int g, int tile, int st) {
+      const uint32_t qa = base + S::kOffQ + tile * S::kTileBytes, ka = base + S::kOffK + st * S::kTileBytes;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        const uint32_t off = (uint32_t)((k >> 2) * 16384 + (k & 3) * 32);
+        mma_ss(s_col[g], desc_k_major(qa + off), desc_k_major(ka + off), kIdescS, k > 0);
+      }
+      mma_commit_to(s_full(g));
+    };
+    for (long long b = lo; b < hi; ++segs) {
+      int b0;
+      const Unit x = unit_at(p, sc, t, plan, b, b0);
+      const int nb = (int)min((long long)(x.blocks - b0), hi - b);
+      const bool dual = x.rows <= 128;
+      if (!wait_bar(q_full(), segs & 1u, ctl)) return;
+      tmem_fence_after_sync();
+      // steps of the segment: (block, group); two tiles: both groups take every block, one tile: they alternate
+      const int steps = dual ? nb : 2 * nb;
+      auto block_of = [&](int i) { return dual ? i : i >> 1; };
+      auto start = [&](int i) -> bool {                       // scores of step i
+        const int blk = block_of(i), g = i & 1;
+        const unsigned m = n + (unsigned)blk;
+        const int st = (int)(m % S::kStages);
+        if (dual || g == 0)
+          if (!wait_bar(k_full(st), (m / S::kStages) & 1u, ctl)) return false;
+        tmem_fence_after_sync();
+        score(g, dual ? 0 : g, st);
+        if (dual || g == 1) mma_commit_to(k_empty(st));
+        return true;
+      };
+      if (!start(0)) return;
+      if (steps > 1 && !start(1)) return;
+      for (int i = 0; i < steps; ++i) {
+        const int blk = block_of(i), g = i & 1;
+        const unsigned m = n + (unsigned)blk;
+        const int st = (int)(m % S::kStages);
+        const int valid = valid_keys(x, b0 + blk);
+        if (dual || g == 0) {
+          if (!wait_bar(v_full(st), (m / S::kStages) & 1u, ctl)) return;
+          if (valid % 16 != 0) {
+            mbar_arrive(c_ask());
+            if (!wait_bar(c_done(), clears & 1u, ctl)) return;
+            ++clears;
+          }
+        }
+        if (!wait_bar(p_full(g), p_par[g], ctl)) return;
+        p_par[g] ^= 1u;
+        tmem_fence_after_sync();
+        const uint32_t va = base + S::kOffV + st * S::kTileBytes;
+        const int ks = (valid + 15) >> 4;
+        for (int k = 0; k < ks; ++k)
+          mma_ts(o_col[g], s_col[g] + 8 * k, desc_n_major(va + 2048u * k, 16384u), kIdescO, !(i < 2 && k == 0));
+        if (dual || g == 1) mma_commit_to(v_empty(st));
+        if (i + 2 < steps) {
+          if (!start(i + 2)) return;
+        } else {
+          mma_commit_to(o_full(g));
+        }
+      }
+      if (steps == 1) mma_commit_to(o_full(1));
+      n += (unsigned)nb;
+      b += nb;
+    }
+  }
+
+  // Rows of V behind the last visible key of a block: cleared, so that 0 * V is 0 whatever the page holds there.
+  __device__ __forceinline__ void clear() {
+    unsigned n = 0, asked = 0;
+    for (long long b = lo; b < hi;) {
+      int b0;
+      const Unit x = unit_at(p, sc, t, plan, b, b0);
+      const int nb = (int)min((long long)(x.blocks - b0), hi - b);
+      for (int blk = 0; blk < nb; ++blk, ++n) {
+        const int valid = valid_keys(x, b0 + blk);
+        if (valid % 16 == 0) continue;
+        const int st = (int)(n % S::kStages);
+        if (!wait_bar(c_ask(), asked & 1u, ctl)) return;     // (the block has landed: the issuer has seen it)
+        ++asked;
+        const int rows = 16 - (valid & 15);
+        for (int i = lane; i < rows * 8 * S::kHalves; i += 32) {
+          const int r = valid + i / (8 * S::kHalves), c = i % (8 * S::kHalves);
+          *reinterpret_cast<uint4*>(smem + S::kOffV + st * S::kTileBytes + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(c_done());
+      }
+      b += nb;
+    }
+  }
+
+  __device__ __forceinline__ void softmax() {
+    const int g = warp >> 2, row = g * 128 + (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + g * 128 + lane_base, o_col = tmem + 256 + g * 128 + lane_base;
+    unsigned segs = 0, s_par = 0;
+    for (long long b = lo; b < hi; ++segs) {
+      int b0;
+      const Unit x = unit_at(p, sc, t, plan, b, b0);
+      const int nb = (int)min((long long)(x.blocks - b0), hi - b);
+      const bool dual = x.rows <= 128;
+      // Q: thread `row` brings row `row` of the unit (with one tile the second group's threads have nothing to bring)
+      int lim;
+      const int tile_row = dual && g == 1 ? row - 128 : row;
+      const int token = row_token(p, sc, x, tile_row, lim);
+      const int head = x.kvh * p.d.G + tile_row % p.d.G;
+      if (!(dual && g == 1)) {
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + (size_t)max(token, 0) * p.q_stride + (size_t)head * HD);
+        unsigned char* dst = smem + S::kOffQ + g * S::kTileBytes + (row & 127) * 128;
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          const uint4 v = token >= 0 ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = v;
+        }
+        fence_async_shared();
+      }
+      tmem_fence_before_sync();                       // (the O of the segment before has been read)
+      mbar_arrive(q_full());
+      const bool warp_works = __ballot_sync(kFullMask, token >= 0) != 0u;
+      const int warp_lim = __reduce_min_sync(kFullMask, lim);
+      float m = -INFINITY, l = 0.f;
+      const int first = dual ? g : 0, step = dual ? 2 : 1;
+      bool ok = true;
+      for (int blk = first; blk < nb; blk += step) {
+        ok = wait_bar(s_full(g), s_par, ctl);
+        if (!ok) break;
+        s_par ^= 1u;
+        tmem_fence_after_sync();
+        if (warp_works) {
+          float s[128];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(s + 32 * c, s_col + 32 * c);
+          tmem_wait_ld();
+          const int k0 = (b0 + blk) * kBlockKeys;
+          if (k0 + kBlockKeys > warp_lim) {
+            const int vis = lim - k0;
+#pragma unroll
+            for (int j = 0; j < 128; ++j) s[j] = j < vis ? s[j] : -INFINITY;
+          }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2e;
+          // NaN scores: fmaxf passes them over, their own exponential keeps them
+          if (__any_sync(kFullMask, top > m + 8.f)) {
+            const float m_new = fmaxf(m, top);
+            if (blk != first) {
+              const float f = m_new == -INFINITY ? 1.f : ex2(m - m_new);
+              l *= f;
+#pragma unroll 1
+              for (int c = 0; c < HD / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld16(o, o_col + 16 * c);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                tmem_st16(o_col + 16 * c, o);
+              }
+            }
+            m = m_new;
+          }
+          const float off = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t pk[64];
+#pragma unroll
+          for (int j = 0; j < 128; j += 2) {
+            const float a = ex2(fmaf(s[j], p.scale_log2e, -off)), c = ex2(fmaf(s[j + 1], p.scale_log2e, -off));
+            sum[j & 2] += a;
+            sum[(j & 2) + 1] += c;
+            pk[j >> 1] = pack2(a, c);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st32(s_col, pk);
+          tmem_st32(s_col + 32, pk + 32);
+          tmem_wait_st();
+        }
+        tmem_fence_before_sync();
+        mbar_arrive(p_full(g));
+      }
+      if (ok) ok = wait_bar(o_full(g), segs & 1u, ctl);
+      tmem_fence_after_sync();
+      // ---- the unit's rows: complete, or a record ----
+      const int cta = (int)blockIdx.x;
+      const bool whole = b0 == 0 && nb == x.blocks && !dual && x.s >= 0;
+      const int rec = cta + x.kvh * plan.unit_total + x.index;
+      const bool have = first < nb;
+      if (warp_works) {
+        const float nan = __int_as_float(0x7fffffff);
+        if (whole) {
+          const float inv = !ok ? nan : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : nan));
+          uint16_t* dst = p.out + (size_t)max(token, 0) * p.out_stride + (size_t)head * HD;
+#pragma unroll 1
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o, o_col + 16 * c);
+            tmem_wait_ld();
+            if (token >= 0) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  w[j] = pack2(l == 0.f ? 0.f : __uint_as_float(o[8 * h + 2 * j]) * inv, l == 0.f ? 0.f : __uint_as_float(o[8 * h + 2 * j + 1]) * inv);
+                reinterpret_cast<uint4*>(dst + 16 * c)[h] = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+          }
+          if (token >= 0 && p.lse) p.lse[(size_t)token * p.NH + head] = !ok ? nan : (l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f);
+        } else {
+          float* dst = p.dense_o + ((size_t)rec * kUnitRows + row) * HD;
+          if (have) {
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o, o_col + 16 * c);
+              tmem_wait_ld();
+              if (token >= 0) {
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                  reinterpret_cast<uint4*>(dst + 16 * c)[h] = make_uint4(o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]);
+              }
+            }
+          }
+          if (token >= 0) p.dense_ml[(size_t)rec * kUnitRows + row] = ok ? make_float2(m, l) : make_float2(nan, nan);
+        }
+        // whoever starts the unit says where its rows' parts are
+        if (b0 == 0 && token >= 0 && tile_row % p.d.G == 0 && !(dual && g == 1)) {
+          const size_t at = (size_t)token * p.d.NKV + x.kvh;
+          int parts = 0;
+          if (!whole) parts = dense_owner(plan, b + x.blocks - 1) - cta + 1;
+          p.dense_desc[at] = make_int2(rec, parts | (dual ? 1 << 15 : 0) | (tile_row << 16));
+          if (x.s >= 0) p.item_desc[at] = make_int2(0, 0);
+        }
+      }
+      b += nb;
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ items
+template <int HD>
+__device__ __forceinline__ void walk_items(const AttnParams& p, const AttnMaps& maps, unsigned char* smem, volatile unsigned* ctl,
+                                           const Scans& sc, const Plan& plan, long long lo, long long hi, int warp, int lane) {
+  using S = AttnSmem<HD>;
+  constexpr int KS = S::kItemKeys, NT = KS / 8, GROUPS = KS / 16, HALVES = S::kHalves;
+  constexpr int KBYTES = KS * HD * 2;                       // 4 KiB of K, then 4 KiB of V
+  const uint32_t ring = smem_u32(smem) + warp * S::kItemStages * S::kItemStageBytes;
+  const uint32_t bars = smem_u32(smem) + S::kOffBars + (4 * S::kStages + 9 + warp * S::kItemStages) * 8;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int oob = p.num_pages << p.page_shift;
+  unsigned filled = 0;                                      // stages filled by this warp so far
+  for (long long item = lo + warp; item < hi; item += kItemWarps) {
+    // item = (request, row block, KV head, chunk), chunk fastest
+    const int flat = (int)(item / p.d.NKV);
+    const int s = find_last(sc.items, p.d.seqs, flat);
+    const Req r = load_request(p, s);
+    const int own = own_keys(p.d, r), chunks = item_chunks(own, plan.ck);
+    long long rest = item - (long long)sc.items[s] * p.d.NKV;
+    const int ch = (int)(rest % chunks);
+    rest /= chunks;
+    const int kvh = (int)(rest % p.d.NKV), rb = (int)(rest / p.d.NKV);
+    const int i0 = rb * p.d.item_tokens(), ni = min(p.d.item_tokens(), r.n - i0), rows = ni * p.d.G;
+    const int k_lo = p.d.prefix_len + ch * plan.ck;
+    const int k_hi = max(k_lo, min(k_lo + plan.ck, limit_of(p.d, r, i0 + ni - 1)));
+    const int row0 = g, row1 = g + 8;
+    const int lim0 = row0 < rows ? limit_of(p.d, r, i0 + row0 / p.d.G) : 0, lim1 = row1 < rows ? limit_of(p.d, r, i0 + row1 / p.d.G) : 0;
+    // page rows of the next 32 groups of 16 keys, one per lane
+    const int* table = p.tables + (size_t)s * p.max_pages;
+    auto group_row = [&](int grp) {
+      const int key = k_lo + grp * 16;
+      if (key >= k_hi) return -1;
+      const int id = table[key >> p.page_shift];
+      if (id < 0 || id >= p.num_pages) return oob;
+      return (id << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+    };
+    const int stages = (k_hi - k_lo + KS - 1) / KS;
+    int held = group_row(lane), held_from = 0;
+    int sent = 0;
+    auto send = [&](bool cleared) {                          // fills the next stage; lane l < 2 * GROUPS * HALVES sends one box
+      const int st = (int)((filled + (unsigned)sent) % S::kItemStages);
+      const int grp0 = sent * GROUPS;
+      if (grp0 + GROUPS > held_from + 32) {
+        held_from = grp0;
+        held = group_row(grp0 + lane);
+      }
+      const int q = lane % (GROUPS * HALVES), kg = q / HALVES, half = q % HALVES;
+      const bool is_v = lane >= GROUPS * HALVES;
+      const int row = __shfl_sync(kFullMask, held, (grp0 + kg - held_from) & 31);
+      const bool mine = lane < 2 * GROUPS * HALVES && row >= 0;
+      const unsigned issue = __ballot_sync(kFullMask, mine);
+      if (cleared) fence_async_shared();
+      if (lane == 0) mbar_expect_tx(bars + st * 8, (uint32_t)__popc(issue) * 2048u);
+      __syncwarp();
+      if (mine)
+        tma_box(ring + st * S::kItemStageBytes + (is_v ? KBYTES : 0) + (kg * HALVES + half) * 2048, is_v ? &maps.v16 : &maps.k16,
+                half * 64, kvh, row, bars + st * 8);
+      ++sent;
+    };
+    while (sent < stages && sent < S::kItemStages) send(false);
+    // Q rows g and g + 8 as the A operand
+    uint32_t qa[HD / 16][4];
+    {
+      const uint16_t* q0 = p.q + (size_t)(r.first + i0 + row0 / p.d.G) * p.q_stride + (size_t)(kvh * p.d.G + row0 % p.d.G) * HD + 2 * t4;
+      const uint16_t* q1 = p.q + (size_t)(r.first + i0 + row1 / p.d.G) * p.q_stride + (size_t)(kvh * p.d.G + row1 % p.d.G) * HD + 2 * t4;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        qa[k][0] = row0 < rows ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k) : 0u;
+        qa[k][1] = row1 < rows ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k) : 0u;
+        qa[k][2] = row0 < rows ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 8) : 0u;
+        qa[k][3] = row1 < rows ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 8) : 0u;
+      }
+    }
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float o[HD / 8][4];
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    bool ok = true;
+    for (int i = 0; i < stages; ++i) {
+      const unsigned f = filled + (unsigned)i;
+      const int st = (int)(f % S::kItemStages);
+      ok = wait_bar(bars + st * 8, (f / S::kItemStages) & 1u, ctl);
+      if (!ok) break;
+      const uint32_t kb = ring + st * S::kItemStageBytes, vb = kb + KBYTES;
+      const int key0 = k_lo + i * KS;
+      const int valid = min(KS, k_hi - key0);
+      bool cleared = false;
+      if (valid < KS) {                                     // rows of V behind the last key: whatever they hold, 0 * V is to be 0
+        unsigned char* vp = smem + warp * S::kItemStages * S::kItemStageBytes + st * S::kItemStageBytes + KBYTES;
+        for (int e = lane; e < (KS - valid) * 8 * HALVES; e += 32) {
+          const int rr = valid + e / (8 * HALVES), c = e % (8 * HALVES);
+          *reinterpret_cast<uint4*>(vp + ((rr >> 4) * HALVES + (c >> 3)) * 2048 + (rr & 15) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+        cleared = true;
+      }
+      float sc4[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        sc4[j][0] = sc4[j][1] = sc4[j][2] = sc4[j][3] = 0.f;
+        const int kr = (j & 1) * 8 + (lane & 7);            // key row inside its group of 16
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {                 // four 16-byte pieces: two k-steps
+          const int piece = 4 * c + (lane >> 3);
+          uint32_t bfr[4];
+          ldsm4(bfr, kb + ((j >> 1) * HALVES + (piece >> 3)) * 2048 + kr * 128 + (((piece & 7) ^ (kr & 7)) << 4));
+          mma16816(sc4[j], qa[2 * c], bfr[0], bfr[1]);
+          mma16816(sc4[j], qa[2 * c + 1], bfr[2], bfr[3]);
+        }
+      }
+      float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int key = key0 + 8 * j + 2 * t4;
+        sc4[j][0] = key < min(lim0, k_hi) ? sc4[j][0] * p.scale_log2e : -INFINITY;
+        sc4[j][1] = key + 1 < min(lim0, k_hi) ? sc4[j][1] * p.scale_log2e : -INFINITY;
+        sc4[j][2] = key < min(lim1, k_hi) ? sc4[j][2] * p.scale_log2e : -INFINITY;
+        sc4[j][3] = key + 1 < min(lim1, k_hi) ? sc4[j][3] * p.scale_log2e : -INFINITY;
+        t0 = fmaxf(t0, fmaxf(sc4[j][0], sc4[j][1]));
+        t1 = fmaxf(t1, fmaxf(sc4[j][2], sc4[j][3]));
+      }
+#pragma unroll
+      for (int d = 1; d <= 2; d <<= 1) {
+        t0 = fmaxf(t0, __shfl_xor_sync(kFullMask, t0, d));
+        t1 = fmaxf(t1, __shfl_xor_sync(kFullMask, t1, d));
+      }
+      const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+      const float f0 = n0 == -INFINITY ? 1.f : ex2(m0 - n0), f1 = n1 == -INFINITY ? 1.f : ex2(m1 - n1);
+      const float off0 = n0 == -INFINITY ? 0.f : n0, off1 = n1 == -INFINITY ? 0.f : n1;
+      m0 = n0; m1 = n1;
+      l0 *= f0; l1 *= f1;
+#pragma unroll
+      for (int j = 0; j < HD / 8; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
+      uint32_t pa[GROUPS][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const float a = ex2(sc4[j][0] - off0), b = ex2(sc4[j][1] - off0), c = ex2(sc4[j][2] - off1), d = ex2(sc4[j][3] - off1);
+        l0 += a + b;
+        l1 += c + d;
+        pa[j >> 1][(j & 1) * 2] = pack2(a, b);
+        pa[j >> 1][(j & 1) * 2 + 1] = pack2(c, d);
+      }
+#pragma unroll
+      for (int kg = 0; kg < GROUPS; ++kg)
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+          const int kr = lane & 15, piece = 2 * c + (lane >> 4);
+          uint32_t bfr[4];
+          ldsm4_t(bfr, vb + (kg * HALVES + (piece >> 3)) * 2048 + kr * 128 + (((piece & 7) ^ (kr & 7)) << 4));
+          mma16816(o[2 * c], pa[kg], bfr[0], bfr[1]);
+          mma16816(o[2 * c + 1], pa[kg], bfr[2], bfr[3]);
+        }
+      __syncwarp();                                         // every lane has read the stage
+      if (sent < stages) send(cleared);
+    }
+    if (!ok) {                                              // leave no copy in flight
+      for (int i = 0; i < sent; ++i) {
+        const unsigned f = filled + (unsigned)i;
+        const long long w0 = clock64();
+        while (!mbar_try_wait(bars + (f % S::kItemStages) * 8, (f / S::kItemStages) & 1u))
+          if (clock64() - w0 > 1000000) break;
+      }
+    }
+    if (ok && stages > 0 && ((k_hi - k_lo) % KS) != 0) fence_async_shared();   // (a cleared stage may be refilled by the next item)
+    filled += (unsigned)sent;
+#pragma unroll
+    for (int d = 1; d <= 2; d <<= 1) {
+      l0 += __shfl_xor_sync(kFullMask, l0, d);
+      l1 += __shfl_xor_sync(kFullMask, l1, d);
+    }
+    const float nan = __int_as_float(0x7fffffff);
+    if (!ok) m0 = m1 = l0 = l1 = nan;
+    const bool whole = p.d.prefix_len == 0 && chunks == 1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = h ? row1 : row0;
+      if (row >= rows) continue;
+      const float m = h ? m1 : m0, l = h ? l1 : l0;
+      const int token = r.first + i0 + row / p.d.G, head = kvh * p.d.G + row % p.d.G;
+      if (whole) {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : nan);
+        uint16_t* dst = p.out + (size_t)token * p.out_stride + (size_t)head * HD + 2 * t4;
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j)
+          *reinterpret_cast<uint32_t*>(dst + 8 * j) = l == 0.f ? 0u : pack2(o[j][2 * h] * inv, o[j][2 * h + 1] * inv);
+        if (p.lse && t4 == 0) p.lse[(size_t)token * p.NH + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      } else {
+        float* dst = p.item_o + ((size_t)item * kItemRows + row) * HD + 2 * t4;
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j) *reinterpret_cast<float2*>(dst + 8 * j) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+        if (t4 == 0) p.item_ml[(size_t)item * kItemRows + row] = make_float2(m, l);
+      }
+      if (ch == 0 && t4 == 0 && row % p.d.G == 0) {
+        const size_t at = (size_t)token * p.d.NKV + kvh;
+        p.item_desc[at] = make_int2((int)item, (whole ? 0 : chunks) | (row << 16));
+        if (p.d.prefix_len == 0) p.dense_desc[at] = make_int2(0, 0);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ kernels
+template <int HD>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ AttnMaps maps) {
+  using S = AttnSmem<HD>;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile unsigned* ctl = reinterpret_cast<volatile unsigned*>(smem + S::kOffCtl);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  Scans sc;
+  sc.long_blocks = reinterpret_cast<int*>(smem + S::kOffScan);
+  sc.long_units = sc.long_blocks + p.d.seqs + 1;
+  sc.short_tokens = sc.long_units + p.d.seqs + 1;
+  sc.items = sc.short_tokens + p.d.seqs + 1;
+  Dense<HD> w{p, maps, smem, smem_u32(smem), ctl, sc, {}, {}, 0, 0, 0u, warp, lane};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(w.k_full(s), 1);
+      mbar_init(w.k_empty(s), 1);
+      mbar_init(w.v_full(s), 1);
+      mbar_init(w.v_empty(s), 1);
+    }
+    mbar_init(w.q_full(), 256);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(w.s_full(g), 1);
+      mbar_init(w.p_full(g), 128);
+      mbar_init(w.o_full(g), 1);
+    }
+    mbar_init(w.c_ask(), 1);
+    mbar_init(w.c_done(), 1);
+    for (int i = 0; i < kItemWarps * S::kItemStages; ++i) mbar_init(w.bar(4 * S::kStages + 9 + i), 1);
+    fence_barrier_init();
+    ctl[0] = 0u;
+  }
+  long long items;
+  build_plan(p, sc, reinterpret_cast<long long*>(smem + S::kOffRed), w.t, w.plan, items);
+  dense_range(w.plan, (int)blockIdx.x, w.lo, w.hi);
+  if (w.lo < w.hi) {
+    if (warp == kIssueWarp) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(w.base + S::kOffCtl + 4) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+      tmem_fence_before_sync();
+    }
+    __syncthreads();
+    tmem_fence_after_sync();
+    w.tmem = ctl[1];
+    unsigned issued = 0;
+    if (warp < kItemWarps) w.softmax();
+    else if (warp == kProducerWarp) issued = w.produce();
+    else if (warp == kIssueWarp) {
+      if (lane == 0) w.issue();
+      __syncwarp();
+    } else if (warp == kClearWarp) w.clear();
+    __syncwarp();
+    if (warp == kProducerWarp && ctl[0] != 0u) {             // aborted: no copy stays in flight
+      const unsigned from = issued > (unsigned)S::kStages ? issued - S::kStages : 0u;
+      for (unsigned n = from; n < issued; ++n) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(w.k_full(n % S::kStages), (n / S::kStages) & 1u) || !mbar_try_wait(w.v_full(n % S::kStages), (n / S::kStages) & 1u))
+          if (clock64() - t0 > 1000000) break;
+      }
+    }
+    tmem_fence_before_sync();
+    __syncthreads();
+    if (warp == kIssueWarp) {
+      tmem_fence_after_sync();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(w.tmem) : "memory");
+    }
+    fence_async_shared();                                    // (the ring's generic writes, before copies land in it again)
+    __syncthreads();
+  }
+  long long lo, hi;
+  item_range(p.d, w.plan, w.t, items, (int)blockIdx.x, lo, hi);
+  if (warp < kItemWarps) walk_items<HD>(p, maps, smem, ctl, sc, w.plan, lo, hi, warp, lane);
+}
+
+// Adds a row's parts: one warp per (token, query head).  With M = max m_r and w_r = 2^(m_r - M):
+//   o = sum_r w_r O_r / sum_r w_r l_r
+template <int HD>
+__global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ AttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int token = (int)(row / p.NH), head = (int)(row % p.NH);
-  if (token >= p.tokens || token >= p.cu_tokens[p.seqs]) return;
-  const int s = request_of(p.cu_tokens, p.seqs, token);
-  const int n = p.cu_tokens[s + 1] - p.cu_tokens[s], i = token - p.cu_tokens[s];
-  long long lim = (long long)p.kv_lengths[s] - n + i + 1;
-  const long long room = max((long long)p.max_pages << p.page_shift, (long long)p.prefix_len);
-  lim = lim < room ? lim : room;
-  const int kvh = head / (p.NH / p.NKV);
-  float q[PER], o[PER], m = -INFINITY, l = 0.f;
+  if (token >= min(p.d.tokens, p.cu_tokens[p.d.seqs])) return;
+  const int kvh = head / p.d.G, g = head % p.d.G;
+  const size_t at = (size_t)token * p.d.NKV + kvh;
+  const int2 dd = p.dense_desc[at], id = p.item_desc[at];
+  const int nseg = dd.y & 0x7fff, dual = (dd.y >> 15) & 1, nd = nseg << dual, ni = id.y & 0xffff;
+  if (nd + ni == 0) return;
+  const size_t drow = (size_t)dd.x * kUnitRows + ((unsigned)dd.y >> 16) + g, irow = (size_t)id.x * kItemRows + ((unsigned)id.y >> 16) + g;
+  auto ml_of = [&](int r) {
+    if (r < nd) return p.dense_ml[drow + (size_t)(r >> dual) * kUnitRows + (dual ? (r & 1) * 128 : 0)];
+    return p.item_ml[irow + (size_t)(r - nd) * kItemRows];
+  };
+  auto o_of = [&](int r) {
+    if (r < nd) return p.dense_o + (drow + (size_t)(r >> dual) * kUnitRows + (dual ? (r & 1) * 128 : 0)) * HD;
+    return p.item_o + (irow + (size_t)(r - nd) * kItemRows) * HD;
+  };
+  constexpr int LPR = HD / 4, PER = 32 / LPR;              // lanes per row, rows per pass
+  float M = -INFINITY, L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int r0 = 0; r0 < nd + ni; r0 += 32) {
+    const bool have = r0 + lane < nd + ni;
+    const float2 ml = have ? ml_of(r0 + lane) : make_float2(-INFINITY, 0.f);
+    float top = ml.x;
 #pragma unroll
-  for (int d = 0; d < PER; ++d) {
-    q[d] = qmk::bf16_bits_to_f32(p.q[(size_t)token * p.q_stride + (size_t)head * HD + lane + 32 * d]);
-    o[d] = 0.f;
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
+    const float Mn = fmaxf(M, top);
+    const float f = Mn == -INFINITY ? 1.f : ex2(M - Mn);
+    M = Mn;
+    float wgt = Mn == -INFINITY ? 0.f : ex2(ml.x - Mn);
+    if (ml.x != ml.x) wgt = ml.x;
+    L = L * f + warp_sum(wgt * ml.y);
+    acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+    const int n = min(32, nd + ni - r0);
+#pragma unroll 8
+    for (int r = 0; r < n; r += PER) {
+      const int rr = r + lane / LPR;
+      const float wr = __shfl_sync(kFullMask, wgt, rr & 31);
+      if (rr < n && wr != 0.f) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(o_of(r0 + rr)) + lane % LPR);
+        acc.x += wr * v.x; acc.y += wr * v.y; acc.z += wr * v.z; acc.w += wr * v.w;
+      }
+    }
   }
-  const int page_mask = (1 << p.page_shift) - 1;
-  for (int j = 0; j < lim; ++j) {
-    const int page = j < p.prefix_len ? p.prefix_table[j >> p.page_shift] : p.tables[(size_t)s * p.max_pages + (j >> p.page_shift)];
-    const bool held = page >= 0 && page < p.num_pages;
-    const size_t at = ((((size_t)(held ? page : 0) << p.page_shift) + (j & page_mask)) * p.NKV + kvh) * HD + lane;
-    float x = 0.f;
 #pragma unroll
-    for (int d = 0; d < PER; ++d) x += held ? q[d] * qmk::bf16_bits_to_f32(p.k_pages[at + 32 * d]) : 0.f;
-    x = qmk::warp_sum(x) * p.scale_log2e;
-    const float m_new = fmaxf(m, x);
-    const float c = m_new == -INFINITY ? 1.f : exp2f(m - m_new), e = m_new == -INFINITY ? 0.f : exp2f(x - m_new);
-    m = m_new;
-    l = l * c + e;
-#pragma unroll
-    for (int d = 0; d < PER; ++d) o[d] = o[d] * c + (held ? e * qmk::bf16_bits_to_f32(p.v_pages[at + 32 * d]) : 0.f);
+  for (int d = LPR; d < 32; d <<= 1) {
+    acc.x += __shfl_xor_sync(kFullMask, acc.x, d);
+    acc.y += __shfl_xor_sync(kFullMask, acc.y, d);
+    acc.z += __shfl_xor_sync(kFullMask, acc.z, d);
+    acc.w += __shfl_xor_sync(kFullMask, acc.w, d);
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-  for (int d = 0; d < PER; ++d)
-    p.out[(size_t)token * p.out_stride + (size_t)head * HD + lane + 32 * d] = qmk::f32_to_bf16_bits(o[d] * inv);
-  if (p.lse && lane == 0) p.lse[(size_t)token * p.NH + head] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  const bool none = L == 0.f;
+  const float inv = none ? 0.f : 1.f / L;
+  if (lane < LPR) {
+    uint2 w = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
+    if (none) w = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2*>(p.out + (size_t)token * p.out_stride + (size_t)head * HD + 4 * lane) = w;
+  }
+  if (p.lse && lane == 0) p.lse[(size_t)token * p.NH + head] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 }  // namespace qmkp

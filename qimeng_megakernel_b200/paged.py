@@ -30,6 +30,7 @@ from . import _lib
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
 MAX_GROUP = 16            # query heads per KV head
+MAX_SEQS = 2048           # requests of one attention call
 
 
 @dataclass
@@ -227,8 +228,10 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         raise ValueError(f"head_dim {size} (cache {kv_size}): expected one of {HEAD_DIMS}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads != 0 or heads // kv_heads > MAX_GROUP:
         raise ValueError(f"{heads} query heads over {kv_heads} KV heads: expected 1..{MAX_GROUP} per KV head")
-    if seqs < 1 or max_pages < 1 or num_pages < 1:
+    if max_pages < 1 or num_pages < 1:
         raise ValueError("block_tables and pages must not be empty")
+    if not 1 <= seqs <= MAX_SEQS:
+        raise ValueError(f"{seqs} requests: expected 1..{MAX_SEQS} requests")
     if kv_lengths.shape[0] != seqs or cu_tokens.shape[0] != seqs + 1:
         raise ValueError(f"expected kv_lengths [{seqs}] and cu_tokens [{seqs + 1}], got {kv_lengths.shape[0]} and "
                          f"{cu_tokens.shape[0]}")
@@ -264,6 +267,8 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         return out
     lib = _lib.load()
     need = lib.qmk_prefix_attention_workspace(tokens, seqs, heads, kv_heads, size, prefix_len, device.index)
+    if need < 0:
+        raise _lib.QmkError(int(need))
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     else:

@@ -1,0 +1,187 @@
+// Replays the plan of the prefix attention (qmk_prefix_plan.h) on the CPU: every (KV head, row, visible key) has to be
+// walked exactly once, by a block of a unit or by an item; every partial result has to have a record of its own inside the
+// workspace's bounds; and the records that a row's description names have to be the ones that were written for it.
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <vector>
+
+#include "../qimeng_megakernel_b200/csrc/qmk_prefix_plan.h"
+
+using namespace qmkp;
+
+#define CHECK(c)                                                      \
+  do {                                                                \
+    if (!(c)) {                                                       \
+      std::printf("line %d: %s (case %d)\n", __LINE__, #c, g_case);  \
+      std::exit(1);                                                   \
+    }                                                                 \
+  } while (0)
+static int g_case;
+
+struct Walk { std::vector<std::vector<int>> seen; };   // [row of the step * NKV + kvh][key] -> times
+
+int main() {
+  std::mt19937 rng(7);
+  auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
+  for (g_case = 0; g_case < 1500; ++g_case) {
+    PlanDims d;
+    d.G = pick(1, 16);
+    d.NKV = pick(1, 4);
+    d.seqs = pick(1, pick(0, 3) ? 6 : 40);
+    d.ctas = pick(0, 1) ? 148 : pick(1, 30);
+    d.prefix_len = pick(0, 3) ? 16 * pick(0, 60) : 0;
+    const int page = 16, max_pages = d.prefix_len / page + pick(1, 40);
+    d.room = max_pages * page > d.prefix_len ? max_pages * page : d.prefix_len;
+    std::vector<int> cu(1, 0), kv;
+    const int kind = pick(0, 3);
+    for (int s = 0; s < d.seqs; ++s) {
+      const int n = kind == 0 ? 1 : (kind == 1 ? pick(0, 5) : (kind == 2 ? pick(0, 400 / d.G) : pick(0, 2) * pick(0, 600)));
+      cu.push_back(cu.back() + n);
+      kv.push_back(pick(0, 9) ? d.prefix_len + pick(0, max_pages * page - d.prefix_len + 5) : pick(-3, d.prefix_len + n));
+    }
+    d.tokens = cu.back() + pick(-3, 5);
+    if (d.tokens < 1) d.tokens = 1;
+
+    std::vector<Req> req;
+    std::vector<int> lb(1, 0), lu(1, 0), stk(1, 0), it(1, 0);
+    Totals t{0, 0, 0, 0};
+    for (int s = 0; s < d.seqs; ++s) {
+      const Req r = request(d, cu[s], cu[s + 1], kv[s]);
+      req.push_back(r);
+      int blocks = 0;
+      if (is_long(d, r)) {
+        for (int u = 0; u < units_of(d, r); ++u) blocks += unit_blocks(d, r, u);
+        t.long_blocks += blocks;
+        t.long_units += units_of(d, r);
+      } else {
+        t.short_tokens += r.n;
+        t.item_keys += (long long)own_keys(d, r) * item_rows_blocks(d, r);
+      }
+      lb.push_back((int)t.long_blocks);
+      lu.push_back(t.long_units);
+      stk.push_back(t.short_tokens);
+    }
+    const Plan p = make_plan(d, t);
+    long long per_head = 0;
+    for (int s = 0; s < d.seqs; ++s) {
+      if (!is_long(d, req[s])) per_head += (long long)item_rows_blocks(d, req[s]) * item_chunks(own_keys(d, req[s]), p.ck);
+      it.push_back((int)per_head);
+    }
+    const long long items = per_head * d.NKV;
+    CHECK(items <= max_items(d));
+    CHECK(p.unit_total <= max_units(d));
+    CHECK(p.dense_ctas <= d.ctas && (p.dense_blocks == 0) == (p.dense_ctas == 0));
+
+    Walk w;
+    w.seen.resize((size_t)d.tokens * d.NKV);
+    std::vector<int> limit(d.tokens, -1), owner(d.tokens, -1);
+    for (int s = 0; s < d.seqs; ++s)
+      for (int i = 0; i < req[s].n; ++i) {
+        CHECK(owner[req[s].first + i] < 0);
+        owner[req[s].first + i] = s;
+        limit[req[s].first + i] = limit_of(d, req[s], i);
+      }
+    for (int tok = 0; tok < d.tokens; ++tok)
+      if (limit[tok] >= 0)
+        for (int h = 0; h < d.NKV; ++h) w.seen[(size_t)tok * d.NKV + h].assign((size_t)limit[tok], 0);
+    std::vector<char> record((size_t)max_dense_records(d), 0);
+    struct Named { int rec, n; };
+    std::vector<Named> named((size_t)d.tokens * d.NKV, Named{-1, 0});
+    std::vector<std::vector<int>> written((size_t)d.tokens * d.NKV);
+    long long walked = 0, at_item = 0;
+    for (int c = 0; c < d.ctas; ++c) {
+      long long lo, hi;
+      dense_range(p, c, lo, hi);
+      if (c < p.dense_ctas) {
+        CHECK(lo == walked && hi > lo);
+        walked = hi;
+      }
+      for (long long b = lo; b < hi;) {
+        // the unit of block b, found by walking all of them
+        const int kvh = (int)(b / p.blocks);
+        long long rest = b % p.blocks;
+        int index = 0, blocks = 0, s = -1, u = 0;
+        bool found = false;
+        for (int q = 0; q < d.seqs && !found; ++q) {
+          if (!is_long(d, req[q])) continue;
+          for (u = 0; u < units_of(d, req[q]); ++u, ++index) {
+            blocks = unit_blocks(d, req[q], u);
+            if (rest < blocks) { s = q; found = true; break; }
+            rest -= blocks;
+          }
+        }
+        if (found) {
+          CHECK(lb[s] <= b % p.blocks && b % p.blocks < lb[s + 1]);
+          CHECK(index == lu[s] + u);
+        } else {
+          blocks = d.prefix_blocks();
+          u = (int)(rest / blocks);
+          rest -= (long long)u * blocks;
+          index = t.long_units + u;
+        }
+        const int b0 = (int)rest, b1 = (int)(blocks - b0 < hi - b ? blocks : b0 + (hi - b));
+        const int rec = c + kvh * p.unit_total + index;
+        CHECK(rec < max_dense_records(d) && !record[rec]);
+        record[rec] = 1;
+        const int parts = dense_owner(p, b - b0 + blocks - 1) - dense_owner(p, b - b0) + 1;
+        CHECK(dense_owner(p, b) == c && dense_owner(p, b + (b1 - b0) - 1) == c);
+        for (int i = 0; i < d.unit_tokens(); ++i) {
+          int tok, lim;
+          if (s >= 0) {
+            const int k = u * d.unit_tokens() + i;
+            if (k >= req[s].n) break;
+            tok = req[s].first + k;
+            lim = limit_of(d, req[s], k);
+            CHECK(lim <= unit_limit(d, req[s], u));
+          } else {
+            const int k = u * d.unit_tokens() + i;
+            if (k >= t.short_tokens) break;
+            int q = 0;
+            while (!(stk[q] <= k && k < stk[q + 1])) ++q;
+            tok = req[q].first + k - stk[q];
+            lim = limit_of(d, req[q], k - stk[q]);
+            lim = lim < d.prefix_len ? lim : d.prefix_len;
+          }
+          auto& seen = w.seen[(size_t)tok * d.NKV + kvh];
+          for (int key = b0 * kBlockKeys; key < b1 * kBlockKeys && key < lim; ++key) ++seen[key];
+          if (b0 == 0) named[(size_t)tok * d.NKV + kvh] = Named{rec, parts};
+          written[(size_t)tok * d.NKV + kvh].push_back(rec);
+        }
+        b += b1 - b0;
+      }
+      long long ilo, ihi;
+      item_range(d, p, t, items, c, ilo, ihi);
+      CHECK(ilo == at_item && ihi >= ilo);
+      at_item = ihi;
+      for (long long item = ilo; item < ihi; ++item) {
+        int s = 0;
+        while (!((long long)it[s] * d.NKV <= item && item < (long long)it[s + 1] * d.NKV)) ++s;
+        CHECK(it[s] <= item / d.NKV && item / d.NKV < it[s + 1]);
+        const Req& r = req[s];
+        const int chunks = item_chunks(own_keys(d, r), p.ck);
+        long long rest = item - (long long)it[s] * d.NKV;
+        const int ch = (int)(rest % chunks);
+        rest /= chunks;
+        const int kvh = (int)(rest % d.NKV), rb = (int)(rest / d.NKV);
+        const int i0 = rb * d.item_tokens(), ni = imin(d.item_tokens(), r.n - i0);
+        CHECK(ni > 0 && ni * d.G <= kItemRows);
+        const int k_lo = d.prefix_len + ch * p.ck, k_hi = imin(k_lo + p.ck, limit_of(d, r, i0 + ni - 1));
+        for (int i = i0; i < i0 + ni; ++i) {
+          auto& seen = w.seen[(size_t)(r.first + i) * d.NKV + kvh];
+          for (int key = k_lo; key < k_hi && key < limit_of(d, r, i); ++key) ++seen[key];
+        }
+      }
+    }
+    CHECK(walked == p.dense_blocks && at_item == items);
+    for (int tok = 0; tok < d.tokens; ++tok)
+      for (int h = 0; h < d.NKV; ++h) {
+        const size_t i = (size_t)tok * d.NKV + h;
+        for (int n : w.seen[i]) CHECK(n == 1);
+        CHECK((int)written[i].size() == named[i].n);
+        for (int k = 0; k < named[i].n; ++k) CHECK(written[i][k] == named[i].rec + k);
+      }
+  }
+  std::printf("prefix plan ok\n");
+  return 0;
+}
