@@ -11,9 +11,10 @@
 // O += P V.  Two groups alternate, so that the tensor pipe works for one while the other does its exponentials: each has
 // a tile of 128 rows, or, where a unit has only one tile, they share it and take alternate blocks.  m is raised (and O
 // rescaled) only when a row's maximum grows by more than 2^8; P then stays below 2^8, which costs no accuracy.
-//   tensor memory: S0 | S1 (128 columns each, P over S), O0 | O1 (HD columns each)
-//   warps 0-3, 4-7 softmax groups; 8 loads K and V blocks (one TMA box per page and 64 dimensions); 9 issues the products;
-//   10 clears the V rows behind the last key of a block that ends inside it
+// A group works in steps of 64 keys with two buffers for S, so that its next scores are there when it has written a P.
+//   tensor memory: S (2 groups x 2 buffers x 64 columns, P over S), O0 | O1 (HD columns each)
+//   warps 0-3, 4-7 softmax groups; 8 and 11 load K and V blocks (one TMA box per page and 64 dimensions); 9 issues the
+//   products; 10 clears the V rows behind the last key of a block that ends inside it
 //
 // Items.  What a short request holds behind the prefix: a warp per item, up to 16 rows x ck keys, mma.sync on 16-row tiles,
 // K and V through a ring of its own in shared memory (the ring of the blocks, free by then).
@@ -59,7 +60,10 @@ struct AttnMaps {
 };
 
 constexpr int kAttnThreads = 384;
-constexpr int kProducerWarp = 8, kIssueWarp = 9, kClearWarp = 10;
+constexpr int kKeyWarp = 8, kIssueWarp = 9, kClearWarp = 10, kValueWarp = 11;
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+constexpr int kPolyEvery = 4;                        // one pair of exponentials in so many goes to the multiply-add pipe
 constexpr long long kWaitCycles = 4000000000ll;      // about two seconds
 
 template <int HD>
@@ -76,7 +80,8 @@ struct AttnSmem {
   static constexpr int kItemKeys = HD == 64 ? 32 : 16;          // keys of a stage
   static constexpr int kItemRing = kItemWarps * kItemStages * kItemStageBytes;
   static constexpr int kOffBars = kRing > kItemRing ? kRing : kItemRing;
-  static constexpr int kNumBars = 4 * kStages + 1 + 2 + 2 + 2 + 2 + kItemWarps * kItemStages;
+  static constexpr int kDenseBars = 4 * kStages + 1 + 4 + 4 + 2 + 2;
+  static constexpr int kNumBars = kDenseBars + kItemWarps * kItemStages;
   static constexpr int kOffCtl = kOffBars + kNumBars * 8;       // words: 0 abort, 1 tensor memory base
   static constexpr int kOffRed = (kOffCtl + 16 + 7) / 8 * 8;    // long long [4][16] scratch of the scans
   static constexpr int kOffTot = kOffRed + 4 * 16 * 8;          // Totals, Plan
@@ -151,6 +156,49 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
   return u;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// Two floats in a register pair.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+// 2^x of a pair on the fused multiply-add pipe, for x <= 127; below -126 the result is about 2^-126.  x = n + f with n the
+// nearest whole number (an addition of 1.5 * 2^23 rounds to it and leaves it in the low bits), 2^f on [-1/2, 1/2] by the
+// polynomial of degree 4 with the smallest largest relative error (2.6e-6, found by Remez exchange), n into the exponent.
+__device__ __forceinline__ void ex2_pair(f32x2 x, float& lo, float& hi) {
+  float a, b;
+  unpair(x, a, b);
+  x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const f32x2 magic = pair(12582912.f, 12582912.f), back = pair(-12582912.f, -12582912.f), minus = pair(-1.f, -1.f);
+  const f32x2 t = add2(x, magic);
+  const f32x2 f = fma2(add2(t, back), minus, x);
+  f32x2 r = fma2(f, pair(0.009570102207362652f, 0.009570102207362652f), pair(0.05591785907745361f, 0.05591785907745361f));
+  r = fma2(r, f, pair(0.240247443318367f, 0.240247443318367f));
+  r = fma2(r, f, pair(0.6931217908859253f, 0.6931217908859253f));
+  r = fma2(r, f, pair(0.9999992847442627f, 0.9999992847442627f));
+  float n0, n1;
+  unpair(t, n0, n1);
+  unpair(r, lo, hi);
+  lo = __uint_as_float(__float_as_uint(lo) + (__float_as_uint(n0) << 23));
+  hi = __uint_as_float(__float_as_uint(hi) + (__float_as_uint(n1) << 23));
+}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -166,6 +214,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// One lane of the (whole) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0u;
+}
 // Bounded wait on a phase of a barrier; false once the CTA has been aborted.
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile unsigned* ctl) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -233,8 +287,13 @@ __device__ __forceinline__ void scan_values(long long (&v)[N], long long (&total
   }
   __syncthreads();
 }
-__device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc, long long* red, Totals& t, Plan& plan,
-                                           long long& items) {
+struct Work {                  // in shared memory
+  Totals t;
+  Plan plan;
+  long long items;
+};
+__device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc, long long* red, Work* out) {
+  Totals t;
   const int seqs = p.d.seqs;
   long long base[4] = {0, 0, 0, 0};
   for (int s0 = 0; s0 < seqs; s0 += kAttnThreads) {
@@ -266,7 +325,7 @@ __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc,
     sc.short_tokens[seqs] = (int)base[2];
   }
   t.long_blocks = base[0]; t.long_units = (int)base[1]; t.short_tokens = (int)base[2]; t.item_keys = base[3];
-  plan = make_plan(p.d, t);
+  const Plan plan = make_plan(p.d, t);
   long long at = 0;
   for (int s0 = 0; s0 < seqs; s0 += kAttnThreads) {
     const int s = s0 + (int)threadIdx.x;
@@ -279,8 +338,12 @@ __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc,
     if (s < seqs) sc.items[s] = (int)(at + v[0]);
     at += tot[0];
   }
-  if (threadIdx.x == 0) sc.items[seqs] = (int)at;
-  items = at * p.d.NKV;
+  if (threadIdx.x == 0) {
+    sc.items[seqs] = (int)at;
+    out->t = t;
+    out->plan = plan;
+    out->items = at * p.d.NKV;
+  }
   __syncthreads();
 }
 
@@ -353,8 +416,8 @@ struct Dense {
   uint32_t base;               // shared address of smem
   volatile unsigned* ctl;
   Scans sc;
-  Totals t;
-  Plan plan;
+  const Totals& t;             // (in shared memory: read where they are needed, not held in registers)
+  const Plan& plan;
   long long lo, hi;            // blocks of this CTA
   uint32_t tmem;
   int warp, lane;
@@ -365,11 +428,16 @@ struct Dense {
   __device__ __forceinline__ uint32_t v_full(int s) const { return bar(2 * S::kStages + s); }
   __device__ __forceinline__ uint32_t v_empty(int s) const { return bar(3 * S::kStages + s); }
   __device__ __forceinline__ uint32_t q_full() const { return bar(4 * S::kStages); }
-  __device__ __forceinline__ uint32_t s_full(int g) const { return bar(4 * S::kStages + 1 + g); }
-  __device__ __forceinline__ uint32_t p_full(int g) const { return bar(4 * S::kStages + 3 + g); }
-  __device__ __forceinline__ uint32_t o_full(int g) const { return bar(4 * S::kStages + 5 + g); }
-  __device__ __forceinline__ uint32_t c_ask() const { return bar(4 * S::kStages + 7); }     // issuer -> warp 10: clear this block's V
-  __device__ __forceinline__ uint32_t c_done() const { return bar(4 * S::kStages + 8); }    // and back
+  __device__ __forceinline__ uint32_t s_full(int g, int buf) const { return bar(4 * S::kStages + 1 + 2 * g + buf); }
+  __device__ __forceinline__ uint32_t p_full(int g, int buf) const { return bar(4 * S::kStages + 5 + 2 * g + buf); }
+  __device__ __forceinline__ uint32_t o_full(int g) const { return bar(4 * S::kStages + 9 + g); }
+  __device__ __forceinline__ uint32_t c_ask() const { return bar(4 * S::kStages + 11); }    // issuer -> warp 10: clear this block's V
+  __device__ __forceinline__ uint32_t c_done() const { return bar(4 * S::kStages + 12); }   // and back
+
+  // Steps of a group in a segment of nb blocks: halves of 64 keys of the blocks it takes (with two tiles every block, with
+  // one the blocks of its parity).
+  __device__ __forceinline__ static int steps_of(int nb, bool dual, int g) { return 2 * (dual ? (nb + 1 - g) >> 1 : nb); }
+  __device__ __forceinline__ static int block_of(int j, bool dual, int g) { return dual ? (j & ~1) + g : j >> 1; }
 
   // keys of block b of a unit that rows can see, and whether the V rows behind them have to be cleared
   __device__ __forceinline__ static int valid_keys(const Unit& x, int b) { return max(0, min(kBlockKeys, x.limit - b * kBlockKeys)); }
@@ -380,12 +448,15 @@ struct Dense {
     else id = x.s >= 0 ? p.tables[(size_t)x.s * p.max_pages + (key >> p.page_shift)] : -1;
     return id;
   }
-  // K and V of the CTA's blocks: lane l loads box l of a block (a page, or 128 rows of one, of 64 dimensions).
+  // K (or V) of the CTA's blocks: lane l loads box l of a block (a page, or 128 rows of one, of 64 dimensions).  K and V have
+  // a warp each: the scores run up to two blocks ahead of the products with V.
+  template <bool kV>
   __device__ __forceinline__ unsigned produce() {
     const int box_rows = min(1 << p.page_shift, kBlockKeys);
     const int key_of_lane = (lane / S::kHalves) * box_rows, half = lane % S::kHalves;
     const int boxes = kBlockKeys / box_rows * S::kHalves;
     const int oob = p.num_pages << p.page_shift;             // behind the last row: reads as zeros
+    const uint32_t dst = base + (kV ? S::kOffV : S::kOffK) + (uint32_t)(half * kBlockKeys * 128 + key_of_lane * 128);
     unsigned n = 0;
     for (long long b = lo; b < hi;) {
       int b0;
@@ -401,95 +472,107 @@ struct Dense {
       int row = row_of(b0);
       for (int blk = b0; blk < b1; ++blk, ++n) {
         const int st = n % S::kStages;
-        const uint32_t par = ((n / S::kStages) & 1u) ^ 1u;
+        const uint32_t full = kV ? v_full(st) : k_full(st), empty = kV ? v_empty(st) : k_empty(st);
         const unsigned issue = __ballot_sync(kFullMask, row >= 0);
         const uint32_t bytes = (uint32_t)__popc(issue) * (uint32_t)(box_rows * 128);
-        const uint32_t dst = (uint32_t)(half * kBlockKeys * 128 + key_of_lane * 128);
         const int next = blk + 1 < b1 ? row_of(blk + 1) : -1;
-        if (!wait_bar(k_empty(st), par, ctl)) return n;
-        if (lane == 0) mbar_expect_tx(k_full(st), bytes);
+        if (!wait_bar(empty, ((n / S::kStages) & 1u) ^ 1u, ctl)) return n;
+        if (lane == 0) mbar_expect_tx(full, bytes);
         __syncwarp();
-        if (row >= 0) tma_box(base + S::kOffK + st * S::kTileBytes + dst, &maps.k, half * 64, x.kvh, row, k_full(st));
-        if (!wait_bar(v_empty(st), par, ctl)) {
-          wait_bar(k_full(st), par ^ 1u, ctl);
-          return n;
-        }
-        if (lane == 0) mbar_expect_tx(v_full(st), bytes);
-        __syncwarp();
-        if (row >= 0) tma_box(base + S::kOffV + st * S::kTileBytes + dst, &maps.v, half * 64, x.kvh, row, v_full(st));
+        if (row >= 0) tma_box(dst + st * S::kTileBytes, kV ? &maps.v : &maps.k, half * 64, x.kvh, row, full);
         row = next;
       }
       b += b1 - b0;
     }
     return n;
   }
+  // After an abort: no copy stays in flight.
+  template <bool kV>
+  __device__ __forceinline__ void drain(unsigned issued) const {
+    const unsigned from = issued > (unsigned)S::kStages ? issued - S::kStages : 0u;
+    for (unsigned n = from; n < issued; ++n) {
+      const long long t0 = clock64();
+      while (!mbar_try_wait(kV ? v_full(n % S::kStages) : k_full(n % S::kStages), (n / S::kStages) & 1u))
+        if (clock64() - t0 > 1000000) break;
+    }
+  }
 
-  // S = Q K^T and O += P V for the CTA's blocks (one lane).
+  // S = Q K^T and O += P V for the CTA's blocks (one lane).  Step j of a group: its P is waited for, P V is issued, and the
+  // scores of step j + 2 into the buffer that P leaves; those of step j + 1 are there already.
   __device__ __forceinline__ void issue() {
-    constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)HD >> 3) << 17) | ((128u >> 4) << 24);
-    const uint32_t s_col[2] = {tmem, tmem + 128}, o_col[2] = {tmem + 256, tmem + 384};
-    unsigned n = 0, segs = 0, p_par[2] = {0, 0}, clears = 0;
-    auto score = [&](int g, int tile, int st) {
-      const uint32_t qa = base + S::kOffQ + tile * S::kTileBytes, ka = base + S::kOffK + st * S::kTileBytes;
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        const uint32_t off = (uint32_t)((k >> 2) * 16384 + (k & 3) * 32);
-        mma_ss(s_col[g], desc_k_major(qa + off), desc_k_major(ka + off), kIdescS, k > 0);
-      }
-      mma_commit_to(s_full(g));
-    };
+    unsigned n = 0, segs = 0, p_par = 0, clears = 0;         // (bit 2g + buf of p_par: parity of that P's next phase)
     for (long long b = lo; b < hi; ++segs) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
       const int nb = (int)min((long long)(x.blocks - b0), hi - b);
       const bool dual = x.rows <= 128;
-      if (!wait_bar(q_full(), segs & 1u, ctl)) return;
-      tmem_fence_after_sync();
-      // steps of the segment: (block, group); two tiles: both groups take every block, one tile: they alternate
-      const int steps = dual ? nb : 2 * nb;
-      auto block_of = [&](int i) { return dual ? i : i >> 1; };
-      auto start = [&](int i) -> bool {                       // scores of step i
-        const int blk = block_of(i), g = i & 1;
-        const unsigned m = n + (unsigned)blk;
-        const int st = (int)(m % S::kStages);
-        if (dual || g == 0)
+      const int steps0 = steps_of(nb, dual, 0), steps1 = steps_of(nb, dual, 1);
+      auto score = [&](int g, int j) -> bool {
+        const unsigned m = n + (unsigned)block_of(j, dual, g);
+        const int st = (int)(m % S::kStages), half = j & 1;
+        if (half == 0 && (dual || g == 0)) {
           if (!wait_bar(k_full(st), (m / S::kStages) & 1u, ctl)) return false;
-        tmem_fence_after_sync();
-        score(g, dual ? 0 : g, st);
-        if (dual || g == 1) mma_commit_to(k_empty(st));
+          tmem_fence_after_sync();
+        }
+        const uint64_t qd = desc_k_major(base + S::kOffQ + (dual ? 0 : g) * S::kTileBytes);
+        const uint64_t kd = desc_k_major(base + S::kOffK + st * S::kTileBytes + half * 8192);
+        const uint32_t sd = tmem + (uint32_t)(g * 128 + half * 64);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t off = (uint32_t)((k >> 2) * (16384 >> 4) + (k & 3) * (32 >> 4));
+          if (k == 0) mma_ss(sd, qd + off, kd + off, kIdescS, 0u);
+          else mma_ss(sd, qd + off, kd + off, kIdescS, 1u);
+        }
+        mma_commit_to(s_full(g, half));
+        if (half == 1 && (dual || g == 1)) mma_commit_to(k_empty(st));
         return true;
       };
-      if (!start(0)) return;
-      if (steps > 1 && !start(1)) return;
-      for (int i = 0; i < steps; ++i) {
-        const int blk = block_of(i), g = i & 1;
-        const unsigned m = n + (unsigned)blk;
-        const int st = (int)(m % S::kStages);
-        const int valid = valid_keys(x, b0 + blk);
-        if (dual || g == 0) {
-          if (!wait_bar(v_full(st), (m / S::kStages) & 1u, ctl)) return;
-          if (valid % 16 != 0) {
-            mbar_arrive(c_ask());
-            if (!wait_bar(c_done(), clears & 1u, ctl)) return;
-            ++clears;
+      if (!wait_bar(q_full(), segs & 1u, ctl)) return;
+      tmem_fence_after_sync();
+      for (int j = 0; j < 2; ++j) {
+        if (!score(0, j)) return;
+        if (j < steps1 && !score(1, j)) return;
+      }
+      for (int j = 0; j < steps0; ++j) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (g == 1 && j >= steps1) break;
+          const int blk = block_of(j, dual, g), half = j & 1;
+          const unsigned m = n + (unsigned)blk;
+          const int st = (int)(m % S::kStages);
+          const int valid = valid_keys(x, b0 + blk);
+          if (half == 0 && (dual || g == 0)) {
+            if (!wait_bar(v_full(st), (m / S::kStages) & 1u, ctl)) return;
+            if (valid % 16 != 0) {
+              mbar_arrive(c_ask());
+              if (!wait_bar(c_done(), clears & 1u, ctl)) return;
+              ++clears;
+            }
+          }
+          if (!wait_bar(p_full(g, half), (p_par >> (2 * g + half)) & 1u, ctl)) return;
+          p_par ^= 1u << (2 * g + half);
+          tmem_fence_after_sync();
+          const uint64_t vd = desc_n_major(base + S::kOffV + st * S::kTileBytes + half * 8192, 16384u);
+          const uint32_t od = tmem + 256u + (uint32_t)g * 128u, pd = tmem + (uint32_t)(g * 128 + half * 64);
+          const int mine = valid - 64 * half;                // visible keys of this half
+          if (mine >= 64) {
+            mma_ts(od, pd, vd, kIdescO, j > 0);
+#pragma unroll
+            for (int k = 1; k < 4; ++k) mma_ts(od, pd + 8u * k, vd + (uint32_t)(k * (2048 >> 4)), kIdescO, 1u);
+          } else {
+#pragma unroll 1
+            for (int k = 0; 16 * k < mine; ++k) mma_ts(od, pd + 8u * k, vd + (uint32_t)(k * (2048 >> 4)), kIdescO, j > 0 || k > 0);
+          }
+          if (half == 1 && (dual || g == 1)) mma_commit_to(v_empty(st));
+          if (j + 2 < (g == 0 ? steps0 : steps1)) {
+            if (!score(g, j + 2)) return;
+          } else {
+            mma_commit_to(o_full(g));                        // (twice a segment: after the last two steps)
           }
         }
-        if (!wait_bar(p_full(g), p_par[g], ctl)) return;
-        p_par[g] ^= 1u;
-        tmem_fence_after_sync();
-        const uint32_t va = base + S::kOffV + st * S::kTileBytes;
-        const int ks = (valid + 15) >> 4;
-        for (int k = 0; k < ks; ++k)
-          mma_ts(o_col[g], s_col[g] + 8 * k, desc_n_major(va + 2048u * k, 16384u), kIdescO, !(i < 2 && k == 0));
-        if (dual || g == 1) mma_commit_to(v_empty(st));
-        if (i + 2 < steps) {
-          if (!start(i + 2)) return;
-        } else {
-          mma_commit_to(o_full(g));
-        }
       }
-      if (steps == 1) mma_commit_to(o_full(1));
       n += (unsigned)nb;
       b += nb;
     }
@@ -526,8 +609,8 @@ struct Dense {
     const int g = warp >> 2, row = g * 128 + (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + g * 128 + lane_base, o_col = tmem + 256 + g * 128 + lane_base;
-    unsigned segs = 0, s_par = 0;
-    for (long long b = lo; b < hi; ++segs) {
+    unsigned s_par = 0;                                      // bit buf: parity of that S's next phase
+    for (long long b = lo; b < hi;) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
       const int nb = (int)min((long long)(x.blocks - b0), hi - b);
@@ -552,32 +635,43 @@ struct Dense {
       const bool warp_works = __ballot_sync(kFullMask, token >= 0) != 0u;
       const int warp_lim = __reduce_min_sync(kFullMask, lim);
       float m = -INFINITY, l = 0.f;
-      const int first = dual ? g : 0, step = dual ? 2 : 1;
+      const int steps = steps_of(nb, dual, g);
       bool ok = true;
-      for (int blk = first; blk < nb; blk += step) {
-        ok = wait_bar(s_full(g), s_par, ctl);
+      for (int j = 0; j < steps; ++j) {
+        const int half = j & 1;
+        ok = wait_bar(s_full(g, half), (s_par >> half) & 1u, ctl);
         if (!ok) break;
-        s_par ^= 1u;
+        s_par ^= 1u << half;
         tmem_fence_after_sync();
         if (warp_works) {
-          float s[128];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(s + 32 * c, s_col + 32 * c);
+          const uint32_t sh = s_col + 64 * half;
+          float s[64];
+          tmem_ld32(s, sh);
+          tmem_ld32(s + 32, sh + 32);
           tmem_wait_ld();
-          const int k0 = (b0 + blk) * kBlockKeys;
-          if (k0 + kBlockKeys > warp_lim) {
+          const int k0 = (b0 + block_of(j, dual, g)) * kBlockKeys + 64 * half;
+          bool plain = k0 + 64 <= warp_lim;
+          if (!plain) {
             const int vis = lim - k0;
 #pragma unroll
-            for (int j = 0; j < 128; ++j) s[j] = j < vis ? s[j] : -INFINITY;
+            for (int c = 0; c < 64; ++c) s[c] = c < vis ? s[c] : -INFINITY;
           }
           float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+          for (int i = 4; i + 8 <= 64; i += 8)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], s[i + c], s[i + 4 + c]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[60 + c]);
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2e;
-          // NaN scores: fmaxf passes them over, their own exponential keeps them
+          // NaN scores: the maximum passes them over, their own exponential keeps them
           if (__any_sync(kFullMask, top > m + 8.f)) {
             const float m_new = fmaxf(m, top);
-            if (blk != first) {
+            if (j > 0) {
+              // O may be touched once P V of step j - 1 is through: the scores of step j + 1 were issued behind it
+              ok = j + 1 < steps ? wait_bar(s_full(g, half ^ 1), (s_par >> (half ^ 1)) & 1u, ctl) : wait_bar(o_full(g), 0u, ctl);
+              if (!ok) break;
+              tmem_fence_after_sync();
               const float f = m_new == -INFINITY ? 1.f : ex2(m - m_new);
               l *= f;
 #pragma unroll 1
@@ -586,37 +680,54 @@ struct Dense {
                 tmem_ld16(o, o_col + 16 * c);
                 tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
                 tmem_st16(o_col + 16 * c, o);
               }
             }
             m = m_new;
           }
+          // the polynomial has no zero: rows with hidden keys, or with nothing seen yet, go without it
+          plain = plain && __all_sync(kFullMask, m != -INFINITY);
           const float off = m == -INFINITY ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t pk[64];
+          const f32x2 scale2 = pair(p.scale_log2e, p.scale_log2e), off2 = pair(-off, -off);
+          f32x2 sum2[2] = {0ull, 0ull};
+          auto exps = [&](auto with_poly) {
 #pragma unroll
-          for (int j = 0; j < 128; j += 2) {
-            const float a = ex2(fmaf(s[j], p.scale_log2e, -off)), c = ex2(fmaf(s[j + 1], p.scale_log2e, -off));
-            sum[j & 2] += a;
-            sum[(j & 2) + 1] += c;
-            pk[j >> 1] = pack2(a, c);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_st32(s_col, pk);
-          tmem_st32(s_col + 32, pk + 32);
+            for (int c = 0; c < 2; ++c) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const f32x2 e = fma2(pair(s[32 * c + 2 * i], s[32 * c + 2 * i + 1]), scale2, off2);
+                float a, d;
+                if (decltype(with_poly)::value && i % kPolyEvery == kPolyEvery - 1) {
+                  ex2_pair(e, a, d);
+                } else {
+                  unpair(e, a, d);
+                  a = ex2(a);
+                  d = ex2(d);
+                }
+                sum2[i & 1] = add2(sum2[i & 1], pair(a, d));
+                pk[i] = pack2(a, d);
+              }
+              tmem_st16(sh + 16 * c, pk);
+            }
+          };
+          if (plain) exps(Yes{}); else exps(No{});
+          float sa, sb;
+          unpair(add2(sum2[0], sum2[1]), sa, sb);
+          l += sa + sb;
           tmem_wait_st();
         }
         tmem_fence_before_sync();
-        mbar_arrive(p_full(g));
+        mbar_arrive(p_full(g, half));
       }
-      if (ok) ok = wait_bar(o_full(g), segs & 1u, ctl);
+      if (ok && steps > 0) ok = wait_bar(o_full(g), 0u, ctl) && wait_bar(o_full(g), 1u, ctl);
       tmem_fence_after_sync();
       // ---- the unit's rows: complete, or a record ----
       const int cta = (int)blockIdx.x;
       const bool whole = b0 == 0 && nb == x.blocks && !dual && x.s >= 0;
       const int rec = cta + x.kvh * plan.unit_total + x.index;
-      const bool have = first < nb;
+      const bool have = steps > 0;
       if (warp_works) {
         const float nan = __int_as_float(0x7fffffff);
         if (whole) {
@@ -678,7 +789,7 @@ __device__ __forceinline__ void walk_items(const AttnParams& p, const AttnMaps& 
   constexpr int KS = S::kItemKeys, NT = KS / 8, GROUPS = KS / 16, HALVES = S::kHalves;
   constexpr int KBYTES = KS * HD * 2;                       // 4 KiB of K, then 4 KiB of V
   const uint32_t ring = smem_u32(smem) + warp * S::kItemStages * S::kItemStageBytes;
-  const uint32_t bars = smem_u32(smem) + S::kOffBars + (4 * S::kStages + 9 + warp * S::kItemStages) * 8;
+  const uint32_t bars = smem_u32(smem) + S::kOffBars + (S::kDenseBars + warp * S::kItemStages) * 8;
   const int g = lane >> 2, t4 = lane & 3;
   const int oob = p.num_pages << p.page_shift;
   unsigned filled = 0;                                      // stages filled by this warp so far
@@ -885,7 +996,8 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
   sc.long_units = sc.long_blocks + p.d.seqs + 1;
   sc.short_tokens = sc.long_units + p.d.seqs + 1;
   sc.items = sc.short_tokens + p.d.seqs + 1;
-  Dense<HD> w{p, maps, smem, smem_u32(smem), ctl, sc, {}, {}, 0, 0, 0u, warp, lane};
+  Work* work = reinterpret_cast<Work*>(smem + S::kOffTot);
+  Dense<HD> w{p, maps, smem, smem_u32(smem), ctl, sc, work->t, work->plan, 0, 0, 0u, warp, lane};
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(w.k_full(s), 1);
@@ -895,19 +1007,20 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
     }
     mbar_init(w.q_full(), 256);
     for (int g = 0; g < 2; ++g) {
-      mbar_init(w.s_full(g), 1);
-      mbar_init(w.p_full(g), 128);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(w.s_full(g, h), 1);
+        mbar_init(w.p_full(g, h), 128);
+      }
       mbar_init(w.o_full(g), 1);
     }
     mbar_init(w.c_ask(), 1);
     mbar_init(w.c_done(), 1);
-    for (int i = 0; i < kItemWarps * S::kItemStages; ++i) mbar_init(w.bar(4 * S::kStages + 9 + i), 1);
+    for (int i = 0; i < kItemWarps * S::kItemStages; ++i) mbar_init(w.bar(S::kDenseBars + i), 1);
     fence_barrier_init();
     ctl[0] = 0u;
   }
-  long long items;
-  build_plan(p, sc, reinterpret_cast<long long*>(smem + S::kOffRed), w.t, w.plan, items);
-  dense_range(w.plan, (int)blockIdx.x, w.lo, w.hi);
+  build_plan(p, sc, reinterpret_cast<long long*>(smem + S::kOffRed), work);
+  dense_range(work->plan, (int)blockIdx.x, w.lo, w.hi);
   if (w.lo < w.hi) {
     if (warp == kIssueWarp) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(w.base + S::kOffCtl + 4) : "memory");
@@ -917,22 +1030,22 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
     __syncthreads();
     tmem_fence_after_sync();
     w.tmem = ctl[1];
-    unsigned issued = 0;
-    if (warp < kItemWarps) w.softmax();
-    else if (warp == kProducerWarp) issued = w.produce();
-    else if (warp == kIssueWarp) {
-      if (lane == 0) w.issue();
+    if (warp < kItemWarps) {
+      w.softmax();
+    } else if (warp == kKeyWarp) {
+      const unsigned n = w.template produce<false>();
       __syncwarp();
-    } else if (warp == kClearWarp) w.clear();
-    __syncwarp();
-    if (warp == kProducerWarp && ctl[0] != 0u) {             // aborted: no copy stays in flight
-      const unsigned from = issued > (unsigned)S::kStages ? issued - S::kStages : 0u;
-      for (unsigned n = from; n < issued; ++n) {
-        const long long t0 = clock64();
-        while (!mbar_try_wait(w.k_full(n % S::kStages), (n / S::kStages) & 1u) || !mbar_try_wait(w.v_full(n % S::kStages), (n / S::kStages) & 1u))
-          if (clock64() - t0 > 1000000) break;
-      }
+      if (ctl[0] != 0u) w.template drain<false>(n);
+    } else if (warp == kValueWarp) {
+      const unsigned n = w.template produce<true>();
+      __syncwarp();
+      if (ctl[0] != 0u) w.template drain<true>(n);
+    } else if (warp == kIssueWarp) {
+      if (elect_one()) w.issue();
+    } else {
+      w.clear();
     }
+    __syncwarp();
     tmem_fence_before_sync();
     __syncthreads();
     if (warp == kIssueWarp) {
@@ -943,8 +1056,8 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
     __syncthreads();
   }
   long long lo, hi;
-  item_range(p.d, w.plan, w.t, items, (int)blockIdx.x, lo, hi);
-  if (warp < kItemWarps) walk_items<HD>(p, maps, smem, ctl, sc, w.plan, lo, hi, warp, lane);
+  item_range(p.d, work->plan, work->t, work->items, (int)blockIdx.x, lo, hi);
+  if (warp < kItemWarps) walk_items<HD>(p, maps, smem, ctl, sc, work->plan, lo, hi, warp, lane);
 }
 
 // Adds a row's parts: one warp per (token, query head).  With M = max m_r and w_r = 2^(m_r - M):
