@@ -13,8 +13,8 @@
 // rescaled) only when a row's maximum grows by more than 2^8; P then stays below 2^8, which costs no accuracy.
 // A group works in steps of 64 keys with two buffers for S, so that its next scores are there when it has written a P.
 //   tensor memory: S (2 groups x 2 buffers x 64 columns, P over S), O0 | O1 (HD columns each)
-//   warps 0-3, 4-7 softmax groups; 8 and 11 load K and V blocks (one TMA box per page and 64 dimensions); 9 issues the
-//   products; 10 clears the V rows behind the last key of a block that ends inside it
+//   warps 0-3, 4-7 softmax groups; 8 and 11 load K and V blocks (one TMA box per page and 64 dimensions); 9 and 10 issue the
+//   products of a group each
 //
 // Items.  What a short request holds behind the prefix: a warp per item, up to 16 rows x ck keys, mma.sync on 16-row tiles,
 // K and V through a ring of its own in shared memory (the ring of the blocks, free by then).
@@ -60,7 +60,7 @@ struct AttnMaps {
 };
 
 constexpr int kAttnThreads = 384;
-constexpr int kKeyWarp = 8, kIssueWarp = 9, kClearWarp = 10, kValueWarp = 11;
+constexpr int kKeyWarp = 8, kIssueWarp = 9, kValueWarp = 11;   // (warps 9 and 10 issue, one for each group)
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 constexpr int kPolyEvery = 4;                        // one pair of exponentials in so many goes to the multiply-add pipe
@@ -80,7 +80,7 @@ struct AttnSmem {
   static constexpr int kItemKeys = HD == 64 ? 32 : 16;          // keys of a stage
   static constexpr int kItemRing = kItemWarps * kItemStages * kItemStageBytes;
   static constexpr int kOffBars = kRing > kItemRing ? kRing : kItemRing;
-  static constexpr int kDenseBars = 4 * kStages + 1 + 4 + 4 + 2 + 2;
+  static constexpr int kDenseBars = 4 * kStages + 1 + 4 + 4 + 2 + 1;
   static constexpr int kNumBars = kDenseBars + kItemWarps * kItemStages;
   static constexpr int kOffCtl = kOffBars + kNumBars * 8;       // words: 0 abort, 1 tensor memory base
   static constexpr int kOffRed = (kOffCtl + 16 + 7) / 8 * 8;    // long long [4][16] scratch of the scans
@@ -431,8 +431,7 @@ struct Dense {
   __device__ __forceinline__ uint32_t s_full(int g, int buf) const { return bar(4 * S::kStages + 1 + 2 * g + buf); }
   __device__ __forceinline__ uint32_t p_full(int g, int buf) const { return bar(4 * S::kStages + 5 + 2 * g + buf); }
   __device__ __forceinline__ uint32_t o_full(int g) const { return bar(4 * S::kStages + 9 + g); }
-  __device__ __forceinline__ uint32_t c_ask() const { return bar(4 * S::kStages + 11); }    // issuer -> warp 10: clear this block's V
-  __device__ __forceinline__ uint32_t c_done() const { return bar(4 * S::kStages + 12); }   // and back
+  __device__ __forceinline__ uint32_t v_clear() const { return bar(4 * S::kStages + 11); }
 
   // Steps of a group in a segment of nb blocks: halves of 64 keys of the blocks it takes (with two tiles every block, with
   // one the blocks of its parity).
@@ -497,80 +496,87 @@ struct Dense {
     }
   }
 
-  // S = Q K^T and O += P V for the CTA's blocks (one lane).  Step j of a group: its P is waited for, P V is issued, and the
-  // scores of step j + 2 into the buffer that P leaves; those of step j + 1 are there already.
-  __device__ __forceinline__ void issue() {
+  // S = Q K^T and O += P V of group g for the CTA's blocks (one lane of a warp per group: a lane spends about as long on
+  // issuing a step as a group on its exponentials).  For every half of 64 keys: its P is waited for, P V is issued, and then the
+  // scores of the same half of the next block into the buffer that P leaves; those of the other half are there already.
+  // A block is released by both groups; with one tile the other group's part is an arrival without products.
+  __device__ __forceinline__ void issue(int g) {
     constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)HD >> 3) << 17) | ((128u >> 4) << 24);
-    unsigned n = 0, segs = 0, p_par = 0, clears = 0;         // (bit 2g + buf of p_par: parity of that P's next phase)
+    const uint64_t kd0 = desc_k_major(base + S::kOffK), vd0 = desc_n_major(base + S::kOffV, 16384u);
+    const uint32_t sd = tmem + (uint32_t)g * 128u, od = tmem + 256u + (uint32_t)g * 128u;
+    unsigned n = 0, segs = 0, p_par = 0;                     // (p_par: parity of the next P, both halves)
     for (long long b = lo; b < hi; ++segs) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
       const int nb = (int)min((long long)(x.blocks - b0), hi - b);
       const bool dual = x.rows <= 128;
-      const int steps0 = steps_of(nb, dual, 0), steps1 = steps_of(nb, dual, 1);
-      auto score = [&](int g, int j) -> bool {
-        const unsigned m = n + (unsigned)block_of(j, dual, g);
-        const int st = (int)(m % S::kStages), half = j & 1;
-        if (half == 0 && (dual || g == 0)) {
-          if (!wait_bar(k_full(st), (m / S::kStages) & 1u, ctl)) return false;
-          tmem_fence_after_sync();
-        }
-        const uint64_t qd = desc_k_major(base + S::kOffQ + (dual ? 0 : g) * S::kTileBytes);
-        const uint64_t kd = desc_k_major(base + S::kOffK + st * S::kTileBytes + half * 8192);
-        const uint32_t sd = tmem + (uint32_t)(g * 128 + half * 64);
+      const uint64_t qd = desc_k_major(base + S::kOffQ + (dual ? 0 : g) * S::kTileBytes);
+      const int step = dual ? 2 : 1;
+      auto score = [&](int st, int half) {
+        const uint64_t kd = kd0 + (uint32_t)(st * (S::kTileBytes >> 4) + half * (8192 >> 4));
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint32_t off = (uint32_t)((k >> 2) * (16384 >> 4) + (k & 3) * (32 >> 4));
-          if (k == 0) mma_ss(sd, qd + off, kd + off, kIdescS, 0u);
-          else mma_ss(sd, qd + off, kd + off, kIdescS, 1u);
+          if (k == 0) mma_ss(sd + 64u * half, qd + off, kd + off, kIdescS, 0u);
+          else mma_ss(sd + 64u * half, qd + off, kd + off, kIdescS, 1u);
         }
         mma_commit_to(s_full(g, half));
-        if (half == 1 && (dual || g == 1)) mma_commit_to(k_empty(st));
-        return true;
+      };
+      auto release = [&](uint32_t empty) {
+        mma_commit_to(empty);
+        if (dual) mbar_arrive(empty);
       };
       if (!wait_bar(q_full(), segs & 1u, ctl)) return;
-      tmem_fence_after_sync();
-      for (int j = 0; j < 2; ++j) {
-        if (!score(0, j)) return;
-        if (j < steps1 && !score(1, j)) return;
-      }
-      for (int j = 0; j < steps0; ++j) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (g == 1 && j >= steps1) break;
-          const int blk = block_of(j, dual, g), half = j & 1;
-          const unsigned m = n + (unsigned)blk;
-          const int st = (int)(m % S::kStages);
+      int blk = dual ? g : 0;
+      if (blk < nb) {
+        unsigned m = n + (unsigned)blk;
+        int st = (int)(m % S::kStages);
+        if (!wait_bar(k_full(st), (m / S::kStages) & 1u, ctl)) return;
+        tmem_fence_after_sync();
+        score(st, 0);
+        score(st, 1);
+        release(k_empty(st));
+        uint32_t more = 0;                                   // 0 for the first products of the segment: O is overwritten
+        for (; blk < nb; blk += step) {
+          const uint64_t vd = vd0 + (uint32_t)(st * (S::kTileBytes >> 4));
           const int valid = valid_keys(x, b0 + blk);
-          if (half == 0 && (dual || g == 0)) {
-            if (!wait_bar(v_full(st), (m / S::kStages) & 1u, ctl)) return;
-            if (valid % 16 != 0) {
-              mbar_arrive(c_ask());
-              if (!wait_bar(c_done(), clears & 1u, ctl)) return;
-              ++clears;
+          const bool next = blk + step < nb;
+          const unsigned mn = m + (unsigned)step;
+          const int stn = (int)(mn % S::kStages);
+          if (!wait_bar(v_full(st), (m / S::kStages) & 1u, ctl)) return;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (!wait_bar(p_full(g, half), p_par, ctl)) return;
+            tmem_fence_after_sync();
+            const int mine = valid - 64 * half;              // visible keys of this half
+            if (mine >= 64) {
+              mma_ts(od, sd + 64u * half, vd + (uint32_t)(half * (8192 >> 4)), kIdescO, more);
+#pragma unroll
+              for (int k = 1; k < 4; ++k)
+                mma_ts(od, sd + 64u * half + 8u * k, vd + (uint32_t)(half * (8192 >> 4) + k * (2048 >> 4)), kIdescO, 1u);
+              more = 1u;
+            } else {
+#pragma unroll 1
+              for (int k = 0; 16 * k < mine; ++k) {
+                mma_ts(od, sd + 64u * half + 8u * k, vd + (uint32_t)(half * (8192 >> 4) + k * (2048 >> 4)), kIdescO, more);
+                more = 1u;
+              }
+            }
+            if (half == 1) release(v_empty(st));
+            if (next) {
+              if (half == 0) {
+                if (!wait_bar(k_full(stn), (mn / S::kStages) & 1u, ctl)) return;
+              }
+              score(stn, half);
+              if (half == 1) release(k_empty(stn));
+            } else {
+              mma_commit_to(o_full(g));                      // (twice a segment: after its last two halves)
             }
           }
-          if (!wait_bar(p_full(g, half), (p_par >> (2 * g + half)) & 1u, ctl)) return;
-          p_par ^= 1u << (2 * g + half);
-          tmem_fence_after_sync();
-          const uint64_t vd = desc_n_major(base + S::kOffV + st * S::kTileBytes + half * 8192, 16384u);
-          const uint32_t od = tmem + 256u + (uint32_t)g * 128u, pd = tmem + (uint32_t)(g * 128 + half * 64);
-          const int mine = valid - 64 * half;                // visible keys of this half
-          if (mine >= 64) {
-            mma_ts(od, pd, vd, kIdescO, j > 0);
-#pragma unroll
-            for (int k = 1; k < 4; ++k) mma_ts(od, pd + 8u * k, vd + (uint32_t)(k * (2048 >> 4)), kIdescO, 1u);
-          } else {
-#pragma unroll 1
-            for (int k = 0; 16 * k < mine; ++k) mma_ts(od, pd + 8u * k, vd + (uint32_t)(k * (2048 >> 4)), kIdescO, j > 0 || k > 0);
-          }
-          if (half == 1 && (dual || g == 1)) mma_commit_to(v_empty(st));
-          if (j + 2 < (g == 0 ? steps0 : steps1)) {
-            if (!score(g, j + 2)) return;
-          } else {
-            mma_commit_to(o_full(g));                        // (twice a segment: after the last two steps)
-          }
+          p_par ^= 1u;
+          m = mn;
+          st = stn;
         }
       }
       n += (unsigned)nb;
@@ -578,38 +584,25 @@ struct Dense {
     }
   }
 
-  // Rows of V behind the last visible key of a block: cleared, so that 0 * V is 0 whatever the page holds there.
-  __device__ __forceinline__ void clear() {
-    unsigned n = 0, asked = 0;
-    for (long long b = lo; b < hi;) {
-      int b0;
-      const Unit x = unit_at(p, sc, t, plan, b, b0);
-      const int nb = (int)min((long long)(x.blocks - b0), hi - b);
-      for (int blk = 0; blk < nb; ++blk, ++n) {
-        const int valid = valid_keys(x, b0 + blk);
-        if (valid % 16 == 0) continue;
-        const int st = (int)(n % S::kStages);
-        if (!wait_bar(c_ask(), asked & 1u, ctl)) return;     // (the block has landed: the issuer has seen it)
-        ++asked;
-        const int rows = 16 - (valid & 15);
-        for (int i = lane; i < rows * 8 * S::kHalves; i += 32) {
-          const int r = valid + i / (8 * S::kHalves), c = i % (8 * S::kHalves);
-          *reinterpret_cast<uint4*>(smem + S::kOffV + st * S::kTileBytes + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) =
-              make_uint4(0, 0, 0, 0);
-        }
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(c_done());
-      }
-      b += nb;
+  // Rows of V behind the last visible key of a block: cleared, so that 0 * V is 0 whatever the page holds there.  (One warp,
+  // before its P is handed over; rows from the next multiple of 16 on are not read.)
+  __device__ __forceinline__ void clear_rows(int st, int valid) {
+    const int rows = 16 - (valid & 15);
+    for (int i = lane; i < rows * 8 * S::kHalves; i += 32) {
+      const int r = valid + i / (8 * S::kHalves), c = i % (8 * S::kHalves);
+      *reinterpret_cast<uint4*>(smem + S::kOffV + st * S::kTileBytes + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) =
+          make_uint4(0, 0, 0, 0);
     }
+    fence_async_shared();
+    __syncwarp();
   }
 
   __device__ __forceinline__ void softmax() {
     const int g = warp >> 2, row = g * 128 + (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + g * 128 + lane_base, o_col = tmem + 256 + g * 128 + lane_base;
-    unsigned s_par = 0;                                      // bit buf: parity of that S's next phase
+    unsigned s_par = 0;                                      // parity of the next S, both halves
+    unsigned n = 0, clears = 0;
     for (long long b = lo; b < hi;) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
@@ -631,6 +624,7 @@ struct Dense {
         fence_async_shared();
       }
       tmem_fence_before_sync();                       // (the O of the segment before has been read)
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // (a group without steps must not arrive for two segments at once)
       mbar_arrive(q_full());
       const bool warp_works = __ballot_sync(kFullMask, token >= 0) != 0u;
       const int warp_lim = __reduce_min_sync(kFullMask, lim);
@@ -639,9 +633,8 @@ struct Dense {
       bool ok = true;
       for (int j = 0; j < steps; ++j) {
         const int half = j & 1;
-        ok = wait_bar(s_full(g, half), (s_par >> half) & 1u, ctl);
+        ok = wait_bar(s_full(g, half), s_par, ctl);
         if (!ok) break;
-        s_par ^= 1u << half;
         tmem_fence_after_sync();
         if (warp_works) {
           const uint32_t sh = s_col + 64 * half;
@@ -669,7 +662,7 @@ struct Dense {
             const float m_new = fmaxf(m, top);
             if (j > 0) {
               // O may be touched once P V of step j - 1 is through: the scores of step j + 1 were issued behind it
-              ok = j + 1 < steps ? wait_bar(s_full(g, half ^ 1), (s_par >> (half ^ 1)) & 1u, ctl) : wait_bar(o_full(g), 0u, ctl);
+              ok = j + 1 < steps ? wait_bar(s_full(g, half ^ 1), half ? s_par ^ 1u : s_par, ctl) : wait_bar(o_full(g), 0u, ctl);
               if (!ok) break;
               tmem_fence_after_sync();
               const float f = m_new == -INFINITY ? 1.f : ex2(m - m_new);
@@ -718,8 +711,26 @@ struct Dense {
           l += sa + sb;
           tmem_wait_st();
         }
+        if (half == 0 && (warp & 3) == 0) {
+          const int blk = block_of(j, dual, g), valid = valid_keys(x, b0 + blk);
+          if (valid % 16 != 0) {
+            const unsigned at = n + (unsigned)blk;
+            const int st = (int)(at % S::kStages);
+            if (dual || g == 0) {
+              ok = wait_bar(v_full(st), (at / S::kStages) & 1u, ctl);
+              if (!ok) break;
+              clear_rows(st, valid);
+              if (!dual && lane == 0) mbar_arrive(v_clear());
+            } else {                                         // (the block of both groups is cleared by the first)
+              ok = wait_bar(v_clear(), clears & 1u, ctl);
+              if (!ok) break;
+              ++clears;
+            }
+          }
+        }
         tmem_fence_before_sync();
         mbar_arrive(p_full(g, half));
+        s_par ^= (unsigned)half;
       }
       if (ok && steps > 0) ok = wait_bar(o_full(g), 0u, ctl) && wait_bar(o_full(g), 1u, ctl);
       tmem_fence_after_sync();
@@ -776,6 +787,7 @@ struct Dense {
           if (x.s >= 0) p.item_desc[at] = make_int2(0, 0);
         }
       }
+      n += (unsigned)nb;
       b += nb;
     }
   }
@@ -1001,9 +1013,9 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(w.k_full(s), 1);
-      mbar_init(w.k_empty(s), 1);
+      mbar_init(w.k_empty(s), 2);
       mbar_init(w.v_full(s), 1);
-      mbar_init(w.v_empty(s), 1);
+      mbar_init(w.v_empty(s), 2);
     }
     mbar_init(w.q_full(), 256);
     for (int g = 0; g < 2; ++g) {
@@ -1013,8 +1025,7 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
       }
       mbar_init(w.o_full(g), 1);
     }
-    mbar_init(w.c_ask(), 1);
-    mbar_init(w.c_done(), 1);
+    mbar_init(w.v_clear(), 1);
     for (int i = 0; i < kItemWarps * S::kItemStages; ++i) mbar_init(w.bar(S::kDenseBars + i), 1);
     fence_barrier_init();
     ctl[0] = 0u;
@@ -1040,10 +1051,8 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
       const unsigned n = w.template produce<true>();
       __syncwarp();
       if (ctl[0] != 0u) w.template drain<true>(n);
-    } else if (warp == kIssueWarp) {
-      if (elect_one()) w.issue();
     } else {
-      w.clear();
+      if (elect_one()) w.issue(warp - kIssueWarp);
     }
     __syncwarp();
     tmem_fence_before_sync();
