@@ -109,18 +109,18 @@ static PlanDims plan_dims(int tokens, int seqs, int num_heads, int num_kv_heads,
 }
 
 // Regions of the workspace; every one starts on a 256-byte boundary.
-struct WorkspaceLayout { long long dense_ml, dense_o, item_ml, item_o, dense_desc, item_desc, total; };
+struct WorkspaceLayout { long long dense_ml, dense_o, strip_ml, strip_o, dense_desc, strip_desc, total; };
 static WorkspaceLayout workspace_layout(const PlanDims& d, int head_dim) {
   WorkspaceLayout w;
   long long at = 0;
   auto take = [&](long long bytes) { const long long here = at; at += (bytes + 255) / 256 * 256; return here; };
-  const long long records = max_dense_records(d), items = max_items(d);
+  const long long records = max_dense_records(d), strips = max_strip_records(d);
   w.dense_ml = take(records * kUnitRows * 8);
-  w.item_ml = take(items * kItemRows * 8);
+  w.strip_ml = take(strips * kStripRows * 8);
   w.dense_desc = take((long long)d.tokens * d.NKV * 8);
-  w.item_desc = take((long long)d.tokens * d.NKV * 8);
+  w.strip_desc = take((long long)d.tokens * d.NKV * d.G * 8);
   w.dense_o = take(records * kUnitRows * head_dim * 4);
-  w.item_o = take(items * kItemRows * head_dim * 4);
+  w.strip_o = take(strips * kStripRows * head_dim * 4);
   w.total = at;
   return w;
 }
@@ -128,7 +128,7 @@ static WorkspaceLayout workspace_layout(const PlanDims& d, int head_dim) {
 static bool attention_sizes_ok(int tokens, int seqs, int num_heads, int num_kv_heads, int head_dim, int prefix_len) {
   return tokens >= 1 && tokens <= (1 << 20) && seqs >= 1 && seqs <= kMaxSeqs && (head_dim == 64 || head_dim == 128) &&
          num_kv_heads >= 1 && num_heads >= 1 && num_heads <= 1024 && num_heads % num_kv_heads == 0 &&
-         num_heads / num_kv_heads <= kItemRows && prefix_len >= 0;
+         num_heads / num_kv_heads <= kMaxGroup && prefix_len >= 0;
 }
 
 extern "C" int64_t qmk_prefix_attention_workspace(int32_t tokens, int32_t seqs, int32_t num_heads, int32_t num_kv_heads,
@@ -183,7 +183,7 @@ static bool pool_map(encode_fn enc, CUtensorMap* m, const void* base, const qmk_
   const cuuint64_t strides[2] = {(cuuint64_t)a->head_dim * 2, (cuuint64_t)a->head_dim * 2 * a->num_kv_heads};
   const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, es[3] = {1, 1, 1};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -228,8 +228,9 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
   p.d = plan_dims(a->tokens, a->seqs, a->num_heads, a->num_kv_heads, a->prefix_len, ctas);
   const long long room = (long long)a->max_pages * a->page_size;
   p.d.room = (int)(room > a->prefix_len ? room : a->prefix_len);
-  // 32-bit counts on the device: blocks of a KV head, items
-  if (max_units(p.d) * (p.d.room / kBlockKeys + 1) > 0x7fffffffll || max_items(p.d) > 0x7fffffffll) return QMK_ERR_INVALID_ARG;
+  // 32-bit counts on the device: blocks and pieces of a KV head, records
+  if (max_units(p.d) * (p.d.room / kBlockKeys + 1) > 0x7fffffffll || max_strip_records(p.d) > 0x7fffffffll ||
+      max_strips(p.d) / p.d.NKV * (p.d.room / kPieceKeys + 1) > 0x7fffffffll) return QMK_ERR_INVALID_ARG;
   const WorkspaceLayout w = workspace_layout(p.d, a->head_dim);
   if (a->workspace_bytes < w.total) return QMK_ERR_INVALID_ARG;
   p.q = (const uint16_t*)a->q; p.out = (uint16_t*)a->out; p.lse = a->lse;
@@ -239,8 +240,8 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
   p.scale_log2e = a->scale * 1.4426950408889634f;
   unsigned char* ws = (unsigned char*)a->workspace;
   p.dense_ml = (float2*)(ws + w.dense_ml); p.dense_o = (float*)(ws + w.dense_o);
-  p.item_ml = (float2*)(ws + w.item_ml); p.item_o = (float*)(ws + w.item_o);
-  p.dense_desc = (int2*)(ws + w.dense_desc); p.item_desc = (int2*)(ws + w.item_desc);
+  p.strip_ml = (float2*)(ws + w.strip_ml); p.strip_o = (float*)(ws + w.strip_o);
+  p.dense_desc = (int2*)(ws + w.dense_desc); p.strip_desc = (int2*)(ws + w.strip_desc);
   encode_fn enc = tensor_map_encoder();
   if (!enc) {
     snprintf(g_paged_err, sizeof(g_paged_err), "cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)");

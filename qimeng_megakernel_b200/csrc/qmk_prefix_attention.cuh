@@ -16,8 +16,9 @@
 //   warps 0-3, 4-7 softmax groups; 8 and 11 load K and V blocks (one TMA box per page and 64 dimensions); 9 and 10 issue the
 //   products of a group each
 //
-// Items.  What a short request holds behind the prefix: a warp per item, up to 16 rows x ck keys, mma.sync on 16-row tiles,
-// K and V through a ring of its own in shared memory (the ring of the blocks, free by then).
+// Strips.  What a short request holds behind the prefix: 8 rows x a run of 32-key pieces per warp, on mma.sync with the keys
+// (for P V the dimensions) as the long side of the tile, K and V through a ring of the warp's own in shared memory (the ring of
+// the blocks, free by then).
 //
 // Both parts leave partial results (m, l, unnormalised O, all in 32 bits) unless a row is complete; merge_kernel adds them
 // up in a fixed order, so a call gives the same bits every time.  Nothing is kept between calls.
@@ -49,10 +50,10 @@ struct AttnParams {
   // workspace
   float* dense_o;              // [records, 256, HD]
   float2* dense_ml;            // [records, 256]   (m in log2 units, l)
-  float* item_o;               // [items, 16, HD]
-  float2* item_ml;             // [items, 16]
+  float* strip_o;              // [records, 8, HD]
+  float2* strip_ml;            // [records, 8]
   int2* dense_desc;            // [tokens, NKV]    {first record, records | dual << 15 | row << 16}; records 0: none
-  int2* item_desc;             // [tokens, NKV]    {first record, records | row << 16}
+  int2* strip_desc;            // [tokens, NH]     {first record, records | row << 16}
 };
 struct AttnMaps {
   CUtensorMap k, v;            // {HD, NKV, slots}, box {64, 1, min(page, 128)}
@@ -75,13 +76,13 @@ struct AttnSmem {
   static constexpr int kOffK = 2 * kTileBytes;
   static constexpr int kOffV = kOffK + kStages * kTileBytes;
   static constexpr int kRing = kOffV + kStages * kTileBytes;
-  // items: per warp a ring of kItemStages stages of 8 KiB
-  static constexpr int kItemStages = 3, kItemStageBytes = 8192;
-  static constexpr int kItemKeys = HD == 64 ? 32 : 16;          // keys of a stage
-  static constexpr int kItemRing = kItemWarps * kItemStages * kItemStageBytes;
-  static constexpr int kOffBars = kRing > kItemRing ? kRing : kItemRing;
-  static constexpr int kDenseBars = 4 * kStages + 1 + 4 + 4 + 2 + 1;
-  static constexpr int kNumBars = kDenseBars + kItemWarps * kItemStages;
+  // strips: per warp a ring of kStripStages stages of 8 KiB
+  static constexpr int kStripStages = 3, kStripStageBytes = 8192;
+  static constexpr int kStageKeys = HD == 64 ? 32 : 16;         // keys of a stage
+  static constexpr int kStripRing = kStripWarps * kStripStages * kStripStageBytes;
+  static constexpr int kOffBars = kRing > kStripRing ? kRing : kStripRing;
+  static constexpr int kDenseBars = 4 * kStages + 15;
+  static constexpr int kNumBars = kDenseBars + kStripWarps * kStripStages;
   static constexpr int kOffCtl = kOffBars + kNumBars * 8;       // words: 0 abort, 1 tensor memory base
   static constexpr int kOffRed = (kOffCtl + 16 + 7) / 8 * 8;    // long long [4][16] scratch of the scans
   static constexpr int kOffTot = kOffRed + 4 * 16 * 8;          // Totals, Plan
@@ -207,6 +208,11 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {   // of an 8 x 8 fragment of 16-bit values
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -241,7 +247,7 @@ struct Scans {                 // prefix sums over the requests, in shared memor
   int* long_blocks;
   int* long_units;
   int* short_tokens;
-  int* items;                  // row blocks x chunks (one KV head)
+  int* pieces;                 // of one KV head
 };
 __device__ __forceinline__ Req load_request(const AttnParams& p, int s) {
   return request(p.d, p.cu_tokens[s], p.cu_tokens[s + 1], p.kv_lengths[s]);
@@ -290,10 +296,8 @@ __device__ __forceinline__ void scan_values(long long (&v)[N], long long (&total
 struct Work {                  // in shared memory
   Totals t;
   Plan plan;
-  long long items;
 };
 __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc, long long* red, Work* out) {
-  Totals t;
   const int seqs = p.d.seqs;
   long long base[4] = {0, 0, 0, 0};
   for (int s0 = 0; s0 < seqs; s0 += kAttnThreads) {
@@ -307,7 +311,7 @@ __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc,
         v[1] = n;
       } else {
         v[2] = r.n;
-        v[3] = (long long)own_keys(p.d, r) * item_rows_blocks(p.d, r);
+        v[3] = (long long)strips_of(p.d, r) * pieces_of(p.d, r);
       }
     }
     scan_values<4>(v, tot, red);
@@ -315,6 +319,7 @@ __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc,
       sc.long_blocks[s] = (int)(base[0] + v[0]);
       sc.long_units[s] = (int)(base[1] + v[1]);
       sc.short_tokens[s] = (int)(base[2] + v[2]);
+      sc.pieces[s] = (int)(base[3] + v[3]);
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) base[k] += tot[k];
@@ -323,26 +328,9 @@ __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc,
     sc.long_blocks[seqs] = (int)base[0];
     sc.long_units[seqs] = (int)base[1];
     sc.short_tokens[seqs] = (int)base[2];
-  }
-  t.long_blocks = base[0]; t.long_units = (int)base[1]; t.short_tokens = (int)base[2]; t.item_keys = base[3];
-  const Plan plan = make_plan(p.d, t);
-  long long at = 0;
-  for (int s0 = 0; s0 < seqs; s0 += kAttnThreads) {
-    const int s = s0 + (int)threadIdx.x;
-    long long v[1] = {0}, tot[1];
-    if (s < seqs) {
-      const Req r = load_request(p, s);
-      if (!is_long(p.d, r)) v[0] = (long long)item_rows_blocks(p.d, r) * item_chunks(own_keys(p.d, r), plan.ck);
-    }
-    scan_values<1>(v, tot, red);
-    if (s < seqs) sc.items[s] = (int)(at + v[0]);
-    at += tot[0];
-  }
-  if (threadIdx.x == 0) {
-    sc.items[seqs] = (int)at;
-    out->t = t;
-    out->plan = plan;
-    out->items = at * p.d.NKV;
+    sc.pieces[seqs] = (int)base[3];
+    out->t = Totals{base[0], (int)base[1], (int)base[2], base[3]};
+    out->plan = make_plan(p.d, out->t);
   }
   __syncthreads();
 }
@@ -427,11 +415,13 @@ struct Dense {
   __device__ __forceinline__ uint32_t k_empty(int s) const { return bar(S::kStages + s); }
   __device__ __forceinline__ uint32_t v_full(int s) const { return bar(2 * S::kStages + s); }
   __device__ __forceinline__ uint32_t v_empty(int s) const { return bar(3 * S::kStages + s); }
-  __device__ __forceinline__ uint32_t q_full() const { return bar(4 * S::kStages); }
-  __device__ __forceinline__ uint32_t s_full(int g, int buf) const { return bar(4 * S::kStages + 1 + 2 * g + buf); }
-  __device__ __forceinline__ uint32_t p_full(int g, int buf) const { return bar(4 * S::kStages + 5 + 2 * g + buf); }
-  __device__ __forceinline__ uint32_t o_full(int g) const { return bar(4 * S::kStages + 9 + g); }
-  __device__ __forceinline__ uint32_t v_clear() const { return bar(4 * S::kStages + 11); }
+  // A waiter tells a phase by its parity alone, so every barrier below is one whose next phase cannot complete before all its
+  // waiters have seen the last one.
+  __device__ __forceinline__ uint32_t s_full(int g, int half) const { return bar(4 * S::kStages + 2 * g + half); }
+  __device__ __forceinline__ uint32_t p_full(int g, int half) const { return bar(4 * S::kStages + 4 + 2 * g + half); }
+  __device__ __forceinline__ uint32_t o_full(int g, int half) const { return bar(4 * S::kStages + 8 + 2 * g + half); }   // once a segment
+  __device__ __forceinline__ uint32_t q_full(int g) const { return bar(4 * S::kStages + 12 + g); }   // segments in which g has steps
+  __device__ __forceinline__ uint32_t v_clear() const { return bar(4 * S::kStages + 14); }
 
   // Steps of a group in a segment of nb blocks: halves of 64 keys of the blocks it takes (with two tiles every block, with
   // one the blocks of its parity).
@@ -506,7 +496,7 @@ struct Dense {
     const uint64_t kd0 = desc_k_major(base + S::kOffK), vd0 = desc_n_major(base + S::kOffV, 16384u);
     const uint32_t sd = tmem + (uint32_t)g * 128u, od = tmem + 256u + (uint32_t)g * 128u;
     unsigned n = 0, segs = 0, p_par = 0;                     // (p_par: parity of the next P, both halves)
-    for (long long b = lo; b < hi; ++segs) {
+    for (long long b = lo; b < hi;) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
       const int nb = (int)min((long long)(x.blocks - b0), hi - b);
@@ -527,9 +517,10 @@ struct Dense {
         mma_commit_to(empty);
         if (dual) mbar_arrive(empty);
       };
-      if (!wait_bar(q_full(), segs & 1u, ctl)) return;
       int blk = dual ? g : 0;
       if (blk < nb) {
+        if (!wait_bar(q_full(g), segs & 1u, ctl)) return;
+        ++segs;
         unsigned m = n + (unsigned)blk;
         int st = (int)(m % S::kStages);
         if (!wait_bar(k_full(st), (m / S::kStages) & 1u, ctl)) return;
@@ -571,7 +562,7 @@ struct Dense {
               score(stn, half);
               if (half == 1) release(k_empty(stn));
             } else {
-              mma_commit_to(o_full(g));                      // (twice a segment: after its last two halves)
+              mma_commit_to(o_full(g, half));
             }
           }
           p_par ^= 1u;
@@ -602,7 +593,7 @@ struct Dense {
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + g * 128 + lane_base, o_col = tmem + 256 + g * 128 + lane_base;
     unsigned s_par = 0;                                      // parity of the next S, both halves
-    unsigned n = 0, clears = 0;
+    unsigned n = 0, clears = 0, o_par = 0;
     for (long long b = lo; b < hi;) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
@@ -624,11 +615,13 @@ struct Dense {
         fence_async_shared();
       }
       tmem_fence_before_sync();                       // (the O of the segment before has been read)
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // (a group without steps must not arrive for two segments at once)
-      mbar_arrive(q_full());
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // (nobody arrives for a segment before all have left the last)
+      mbar_arrive(q_full(0));
+      if (steps_of(nb, dual, 1) > 0) mbar_arrive(q_full(1));
       const bool warp_works = __ballot_sync(kFullMask, token >= 0) != 0u;
       const int warp_lim = __reduce_min_sync(kFullMask, lim);
       float m = -INFINITY, l = 0.f;
+      bool seen = false;                              // every row of the warp has an m
       const int steps = steps_of(nb, dual, g);
       bool ok = true;
       for (int j = 0; j < steps; ++j) {
@@ -643,12 +636,37 @@ struct Dense {
           tmem_ld32(s + 32, sh + 32);
           tmem_wait_ld();
           const int k0 = (b0 + block_of(j, dual, g)) * kBlockKeys + 64 * half;
-          bool plain = k0 + 64 <= warp_lim;
+          const bool plain = k0 + 64 <= warp_lim;
           if (!plain) {
             const int vis = lim - k0;
 #pragma unroll
             for (int c = 0; c < 64; ++c) s[c] = c < vis ? s[c] : -INFINITY;
           }
+          const f32x2 scale2 = pair(p.scale_log2e, p.scale_log2e);
+          f32x2 sum2[2];
+          uint32_t pk[32];
+          // 2^(scale s - m) of the row, packed, and their sum
+          auto exps = [&](auto with_poly) {
+            const float off = m == -INFINITY ? 0.f : m;
+            const f32x2 off2 = pair(-off, -off);
+            sum2[0] = sum2[1] = 0ull;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const f32x2 e = fma2(pair(s[2 * i], s[2 * i + 1]), scale2, off2);
+              float a, d;
+              if (decltype(with_poly)::value && i % kPolyEvery == kPolyEvery - 1) {
+                ex2_pair(e, a, d);
+              } else {
+                unpair(e, a, d);
+                a = ex2(a);
+                d = ex2(d);
+              }
+              sum2[i & 1] = add2(sum2[i & 1], pair(a, d));
+              pk[i] = pack2(a, d);
+            }
+          };
+          // The row's maximum is worked out beside the exponentials, which take the m there is (it rarely has to rise); the
+          // polynomial has no zero: rows with hidden keys, or with nothing seen yet, go without it.
           float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
           for (int i = 4; i + 8 <= 64; i += 8)
@@ -657,55 +675,35 @@ struct Dense {
 #pragma unroll
           for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[60 + c]);
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2e;
-          // NaN scores: the maximum passes them over, their own exponential keeps them
-          if (__any_sync(kFullMask, top > m + 8.f)) {
-            const float m_new = fmaxf(m, top);
-            if (j > 0) {
-              // O may be touched once P V of step j - 1 is through: the scores of step j + 1 were issued behind it
-              ok = j + 1 < steps ? wait_bar(s_full(g, half ^ 1), half ? s_par ^ 1u : s_par, ctl) : wait_bar(o_full(g), 0u, ctl);
-              if (!ok) break;
-              tmem_fence_after_sync();
-              const float f = m_new == -INFINITY ? 1.f : ex2(m - m_new);
-              l *= f;
+          if (plain && seen) exps(Yes{});
+          // (NaN scores: the maximum passes them over, their own exponential keeps them)
+          const bool raise = __any_sync(kFullMask, top > m + 8.f);
+          if (raise || !(plain && seen)) {
+            if (raise) {
+              const float m_new = fmaxf(m, top);
+              if (j > 0) {
+                // O may be touched once P V of step j - 1 is through: the scores of step j + 1 were issued behind it
+                ok = j + 1 < steps ? wait_bar(s_full(g, half ^ 1), half ? s_par ^ 1u : s_par, ctl) : wait_bar(o_full(g, 0), o_par, ctl);
+                if (!ok) break;
+                tmem_fence_after_sync();
+                const float f = m_new == -INFINITY ? 1.f : ex2(m - m_new);
+                l *= f;
 #pragma unroll 1
-              for (int c = 0; c < HD / 16; ++c) {
-                uint32_t o[16];
-                tmem_ld16(o, o_col + 16 * c);
-                tmem_wait_ld();
+                for (int c = 0; c < HD / 16; ++c) {
+                  uint32_t o[16];
+                  tmem_ld16(o, o_col + 16 * c);
+                  tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tmem_st16(o_col + 16 * c, o);
-              }
-            }
-            m = m_new;
-          }
-          // the polynomial has no zero: rows with hidden keys, or with nothing seen yet, go without it
-          plain = plain && __all_sync(kFullMask, m != -INFINITY);
-          const float off = m == -INFINITY ? 0.f : m;
-          const f32x2 scale2 = pair(p.scale_log2e, p.scale_log2e), off2 = pair(-off, -off);
-          f32x2 sum2[2] = {0ull, 0ull};
-          auto exps = [&](auto with_poly) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const f32x2 e = fma2(pair(s[32 * c + 2 * i], s[32 * c + 2 * i + 1]), scale2, off2);
-                float a, d;
-                if (decltype(with_poly)::value && i % kPolyEvery == kPolyEvery - 1) {
-                  ex2_pair(e, a, d);
-                } else {
-                  unpair(e, a, d);
-                  a = ex2(a);
-                  d = ex2(d);
+                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                  tmem_st16(o_col + 16 * c, o);
                 }
-                sum2[i & 1] = add2(sum2[i & 1], pair(a, d));
-                pk[i] = pack2(a, d);
               }
-              tmem_st16(sh + 16 * c, pk);
+              m = m_new;
+              seen = __all_sync(kFullMask, m != -INFINITY);
             }
-          };
-          if (plain) exps(Yes{}); else exps(No{});
+            exps(No{});
+          }
+          tmem_st32(sh, pk);
           float sa, sb;
           unpair(add2(sum2[0], sum2[1]), sa, sb);
           l += sa + sb;
@@ -732,7 +730,8 @@ struct Dense {
         mbar_arrive(p_full(g, half));
         s_par ^= (unsigned)half;
       }
-      if (ok && steps > 0) ok = wait_bar(o_full(g), 0u, ctl) && wait_bar(o_full(g), 1u, ctl);
+      if (ok && steps > 0) ok = wait_bar(o_full(g, 1), o_par, ctl);
+      if (steps > 0) o_par ^= 1u;
       tmem_fence_after_sync();
       // ---- the unit's rows: complete, or a record ----
       const int cta = (int)blockIdx.x;
@@ -784,7 +783,8 @@ struct Dense {
           int parts = 0;
           if (!whole) parts = dense_owner(plan, b + x.blocks - 1) - cta + 1;
           p.dense_desc[at] = make_int2(rec, parts | (dual ? 1 << 15 : 0) | (tile_row << 16));
-          if (x.s >= 0) p.item_desc[at] = make_int2(0, 0);
+          if (x.s >= 0)
+            for (int i = 0; i < p.d.G; ++i) p.strip_desc[(size_t)token * p.NH + head + i] = make_int2(0, 0);
         }
       }
       n += (unsigned)nb;
@@ -793,34 +793,35 @@ struct Dense {
   }
 };
 
-// ------------------------------------------------------------------------------------------------ items
+// ------------------------------------------------------------------------------------------------ strips
+// g = lane / 4, t = lane % 4.  S^T = K Q^T: tiles of 16 keys x 8 rows (lane: keys g, g + 8 of rows 2t, 2t + 1); O^T = V^T P^T: tiles
+// of 16 dimensions x 8 rows.  The P^T operand is the transpose of the S^T fragment: one movmatrix per 8 keys.  A lane's columns
+// are the same two rows in both products, so a row's maximum and scale never leave its lanes.
 template <int HD>
-__device__ __forceinline__ void walk_items(const AttnParams& p, const AttnMaps& maps, unsigned char* smem, volatile unsigned* ctl,
-                                           const Scans& sc, const Plan& plan, long long lo, long long hi, int warp, int lane) {
+__device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps& maps, unsigned char* smem, volatile unsigned* ctl,
+                                            const Scans& sc, const Plan& plan, int warp, int lane) {
   using S = AttnSmem<HD>;
-  constexpr int KS = S::kItemKeys, NT = KS / 8, GROUPS = KS / 16, HALVES = S::kHalves;
+  constexpr int KS = S::kStageKeys, TILES = KS / 16, HALVES = S::kHalves;
   constexpr int KBYTES = KS * HD * 2;                       // 4 KiB of K, then 4 KiB of V
-  const uint32_t ring = smem_u32(smem) + warp * S::kItemStages * S::kItemStageBytes;
-  const uint32_t bars = smem_u32(smem) + S::kOffBars + (S::kDenseBars + warp * S::kItemStages) * 8;
+  const uint32_t ring = smem_u32(smem) + warp * S::kStripStages * S::kStripStageBytes;
+  const uint32_t bars = smem_u32(smem) + S::kOffBars + (S::kDenseBars + warp * S::kStripStages) * 8;
   const int g = lane >> 2, t4 = lane & 3;
   const int oob = p.num_pages << p.page_shift;
   unsigned filled = 0;                                      // stages filled by this warp so far
-  for (long long item = lo + warp; item < hi; item += kItemWarps) {
-    // item = (request, row block, KV head, chunk), chunk fastest
-    const int flat = (int)(item / p.d.NKV);
-    const int s = find_last(sc.items, p.d.seqs, flat);
+  long long lo, hi;
+  const int number = piece_range(p.d, plan, (int)blockIdx.x, warp, lo, hi);
+  for (long long f = lo; f < hi;) {
+    const int s = find_last(sc.pieces, p.d.seqs, (int)(f / p.d.NKV));
     const Req r = load_request(p, s);
-    const int own = own_keys(p.d, r), chunks = item_chunks(own, plan.ck);
-    long long rest = item - (long long)sc.items[s] * p.d.NKV;
-    const int ch = (int)(rest % chunks);
-    rest /= chunks;
-    const int kvh = (int)(rest % p.d.NKV), rb = (int)(rest / p.d.NKV);
-    const int i0 = rb * p.d.item_tokens(), ni = min(p.d.item_tokens(), r.n - i0), rows = ni * p.d.G;
-    const int k_lo = p.d.prefix_len + ch * plan.ck;
-    const int k_hi = max(k_lo, min(k_lo + plan.ck, limit_of(p.d, r, i0 + ni - 1)));
-    const int row0 = g, row1 = g + 8;
-    const int lim0 = row0 < rows ? limit_of(p.d, r, i0 + row0 / p.d.G) : 0, lim1 = row1 < rows ? limit_of(p.d, r, i0 + row1 / p.d.G) : 0;
-    // page rows of the next 32 groups of 16 keys, one per lane
+    const int per = pieces_of(p.d, r);
+    long long rest = f - (long long)sc.pieces[s] * p.d.NKV;
+    const int c0 = (int)(rest % per), n = (int)min((long long)(per - c0), hi - f);
+    rest /= per;
+    const int kvh = (int)(rest % p.d.NKV), strip = (int)(rest / p.d.NKV);
+    const int base_row = strip * kStripRows, rows = min(kStripRows, r.n * p.d.G - base_row);
+    const int k_lo = p.d.prefix_len + c0 * kPieceKeys;
+    const int k_hi = max(k_lo, min(k_lo + n * kPieceKeys, limit_of(p.d, r, (base_row + rows - 1) / p.d.G)));
+    // pool rows of the next 32 groups of 16 keys, one per lane
     const int* table = p.tables + (size_t)s * p.max_pages;
     auto group_row = [&](int grp) {
       const int key = k_lo + grp * 16;
@@ -832,165 +833,176 @@ __device__ __forceinline__ void walk_items(const AttnParams& p, const AttnMaps& 
     const int stages = (k_hi - k_lo + KS - 1) / KS;
     int held = group_row(lane), held_from = 0;
     int sent = 0;
-    auto send = [&](bool cleared) {                          // fills the next stage; lane l < 2 * GROUPS * HALVES sends one box
-      const int st = (int)((filled + (unsigned)sent) % S::kItemStages);
-      const int grp0 = sent * GROUPS;
-      if (grp0 + GROUPS > held_from + 32) {
+    auto send = [&]() {                                      // fills the next stage; lane l < 2 * TILES * HALVES sends one box
+      const int st = (int)((filled + (unsigned)sent) % S::kStripStages);
+      const int grp0 = sent * TILES;
+      if (grp0 + TILES > held_from + 32) {
         held_from = grp0;
         held = group_row(grp0 + lane);
       }
-      const int q = lane % (GROUPS * HALVES), kg = q / HALVES, half = q % HALVES;
-      const bool is_v = lane >= GROUPS * HALVES;
+      const int q = lane % (TILES * HALVES), kg = q / HALVES, half = q % HALVES;
+      const bool is_v = lane >= TILES * HALVES;
       const int row = __shfl_sync(kFullMask, held, (grp0 + kg - held_from) & 31);
-      const bool mine = lane < 2 * GROUPS * HALVES && row >= 0;
+      const bool mine = lane < 2 * TILES * HALVES && row >= 0;
       const unsigned issue = __ballot_sync(kFullMask, mine);
-      if (cleared) fence_async_shared();
       if (lane == 0) mbar_expect_tx(bars + st * 8, (uint32_t)__popc(issue) * 2048u);
       __syncwarp();
       if (mine)
-        tma_box(ring + st * S::kItemStageBytes + (is_v ? KBYTES : 0) + (kg * HALVES + half) * 2048, is_v ? &maps.v16 : &maps.k16,
+        tma_box(ring + st * S::kStripStageBytes + (is_v ? KBYTES : 0) + (kg * HALVES + half) * 2048, is_v ? &maps.v16 : &maps.k16,
                 half * 64, kvh, row, bars + st * 8);
       ++sent;
     };
-    while (sent < stages && sent < S::kItemStages) send(false);
-    // Q rows g and g + 8 as the A operand
-    uint32_t qa[HD / 16][4];
+    while (sent < stages && sent < S::kStripStages) send();
+    // row g of the strip as the column-major operand; the two rows this lane's results belong to
+    uint32_t qb[HD / 16][2];
     {
-      const uint16_t* q0 = p.q + (size_t)(r.first + i0 + row0 / p.d.G) * p.q_stride + (size_t)(kvh * p.d.G + row0 % p.d.G) * HD + 2 * t4;
-      const uint16_t* q1 = p.q + (size_t)(r.first + i0 + row1 / p.d.G) * p.q_stride + (size_t)(kvh * p.d.G + row1 % p.d.G) * HD + 2 * t4;
+      const int i = min(g, rows - 1) + base_row;
+      const uint16_t* qp = p.q + (size_t)(r.first + i / p.d.G) * p.q_stride + (size_t)(kvh * p.d.G + i % p.d.G) * HD + 2 * t4;
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
-        qa[k][0] = row0 < rows ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k) : 0u;
-        qa[k][1] = row1 < rows ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k) : 0u;
-        qa[k][2] = row0 < rows ? *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 8) : 0u;
-        qa[k][3] = row1 < rows ? *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 8) : 0u;
+        qb[k][0] = *reinterpret_cast<const uint32_t*>(qp + 16 * k);
+        qb[k][1] = *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8);
       }
     }
+    const int lim0 = min(k_hi, limit_of(p.d, r, (base_row + min(2 * t4, rows - 1)) / p.d.G));
+    const int lim1 = min(k_hi, limit_of(p.d, r, (base_row + min(2 * t4 + 1, rows - 1)) / p.d.G));
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    float o[HD / 8][4];
+    float o[HD / 16][4];
 #pragma unroll
-    for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int j = 0; j < HD / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     bool ok = true;
     for (int i = 0; i < stages; ++i) {
-      const unsigned f = filled + (unsigned)i;
-      const int st = (int)(f % S::kItemStages);
-      ok = wait_bar(bars + st * 8, (f / S::kItemStages) & 1u, ctl);
+      const unsigned at = filled + (unsigned)i;
+      const int st = (int)(at % S::kStripStages);
+      ok = wait_bar(bars + st * 8, (at / S::kStripStages) & 1u, ctl);
       if (!ok) break;
-      const uint32_t kb = ring + st * S::kItemStageBytes, vb = kb + KBYTES;
+      const uint32_t kb = ring + st * S::kStripStageBytes, vb = kb + KBYTES;
       const int key0 = k_lo + i * KS;
       const int valid = min(KS, k_hi - key0);
-      bool cleared = false;
       if (valid < KS) {                                     // rows of V behind the last key: whatever they hold, 0 * V is to be 0
-        unsigned char* vp = smem + warp * S::kItemStages * S::kItemStageBytes + st * S::kItemStageBytes + KBYTES;
+        unsigned char* vp = smem + warp * S::kStripStages * S::kStripStageBytes + st * S::kStripStageBytes + KBYTES;
         for (int e = lane; e < (KS - valid) * 8 * HALVES; e += 32) {
           const int rr = valid + e / (8 * HALVES), c = e % (8 * HALVES);
           *reinterpret_cast<uint4*>(vp + ((rr >> 4) * HALVES + (c >> 3)) * 2048 + (rr & 15) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
+        fence_async_shared();                               // (before a copy lands here again)
         __syncwarp();
-        cleared = true;
       }
-      float sc4[NT][4];
+      float x[TILES][4];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        sc4[j][0] = sc4[j][1] = sc4[j][2] = sc4[j][3] = 0.f;
-        const int kr = (j & 1) * 8 + (lane & 7);            // key row inside its group of 16
+      for (int j = 0; j < TILES; ++j) {
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+        x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
+        const int kr = lane & 15;
 #pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {                 // four 16-byte pieces: two k-steps
-          const int piece = 4 * c + (lane >> 3);
-          uint32_t bfr[4];
-          ldsm4(bfr, kb + ((j >> 1) * HALVES + (piece >> 3)) * 2048 + kr * 128 + (((piece & 7) ^ (kr & 7)) << 4));
-          mma16816(sc4[j], qa[2 * c], bfr[0], bfr[1]);
-          mma16816(sc4[j], qa[2 * c + 1], bfr[2], bfr[3]);
+        for (int k = 0; k < HD / 16; ++k) {                 // (two chains of products)
+          const int piece = 2 * k + (lane >> 4);
+          uint32_t a[4];
+          ldsm4(a, kb + (j * HALVES + (piece >> 3)) * 2048 + kr * 128 + (((piece & 7) ^ (kr & 7)) << 4));
+          if (k & 1) mma16816(y, a, qb[k][0], qb[k][1]);
+          else mma16816(x[j], a, qb[k][0], qb[k][1]);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[j][c] = (x[j][c] + y[c]) * p.scale_log2e;
+      }
+      if (key0 + KS > min(lim0, lim1)) {
+#pragma unroll
+        for (int j = 0; j < TILES; ++j) {
+          const int key = key0 + 16 * j + g;
+          x[j][0] = key < lim0 ? x[j][0] : -INFINITY;
+          x[j][1] = key < lim1 ? x[j][1] : -INFINITY;
+          x[j][2] = key + 8 < lim0 ? x[j][2] : -INFINITY;
+          x[j][3] = key + 8 < lim1 ? x[j][3] : -INFINITY;
         }
       }
-      float t0 = -INFINITY, t1 = -INFINITY;
+      float t0 = fmaxf(x[0][0], x[0][2]), t1 = fmaxf(x[0][1], x[0][3]);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int key = key0 + 8 * j + 2 * t4;
-        sc4[j][0] = key < min(lim0, k_hi) ? sc4[j][0] * p.scale_log2e : -INFINITY;
-        sc4[j][1] = key + 1 < min(lim0, k_hi) ? sc4[j][1] * p.scale_log2e : -INFINITY;
-        sc4[j][2] = key < min(lim1, k_hi) ? sc4[j][2] * p.scale_log2e : -INFINITY;
-        sc4[j][3] = key + 1 < min(lim1, k_hi) ? sc4[j][3] * p.scale_log2e : -INFINITY;
-        t0 = fmaxf(t0, fmaxf(sc4[j][0], sc4[j][1]));
-        t1 = fmaxf(t1, fmaxf(sc4[j][2], sc4[j][3]));
+      for (int j = 1; j < TILES; ++j) { t0 = max3(t0, x[j][0], x[j][2]); t1 = max3(t1, x[j][1], x[j][3]); }
+      // m is raised only when a lane's part of a row asks for more than 2^8: then the row's lanes agree on the new one
+      if (__any_sync(kFullMask, t0 > m0 + 8.f || t1 > m1 + 8.f)) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          t0 = fmaxf(t0, __shfl_xor_sync(kFullMask, t0, d));
+          t1 = fmaxf(t1, __shfl_xor_sync(kFullMask, t1, d));
+        }
+        const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+        const float f0 = n0 == -INFINITY ? 1.f : ex2(m0 - n0), f1 = n1 == -INFINITY ? 1.f : ex2(m1 - n1);
+        m0 = n0; m1 = n1;
+        l0 *= f0; l1 *= f1;
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j) { o[j][0] *= f0; o[j][1] *= f1; o[j][2] *= f0; o[j][3] *= f1; }
+      }
+      const float off0 = m0 == -INFINITY ? 0.f : m0, off1 = m1 == -INFINITY ? 0.f : m1;
+      uint32_t pb[TILES][2];
+#pragma unroll
+      for (int j = 0; j < TILES; ++j) {
+        const float a = ex2(x[j][0] - off0), b = ex2(x[j][1] - off1), c = ex2(x[j][2] - off0), d = ex2(x[j][3] - off1);
+        l0 += a + c;
+        l1 += b + d;
+        pb[j][0] = transpose8(pack2(a, b));
+        pb[j][1] = transpose8(pack2(c, d));
       }
 #pragma unroll
-      for (int d = 1; d <= 2; d <<= 1) {
-        t0 = fmaxf(t0, __shfl_xor_sync(kFullMask, t0, d));
-        t1 = fmaxf(t1, __shfl_xor_sync(kFullMask, t1, d));
-      }
-      const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-      const float f0 = n0 == -INFINITY ? 1.f : ex2(m0 - n0), f1 = n1 == -INFINITY ? 1.f : ex2(m1 - n1);
-      const float off0 = n0 == -INFINITY ? 0.f : n0, off1 = n1 == -INFINITY ? 0.f : n1;
-      m0 = n0; m1 = n1;
-      l0 *= f0; l1 *= f1;
-#pragma unroll
-      for (int j = 0; j < HD / 8; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
-      uint32_t pa[GROUPS][4];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const float a = ex2(sc4[j][0] - off0), b = ex2(sc4[j][1] - off0), c = ex2(sc4[j][2] - off1), d = ex2(sc4[j][3] - off1);
-        l0 += a + b;
-        l1 += c + d;
-        pa[j >> 1][(j & 1) * 2] = pack2(a, b);
-        pa[j >> 1][(j & 1) * 2 + 1] = pack2(c, d);
-      }
-#pragma unroll
-      for (int kg = 0; kg < GROUPS; ++kg)
+      for (int j = 0; j < TILES; ++j)
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c) {
-          const int kr = lane & 15, piece = 2 * c + (lane >> 4);
-          uint32_t bfr[4];
-          ldsm4_t(bfr, vb + (kg * HALVES + (piece >> 3)) * 2048 + kr * 128 + (((piece & 7) ^ (kr & 7)) << 4));
-          mma16816(o[2 * c], pa[kg], bfr[0], bfr[1]);
-          mma16816(o[2 * c + 1], pa[kg], bfr[2], bfr[3]);
+          const int kr = (lane & 7) + ((lane >> 4) & 1) * 8, piece = 2 * c + ((lane >> 3) & 1);
+          uint32_t a[4];
+          ldsm4_t(a, vb + (j * HALVES + (piece >> 3)) * 2048 + kr * 128 + (((piece & 7) ^ (kr & 7)) << 4));
+          mma16816(o[c], a, pb[j][0], pb[j][1]);
         }
       __syncwarp();                                         // every lane has read the stage
-      if (sent < stages) send(cleared);
+      if (sent < stages) send();
     }
     if (!ok) {                                              // leave no copy in flight
       for (int i = 0; i < sent; ++i) {
-        const unsigned f = filled + (unsigned)i;
+        const unsigned at = filled + (unsigned)i;
         const long long w0 = clock64();
-        while (!mbar_try_wait(bars + (f % S::kItemStages) * 8, (f / S::kItemStages) & 1u))
+        while (!mbar_try_wait(bars + (at % S::kStripStages) * 8, (at / S::kStripStages) & 1u))
           if (clock64() - w0 > 1000000) break;
       }
     }
-    if (ok && stages > 0 && ((k_hi - k_lo) % KS) != 0) fence_async_shared();   // (a cleared stage may be refilled by the next item)
     filled += (unsigned)sent;
 #pragma unroll
-    for (int d = 1; d <= 2; d <<= 1) {
+    for (int d = 4; d < 32; d <<= 1) {
       l0 += __shfl_xor_sync(kFullMask, l0, d);
       l1 += __shfl_xor_sync(kFullMask, l1, d);
     }
     const float nan = __int_as_float(0x7fffffff);
     if (!ok) m0 = m1 = l0 = l1 = nan;
-    const bool whole = p.d.prefix_len == 0 && chunks == 1;
+    const bool whole = p.d.prefix_len == 0 && n == per;
+    const int rec = number + strip_number(p.d, s, sc.short_tokens[s], strip, kvh);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = h ? row1 : row0;
+      const int row = 2 * t4 + h;
       if (row >= rows) continue;
       const float m = h ? m1 : m0, l = h ? l1 : l0;
-      const int token = r.first + i0 + row / p.d.G, head = kvh * p.d.G + row % p.d.G;
+      const int token = r.first + (base_row + row) / p.d.G, gq = (base_row + row) % p.d.G, head = kvh * p.d.G + gq;
       if (whole) {
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : nan);
-        uint16_t* dst = p.out + (size_t)token * p.out_stride + (size_t)head * HD + 2 * t4;
+        uint16_t* dst = p.out + (size_t)token * p.out_stride + (size_t)head * HD + g;
 #pragma unroll
-        for (int j = 0; j < HD / 8; ++j)
-          *reinterpret_cast<uint32_t*>(dst + 8 * j) = l == 0.f ? 0u : pack2(o[j][2 * h] * inv, o[j][2 * h + 1] * inv);
-        if (p.lse && t4 == 0) p.lse[(size_t)token * p.NH + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        for (int j = 0; j < HD / 16; ++j) {
+          dst[16 * j] = f32_to_bf16_bits(l == 0.f ? 0.f : o[j][h] * inv);
+          dst[16 * j + 8] = f32_to_bf16_bits(l == 0.f ? 0.f : o[j][2 + h] * inv);
+        }
+        if (p.lse && g == 0) p.lse[(size_t)token * p.NH + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       } else {
-        float* dst = p.item_o + ((size_t)item * kItemRows + row) * HD + 2 * t4;
+        float* dst = p.strip_o + ((size_t)rec * kStripRows + row) * HD + g;
 #pragma unroll
-        for (int j = 0; j < HD / 8; ++j) *reinterpret_cast<float2*>(dst + 8 * j) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
-        if (t4 == 0) p.item_ml[(size_t)item * kItemRows + row] = make_float2(m, l);
+        for (int j = 0; j < HD / 16; ++j) {
+          dst[16 * j] = o[j][h];
+          dst[16 * j + 8] = o[j][2 + h];
+        }
+        if (g == 0) p.strip_ml[(size_t)rec * kStripRows + row] = make_float2(m, l);
       }
-      if (ch == 0 && t4 == 0 && row % p.d.G == 0) {
-        const size_t at = (size_t)token * p.d.NKV + kvh;
-        p.item_desc[at] = make_int2((int)item, (whole ? 0 : chunks) | (row << 16));
-        if (p.d.prefix_len == 0) p.dense_desc[at] = make_int2(0, 0);
+      if (c0 == 0 && g == 0) {                              // whoever starts the strip says where its rows' parts are
+        const int parts = whole ? 0 : piece_owner(plan, f + per - 1) - number + 1;
+        p.strip_desc[(size_t)token * p.NH + head] = make_int2(rec, parts | (row << 16));
+        if (p.d.prefix_len == 0 && gq == 0) p.dense_desc[(size_t)token * p.d.NKV + kvh] = make_int2(0, 0);
       }
     }
+    f += n;
   }
 }
 
@@ -1007,7 +1019,7 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
   sc.long_blocks = reinterpret_cast<int*>(smem + S::kOffScan);
   sc.long_units = sc.long_blocks + p.d.seqs + 1;
   sc.short_tokens = sc.long_units + p.d.seqs + 1;
-  sc.items = sc.short_tokens + p.d.seqs + 1;
+  sc.pieces = sc.short_tokens + p.d.seqs + 1;
   Work* work = reinterpret_cast<Work*>(smem + S::kOffTot);
   Dense<HD> w{p, maps, smem, smem_u32(smem), ctl, sc, work->t, work->plan, 0, 0, 0u, warp, lane};
   if (threadIdx.x == 0) {
@@ -1017,16 +1029,16 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
       mbar_init(w.v_full(s), 1);
       mbar_init(w.v_empty(s), 2);
     }
-    mbar_init(w.q_full(), 256);
     for (int g = 0; g < 2; ++g) {
       for (int h = 0; h < 2; ++h) {
         mbar_init(w.s_full(g, h), 1);
         mbar_init(w.p_full(g, h), 128);
+        mbar_init(w.o_full(g, h), 1);
       }
-      mbar_init(w.o_full(g), 1);
+      mbar_init(w.q_full(g), 256);
     }
     mbar_init(w.v_clear(), 1);
-    for (int i = 0; i < kItemWarps * S::kItemStages; ++i) mbar_init(w.bar(S::kDenseBars + i), 1);
+    for (int i = 0; i < kStripWarps * S::kStripStages; ++i) mbar_init(w.bar(S::kDenseBars + i), 1);
     fence_barrier_init();
     ctl[0] = 0u;
   }
@@ -1041,7 +1053,7 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
     __syncthreads();
     tmem_fence_after_sync();
     w.tmem = ctl[1];
-    if (warp < kItemWarps) {
+    if (warp < kStripWarps) {
       w.softmax();
     } else if (warp == kKeyWarp) {
       const unsigned n = w.template produce<false>();
@@ -1064,13 +1076,13 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
     fence_async_shared();                                    // (the ring's generic writes, before copies land in it again)
     __syncthreads();
   }
-  long long lo, hi;
-  item_range(p.d, work->plan, work->t, work->items, (int)blockIdx.x, lo, hi);
-  if (warp < kItemWarps) walk_items<HD>(p, maps, smem, ctl, sc, work->plan, lo, hi, warp, lane);
+  if (warp < kStripWarps) walk_strips<HD>(p, maps, smem, ctl, sc, work->plan, warp, lane);
 }
 
 // Adds a row's parts: one warp per (token, query head).  With M = max m_r and w_r = 2^(m_r - M):
 //   o = sum_r w_r O_r / sum_r w_r l_r
+// Lane r reads the statistics of part r; then all parts' values are on their way at once (a part of weight zero may hold
+// anything and is left out by a selection).
 template <int HD>
 __global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1079,25 +1091,20 @@ __global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ Attn
   const int token = (int)(row / p.NH), head = (int)(row % p.NH);
   if (token >= min(p.d.tokens, p.cu_tokens[p.d.seqs])) return;
   const int kvh = head / p.d.G, g = head % p.d.G;
-  const size_t at = (size_t)token * p.d.NKV + kvh;
-  const int2 dd = p.dense_desc[at], id = p.item_desc[at];
-  const int nseg = dd.y & 0x7fff, dual = (dd.y >> 15) & 1, nd = nseg << dual, ni = id.y & 0xffff;
-  if (nd + ni == 0) return;
-  const size_t drow = (size_t)dd.x * kUnitRows + ((unsigned)dd.y >> 16) + g, irow = (size_t)id.x * kItemRows + ((unsigned)id.y >> 16) + g;
-  auto ml_of = [&](int r) {
-    if (r < nd) return p.dense_ml[drow + (size_t)(r >> dual) * kUnitRows + (dual ? (r & 1) * 128 : 0)];
-    return p.item_ml[irow + (size_t)(r - nd) * kItemRows];
-  };
-  auto o_of = [&](int r) {
-    if (r < nd) return p.dense_o + (drow + (size_t)(r >> dual) * kUnitRows + (dual ? (r & 1) * 128 : 0)) * HD;
-    return p.item_o + (irow + (size_t)(r - nd) * kItemRows) * HD;
-  };
-  constexpr int LPR = HD / 4, PER = 32 / LPR;              // lanes per row, rows per pass
+  const int2 dd = p.dense_desc[(size_t)token * p.d.NKV + kvh], sd = p.strip_desc[(size_t)token * p.NH + head];
+  const int nseg = dd.y & 0x7fff, dual = (dd.y >> 15) & 1, nd = nseg << dual, parts = nd + (sd.y & 0xffff);
+  if (parts == 0) return;
+  // row of part r: dense parts are 256 rows apart (with one tile two of them 128 rows), strips 8
+  const size_t drow = (size_t)dd.x * kUnitRows + ((unsigned)dd.y >> 16) + g, srow = (size_t)sd.x * kStripRows + ((unsigned)sd.y >> 16);
+  auto dense_row = [&](int r) { return drow + (size_t)(r >> dual) * kUnitRows + (dual ? (r & 1) * 128 : 0); };
+  auto strip_row = [&](int r) { return srow + (size_t)(r - nd) * kStripRows; };
+  constexpr int LPR = HD / 4, PER = 32 / LPR;              // lanes per row, parts per pass
   float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int r0 = 0; r0 < nd + ni; r0 += 32) {
-    const bool have = r0 + lane < nd + ni;
-    const float2 ml = have ? ml_of(r0 + lane) : make_float2(-INFINITY, 0.f);
+  for (int r0 = 0; r0 < parts; r0 += 32) {
+    const int mine = r0 + lane;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (mine < parts) ml = mine < nd ? p.dense_ml[dense_row(mine)] : p.strip_ml[strip_row(mine)];
     float top = ml.x;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
@@ -1108,14 +1115,26 @@ __global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ Attn
     if (ml.x != ml.x) wgt = ml.x;
     L = L * f + warp_sum(wgt * ml.y);
     acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-    const int n = min(32, nd + ni - r0);
-#pragma unroll 8
-    for (int r = 0; r < n; r += PER) {
-      const int rr = r + lane / LPR;
-      const float wr = __shfl_sync(kFullMask, wgt, rr & 31);
-      if (rr < n && wr != 0.f) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(o_of(r0 + rr)) + lane % LPR);
-        acc.x += wr * v.x; acc.y += wr * v.y; acc.z += wr * v.z; acc.w += wr * v.w;
+    const int n = min(32, parts - r0);
+    constexpr int BATCH = 8;
+    for (int b = 0; b < n; b += BATCH * PER) {
+      float4 v[BATCH];
+      float w[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int r = b + i * PER + lane / LPR;
+        const int at = min(r, n - 1) + r0;
+        w[i] = __shfl_sync(kFullMask, wgt, r & 31);
+        if (r >= n) w[i] = 0.f;
+        const float* src = at < nd ? p.dense_o + dense_row(at) * HD : p.strip_o + strip_row(at) * HD;
+        v[i] = __ldcg(reinterpret_cast<const float4*>(src) + lane % LPR);
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        acc.x += w[i] != 0.f ? w[i] * v[i].x : 0.f;
+        acc.y += w[i] != 0.f ? w[i] * v[i].y : 0.f;
+        acc.z += w[i] != 0.f ? w[i] * v[i].z : 0.f;
+        acc.w += w[i] != 0.f ? w[i] * v[i].w : 0.f;
       }
     }
   }

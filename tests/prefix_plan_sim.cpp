@@ -1,5 +1,5 @@
 // Replays the plan of the prefix attention (qmk_prefix_plan.h) on the CPU: every (KV head, row, visible key) has to be
-// walked exactly once, by a block of a unit or by an item; every partial result has to have a record of its own inside the
+// walked exactly once, by a block of a unit or by a piece of a strip; every partial result has to have a record of its own inside the
 // workspace's bounds; and the records that a row's description names have to be the ones that were written for it.
 #include <cstdio>
 #include <cstdlib>
@@ -44,7 +44,7 @@ int main() {
     if (d.tokens < 1) d.tokens = 1;
 
     std::vector<Req> req;
-    std::vector<int> lb(1, 0), lu(1, 0), stk(1, 0), it(1, 0);
+    std::vector<int> lb(1, 0), lu(1, 0), stk(1, 0), pc(1, 0);
     Totals t{0, 0, 0, 0};
     for (int s = 0; s < d.seqs; ++s) {
       const Req r = request(d, cu[s], cu[s + 1], kv[s]);
@@ -56,20 +56,16 @@ int main() {
         t.long_units += units_of(d, r);
       } else {
         t.short_tokens += r.n;
-        t.item_keys += (long long)own_keys(d, r) * item_rows_blocks(d, r);
+        t.pieces += (long long)strips_of(d, r) * pieces_of(d, r);
       }
       lb.push_back((int)t.long_blocks);
       lu.push_back(t.long_units);
       stk.push_back(t.short_tokens);
+      pc.push_back((int)t.pieces);
     }
     const Plan p = make_plan(d, t);
-    long long per_head = 0;
-    for (int s = 0; s < d.seqs; ++s) {
-      if (!is_long(d, req[s])) per_head += (long long)item_rows_blocks(d, req[s]) * item_chunks(own_keys(d, req[s]), p.ck);
-      it.push_back((int)per_head);
-    }
-    const long long items = per_head * d.NKV;
-    CHECK(items <= max_items(d));
+    const long long pieces = t.pieces * d.NKV;
+    CHECK(p.share[0] + p.share[1] == pieces && p.share[0] >= 0 && p.share[1] >= 0);
     CHECK(p.unit_total <= max_units(d));
     CHECK(p.dense_ctas <= d.ctas && (p.dense_blocks == 0) == (p.dense_ctas == 0));
 
@@ -89,7 +85,10 @@ int main() {
     struct Named { int rec, n; };
     std::vector<Named> named((size_t)d.tokens * d.NKV, Named{-1, 0});
     std::vector<std::vector<int>> written((size_t)d.tokens * d.NKV);
-    long long walked = 0, at_item = 0;
+    long long walked = 0;
+    std::vector<char> strip_record((size_t)max_strip_records(d), 0), piece_done((size_t)pieces, 0);
+    std::vector<Named> strip_named((size_t)d.tokens * d.G * d.NKV, Named{-1, 0});
+    std::vector<std::vector<int>> strip_written((size_t)d.tokens * d.G * d.NKV);
     for (int c = 0; c < d.ctas; ++c) {
       long long lo, hi;
       dense_range(p, c, lo, hi);
@@ -150,30 +149,57 @@ int main() {
         }
         b += b1 - b0;
       }
-      long long ilo, ihi;
-      item_range(d, p, t, items, c, ilo, ihi);
-      CHECK(ilo == at_item && ihi >= ilo);
-      at_item = ihi;
-      for (long long item = ilo; item < ihi; ++item) {
-        int s = 0;
-        while (!((long long)it[s] * d.NKV <= item && item < (long long)it[s + 1] * d.NKV)) ++s;
-        CHECK(it[s] <= item / d.NKV && item / d.NKV < it[s + 1]);
-        const Req& r = req[s];
-        const int chunks = item_chunks(own_keys(d, r), p.ck);
-        long long rest = item - (long long)it[s] * d.NKV;
-        const int ch = (int)(rest % chunks);
-        rest /= chunks;
-        const int kvh = (int)(rest % d.NKV), rb = (int)(rest / d.NKV);
-        const int i0 = rb * d.item_tokens(), ni = imin(d.item_tokens(), r.n - i0);
-        CHECK(ni > 0 && ni * d.G <= kItemRows);
-        const int k_lo = d.prefix_len + ch * p.ck, k_hi = imin(k_lo + p.ck, limit_of(d, r, i0 + ni - 1));
-        for (int i = i0; i < i0 + ni; ++i) {
-          auto& seen = w.seen[(size_t)(r.first + i) * d.NKV + kvh];
-          for (int key = k_lo; key < k_hi && key < limit_of(d, r, i); ++key) ++seen[key];
+      for (int warp = 0; warp < kStripWarps; ++warp) {
+        long long flo, fhi;
+        const int number = piece_range(d, p, c, warp, flo, fhi);
+        CHECK((number < 0) == (flo == fhi));
+        for (long long f = flo; f < fhi;) {
+          int s = 0;
+          while (!((long long)pc[s] * d.NKV <= f && f < (long long)pc[s + 1] * d.NKV)) ++s;
+          CHECK(pc[s] <= f / d.NKV && f / d.NKV < pc[s + 1]);
+          const Req& r = req[s];
+          const int per = pieces_of(d, r);
+          long long rest = f - (long long)pc[s] * d.NKV;
+          const int c0 = (int)(rest % per), n = (int)(per - c0 < fhi - f ? per - c0 : fhi - f);
+          rest /= per;
+          const int kvh = (int)(rest % d.NKV), strip = (int)(rest / d.NKV);
+          const int rec = number + strip_number(d, s, stk[s], strip, kvh);
+          CHECK(rec < max_strip_records(d) && !strip_record[rec]);
+          strip_record[rec] = 1;
+          for (long long k = f; k < f + n; ++k) { CHECK(!piece_done[k]); piece_done[k] = 1; CHECK(piece_owner(p, k) == number); }
+          const int row0 = strip * kStripRows, rows = imin(kStripRows, r.n * d.G - row0);
+          CHECK(rows > 0);
+          const int last = limit_of(d, r, (row0 + rows - 1) / d.G);
+          const int k_lo = d.prefix_len + c0 * kPieceKeys, k_hi = imin(d.prefix_len + (c0 + n) * kPieceKeys, last);
+          for (int i = 0; i < rows; ++i) {
+            const int tok = r.first + (row0 + i) / d.G, gq = (row0 + i) % d.G, lim = limit_of(d, r, (row0 + i) / d.G);
+            CHECK(lim <= last);
+            const size_t at = ((size_t)tok * d.NKV + kvh) * d.G + gq;
+            if (gq == 0) {                                    // (heads of a token see the same keys)
+              auto& seen = w.seen[(size_t)tok * d.NKV + kvh];
+              for (int key = k_lo; key < k_hi && key < lim; ++key) ++seen[key];
+            }
+            if (c0 == 0) strip_named[at] = Named{rec, piece_owner(p, f + per - 1) - number + 1};
+            strip_written[at].push_back(rec);
+          }
+          f += n;
         }
       }
     }
-    CHECK(walked == p.dense_blocks && at_item == items);
+    for (char x : piece_done) CHECK(x);
+    for (int tok = 0; tok < d.tokens; ++tok) {
+      if (owner[tok] < 0 || is_long(d, req[owner[tok]])) continue;
+      for (int h = 0; h < d.NKV * d.G; ++h) {
+        const size_t at = (size_t)tok * d.NKV * d.G + h;
+        std::vector<int>& v = strip_written[at];
+        for (size_t a = 0; a < v.size(); ++a)                  // (warps are visited CTA by CTA, not in their order)
+          for (size_t b2 = a + 1; b2 < v.size(); ++b2)
+            if (v[b2] < v[a]) { const int x = v[a]; v[a] = v[b2]; v[b2] = x; }
+        CHECK((int)v.size() == strip_named[at].n);
+        for (int k = 0; k < strip_named[at].n; ++k) CHECK(v[k] == strip_named[at].rec + k);
+      }
+    }
+    CHECK(walked == p.dense_blocks);
     for (int tok = 0; tok < d.tokens; ++tok)
       for (int h = 0; h < d.NKV; ++h) {
         const size_t i = (size_t)tok * d.NKV + h;
