@@ -125,6 +125,13 @@ static WorkspaceLayout workspace_layout(const PlanDims& d, int head_dim) {
   return w;
 }
 
+// The device counts blocks, pieces and records in 32 bits.
+static bool counts_fit(const PlanDims& d) {
+  const long long most = 0x7fffffffll, strips = max_strips(d), by_request = (long long)d.seqs * (kLongRows / kStripRows) * d.NKV;
+  return max_units(d) * d.NKV * (d.room / kBlockKeys + 1) <= most && max_strip_records(d) <= most &&
+         (strips < by_request ? strips : by_request) * (d.room / kPieceKeys + 1) <= most;
+}
+
 static bool attention_sizes_ok(int tokens, int seqs, int num_heads, int num_kv_heads, int head_dim, int prefix_len) {
   return tokens >= 1 && tokens <= (1 << 20) && seqs >= 1 && seqs <= kMaxSeqs && (head_dim == 64 || head_dim == 128) &&
          num_kv_heads >= 1 && num_heads >= 1 && num_heads <= 1024 && num_heads % num_kv_heads == 0 &&
@@ -228,9 +235,7 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
   p.d = plan_dims(a->tokens, a->seqs, a->num_heads, a->num_kv_heads, a->prefix_len, ctas);
   const long long room = (long long)a->max_pages * a->page_size;
   p.d.room = (int)(room > a->prefix_len ? room : a->prefix_len);
-  // 32-bit counts on the device: blocks and pieces of a KV head, records
-  if (max_units(p.d) * (p.d.room / kBlockKeys + 1) > 0x7fffffffll || max_strip_records(p.d) > 0x7fffffffll ||
-      max_strips(p.d) / p.d.NKV * (p.d.room / kPieceKeys + 1) > 0x7fffffffll) return QMK_ERR_INVALID_ARG;
+  if (!counts_fit(p.d)) return QMK_ERR_INVALID_ARG;
   const WorkspaceLayout w = workspace_layout(p.d, a->head_dim);
   if (a->workspace_bytes < w.total) return QMK_ERR_INVALID_ARG;
   p.q = (const uint16_t*)a->q; p.out = (uint16_t*)a->out; p.lse = a->lse;

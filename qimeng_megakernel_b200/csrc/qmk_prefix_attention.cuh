@@ -4,21 +4,21 @@
 //   o = sum_{j < lim} softmax_j(scale * q . k_j) v_j,    lse = log sum_{j < lim} exp(scale * q . k_j)
 //   position j lies in page prefix_table[j / page] for j < prefix_len and in block_tables[s][j / page] behind it
 //
-// One persistent CTA per SM works through its share of the plan (qmk_prefix_plan.h) in two parts.
+// One persistent CTA per SM works through its share of the plan (qmk_prefix_plan.h): blocks or strips.
 //
 // Blocks.  Up to 256 rows against 128 keys at a time with tcgen05.mma, in the manner of a running softmax: S = Q K^T into
-// tensor memory, a group of four warps (one thread per row) turns S into P = exp2(S - m), rounded to bf16 and put over S, and
-// O += P V.  Two groups alternate, so that the tensor pipe works for one while the other does its exponentials: each has
-// a tile of 128 rows, or, where a unit has only one tile, they share it and take alternate blocks.  m is raised (and O
-// rescaled) only when a row's maximum grows by more than 2^8; P then stays below 2^8, which costs no accuracy.
-// A group works in steps of 64 keys with two buffers for S, so that its next scores are there when it has written a P.
+// tensor memory, softmax warps (one thread per row) turn S into P = exp2(S - m), rounded to bf16 and put over S, and O += P V.
+// Two groups alternate, so that the tensor pipe works for one while the other does its exponentials: each has a tile of 128
+// rows, or, where a unit has only one tile, they share it and take alternate blocks.  A group works in steps of 64 keys with
+// two buffers for S, so that its next scores are there when it has written a P.  m is the row's first maximum and is raised
+// (and O rescaled) only when a step's sum of exponentials passes 2^40: P keeps bf16's relative precision up to there, and a
+// step looks for no maximum.
 //   tensor memory: S (2 groups x 2 buffers x 64 columns, P over S), O0 | O1 (HD columns each)
 //   warps 0-3, 4-7 softmax groups; 8 and 11 load K and V blocks (one TMA box per page and 64 dimensions); 9 and 10 issue the
 //   products of a group each
 //
 // Strips.  What a short request holds behind the prefix: 8 rows x a run of 32-key pieces per warp, on mma.sync with the keys
-// (for P V the dimensions) as the long side of the tile, K and V through a ring of the warp's own in shared memory (the ring of
-// the blocks, free by then).
+// (for P V the dimensions) as the long side of the tile, K and V through a ring of the warp's own in shared memory.
 //
 // Both parts leave partial results (m, l, unnormalised O, all in 32 bits) unless a row is complete; merge_kernel adds them
 // up in a fixed order, so a call gives the same bits every time.  Nothing is kept between calls.
@@ -61,7 +61,7 @@ struct AttnMaps {
 };
 
 constexpr int kAttnThreads = 384;
-constexpr int kKeyWarp = 8, kIssueWarp = 9, kValueWarp = 11;   // (warps 9 and 10 issue, one for each group)
+constexpr int kSoftmaxWarps = 8, kKeyWarp = 8, kIssueWarp = 9, kValueWarp = 11;   // (9 and 10 issue, one for each group)
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 constexpr int kPolyEvery = 4;                        // one pair of exponentials in so many goes to the multiply-add pipe
@@ -84,9 +84,9 @@ struct AttnSmem {
   static constexpr int kDenseBars = 4 * kStages + 15;
   static constexpr int kNumBars = kDenseBars + kStripWarps * kStripStages;
   static constexpr int kOffCtl = kOffBars + kNumBars * 8;       // words: 0 abort, 1 tensor memory base
-  static constexpr int kOffRed = (kOffCtl + 16 + 7) / 8 * 8;    // long long [4][16] scratch of the scans
-  static constexpr int kOffTot = kOffRed + 4 * 16 * 8;          // Totals, Plan
-  static constexpr int kOffScan = (kOffTot + 128 + 15) / 16 * 16;   // int [4][seqs + 1]
+  static constexpr int kOffRed = (kOffCtl + 16 + 15) / 16 * 16;   // int4 [12] scratch of the scan
+  static constexpr int kOffWork = kOffRed + kAttnThreads / 32 * 16;   // Work
+  static constexpr int kOffScan = (kOffWork + 128 + 15) / 16 * 16;   // int [4][seqs + 1]
   static __host__ __device__ constexpr int total(int seqs) { return kOffScan + 4 * (seqs + 1) * 4; }
 };
 
@@ -261,75 +261,63 @@ __device__ __forceinline__ int find_last(const int* a, int n, int v) {
   }
   return lo;
 }
-// Exclusive prefix sums of up to four values over the CTA's threads; the totals come back too.
-template <int N>
-__device__ __forceinline__ void scan_values(long long (&v)[N], long long (&total)[N], long long* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int W = kAttnThreads / 32;
-  long long incl[N];
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    long long x = v[k];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(kFullMask, x, o);
-      if (lane >= o) x += u;
-    }
-    incl[k] = x;
-    if (lane == 31) red[k * 16 + warp] = x;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    long long before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const long long x = red[k * 16 + w];
-      before += w < warp ? x : 0;
-      all += x;
-    }
-    v[k] = before + incl[k] - v[k];
-    total[k] = all;
-  }
-  __syncthreads();
-}
 struct Work {                  // in shared memory
   Totals t;
   Plan plan;
 };
-__device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc, long long* red, Work* out) {
-  const int seqs = p.d.seqs;
-  long long base[4] = {0, 0, 0, 0};
+// Prefix sums of the requests' numbers and the plan.  One pass takes as many requests as the CTA has threads; only warps that
+// have some take part in the sums.
+__device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc, int4* red, Work* out) {
+  const int seqs = p.d.seqs, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int4 base = make_int4(0, 0, 0, 0);
   for (int s0 = 0; s0 < seqs; s0 += kAttnThreads) {
     const int s = s0 + (int)threadIdx.x;
-    long long v[4] = {0, 0, 0, 0}, tot[4];
-    if (s < seqs) {
-      const Req r = load_request(p, s);
-      if (is_long(p.d, r)) {
-        const int n = units_of(p.d, r);
-        for (int u = 0; u < n; ++u) v[0] += unit_blocks(p.d, r, u);
-        v[1] = n;
-      } else {
-        v[2] = r.n;
-        v[3] = (long long)strips_of(p.d, r) * pieces_of(p.d, r);
+    const int warps = (min(seqs - s0, kAttnThreads) + 31) / 32;
+    int4 v = make_int4(0, 0, 0, 0), x;
+    if (warp < warps) {
+      if (s < seqs) {
+        const Req r = load_request(p, s);
+        if (is_long(p.d, r)) {
+          const int n = units_of(p.d, r);
+          for (int u = 0; u < n; ++u) v.x += unit_blocks(p.d, r, u);
+          v.y = n;
+        } else {
+          v.z = r.n;
+          v.w = strips_of(p.d, r) * pieces_of(p.d, r);
+        }
+      }
+      x = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(kFullMask, x.x, o), b = __shfl_up_sync(kFullMask, x.y, o);
+        const int c = __shfl_up_sync(kFullMask, x.z, o), d = __shfl_up_sync(kFullMask, x.w, o);
+        if (lane >= o) { x.x += a; x.y += b; x.z += c; x.w += d; }
+      }
+      if (lane == 31) red[warp] = x;
+    }
+    __syncthreads();
+    if (warp < warps) {
+      int4 at = base;
+      for (int w = 0; w < warps; ++w) {
+        const int4 y = red[w];
+        if (w < warp) { at.x += y.x; at.y += y.y; at.z += y.z; at.w += y.w; }
+        base.x += y.x; base.y += y.y; base.z += y.z; base.w += y.w;
+      }
+      if (s < seqs) {
+        sc.long_blocks[s] = at.x + x.x - v.x;
+        sc.long_units[s] = at.y + x.y - v.y;
+        sc.short_tokens[s] = at.z + x.z - v.z;
+        sc.pieces[s] = at.w + x.w - v.w;
       }
     }
-    scan_values<4>(v, tot, red);
-    if (s < seqs) {
-      sc.long_blocks[s] = (int)(base[0] + v[0]);
-      sc.long_units[s] = (int)(base[1] + v[1]);
-      sc.short_tokens[s] = (int)(base[2] + v[2]);
-      sc.pieces[s] = (int)(base[3] + v[3]);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) base[k] += tot[k];
+    if (s0 + kAttnThreads < seqs) __syncthreads();           // (the scratch is written again)
   }
-  if (threadIdx.x == 0) {
-    sc.long_blocks[seqs] = (int)base[0];
-    sc.long_units[seqs] = (int)base[1];
-    sc.short_tokens[seqs] = (int)base[2];
-    sc.pieces[seqs] = (int)base[3];
-    out->t = Totals{base[0], (int)base[1], (int)base[2], base[3]};
+  if (threadIdx.x == 0) {                                    // (its warp has taken part in every pass)
+    sc.long_blocks[seqs] = base.x;
+    sc.long_units[seqs] = base.y;
+    sc.short_tokens[seqs] = base.z;
+    sc.pieces[seqs] = base.w;
+    out->t = Totals{base.x, base.y, base.z, base.w};
     out->plan = make_plan(p.d, out->t);
   }
   __syncthreads();
@@ -343,13 +331,13 @@ struct Unit {
   int rows;             // packed rows that exist
   Req r;
 };
-__device__ __forceinline__ Unit unit_at(const AttnParams& p, const Scans& sc, const Totals& t, const Plan& plan, long long b,
+__device__ __forceinline__ Unit unit_at(const AttnParams& p, const Scans& sc, const Totals& t, const Plan& plan, int b,
                                         int& block) {
   Unit x;
-  x.kvh = (int)(b / plan.blocks);
-  long long rest = b - (long long)x.kvh * plan.blocks;
+  x.kvh = b / plan.blocks;
+  int rest = b - x.kvh * plan.blocks;
   if (rest < t.long_blocks) {
-    int lo = find_last(sc.long_blocks, p.d.seqs, (int)rest);
+    int lo = find_last(sc.long_blocks, p.d.seqs, rest);
     rest -= sc.long_blocks[lo];
     x.s = lo;
     x.r = load_request(p, lo);
@@ -366,14 +354,14 @@ __device__ __forceinline__ Unit unit_at(const AttnParams& p, const Scans& sc, co
     rest -= t.long_blocks;
     x.s = -1;
     x.blocks = p.d.prefix_blocks();
-    x.u = (int)(rest / x.blocks);
-    rest -= (long long)x.u * x.blocks;
+    x.u = rest / x.blocks;
+    rest -= x.u * x.blocks;
     x.index = t.long_units + x.u;
     x.limit = p.d.prefix_len;
     x.rows = min(p.d.unit_tokens(), t.short_tokens - x.u * p.d.unit_tokens()) * p.d.G;
     x.r = Req{0, 0, 0};
   }
-  block = (int)rest;
+  block = rest;
   return x;
 }
 // The row `row` of a unit: token (-1: none) and the keys it sees of the unit's.
@@ -406,7 +394,7 @@ struct Dense {
   Scans sc;
   const Totals& t;             // (in shared memory: read where they are needed, not held in registers)
   const Plan& plan;
-  long long lo, hi;            // blocks of this CTA
+  int lo, hi;                  // blocks of this CTA
   uint32_t tmem;
   int warp, lane;
 
@@ -447,10 +435,10 @@ struct Dense {
     const int oob = p.num_pages << p.page_shift;             // behind the last row: reads as zeros
     const uint32_t dst = base + (kV ? S::kOffV : S::kOffK) + (uint32_t)(half * kBlockKeys * 128 + key_of_lane * 128);
     unsigned n = 0;
-    for (long long b = lo; b < hi;) {
+    for (int b = lo; b < hi;) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
-      const int b1 = (int)min((long long)x.blocks, b0 + (hi - b));
+      const int b1 = min(x.blocks, b0 + (hi - b));
       auto row_of = [&](int blk) {                           // row of the pool that this lane's box starts at, -1: no box
         const int key = blk * kBlockKeys + key_of_lane;
         if (lane >= boxes || key >= x.limit) return -1;
@@ -496,10 +484,10 @@ struct Dense {
     const uint64_t kd0 = desc_k_major(base + S::kOffK), vd0 = desc_n_major(base + S::kOffV, 16384u);
     const uint32_t sd = tmem + (uint32_t)g * 128u, od = tmem + 256u + (uint32_t)g * 128u;
     unsigned n = 0, segs = 0, p_par = 0;                     // (p_par: parity of the next P, both halves)
-    for (long long b = lo; b < hi;) {
+    for (int b = lo; b < hi;) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
-      const int nb = (int)min((long long)(x.blocks - b0), hi - b);
+      const int nb = min(x.blocks - b0, hi - b);
       const bool dual = x.rows <= 128;
       const uint64_t qd = desc_k_major(base + S::kOffQ + (dual ? 0 : g) * S::kTileBytes);
       const int step = dual ? 2 : 1;
@@ -594,10 +582,10 @@ struct Dense {
     const uint32_t s_col = tmem + g * 128 + lane_base, o_col = tmem + 256 + g * 128 + lane_base;
     unsigned s_par = 0;                                      // parity of the next S, both halves
     unsigned n = 0, clears = 0, o_par = 0;
-    for (long long b = lo; b < hi;) {
+    for (int b = lo; b < hi;) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
-      const int nb = (int)min((long long)(x.blocks - b0), hi - b);
+      const int nb = min(x.blocks - b0, hi - b);
       const bool dual = x.rows <= 128;
       // Q: thread `row` brings row `row` of the unit (with one tile the second group's threads have nothing to bring)
       int lim;
@@ -636,50 +624,57 @@ struct Dense {
           tmem_ld32(s + 32, sh + 32);
           tmem_wait_ld();
           const int k0 = (b0 + block_of(j, dual, g)) * kBlockKeys + 64 * half;
-          const bool plain = k0 + 64 <= warp_lim;
-          if (!plain) {
-            const int vis = lim - k0;
-#pragma unroll
-            for (int c = 0; c < 64; ++c) s[c] = c < vis ? s[c] : -INFINITY;
-          }
           const f32x2 scale2 = pair(p.scale_log2e, p.scale_log2e);
-          f32x2 sum2[2];
+          float sum, most;
           uint32_t pk[32];
-          // 2^(scale s - m) of the row, packed, and their sum
+          // 2^(scale s - m) of the row, packed, and their sum.  One pair in kPolyEvery goes to the multiply-add pipe; the
+          // largest exponent of those is noted, the others say themselves when they are too large.
           auto exps = [&](auto with_poly) {
             const float off = m == -INFINITY ? 0.f : m;
             const f32x2 off2 = pair(-off, -off);
-            sum2[0] = sum2[1] = 0ull;
+            f32x2 sum2[2] = {0ull, 0ull};
+            most = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const f32x2 e = fma2(pair(s[2 * i], s[2 * i + 1]), scale2, off2);
               float a, d;
+              unpair(e, a, d);
               if (decltype(with_poly)::value && i % kPolyEvery == kPolyEvery - 1) {
+                most = max3(most, a, d);
                 ex2_pair(e, a, d);
               } else {
-                unpair(e, a, d);
                 a = ex2(a);
                 d = ex2(d);
               }
               sum2[i & 1] = add2(sum2[i & 1], pair(a, d));
               pk[i] = pack2(a, d);
             }
+            float a, d;
+            unpair(add2(sum2[0], sum2[1]), a, d);
+            sum = a + d;
           };
-          // The row's maximum is worked out beside the exponentials, which take the m there is (it rarely has to rise); the
-          // polynomial has no zero: rows with hidden keys, or with nothing seen yet, go without it.
-          float mx[4] = {s[0], s[1], s[2], s[3]};
+          bool done = false;
+          const bool plain = k0 + 64 <= warp_lim;
+          if (plain && seen) {
+            exps(Yes{});
+            done = __all_sync(kFullMask, sum <= 1099511627776.f && most <= 40.f);
+          }
+          if (!done) {                                  // the first step, hidden keys, a score far above m, or a NaN
+            if (!plain) {
+              const int vis = lim - k0;
 #pragma unroll
-          for (int i = 4; i + 8 <= 64; i += 8)
+              for (int c = 0; c < 64; ++c) s[c] = c < vis ? s[c] : -INFINITY;
+            }
+            float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], s[i + c], s[i + 4 + c]);
+            for (int i = 4; i + 8 <= 64; i += 8)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[60 + c]);
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2e;
-          if (plain && seen) exps(Yes{});
-          // (NaN scores: the maximum passes them over, their own exponential keeps them)
-          const bool raise = __any_sync(kFullMask, top > m + 8.f);
-          if (raise || !(plain && seen)) {
-            if (raise) {
+              for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], s[i + c], s[i + 4 + c]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[60 + c]);
+            // (NaN scores: the maximum passes them over, their own exponential keeps them)
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2e;
+            if (__any_sync(kFullMask, top > m)) {
               const float m_new = fmaxf(m, top);
               if (j > 0) {
                 // O may be touched once P V of step j - 1 is through: the scores of step j + 1 were issued behind it
@@ -703,10 +698,8 @@ struct Dense {
             }
             exps(No{});
           }
+          l += sum;
           tmem_st32(sh, pk);
-          float sa, sb;
-          unpair(add2(sum2[0], sum2[1]), sa, sb);
-          l += sa + sb;
           tmem_wait_st();
         }
         if (half == 0 && (warp & 3) == 0) {
@@ -781,7 +774,7 @@ struct Dense {
         if (b0 == 0 && token >= 0 && tile_row % p.d.G == 0 && !(dual && g == 1)) {
           const size_t at = (size_t)token * p.d.NKV + x.kvh;
           int parts = 0;
-          if (!whole) parts = dense_owner(plan, b + x.blocks - 1) - cta + 1;
+          if (!whole) parts = plan.dense.owner(b + x.blocks - 1) - cta + 1;
           p.dense_desc[at] = make_int2(rec, parts | (dual ? 1 << 15 : 0) | (tile_row << 16));
           if (x.s >= 0)
             for (int i = 0; i < p.d.G; ++i) p.strip_desc[(size_t)token * p.NH + head + i] = make_int2(0, 0);
@@ -808,16 +801,15 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
   const int g = lane >> 2, t4 = lane & 3;
   const int oob = p.num_pages << p.page_shift;
   unsigned filled = 0;                                      // stages filled by this warp so far
-  long long lo, hi;
+  int lo, hi;
   const int number = piece_range(p.d, plan, (int)blockIdx.x, warp, lo, hi);
-  for (long long f = lo; f < hi;) {
-    const int s = find_last(sc.pieces, p.d.seqs, (int)(f / p.d.NKV));
+  for (int f = lo; f < hi;) {
+    const int s = find_last(sc.pieces, p.d.seqs, f / p.d.NKV);
     const Req r = load_request(p, s);
     const int per = pieces_of(p.d, r);
-    long long rest = f - (long long)sc.pieces[s] * p.d.NKV;
-    const int c0 = (int)(rest % per), n = (int)min((long long)(per - c0), hi - f);
-    rest /= per;
-    const int kvh = (int)(rest % p.d.NKV), strip = (int)(rest / p.d.NKV);
+    const int rest = f - sc.pieces[s] * p.d.NKV, column = rest / per;
+    const int c0 = rest - column * per, n = min(per - c0, hi - f);
+    const int strip = column / p.d.NKV, kvh = column - strip * p.d.NKV;
     const int base_row = strip * kStripRows, rows = min(kStripRows, r.n * p.d.G - base_row);
     const int k_lo = p.d.prefix_len + c0 * kPieceKeys;
     const int k_hi = max(k_lo, min(k_lo + n * kPieceKeys, limit_of(p.d, r, (base_row + rows - 1) / p.d.G)));
@@ -997,7 +989,7 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
         if (g == 0) p.strip_ml[(size_t)rec * kStripRows + row] = make_float2(m, l);
       }
       if (c0 == 0 && g == 0) {                              // whoever starts the strip says where its rows' parts are
-        const int parts = whole ? 0 : piece_owner(plan, f + per - 1) - number + 1;
+        const int parts = whole ? 0 : plan.strips.owner(f + per - 1) - number + 1;
         p.strip_desc[(size_t)token * p.NH + head] = make_int2(rec, parts | (row << 16));
         if (p.d.prefix_len == 0 && gq == 0) p.dense_desc[(size_t)token * p.d.NKV + kvh] = make_int2(0, 0);
       }
@@ -1020,63 +1012,59 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
   sc.long_units = sc.long_blocks + p.d.seqs + 1;
   sc.short_tokens = sc.long_units + p.d.seqs + 1;
   sc.pieces = sc.short_tokens + p.d.seqs + 1;
-  Work* work = reinterpret_cast<Work*>(smem + S::kOffTot);
+  Work* work = reinterpret_cast<Work*>(smem + S::kOffWork);
   Dense<HD> w{p, maps, smem, smem_u32(smem), ctl, sc, work->t, work->plan, 0, 0, 0u, warp, lane};
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(w.k_full(s), 1);
-      mbar_init(w.k_empty(s), 2);
-      mbar_init(w.v_full(s), 1);
-      mbar_init(w.v_empty(s), 2);
+  if (warp == kKeyWarp) {
+    if (lane < 4) {
+      const CUtensorMap* m = lane == 0 ? &maps.k : (lane == 1 ? &maps.v : (lane == 2 ? &maps.k16 : &maps.v16));
+      asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
     }
-    for (int g = 0; g < 2; ++g) {
-      for (int h = 0; h < 2; ++h) {
-        mbar_init(w.s_full(g, h), 1);
-        mbar_init(w.p_full(g, h), 128);
-        mbar_init(w.o_full(g, h), 1);
-      }
-      mbar_init(w.q_full(g), 256);
+    // barriers: arrivals they wait for
+    for (int i = lane; i < S::kNumBars; i += 32) {
+      int count = 1;
+      const int r = i - 4 * S::kStages;
+      if (r < 0) count = (i / S::kStages) & 1 ? 2 : 1;       // full: the copy's bytes; empty: both groups
+      else if (r >= 4 && r < 8) count = 128;                 // p_full: a group's four warps
+      else if (r == 12 || r == 13) count = 256;              // q_full: all softmax warps
+      mbar_init(w.bar(i), count);
     }
-    mbar_init(w.v_clear(), 1);
-    for (int i = 0; i < kStripWarps * S::kStripStages; ++i) mbar_init(w.bar(S::kDenseBars + i), 1);
+    if (lane == 0) ctl[0] = 0u;
     fence_barrier_init();
-    ctl[0] = 0u;
   }
-  build_plan(p, sc, reinterpret_cast<long long*>(smem + S::kOffRed), work);
+  build_plan(p, sc, reinterpret_cast<int4*>(smem + S::kOffRed), work);
+  if ((int)blockIdx.x >= work->plan.dense_ctas) {
+    if (warp < kStripWarps) walk_strips<HD>(p, maps, smem, ctl, sc, work->plan, warp, lane);
+    return;
+  }
   dense_range(work->plan, (int)blockIdx.x, w.lo, w.hi);
-  if (w.lo < w.hi) {
-    if (warp == kIssueWarp) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(w.base + S::kOffCtl + 4) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-      tmem_fence_before_sync();
-    }
-    __syncthreads();
-    tmem_fence_after_sync();
-    w.tmem = ctl[1];
-    if (warp < kStripWarps) {
-      w.softmax();
-    } else if (warp == kKeyWarp) {
-      const unsigned n = w.template produce<false>();
-      __syncwarp();
-      if (ctl[0] != 0u) w.template drain<false>(n);
-    } else if (warp == kValueWarp) {
-      const unsigned n = w.template produce<true>();
-      __syncwarp();
-      if (ctl[0] != 0u) w.template drain<true>(n);
-    } else {
-      if (elect_one()) w.issue(warp - kIssueWarp);
-    }
-    __syncwarp();
+  if (warp == kIssueWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(w.base + S::kOffCtl + 4) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     tmem_fence_before_sync();
-    __syncthreads();
-    if (warp == kIssueWarp) {
-      tmem_fence_after_sync();
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(w.tmem) : "memory");
-    }
-    fence_async_shared();                                    // (the ring's generic writes, before copies land in it again)
-    __syncthreads();
   }
-  if (warp < kStripWarps) walk_strips<HD>(p, maps, smem, ctl, sc, work->plan, warp, lane);
+  __syncthreads();
+  tmem_fence_after_sync();
+  w.tmem = ctl[1];
+  if (warp < kSoftmaxWarps) {
+    w.softmax();
+  } else if (warp == kKeyWarp) {
+    const unsigned n = w.template produce<false>();
+    __syncwarp();
+    if (ctl[0] != 0u) w.template drain<false>(n);
+  } else if (warp == kValueWarp) {
+    const unsigned n = w.template produce<true>();
+    __syncwarp();
+    if (ctl[0] != 0u) w.template drain<true>(n);
+  } else {
+    if (elect_one()) w.issue(warp - kIssueWarp);
+  }
+  __syncwarp();
+  tmem_fence_before_sync();
+  __syncthreads();
+  if (warp == kIssueWarp) {
+    tmem_fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(w.tmem) : "memory");
+  }
 }
 
 // Adds a row's parts: one warp per (token, query head).  With M = max m_r and w_r = 2^(m_r - M):

@@ -7,8 +7,8 @@
 //   short  (fewer rows: decoding, verification)  their tokens are strung together and cut into units of 256 rows, which
 //          walk the shared prefix; what each request holds behind the prefix is walked by single warps, 8 rows at a time: a
 //          STRIP is (request, 8 of its rows, KV head), cut into pieces of 32 keys
-// The 128-key blocks of all (KV head, unit) pairs, in that order, are dealt to `dense_ctas` CTAs as equal contiguous ranges;
-// the pieces of all strips to warps, so that a CTA's blocks and pieces together come out even.  Every (CTA, unit) and every
+// The 128-key blocks of all (KV head, unit) pairs, in that order, are dealt to the first CTAs as equal contiguous ranges, the
+// pieces of all strips to the warps of the other CTAs, as many CTAs to either as its share of the work.  Every (CTA, unit) and every
 // (warp, strip) that meet leave a partial result: record number (CTA + unit) or (warp + strip), which no other pair has.
 #pragma once
 #include <stdint.h>
@@ -28,7 +28,8 @@ constexpr int kStripRows = 8;       // rows of a strip (the short side of an mma
 constexpr int kMaxGroup = 16;       // query heads of a KV head
 constexpr int kPieceKeys = 32;      // keys of a piece
 constexpr int kStripWarps = 8;      // warps of a CTA that walk strips
-constexpr int kMaxSeqs = 2048;      // requests of a call (their prefix sums are kept in shared memory)
+constexpr int kBlockCost = 8;       // time of a block of 256 rows in pieces (a CTA's eight warps at one each)
+constexpr int kMaxSeqs = 1536;      // requests of a call (their prefix sums are kept in shared memory)
 
 struct PlanDims {
   int tokens, seqs, G, NKV, prefix_len, ctas;
@@ -70,69 +71,75 @@ QMKP_HD int own_keys(const PlanDims& d, const Req& r) { return r.n > 0 ? imax(0,
 QMKP_HD int strips_of(const PlanDims& d, const Req& r) { return (r.n * d.G + kStripRows - 1) / kStripRows; }   // of a KV head
 QMKP_HD int pieces_of(const PlanDims& d, const Req& r) { return imax(1, (own_keys(d, r) + kPieceKeys - 1) / kPieceKeys); }
 
+// `total` things dealt to n takers as contiguous ranges that differ by one at most (with fewer things than takers the first
+// ones get one each, so owners of neighbouring things are always neighbours).
+struct Deal {
+  int n, each, more;                // the first `more` takers get each + 1
+  QMKP_HD int first(int i) const { return each * i + imin(i, more); }
+  QMKP_HD int owner(int b) const {
+    const int head = more * (each + 1);
+    return b < head ? b / (each + 1) : more + (b - head) / each;
+  }
+};
+QMKP_HD Deal deal(int total, int n) {
+  Deal d;
+  d.n = n;
+  d.each = n > 0 ? total / n : 0;
+  d.more = n > 0 ? total - d.each * n : 0;
+  return d;
+}
+
+// (The entry point refuses sizes whose totals do not fit 32 bits.)
 struct Totals {
-  long long long_blocks;            // blocks of all long units (per KV head)
+  int long_blocks;                  // blocks of all long units (per KV head)
   int long_units;
   int short_tokens;
-  long long pieces;                 // pieces of all short requests (per KV head)
+  int pieces;                       // pieces of all short requests (per KV head)
 };
 
 struct Plan {
-  int short_units, unit_total;      // units per KV head
-  long long blocks;                 // per KV head
-  long long dense_blocks;           // all KV heads
-  int dense_ctas;
-  // pieces: warps of the CTAs with blocks (class 0) and of those without (class 1); warps and pieces of a class
-  int warps[2];
-  long long share[2];
+  int unit_total;                   // units per KV head
+  int blocks;                       // per KV head
+  int dense_ctas;                   // CTAs with blocks; the others have pieces
+  Deal dense, strips;               // all blocks to CTAs, all pieces to warps
 };
 constexpr int kMinSegment = 2;      // blocks a CTA takes at least
 
 QMKP_HD Plan make_plan(const PlanDims& d, const Totals& t) {
   Plan p;
-  p.short_units = d.prefix_len > 0 ? (t.short_tokens + d.unit_tokens() - 1) / d.unit_tokens() : 0;
-  p.unit_total = t.long_units + p.short_units;
-  p.blocks = t.long_blocks + (long long)p.short_units * d.prefix_blocks();
-  p.dense_blocks = p.blocks * d.NKV;
-  const long long want = (p.dense_blocks + kMinSegment - 1) / kMinSegment;
-  p.dense_ctas = want < d.ctas ? (int)want : d.ctas;
-  // a block counts as four pieces (its keys)
-  const long long all = t.pieces * d.NKV, load = p.dense_blocks * (kBlockKeys / kPieceKeys);
-  const long long even = (load + all) / d.ctas, mine = p.dense_ctas > 0 ? load / p.dense_ctas : 0;
-  const long long left = even > mine ? (even - mine) * p.dense_ctas : 0;       // room beside the blocks
-  p.share[0] = p.dense_ctas == d.ctas ? all : (left < all ? left : all);
-  p.share[1] = all - p.share[0];
-  for (int c = 0; c < 2; ++c) {
-    const long long w = (long long)kStripWarps * (c == 0 ? p.dense_ctas : d.ctas - p.dense_ctas);
-    p.warps[c] = (int)(w < p.share[c] ? w : p.share[c]);
-  }
+  const int short_units = d.prefix_len > 0 ? (t.short_tokens + d.unit_tokens() - 1) / d.unit_tokens() : 0;
+  p.unit_total = t.long_units + short_units;
+  const int short_blocks = short_units * d.prefix_blocks();
+  p.blocks = t.long_blocks + short_blocks;
+  const int all = p.blocks * d.NKV, pieces = t.pieces * d.NKV;
+  // a block of two tiles counts as kBlockCost pieces, one of a single tile as four (its keys)
+  const bool small = t.short_tokens * d.G <= kLongRows;
+  const float dense = ((float)t.long_blocks * kBlockCost + (float)short_blocks * (small ? 4 : kBlockCost)) * (float)d.NKV;
+  int ctas = pieces == 0 ? d.ctas : (int)((float)d.ctas * (dense / (dense + (float)pieces)) + 0.5f);
+  ctas = imin(imax(ctas, 1), pieces == 0 ? d.ctas : d.ctas - 1);
+  ctas = imin(ctas, (all + kMinSegment - 1) / kMinSegment);
+  p.dense_ctas = ctas;
+  p.dense = deal(all, ctas);
+  p.strips = deal(pieces, (d.ctas - ctas) * kStripWarps);
   return p;
 }
 // Blocks [lo, hi) of CTA c.
-QMKP_HD void dense_range(const Plan& p, int c, long long& lo, long long& hi) {
-  if (c >= p.dense_ctas) { lo = hi = 0; return; }
-  lo = p.dense_blocks * c / p.dense_ctas;
-  hi = p.dense_blocks * (c + 1) / p.dense_ctas;
-}
-QMKP_HD int dense_owner(const Plan& p, long long b) { return (int)(((b + 1) * p.dense_ctas - 1) / p.dense_blocks); }
-
-// Pieces [lo, hi) of a warp of CTA c, and the warp's number among all that have any (-1: none).  Neighbouring numbers are
-// neighbouring CTAs.
-QMKP_HD int piece_range(const PlanDims& d, const Plan& p, int c, int warp, long long& lo, long long& hi) {
-  const int k = c < p.dense_ctas ? 0 : 1;
-  const int i = k == 0 ? warp * p.dense_ctas + c : warp * (d.ctas - p.dense_ctas) + c - p.dense_ctas;
+QMKP_HD void dense_range(const Plan& p, int c, int& lo, int& hi) {
   lo = hi = 0;
-  if (i >= p.warps[k]) return -1;
-  const long long from = k == 0 ? 0 : p.share[0];
-  lo = from + p.share[k] * i / p.warps[k];
-  hi = from + p.share[k] * (i + 1) / p.warps[k];
-  return (k == 0 ? 0 : p.warps[0]) + i;
+  if (c >= p.dense_ctas) return;
+  lo = p.dense.first(c);
+  hi = p.dense.first(c + 1);
 }
-QMKP_HD int piece_owner(const Plan& p, long long f) {
-  if (f < p.share[0]) return (int)(((f + 1) * p.warps[0] - 1) / p.share[0]);
-  f -= p.share[0];
-  return p.warps[0] + (int)(((f + 1) * p.warps[1] - 1) / p.share[1]);
+// Pieces [lo, hi) of a warp of CTA c and the warp's number among those that have any (neighbours sit in neighbouring CTAs).
+QMKP_HD int piece_range(const PlanDims& d, const Plan& p, int c, int warp, int& lo, int& hi) {
+  lo = hi = 0;
+  if (c < p.dense_ctas) return -1;
+  const int i = warp * (d.ctas - p.dense_ctas) + c - p.dense_ctas;
+  lo = p.strips.first(i);
+  hi = p.strips.first(i + 1);
+  return i;
 }
+
 // Pieces are numbered request by request, inside it (strip of a KV head, KV head, piece), the piece fastest.  Strips are
 // numbered in the same order, with gaps: `before` short tokens in front of request s leave room for their strips.
 QMKP_HD int strip_number(const PlanDims& d, int s, int before, int strip, int kvh) {

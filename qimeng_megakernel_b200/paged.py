@@ -30,7 +30,7 @@ from . import _lib
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
 MAX_GROUP = 16            # query heads per KV head
-MAX_SEQS = 2048           # requests of one attention call
+MAX_SEQS = 1536           # requests of one attention call
 
 
 @dataclass

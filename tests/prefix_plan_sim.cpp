@@ -29,7 +29,7 @@ int main() {
     d.G = pick(1, 16);
     d.NKV = pick(1, 4);
     d.seqs = pick(1, pick(0, 3) ? 6 : 40);
-    d.ctas = pick(0, 1) ? 148 : pick(1, 30);
+    d.ctas = pick(0, 1) ? 148 : pick(2, 30);
     d.prefix_len = pick(0, 3) ? 16 * pick(0, 60) : 0;
     const int page = 16, max_pages = d.prefix_len / page + pick(1, 40);
     d.room = max_pages * page > d.prefix_len ? max_pages * page : d.prefix_len;
@@ -64,10 +64,9 @@ int main() {
       pc.push_back((int)t.pieces);
     }
     const Plan p = make_plan(d, t);
-    const long long pieces = t.pieces * d.NKV;
-    CHECK(p.share[0] + p.share[1] == pieces && p.share[0] >= 0 && p.share[1] >= 0);
+    const int pieces = t.pieces * d.NKV, all_blocks = p.blocks * d.NKV;
     CHECK(p.unit_total <= max_units(d));
-    CHECK(p.dense_ctas <= d.ctas && (p.dense_blocks == 0) == (p.dense_ctas == 0));
+    CHECK(p.dense_ctas <= d.ctas && (all_blocks == 0) == (p.dense_ctas == 0) && (pieces == 0 || p.dense_ctas < d.ctas));
 
     Walk w;
     w.seen.resize((size_t)d.tokens * d.NKV);
@@ -85,21 +84,21 @@ int main() {
     struct Named { int rec, n; };
     std::vector<Named> named((size_t)d.tokens * d.NKV, Named{-1, 0});
     std::vector<std::vector<int>> written((size_t)d.tokens * d.NKV);
-    long long walked = 0;
+    int walked = 0;
     std::vector<char> strip_record((size_t)max_strip_records(d), 0), piece_done((size_t)pieces, 0);
     std::vector<Named> strip_named((size_t)d.tokens * d.G * d.NKV, Named{-1, 0});
     std::vector<std::vector<int>> strip_written((size_t)d.tokens * d.G * d.NKV);
     for (int c = 0; c < d.ctas; ++c) {
-      long long lo, hi;
+      int lo, hi;
       dense_range(p, c, lo, hi);
       if (c < p.dense_ctas) {
         CHECK(lo == walked && hi > lo);
         walked = hi;
       }
-      for (long long b = lo; b < hi;) {
+      for (int b = lo; b < hi;) {
         // the unit of block b, found by walking all of them
         const int kvh = (int)(b / p.blocks);
-        long long rest = b % p.blocks;
+        int rest = b % p.blocks;
         int index = 0, blocks = 0, s = -1, u = 0;
         bool found = false;
         for (int q = 0; q < d.seqs && !found; ++q) {
@@ -123,8 +122,8 @@ int main() {
         const int rec = c + kvh * p.unit_total + index;
         CHECK(rec < max_dense_records(d) && !record[rec]);
         record[rec] = 1;
-        const int parts = dense_owner(p, b - b0 + blocks - 1) - dense_owner(p, b - b0) + 1;
-        CHECK(dense_owner(p, b) == c && dense_owner(p, b + (b1 - b0) - 1) == c);
+        const int parts = p.dense.owner(b - b0 + blocks - 1) - p.dense.owner(b - b0) + 1;
+        CHECK(p.dense.owner(b) == c && p.dense.owner(b + (b1 - b0) - 1) == c);
         for (int i = 0; i < d.unit_tokens(); ++i) {
           int tok, lim;
           if (s >= 0) {
@@ -150,23 +149,23 @@ int main() {
         b += b1 - b0;
       }
       for (int warp = 0; warp < kStripWarps; ++warp) {
-        long long flo, fhi;
+        int flo, fhi;
         const int number = piece_range(d, p, c, warp, flo, fhi);
-        CHECK((number < 0) == (flo == fhi));
-        for (long long f = flo; f < fhi;) {
+        CHECK(number >= 0 || flo == fhi);
+        for (int f = flo; f < fhi;) {
           int s = 0;
           while (!((long long)pc[s] * d.NKV <= f && f < (long long)pc[s + 1] * d.NKV)) ++s;
           CHECK(pc[s] <= f / d.NKV && f / d.NKV < pc[s + 1]);
           const Req& r = req[s];
           const int per = pieces_of(d, r);
-          long long rest = f - (long long)pc[s] * d.NKV;
+          int rest = f - pc[s] * d.NKV;
           const int c0 = (int)(rest % per), n = (int)(per - c0 < fhi - f ? per - c0 : fhi - f);
           rest /= per;
           const int kvh = (int)(rest % d.NKV), strip = (int)(rest / d.NKV);
           const int rec = number + strip_number(d, s, stk[s], strip, kvh);
           CHECK(rec < max_strip_records(d) && !strip_record[rec]);
           strip_record[rec] = 1;
-          for (long long k = f; k < f + n; ++k) { CHECK(!piece_done[k]); piece_done[k] = 1; CHECK(piece_owner(p, k) == number); }
+          for (int k = f; k < f + n; ++k) { CHECK(!piece_done[k]); piece_done[k] = 1; CHECK(p.strips.owner(k) == number); }
           const int row0 = strip * kStripRows, rows = imin(kStripRows, r.n * d.G - row0);
           CHECK(rows > 0);
           const int last = limit_of(d, r, (row0 + rows - 1) / d.G);
@@ -179,7 +178,7 @@ int main() {
               auto& seen = w.seen[(size_t)tok * d.NKV + kvh];
               for (int key = k_lo; key < k_hi && key < lim; ++key) ++seen[key];
             }
-            if (c0 == 0) strip_named[at] = Named{rec, piece_owner(p, f + per - 1) - number + 1};
+            if (c0 == 0) strip_named[at] = Named{rec, p.strips.owner(f + per - 1) - number + 1};
             strip_written[at].push_back(rec);
           }
           f += n;
@@ -199,7 +198,7 @@ int main() {
         for (int k = 0; k < strip_named[at].n; ++k) CHECK(v[k] == strip_named[at].rec + k);
       }
     }
-    CHECK(walked == p.dense_blocks);
+    CHECK(walked == all_blocks);
     for (int tok = 0; tok < d.tokens; ++tok)
       for (int h = 0; h < d.NKV; ++h) {
         const size_t i = (size_t)tok * d.NKV + h;

@@ -84,7 +84,7 @@ def test_attention_refusals(paged):
     refused(ValueError, "whole pages", f, prefix=-16)
     refused(ValueError, "prefix_table has 1 pages", f, prefix_table=i32(1))
     refused(ValueError, "needs a prefix_table", f, prefix_table=None)
-    refused(ValueError, "expected 1..2048 requests", f, seqs=2049)
+    refused(ValueError, "expected 1..1536 requests", f, seqs=1537)
     refused(ValueError, "expected kv_lengths", f, kv=i32(3))
     refused(ValueError, "expected kv_lengths", f, cu=i32(2))
     refused(ValueError, "scale 0", f, scale=0.0)
@@ -152,7 +152,7 @@ def test_c_entries_refuse_before_they_launch(paged):
         assert attn(**{name: None}) == -1, name
     for kw in (dict(q=P + 8), dict(out=P + 2), dict(k_pages=P + 8), dict(v_pages=P + 8), dict(q_token_stride=508),
                dict(out_token_stride=516), dict(tokens=0), dict(seqs=0), dict(num_heads=9), dict(num_kv_heads=0),
-               dict(num_heads=34), dict(seqs=2049), dict(tokens=(1 << 20) + 1), dict(head_dim=80), dict(num_pages=1 << 27),
+               dict(num_heads=34), dict(seqs=1537), dict(tokens=(1 << 20) + 1), dict(head_dim=80), dict(num_pages=1 << 27),
                dict(max_pages=(1 << 26) + 1), dict(workspace=None), dict(workspace=P + 128), dict(page_size=48), dict(num_pages=0), dict(max_pages=0),
                dict(prefix_len=33), dict(prefix_len=-16), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf"))):
         assert attn(**kw) == -1, kw
