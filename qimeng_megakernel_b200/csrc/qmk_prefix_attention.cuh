@@ -226,20 +226,26 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
   return one != 0u;
 }
-// Bounded wait on a phase of a barrier; false once the CTA has been aborted.
+// Bounded wait on a phase of a barrier; false once the CTA has been aborted.  The hint (1 ms) lets the hardware park the warp:
+// one that polls takes issue slots from the softmax warps of its scheduler (measured: 3 % of a long step).
+__device__ __forceinline__ uint32_t mbar_try_wait_parked(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000000u) : "memory");
+  return ok;
+}
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile unsigned* ctl) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_try_wait_parked(bar, parity)) return true;
   const long long t0 = clock64();
-  for (;;) {
-#pragma unroll 1
-    for (int i = 0; i < 16; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
+  while (!mbar_try_wait_parked(bar, parity)) {
     if (ctl[0] != 0u) return false;
     if (clock64() - t0 > kWaitCycles) {
       ctl[0] = 1u;
       return false;
     }
   }
+  return true;
 }
 
 // ------------------------------------------------------------------------------------------------ plan
