@@ -101,13 +101,6 @@ static int sm_count(int device) {
   return n;
 }
 
-static PlanDims plan_dims(int tokens, int seqs, int num_heads, int num_kv_heads, int prefix_len, int ctas) {
-  PlanDims d;
-  d.tokens = tokens; d.seqs = seqs; d.G = num_heads / num_kv_heads; d.NKV = num_kv_heads; d.prefix_len = prefix_len;
-  d.ctas = ctas; d.room = prefix_len;
-  return d;
-}
-
 // Regions of the workspace; every one starts on a 256-byte boundary.
 struct WorkspaceLayout { long long dense_ml, dense_o, strip_ml, strip_o, dense_desc, strip_desc, total; };
 static WorkspaceLayout workspace_layout(const PlanDims& d, int head_dim) {
@@ -129,7 +122,7 @@ static WorkspaceLayout workspace_layout(const PlanDims& d, int head_dim) {
 static bool counts_fit(const PlanDims& d) {
   const long long most = 0x7fffffffll, strips = max_strips(d), by_request = (long long)d.seqs * (kLongRows / kStripRows) * d.NKV;
   return max_units(d) * d.NKV * (d.room / kBlockKeys + 1) <= most && max_strip_records(d) <= most &&
-         (strips < by_request ? strips : by_request) * (d.room / kPieceKeys + 1) <= most;
+         (strips < by_request ? strips : by_request) * (d.room / kPieceKeys + 1 + kStripCost) <= most;
 }
 
 static bool attention_sizes_ok(int tokens, int seqs, int num_heads, int num_kv_heads, int head_dim, int prefix_len) {
@@ -143,7 +136,7 @@ extern "C" int64_t qmk_prefix_attention_workspace(int32_t tokens, int32_t seqs, 
   if (!attention_sizes_ok(tokens, seqs, num_heads, num_kv_heads, head_dim, prefix_len)) return QMK_ERR_INVALID_ARG;
   const int ctas = sm_count(device);
   if (ctas < 1) return QMK_ERR_DEVICE;
-  return workspace_layout(plan_dims(tokens, seqs, num_heads, num_kv_heads, prefix_len, ctas), head_dim).total;
+  return workspace_layout(make_dims(tokens, seqs, num_heads / num_kv_heads, num_kv_heads, head_dim, prefix_len, 0, ctas), head_dim).total;
 }
 
 static int attention_args(const qmk_prefix_attention_args* a) {
@@ -232,9 +225,8 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
   if (ctas < 1) return QMK_ERR_DEVICE;
   AttnParams p;
   memset(&p, 0, sizeof(p));
-  p.d = plan_dims(a->tokens, a->seqs, a->num_heads, a->num_kv_heads, a->prefix_len, ctas);
-  const long long room = (long long)a->max_pages * a->page_size;
-  p.d.room = (int)(room > a->prefix_len ? room : a->prefix_len);
+  p.d = make_dims(a->tokens, a->seqs, a->num_heads / a->num_kv_heads, a->num_kv_heads, a->head_dim, a->prefix_len,
+                  a->max_pages * a->page_size, ctas);
   if (!counts_fit(p.d)) return QMK_ERR_INVALID_ARG;
   const WorkspaceLayout w = workspace_layout(p.d, a->head_dim);
   if (a->workspace_bytes < w.total) return QMK_ERR_INVALID_ARG;

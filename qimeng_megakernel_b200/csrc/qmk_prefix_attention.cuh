@@ -52,7 +52,7 @@ struct AttnParams {
   float2* dense_ml;            // [records, 256]   (m in log2 units, l)
   float* strip_o;              // [records, 8, HD]
   float2* strip_ml;            // [records, 8]
-  int2* dense_desc;            // [tokens, NKV]    {first record, records | dual << 15 | row << 16}; records 0: none
+  int2* dense_desc;            // [tokens, NKV]    {first record, records | row << 16}; records 0: none
   int2* strip_desc;            // [tokens, NH]     {first record, records | row << 16}
 };
 struct AttnMaps {
@@ -86,7 +86,8 @@ struct AttnSmem {
   static constexpr int kOffCtl = kOffBars + kNumBars * 8;       // words: 0 abort, 1 tensor memory base
   static constexpr int kOffRed = (kOffCtl + 16 + 15) / 16 * 16;   // int4 [12] scratch of the scan
   static constexpr int kOffWork = kOffRed + kAttnThreads / 32 * 16;   // Work
-  static constexpr int kOffScan = (kOffWork + 128 + 15) / 16 * 16;   // int [4][seqs + 1]
+  static constexpr int kOffMl = (kOffWork + 128 + 15) / 16 * 16;   // float2 [256]  m and l of the groups' rows
+  static constexpr int kOffScan = kOffMl + 256 * 8;             // int [4][seqs + 1]
   static __host__ __device__ constexpr int total(int seqs) { return kOffScan + 4 * (seqs + 1) * 4; }
 };
 
@@ -323,8 +324,21 @@ __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc,
     sc.long_units[seqs] = base.y;
     sc.short_tokens[seqs] = base.z;
     sc.pieces[seqs] = base.w;
-    out->t = Totals{base.x, base.y, base.z, base.w};
-    out->plan = make_plan(p.d, out->t);
+  }
+  if (warp == 0) {                                           // each lane weighs one division of the CTAs
+    const Totals t{base.x, base.y, base.z, base.w};
+    int ctas = plan_choice(p.d, t, lane);
+    float time = plan_time(p.d, t, ctas);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float ot = __shfl_xor_sync(kFullMask, time, o);
+      const int oc = __shfl_xor_sync(kFullMask, ctas, o);
+      if (ot < time || (ot == time && oc < ctas)) { time = ot; ctas = oc; }
+    }
+    if (lane == 0) {
+      out->t = t;
+      out->plan = make_plan(p.d, t, ctas);
+    }
   }
   __syncthreads();
 }
@@ -355,16 +369,16 @@ __device__ __forceinline__ Unit unit_at(const AttnParams& p, const Scans& sc, co
     }
     x.index = sc.long_units[lo] + x.u;
     x.limit = unit_limit(p.d, x.r, x.u);
-    x.rows = min(p.d.unit_tokens(), x.r.n - x.u * p.d.unit_tokens()) * p.d.G;
+    x.rows = min(p.d.unit_tokens, x.r.n - x.u * p.d.unit_tokens) * p.d.G;
   } else {
     rest -= t.long_blocks;
     x.s = -1;
-    x.blocks = p.d.prefix_blocks();
+    x.blocks = p.d.prefix_blocks;
     x.u = rest / x.blocks;
     rest -= x.u * x.blocks;
     x.index = t.long_units + x.u;
     x.limit = p.d.prefix_len;
-    x.rows = min(p.d.unit_tokens(), t.short_tokens - x.u * p.d.unit_tokens()) * p.d.G;
+    x.rows = min(p.d.unit_tokens, t.short_tokens - x.u * p.d.unit_tokens) * p.d.G;
     x.r = Req{0, 0, 0};
   }
   block = rest;
@@ -374,13 +388,13 @@ __device__ __forceinline__ Unit unit_at(const AttnParams& p, const Scans& sc, co
 __device__ __forceinline__ int row_token(const AttnParams& p, const Scans& sc, const Unit& x, int row, int& lim) {
   lim = 0x7fffffff;
   if (row >= x.rows) return -1;
-  const int i = row / p.d.G;
+  const int i = p.d.by_G.div(row);
   if (x.s >= 0) {
-    const int t = x.u * p.d.unit_tokens() + i;
+    const int t = x.u * p.d.unit_tokens + i;
     lim = limit_of(p.d, x.r, t);
     return x.r.first + t;
   }
-  const int at = x.u * p.d.unit_tokens() + i;
+  const int at = x.u * p.d.unit_tokens + i;
   const int s = find_last(sc.short_tokens, p.d.seqs, at);
   const Req r = load_request(p, s);
   const int t = at - sc.short_tokens[s];
@@ -597,7 +611,7 @@ struct Dense {
       int lim;
       const int tile_row = dual && g == 1 ? row - 128 : row;
       const int token = row_token(p, sc, x, tile_row, lim);
-      const int head = x.kvh * p.d.G + tile_row % p.d.G;
+      const int head = x.kvh * p.d.G + p.d.by_G.mod(tile_row);
       if (!(dual && g == 1)) {
         const uint4* src = reinterpret_cast<const uint4*>(p.q + (size_t)max(token, 0) * p.q_stride + (size_t)head * HD);
         unsigned char* dst = smem + S::kOffQ + g * S::kTileBytes + (row & 127) * 128;
@@ -732,58 +746,80 @@ struct Dense {
       if (ok && steps > 0) ok = wait_bar(o_full(g, 1), o_par, ctl);
       if (steps > 0) o_par ^= 1u;
       tmem_fence_after_sync();
-      // ---- the unit's rows: complete, or a record ----
+      // ---- the unit's rows: complete, or a record.  With one tile both groups have a part of every row (in the same lanes
+      // of tensor memory): they add the two up, half of the dimensions each ----
       const int cta = (int)blockIdx.x;
-      const bool whole = b0 == 0 && nb == x.blocks && !dual && x.s >= 0;
+      const bool whole = b0 == 0 && nb == x.blocks && x.s >= 0;
       const int rec = cta + x.kvh * plan.unit_total + x.index;
-      const bool have = steps > 0;
+      float f = 1.f, f_other = 0.f;                   // factors of this group's O and of the other's
+      if (!ok) l = __int_as_float(0x7fffffff);
+      if (dual) {
+        float2* ml = reinterpret_cast<float2*>(smem + S::kOffMl);
+        ml[row] = make_float2(m, l);
+        tmem_fence_before_sync();
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+        tmem_fence_after_sync();
+        const float2 other = ml[row ^ 128];
+        const float top = fmaxf(m, other.x);
+        f = m == -INFINITY ? 0.f : ex2(m - top);
+        f_other = other.x == -INFINITY ? 0.f : ex2(other.x - top);
+        l = l * f + other.y * f_other;
+        if (!(other.y == other.y) || !ok) l = __int_as_float(0x7fffffff);
+        m = top;
+      } else if (steps == 0 || m == -INFINITY) {
+        f = 0.f;
+      }
       if (warp_works) {
-        const float nan = __int_as_float(0x7fffffff);
-        if (whole) {
-          const float inv = !ok ? nan : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : nan));
-          uint16_t* dst = p.out + (size_t)max(token, 0) * p.out_stride + (size_t)head * HD;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const uint32_t other_col = tmem + 256 + (g ^ 1) * 128 + lane_base;
+        uint16_t* out = p.out + (size_t)max(token, 0) * p.out_stride + (size_t)head * HD;
+        float* part = p.dense_o + ((size_t)rec * kUnitRows + tile_row) * HD;
+        const int c0 = dual ? g * (HD / 32) : 0, c1 = dual ? c0 + HD / 32 : HD / 16;
 #pragma unroll 1
-          for (int c = 0; c < HD / 16; ++c) {
-            uint32_t o[16];
-            tmem_ld16(o, o_col + 16 * c);
+        for (int c = c0; c < c1; ++c) {
+          uint32_t o[16];
+          tmem_ld16(o, o_col + 16 * c);
+          if (dual) {
+            uint32_t u[16];
+            tmem_ld16(u, other_col + 16 * c);
             tmem_wait_ld();
-            if (token >= 0) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
+            for (int i = 0; i < 16; ++i)               // (a factor of zero: whatever stands there does not count)
+              o[i] = __float_as_uint((f != 0.f ? f * __uint_as_float(o[i]) : 0.f) + (f_other != 0.f ? f_other * __uint_as_float(u[i]) : 0.f));
+          } else {
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = f != 0.f ? o[i] : 0u;
+          }
+          if (token >= 0) {
+            if (whole) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
                 uint32_t w[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  w[j] = pack2(l == 0.f ? 0.f : __uint_as_float(o[8 * h + 2 * j]) * inv, l == 0.f ? 0.f : __uint_as_float(o[8 * h + 2 * j + 1]) * inv);
-                reinterpret_cast<uint4*>(dst + 16 * c)[h] = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int k = 0; k < 4; ++k) w[k] = pack2(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+                reinterpret_cast<uint4*>(out + 16 * c)[i] = make_uint4(w[0], w[1], w[2], w[3]);
               }
-            }
-          }
-          if (token >= 0 && p.lse) p.lse[(size_t)token * p.NH + head] = !ok ? nan : (l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f);
-        } else {
-          float* dst = p.dense_o + ((size_t)rec * kUnitRows + row) * HD;
-          if (have) {
-#pragma unroll 1
-            for (int c = 0; c < HD / 16; ++c) {
-              uint32_t o[16];
-              tmem_ld16(o, o_col + 16 * c);
-              tmem_wait_ld();
-              if (token >= 0) {
+            } else {
 #pragma unroll
-                for (int h = 0; h < 4; ++h)
-                  reinterpret_cast<uint4*>(dst + 16 * c)[h] = make_uint4(o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]);
-              }
+              for (int i = 0; i < 4; ++i)
+                reinterpret_cast<uint4*>(part + 16 * c)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             }
           }
-          if (token >= 0) p.dense_ml[(size_t)rec * kUnitRows + row] = ok ? make_float2(m, l) : make_float2(nan, nan);
         }
-        // whoever starts the unit says where its rows' parts are
-        if (b0 == 0 && token >= 0 && tile_row % p.d.G == 0 && !(dual && g == 1)) {
-          const size_t at = (size_t)token * p.d.NKV + x.kvh;
-          int parts = 0;
-          if (!whole) parts = plan.dense.owner(b + x.blocks - 1) - cta + 1;
-          p.dense_desc[at] = make_int2(rec, parts | (dual ? 1 << 15 : 0) | (tile_row << 16));
-          if (x.s >= 0)
-            for (int i = 0; i < p.d.G; ++i) p.strip_desc[(size_t)token * p.NH + head + i] = make_int2(0, 0);
+        if (token >= 0 && !(dual && g == 1)) {
+          if (whole) {
+            if (p.lse) p.lse[(size_t)token * p.NH + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+          } else {
+            p.dense_ml[(size_t)rec * kUnitRows + tile_row] = make_float2(l == l ? m : l, l);
+          }
+          // whoever starts the unit says where its rows' parts are
+          if (b0 == 0 && p.d.by_G.mod(tile_row) == 0) {
+            const int parts = whole ? 0 : plan.dense.owner(b + x.blocks - 1) - cta + 1;
+            p.dense_desc[(size_t)token * p.d.NKV + x.kvh] = make_int2(rec, parts | (tile_row << 16));
+            if (x.s >= 0)
+              for (int i = 0; i < p.d.G; ++i) p.strip_desc[(size_t)token * p.NH + head + i] = make_int2(0, 0);
+          }
         }
       }
       n += (unsigned)nb;
@@ -810,15 +846,15 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
   int lo, hi;
   const int number = piece_range(p.d, plan, (int)blockIdx.x, warp, lo, hi);
   for (int f = lo; f < hi;) {
-    const int s = find_last(sc.pieces, p.d.seqs, f / p.d.NKV);
+    const int s = find_last(sc.pieces, p.d.seqs, p.d.by_NKV.div(f));
     const Req r = load_request(p, s);
     const int per = pieces_of(p.d, r);
     const int rest = f - sc.pieces[s] * p.d.NKV, column = rest / per;
     const int c0 = rest - column * per, n = min(per - c0, hi - f);
-    const int strip = column / p.d.NKV, kvh = column - strip * p.d.NKV;
+    const int strip = p.d.by_NKV.div(column), kvh = column - strip * p.d.NKV;
     const int base_row = strip * kStripRows, rows = min(kStripRows, r.n * p.d.G - base_row);
-    const int k_lo = p.d.prefix_len + c0 * kPieceKeys;
-    const int k_hi = max(k_lo, min(k_lo + n * kPieceKeys, limit_of(p.d, r, (base_row + rows - 1) / p.d.G)));
+    const int k_lo = p.d.prefix_len + piece_lo(c0);
+    const int k_hi = max(k_lo, min(p.d.prefix_len + piece_lo(c0 + n), limit_of(p.d, r, p.d.by_G.div(base_row + rows - 1))));
     // pool rows of the next 32 groups of 16 keys, one per lane
     const int* table = p.tables + (size_t)s * p.max_pages;
     auto group_row = [&](int grp) {
@@ -855,15 +891,15 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
     uint32_t qb[HD / 16][2];
     {
       const int i = min(g, rows - 1) + base_row;
-      const uint16_t* qp = p.q + (size_t)(r.first + i / p.d.G) * p.q_stride + (size_t)(kvh * p.d.G + i % p.d.G) * HD + 2 * t4;
+      const uint16_t* qp = p.q + (size_t)(r.first + p.d.by_G.div(i)) * p.q_stride + (size_t)(kvh * p.d.G + p.d.by_G.mod(i)) * HD + 2 * t4;
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
         qb[k][0] = *reinterpret_cast<const uint32_t*>(qp + 16 * k);
         qb[k][1] = *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8);
       }
     }
-    const int lim0 = min(k_hi, limit_of(p.d, r, (base_row + min(2 * t4, rows - 1)) / p.d.G));
-    const int lim1 = min(k_hi, limit_of(p.d, r, (base_row + min(2 * t4 + 1, rows - 1)) / p.d.G));
+    const int lim0 = min(k_hi, limit_of(p.d, r, p.d.by_G.div(base_row + min(2 * t4, rows - 1))));
+    const int lim1 = min(k_hi, limit_of(p.d, r, p.d.by_G.div(base_row + min(2 * t4 + 1, rows - 1))));
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     float o[HD / 16][4];
 #pragma unroll
@@ -975,7 +1011,7 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
       const int row = 2 * t4 + h;
       if (row >= rows) continue;
       const float m = h ? m1 : m0, l = h ? l1 : l0;
-      const int token = r.first + (base_row + row) / p.d.G, gq = (base_row + row) % p.d.G, head = kvh * p.d.G + gq;
+      const int token = r.first + p.d.by_G.div(base_row + row), gq = p.d.by_G.mod(base_row + row), head = kvh * p.d.G + gq;
       if (whole) {
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : nan);
         uint16_t* dst = p.out + (size_t)token * p.out_stride + (size_t)head * HD + g;
@@ -1081,16 +1117,17 @@ template <int HD>
 __global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int token = (int)(row / p.NH), head = (int)(row % p.NH);
-  if (token >= min(p.d.tokens, p.cu_tokens[p.d.seqs])) return;
-  const int kvh = head / p.d.G, g = head % p.d.G;
+  const int row = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 5);   // (at most 2^20 tokens of 2^10 heads)
+  const int token = row / p.NH, head = row - token * p.NH;
+  if (token >= p.d.tokens) return;
+  const int rows = p.cu_tokens[p.d.seqs];
+  const int kvh = p.d.by_G.div(head), g = p.d.by_G.mod(head);
   const int2 dd = p.dense_desc[(size_t)token * p.d.NKV + kvh], sd = p.strip_desc[(size_t)token * p.NH + head];
-  const int nseg = dd.y & 0x7fff, dual = (dd.y >> 15) & 1, nd = nseg << dual, parts = nd + (sd.y & 0xffff);
-  if (parts == 0) return;
-  // row of part r: dense parts are 256 rows apart (with one tile two of them 128 rows), strips 8
+  const int nd = dd.y & 0xffff, parts = nd + (sd.y & 0xffff);
+  if (parts == 0 || token >= rows) return;
+  // row of part r: dense parts are 256 rows apart, strips 8
   const size_t drow = (size_t)dd.x * kUnitRows + ((unsigned)dd.y >> 16) + g, srow = (size_t)sd.x * kStripRows + ((unsigned)sd.y >> 16);
-  auto dense_row = [&](int r) { return drow + (size_t)(r >> dual) * kUnitRows + (dual ? (r & 1) * 128 : 0); };
+  auto dense_row = [&](int r) { return drow + (size_t)r * kUnitRows; };
   auto strip_row = [&](int r) { return srow + (size_t)(r - nd) * kStripRows; };
   constexpr int LPR = HD / 4, PER = 32 / LPR;              // lanes per row, parts per pass
   float M = -INFINITY, L = 0.f;

@@ -27,16 +27,52 @@ constexpr int kLongRows = 128;      // a request with fewer rows shares its unit
 constexpr int kStripRows = 8;       // rows of a strip (the short side of an mma.sync tile)
 constexpr int kMaxGroup = 16;       // query heads of a KV head
 constexpr int kPieceKeys = 32;      // keys of a piece
+constexpr int kStripCost = 2;       // pieces without keys at the head of a strip: what it costs to take one up
 constexpr int kStripWarps = 8;      // warps of a CTA that walk strips
-constexpr int kBlockCost = 8;       // time of a block of 256 rows in pieces (a CTA's eight warps at one each)
 constexpr int kMaxSeqs = 1536;      // requests of a call (their prefix sums are kept in shared memory)
 
-struct PlanDims {
-  int tokens, seqs, G, NKV, prefix_len, ctas;
-  int room;                         // positions a request can have: max(prefix_len, max_pages * page_size)
-  QMKP_HD int unit_tokens() const { return kUnitRows / G; }
-  QMKP_HD int prefix_blocks() const { return (prefix_len + kBlockKeys - 1) / kBlockKeys; }
+// Division by a number known on the host, for 0 <= x < 2^31: with p = 31 + ceil(log2 d) and mul = ceil(2^p / d) < 2^32 the
+// quotient is floor(x * mul / 2^p) (the rounding of mul adds less than x / 2^31 < 1 part of 1 / d).
+struct Divider {
+  unsigned mul;
+  int d, shift;
+  QMKP_HD int div(int x) const {
+    if (d == 1) return x;
+#if defined(__CUDA_ARCH__)
+    return (int)(__umulhi((unsigned)x, mul) >> shift);
+#else
+    return (int)(((unsigned long long)(unsigned)x * mul >> 32) >> shift);
+#endif
+  }
+  QMKP_HD int mod(int x) const { return x - div(x) * d; }
 };
+inline Divider make_divider(int d) {
+  Divider v;
+  v.d = d;
+  int log = 0;
+  while ((1ll << log) < d) ++log;
+  v.shift = 31 + log - 32;
+  v.mul = d == 1 ? 0u : (unsigned)(((1ull << (31 + log)) + (unsigned)d - 1) / (unsigned)d);
+  return v;
+}
+
+struct PlanDims {
+  int tokens, seqs, G, NKV, prefix_len, ctas, head_dim;
+  int room;                         // positions a request can have: max(prefix_len, max_pages * page_size)
+  int unit_tokens;                  // tokens of a unit
+  int prefix_blocks;
+  Divider by_G, by_NKV;
+};
+inline PlanDims make_dims(int tokens, int seqs, int G, int NKV, int head_dim, int prefix_len, int room, int ctas) {
+  PlanDims d;
+  d.tokens = tokens; d.seqs = seqs; d.G = G; d.NKV = NKV; d.prefix_len = prefix_len; d.ctas = ctas; d.head_dim = head_dim;
+  d.room = room > prefix_len ? room : prefix_len;
+  d.unit_tokens = kUnitRows / G;
+  d.prefix_blocks = (prefix_len + kBlockKeys - 1) / kBlockKeys;
+  d.by_G = make_divider(G);
+  d.by_NKV = make_divider(NKV);
+  return d;
+}
 
 struct Req {
   int first, n;                     // first row (token) of the request in the step, tokens
@@ -59,9 +95,9 @@ QMKP_HD int limit_of(const PlanDims& d, const Req& r, int i) {
 QMKP_HD bool is_long(const PlanDims& d, const Req& r) { return (long long)r.n * d.G >= kLongRows; }
 
 // long requests
-QMKP_HD int units_of(const PlanDims& d, const Req& r) { return (r.n + d.unit_tokens() - 1) / d.unit_tokens(); }
+QMKP_HD int units_of(const PlanDims& d, const Req& r) { return (r.n + d.unit_tokens - 1) / d.unit_tokens; }
 QMKP_HD int unit_limit(const PlanDims& d, const Req& r, int u) {
-  return limit_of(d, r, imin((u + 1) * d.unit_tokens(), r.n) - 1);
+  return limit_of(d, r, imin((u + 1) * d.unit_tokens, r.n) - 1);
 }
 QMKP_HD int unit_blocks(const PlanDims& d, const Req& r, int u) {
   return imax(1, (unit_limit(d, r, u) + kBlockKeys - 1) / kBlockKeys);
@@ -69,7 +105,7 @@ QMKP_HD int unit_blocks(const PlanDims& d, const Req& r, int u) {
 // short requests
 QMKP_HD int own_keys(const PlanDims& d, const Req& r) { return r.n > 0 ? imax(0, limit_of(d, r, r.n - 1) - d.prefix_len) : 0; }
 QMKP_HD int strips_of(const PlanDims& d, const Req& r) { return (r.n * d.G + kStripRows - 1) / kStripRows; }   // of a KV head
-QMKP_HD int pieces_of(const PlanDims& d, const Req& r) { return imax(1, (own_keys(d, r) + kPieceKeys - 1) / kPieceKeys); }
+QMKP_HD int pieces_of(const PlanDims& d, const Req& r) { return kStripCost + (own_keys(d, r) + kPieceKeys - 1) / kPieceKeys; }
 
 // `total` things dealt to n takers as contiguous ranges that differ by one at most (with fewer things than takers the first
 // ones get one each, so owners of neighbouring things are always neighbours).
@@ -103,24 +139,35 @@ struct Plan {
   int dense_ctas;                   // CTAs with blocks; the others have pieces
   Deal dense, strips;               // all blocks to CTAs, all pieces to warps
 };
-constexpr int kMinSegment = 2;      // blocks a CTA takes at least
 
-QMKP_HD Plan make_plan(const PlanDims& d, const Totals& t) {
+// Microseconds that a call takes when `ctas` CTAs have the blocks, the longer of the two kinds (measured on B200; a piece at a CTA's share
+// of the memory bandwidth, a block of one tile at its keys' or its steps' time, one of two tiles at its steps').
+QMKP_HD float plan_time(const PlanDims& d, const Totals& t, int ctas) {
+  const int short_units = d.prefix_len > 0 ? (t.short_tokens + d.unit_tokens - 1) / d.unit_tokens : 0;
+  const bool small = t.short_tokens * d.G <= kLongRows, wide = d.head_dim == 128;
+  const float one = wide ? 1.4f : 0.85f, two = wide ? 2.0f : 1.6f, piece = wide ? 0.37f : 0.19f;
+  const float blocks = ((float)t.long_blocks * two + (float)(short_units * d.prefix_blocks) * (small ? one : two)) * (float)d.NKV;
+  const float dense = blocks > 0.f ? 3.5f + (ctas > 0 ? blocks / (float)ctas : 1e30f) : 0.f;
+  const int rest = d.ctas - ctas;
+  const float few = t.pieces > 0 ? 2.5f + (rest > 0 ? (float)t.pieces * (float)d.NKV * piece / (float)rest : 1e30f) : 0.f;
+  return dense > few ? dense : few;
+}
+// The numbers of CTAs that are weighed: i of kPlanChoices.
+constexpr int kPlanChoices = 32;
+QMKP_HD int plan_choice(const PlanDims& d, const Totals& t, int i) {
+  const int all = (t.long_blocks + (d.prefix_len > 0 ? (t.short_tokens + d.unit_tokens - 1) / d.unit_tokens * d.prefix_blocks : 0)) * d.NKV;
+  int ctas = t.pieces == 0 ? d.ctas : (i + 1) * (d.ctas - 1) / kPlanChoices;
+  ctas = imax(ctas, 1);
+  return imin(ctas, all);                // (no blocks: none)
+}
+QMKP_HD Plan make_plan(const PlanDims& d, const Totals& t, int ctas) {
   Plan p;
-  const int short_units = d.prefix_len > 0 ? (t.short_tokens + d.unit_tokens() - 1) / d.unit_tokens() : 0;
+  const int short_units = d.prefix_len > 0 ? (t.short_tokens + d.unit_tokens - 1) / d.unit_tokens : 0;
   p.unit_total = t.long_units + short_units;
-  const int short_blocks = short_units * d.prefix_blocks();
-  p.blocks = t.long_blocks + short_blocks;
-  const int all = p.blocks * d.NKV, pieces = t.pieces * d.NKV;
-  // a block of two tiles counts as kBlockCost pieces, one of a single tile as four (its keys)
-  const bool small = t.short_tokens * d.G <= kLongRows;
-  const float dense = ((float)t.long_blocks * kBlockCost + (float)short_blocks * (small ? 4 : kBlockCost)) * (float)d.NKV;
-  int ctas = pieces == 0 ? d.ctas : (int)((float)d.ctas * (dense / (dense + (float)pieces)) + 0.5f);
-  ctas = imin(imax(ctas, 1), pieces == 0 ? d.ctas : d.ctas - 1);
-  ctas = imin(ctas, (all + kMinSegment - 1) / kMinSegment);
+  p.blocks = t.long_blocks + short_units * d.prefix_blocks;
   p.dense_ctas = ctas;
-  p.dense = deal(all, ctas);
-  p.strips = deal(pieces, (d.ctas - ctas) * kStripWarps);
+  p.dense = deal(p.blocks * d.NKV, ctas);
+  p.strips = deal(t.pieces * d.NKV, (d.ctas - ctas) * kStripWarps);
   return p;
 }
 // Blocks [lo, hi) of CTA c.
@@ -140,6 +187,8 @@ QMKP_HD int piece_range(const PlanDims& d, const Plan& p, int c, int warp, int& 
   return i;
 }
 
+// First key behind the prefix of piece c of a strip.
+QMKP_HD int piece_lo(int c) { return imax(0, c - kStripCost) * kPieceKeys; }
 // Pieces are numbered request by request, inside it (strip of a KV head, KV head, piece), the piece fastest.  Strips are
 // numbered in the same order, with gaps: `before` short tokens in front of request s leave room for their strips.
 QMKP_HD int strip_number(const PlanDims& d, int s, int before, int strip, int kvh) {
@@ -148,7 +197,7 @@ QMKP_HD int strip_number(const PlanDims& d, int s, int before, int strip, int kv
 
 // Upper bounds for the workspace.
 QMKP_HD long long max_units(const PlanDims& d) {
-  const long long per = d.unit_tokens(), a = 2ll * d.tokens / per + 2, b = d.tokens / per + (long long)d.seqs + 2;
+  const long long per = d.unit_tokens, a = 2ll * d.tokens / per + 2, b = d.tokens / per + (long long)d.seqs + 2;
   return a < b ? a : b;
 }
 QMKP_HD long long max_dense_records(const PlanDims& d) { return d.ctas + max_units(d) * d.NKV; }

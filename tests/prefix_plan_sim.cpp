@@ -24,15 +24,17 @@ struct Walk { std::vector<std::vector<int>> seen; };   // [row of the step * NKV
 int main() {
   std::mt19937 rng(7);
   auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
+  for (int d : {1, 2, 3, 5, 7, 8, 16, 48, 127, 1000, 1024}) {
+    const Divider v = make_divider(d);
+    for (int i = 0; i < 20000; ++i) {
+      const int x = i < 5000 ? i : (i < 10000 ? 0x7fffffff - i : (int)(rng() >> 1));
+      CHECK(v.div(x) == x / d && v.mod(x) == x % d);
+    }
+  }
   for (g_case = 0; g_case < 1500; ++g_case) {
-    PlanDims d;
-    d.G = pick(1, 16);
-    d.NKV = pick(1, 4);
-    d.seqs = pick(1, pick(0, 3) ? 6 : 40);
-    d.ctas = pick(0, 1) ? 148 : pick(2, 30);
-    d.prefix_len = pick(0, 3) ? 16 * pick(0, 60) : 0;
-    const int page = 16, max_pages = d.prefix_len / page + pick(1, 40);
-    d.room = max_pages * page > d.prefix_len ? max_pages * page : d.prefix_len;
+    const int G = pick(1, 16), ctas = pick(0, 1) ? 148 : pick(2, 30), page = 16;
+    const int prefix_len = pick(0, 3) ? 16 * pick(0, 60) : 0, max_pages = prefix_len / page + pick(1, 40);
+    PlanDims d = make_dims(1, pick(1, pick(0, 3) ? 6 : 40), G, pick(1, 4), pick(0, 1) ? 64 : 128, prefix_len, max_pages * page, ctas);
     std::vector<int> cu(1, 0), kv;
     const int kind = pick(0, 3);
     for (int s = 0; s < d.seqs; ++s) {
@@ -63,7 +65,12 @@ int main() {
       stk.push_back(t.short_tokens);
       pc.push_back((int)t.pieces);
     }
-    const Plan p = make_plan(d, t);
+    int choice = plan_choice(d, t, 0);
+    for (int i = 1; i < kPlanChoices; ++i) {
+      const int other = plan_choice(d, t, i);
+      if (plan_time(d, t, other) < plan_time(d, t, choice)) choice = other;
+    }
+    const Plan p = make_plan(d, t, choice);
     const int pieces = t.pieces * d.NKV, all_blocks = p.blocks * d.NKV;
     CHECK(p.unit_total <= max_units(d));
     CHECK(p.dense_ctas <= d.ctas && (all_blocks == 0) == (p.dense_ctas == 0) && (pieces == 0 || p.dense_ctas < d.ctas));
@@ -113,7 +120,7 @@ int main() {
           CHECK(lb[s] <= b % p.blocks && b % p.blocks < lb[s + 1]);
           CHECK(index == lu[s] + u);
         } else {
-          blocks = d.prefix_blocks();
+          blocks = d.prefix_blocks;
           u = (int)(rest / blocks);
           rest -= (long long)u * blocks;
           index = t.long_units + u;
@@ -124,16 +131,16 @@ int main() {
         record[rec] = 1;
         const int parts = p.dense.owner(b - b0 + blocks - 1) - p.dense.owner(b - b0) + 1;
         CHECK(p.dense.owner(b) == c && p.dense.owner(b + (b1 - b0) - 1) == c);
-        for (int i = 0; i < d.unit_tokens(); ++i) {
+        for (int i = 0; i < d.unit_tokens; ++i) {
           int tok, lim;
           if (s >= 0) {
-            const int k = u * d.unit_tokens() + i;
+            const int k = u * d.unit_tokens + i;
             if (k >= req[s].n) break;
             tok = req[s].first + k;
             lim = limit_of(d, req[s], k);
             CHECK(lim <= unit_limit(d, req[s], u));
           } else {
-            const int k = u * d.unit_tokens() + i;
+            const int k = u * d.unit_tokens + i;
             if (k >= t.short_tokens) break;
             int q = 0;
             while (!(stk[q] <= k && k < stk[q + 1])) ++q;
@@ -169,7 +176,7 @@ int main() {
           const int row0 = strip * kStripRows, rows = imin(kStripRows, r.n * d.G - row0);
           CHECK(rows > 0);
           const int last = limit_of(d, r, (row0 + rows - 1) / d.G);
-          const int k_lo = d.prefix_len + c0 * kPieceKeys, k_hi = imin(d.prefix_len + (c0 + n) * kPieceKeys, last);
+          const int k_lo = d.prefix_len + piece_lo(c0), k_hi = imin(d.prefix_len + piece_lo(c0 + n), last);
           for (int i = 0; i < rows; ++i) {
             const int tok = r.first + (row0 + i) / d.G, gq = (row0 + i) % d.G, lim = limit_of(d, r, (row0 + i) / d.G);
             CHECK(lim <= last);
