@@ -832,6 +832,28 @@ struct Dense {
 // g = lane / 4, t = lane % 4.  S^T = K Q^T: tiles of 16 keys x 8 rows (lane: keys g, g + 8 of rows 2t, 2t + 1); O^T = V^T P^T: tiles
 // of 16 dimensions x 8 rows.  The P^T operand is the transpose of the S^T fragment: one movmatrix per 8 keys.  A lane's columns
 // are the same two rows in both products, so a row's maximum and scale never leave its lanes.
+// The part of a strip that a warp takes: pieces [c0, c0 + n), `stages` fills of the ring.
+struct StripRun {
+  Req r;
+  int s, per, c0, n, kvh, strip, base_row, rows, k_lo, k_hi, stages;
+};
+__device__ __forceinline__ StripRun strip_at(const AttnParams& p, const Scans& sc, int f, int hi, int stage_keys) {
+  StripRun x;
+  x.s = find_last(sc.pieces, p.d.seqs, p.d.by_NKV.div(f));
+  x.r = load_request(p, x.s);
+  x.per = pieces_of(p.d, x.r);
+  const int rest = f - sc.pieces[x.s] * p.d.NKV, column = rest / x.per;
+  x.c0 = rest - column * x.per;
+  x.n = min(x.per - x.c0, hi - f);
+  x.strip = p.d.by_NKV.div(column);
+  x.kvh = column - x.strip * p.d.NKV;
+  x.base_row = x.strip * kStripRows;
+  x.rows = min(kStripRows, x.r.n * p.d.G - x.base_row);
+  x.k_lo = p.d.prefix_len + piece_lo(x.c0);
+  x.k_hi = max(x.k_lo, min(p.d.prefix_len + piece_lo(x.c0 + x.n), limit_of(p.d, x.r, p.d.by_G.div(x.base_row + x.rows - 1))));
+  x.stages = (x.k_hi - x.k_lo + stage_keys - 1) / stage_keys;
+  return x;
+}
 template <int HD>
 __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps& maps, unsigned char* smem, volatile unsigned* ctl,
                                             const Scans& sc, const Plan& plan, int warp, int lane) {
@@ -842,51 +864,62 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
   const uint32_t bars = smem_u32(smem) + S::kOffBars + (S::kDenseBars + warp * S::kStripStages) * 8;
   const int g = lane >> 2, t4 = lane & 3;
   const int oob = p.num_pages << p.page_shift;
-  unsigned filled = 0;                                      // stages filled by this warp so far
   int lo, hi;
   const int number = piece_range(p.d, plan, (int)blockIdx.x, warp, lo, hi);
-  for (int f = lo; f < hi;) {
-    const int s = find_last(sc.pieces, p.d.seqs, p.d.by_NKV.div(f));
-    const Req r = load_request(p, s);
-    const int per = pieces_of(p.d, r);
-    const int rest = f - sc.pieces[s] * p.d.NKV, column = rest / per;
-    const int c0 = rest - column * per, n = min(per - c0, hi - f);
-    const int strip = p.d.by_NKV.div(column), kvh = column - strip * p.d.NKV;
-    const int base_row = strip * kStripRows, rows = min(kStripRows, r.n * p.d.G - base_row);
-    const int k_lo = p.d.prefix_len + piece_lo(c0);
-    const int k_hi = max(k_lo, min(p.d.prefix_len + piece_lo(c0 + n), limit_of(p.d, r, p.d.by_G.div(base_row + rows - 1))));
-    // pool rows of the next 32 groups of 16 keys, one per lane
-    const int* table = p.tables + (size_t)s * p.max_pages;
-    auto group_row = [&](int grp) {
-      const int key = k_lo + grp * 16;
-      if (key >= k_hi) return -1;
-      const int id = table[key >> p.page_shift];
-      if (id < 0 || id >= p.num_pages) return oob;
-      return (id << p.page_shift) + (key & ((1 << p.page_shift) - 1));
-    };
-    const int stages = (k_hi - k_lo + KS - 1) / KS;
-    int held = group_row(lane), held_from = 0;
-    int sent = 0;
-    auto send = [&]() {                                      // fills the next stage; lane l < 2 * TILES * HALVES sends one box
-      const int st = (int)((filled + (unsigned)sent) % S::kStripStages);
-      const int grp0 = sent * TILES;
-      if (grp0 + TILES > held_from + 32) {
-        held_from = grp0;
-        held = group_row(grp0 + lane);
+  if (lo >= hi) return;
+  // The fills run ahead of the products, into the next strips too: a short strip's table, pages and rows would otherwise be
+  // waited for one after the other.
+  unsigned sent = 0, used = 0;                              // stages filled and consumed by this warp
+  int nf = lo, next = 0, held = -1, held_from = 0;          // strip being filled, its next stage, pool rows of 32 groups of 16 keys
+  StripRun y = strip_at(p, sc, lo, hi, KS);
+  auto group_row = [&](int grp) {
+    const int key = y.k_lo + grp * 16;
+    if (key >= y.k_hi) return -1;
+    const int id = p.tables[(size_t)y.s * p.max_pages + (key >> p.page_shift)];
+    if (id < 0 || id >= p.num_pages) return oob;
+    return (id << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+  };
+  held = group_row(lane);
+  auto send = [&]() {                                        // the next fill; lane l < 2 * TILES * HALVES sends one box
+    while (nf < hi && next >= y.stages) {
+      nf += y.n;
+      if (nf >= hi) return;
+      y = strip_at(p, sc, nf, hi, KS);
+      next = held_from = 0;
+      held = group_row(lane);
+      if (lane < y.rows) {                                   // (its rows of Q, for when it is taken up)
+        const int i = y.base_row + lane;
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(p.q + (size_t)(y.r.first + p.d.by_G.div(i)) * p.q_stride +
+                                                      (size_t)(y.kvh * p.d.G + p.d.by_G.mod(i)) * HD));
       }
-      const int q = lane % (TILES * HALVES), kg = q / HALVES, half = q % HALVES;
-      const bool is_v = lane >= TILES * HALVES;
-      const int row = __shfl_sync(kFullMask, held, (grp0 + kg - held_from) & 31);
-      const bool mine = lane < 2 * TILES * HALVES && row >= 0;
-      const unsigned issue = __ballot_sync(kFullMask, mine);
-      if (lane == 0) mbar_expect_tx(bars + st * 8, (uint32_t)__popc(issue) * 2048u);
-      __syncwarp();
-      if (mine)
-        tma_box(ring + st * S::kStripStageBytes + (is_v ? KBYTES : 0) + (kg * HALVES + half) * 2048, is_v ? &maps.v16 : &maps.k16,
-                half * 64, kvh, row, bars + st * 8);
-      ++sent;
-    };
-    while (sent < stages && sent < S::kStripStages) send();
+    }
+    if (nf >= hi) return;
+    const int st = (int)(sent % S::kStripStages);
+    const int grp0 = next * TILES;
+    if (grp0 + TILES > held_from + 32) {
+      held_from = grp0;
+      held = group_row(grp0 + lane);
+    }
+    const int q = lane % (TILES * HALVES), kg = q / HALVES, half = q % HALVES;
+    const bool is_v = lane >= TILES * HALVES;
+    const int row = __shfl_sync(kFullMask, held, (grp0 + kg - held_from) & 31);
+    const bool mine = lane < 2 * TILES * HALVES && row >= 0;
+    const unsigned issue = __ballot_sync(kFullMask, mine);
+    if (lane == 0) mbar_expect_tx(bars + st * 8, (uint32_t)__popc(issue) * 2048u);
+    __syncwarp();
+    if (mine)
+      tma_box(ring + st * S::kStripStageBytes + (is_v ? KBYTES : 0) + (kg * HALVES + half) * 2048, is_v ? &maps.v16 : &maps.k16,
+              half * 64, y.kvh, row, bars + st * 8);
+    ++sent;
+    ++next;
+  };
+  for (int i = 0; i < S::kStripStages; ++i) send();
+  bool ok = true;
+  for (int f = lo; f < hi;) {
+    const StripRun x = strip_at(p, sc, f, hi, KS);
+    const Req& r = x.r;
+    const int s = x.s, per = x.per, c0 = x.c0, n = x.n, kvh = x.kvh, strip = x.strip, base_row = x.base_row, rows = x.rows;
+    const int k_lo = x.k_lo, k_hi = x.k_hi, stages = x.stages;
     // row g of the strip as the column-major operand; the two rows this lane's results belong to
     uint32_t qb[HD / 16][2];
     {
@@ -904,12 +937,11 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
     float o[HD / 16][4];
 #pragma unroll
     for (int j = 0; j < HD / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    bool ok = true;
     for (int i = 0; i < stages; ++i) {
-      const unsigned at = filled + (unsigned)i;
-      const int st = (int)(at % S::kStripStages);
-      ok = wait_bar(bars + st * 8, (at / S::kStripStages) & 1u, ctl);
+      const int st = (int)(used % S::kStripStages);
+      ok = ok && wait_bar(bars + st * 8, (used / S::kStripStages) & 1u, ctl);
       if (!ok) break;
+      ++used;
       const uint32_t kb = ring + st * S::kStripStageBytes, vb = kb + KBYTES;
       const int key0 = k_lo + i * KS;
       const int valid = min(KS, k_hi - key0);
@@ -986,17 +1018,8 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
           mma16816(o[c], a, pb[j][0], pb[j][1]);
         }
       __syncwarp();                                         // every lane has read the stage
-      if (sent < stages) send();
+      send();
     }
-    if (!ok) {                                              // leave no copy in flight
-      for (int i = 0; i < sent; ++i) {
-        const unsigned at = filled + (unsigned)i;
-        const long long w0 = clock64();
-        while (!mbar_try_wait(bars + (at % S::kStripStages) * 8, (at / S::kStripStages) & 1u))
-          if (clock64() - w0 > 1000000) break;
-      }
-    }
-    filled += (unsigned)sent;
 #pragma unroll
     for (int d = 4; d < 32; d <<= 1) {
       l0 += __shfl_xor_sync(kFullMask, l0, d);
@@ -1037,6 +1060,11 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
       }
     }
     f += n;
+  }
+  for (; used < sent; ++used) {                             // after an abort: no copy stays in flight
+    const long long w0 = clock64();
+    while (!mbar_try_wait(bars + (used % S::kStripStages) * 8, (used / S::kStripStages) & 1u))
+      if (clock64() - w0 > 1000000) break;
   }
 }
 
