@@ -245,7 +245,7 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
     return QMK_ERR_CUDA;
   }
   AttnMaps maps;
-  const int box = a->page_size < kBlockKeys ? a->page_size : kBlockKeys;
+  const int box = a->page_size < 64 ? a->page_size : 64;
   if (!pool_map(enc, &maps.k, a->k_pages, a, box) || !pool_map(enc, &maps.v, a->v_pages, a, box) ||
       !pool_map(enc, &maps.k16, a->k_pages, a, 16) || !pool_map(enc, &maps.v16, a->v_pages, a, 16)) {
     snprintf(g_paged_err, sizeof(g_paged_err), "cuTensorMapEncodeTiled failed");

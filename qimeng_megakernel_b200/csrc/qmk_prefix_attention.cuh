@@ -56,7 +56,7 @@ struct AttnParams {
   int2* strip_desc;            // [tokens, NH]     {first record, records | row << 16}
 };
 struct AttnMaps {
-  CUtensorMap k, v;            // {HD, NKV, slots}, box {64, 1, min(page, 128)}
+  CUtensorMap k, v;            // {HD, NKV, slots}, box {64, 1, min(page, 64)}
   CUtensorMap k16, v16;        // the same, box {64, 1, 16}
 };
 
@@ -70,12 +70,13 @@ constexpr long long kWaitCycles = 4000000000ll;      // about two seconds
 template <int HD>
 struct AttnSmem {
   static constexpr int kHalves = HD / 64;
-  static constexpr int kTileBytes = 128 * HD * 2;               // a 128-row Q tile, or a K or V block
-  static constexpr int kStages = HD == 64 ? 4 : 2;
+  static constexpr int kTileBytes = 128 * HD * 2;               // a 128-row Q tile
+  static constexpr int kHalfBytes = 64 * HD * 2;                // K or V of half a block
+  static constexpr int kStages = HD == 64 ? 8 : 4;              // halves of K, and of V, in the rings
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = 2 * kTileBytes;
-  static constexpr int kOffV = kOffK + kStages * kTileBytes;
-  static constexpr int kRing = kOffV + kStages * kTileBytes;
+  static constexpr int kOffV = kOffK + kStages * kHalfBytes;
+  static constexpr int kRing = kOffV + kStages * kHalfBytes;
   // strips: per warp a ring of kStripStages stages of 8 KiB
   static constexpr int kStripStages = 3, kStripStageBytes = 8192;
   static constexpr int kStageKeys = HD == 64 ? 32 : 16;         // keys of a stage
@@ -436,8 +437,8 @@ struct Dense {
   __device__ __forceinline__ static int steps_of(int nb, bool dual, int g) { return 2 * (dual ? (nb + 1 - g) >> 1 : nb); }
   __device__ __forceinline__ static int block_of(int j, bool dual, int g) { return dual ? (j & ~1) + g : j >> 1; }
 
-  // keys of block b of a unit that rows can see, and whether the V rows behind them have to be cleared
-  __device__ __forceinline__ static int valid_keys(const Unit& x, int b) { return max(0, min(kBlockKeys, x.limit - b * kBlockKeys)); }
+  // keys of half a block of a unit that rows can see
+  __device__ __forceinline__ static int valid_keys(const Unit& x, int b, int half) { return max(0, min(64, x.limit - b * kBlockKeys - 64 * half)); }
 
   __device__ __forceinline__ int page_of(const Unit& x, int key) const {
     int id;
@@ -445,41 +446,41 @@ struct Dense {
     else id = x.s >= 0 ? p.tables[(size_t)x.s * p.max_pages + (key >> p.page_shift)] : -1;
     return id;
   }
-  // K (or V) of the CTA's blocks: lane l loads box l of a block (a page, or 128 rows of one, of 64 dimensions).  K and V have
-  // a warp each: the scores run up to two blocks ahead of the products with V.
+  // K (or V) of the CTA's blocks, half by half: lane l loads box l of a half (a page, or 64 rows of one, of 64 dimensions).  K and
+  // V have a warp each: the scores run up to a block ahead of the products with V.
   template <bool kV>
   __device__ __forceinline__ unsigned produce() {
-    const int box_rows = min(1 << p.page_shift, kBlockKeys);
-    const int key_of_lane = (lane / S::kHalves) * box_rows, half = lane % S::kHalves;
-    const int boxes = kBlockKeys / box_rows * S::kHalves;
+    const int box_rows = min(1 << p.page_shift, 64);
+    const int key_of_lane = (lane / S::kHalves) * box_rows, half_dims = lane % S::kHalves;
+    const int boxes = 64 / box_rows * S::kHalves;
     const int oob = p.num_pages << p.page_shift;             // behind the last row: reads as zeros
-    const uint32_t dst = base + (kV ? S::kOffV : S::kOffK) + (uint32_t)(half * kBlockKeys * 128 + key_of_lane * 128);
+    const uint32_t dst = base + (kV ? S::kOffV : S::kOffK) + (uint32_t)(half_dims * 8192 + key_of_lane * 128);
     unsigned n = 0;
     for (int b = lo; b < hi;) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
-      const int b1 = min(x.blocks, b0 + (hi - b));
-      auto row_of = [&](int blk) {                           // row of the pool that this lane's box starts at, -1: no box
-        const int key = blk * kBlockKeys + key_of_lane;
+      const int nb = min(x.blocks - b0, hi - b), end = 2 * (b0 + nb);
+      auto row_of = [&](int part) {                          // row of the pool that this lane's box of a half starts at, -1: no box
+        const int key = part * 64 + key_of_lane;
         if (lane >= boxes || key >= x.limit) return -1;
         const int id = page_of(x, key);
         if (id < 0 || id >= p.num_pages) return oob;
         return (id << p.page_shift) + (key & ((1 << p.page_shift) - 1));
       };
-      int row = row_of(b0);
-      for (int blk = b0; blk < b1; ++blk, ++n) {
+      int row = row_of(2 * b0);
+      for (int part = 2 * b0; part < end; ++part, ++n) {
         const int st = n % S::kStages;
         const uint32_t full = kV ? v_full(st) : k_full(st), empty = kV ? v_empty(st) : k_empty(st);
         const unsigned issue = __ballot_sync(kFullMask, row >= 0);
         const uint32_t bytes = (uint32_t)__popc(issue) * (uint32_t)(box_rows * 128);
-        const int next = blk + 1 < b1 ? row_of(blk + 1) : -1;
+        const int next = part + 1 < end ? row_of(part + 1) : -1;
         if (!wait_bar(empty, ((n / S::kStages) & 1u) ^ 1u, ctl)) return n;
         if (lane == 0) mbar_expect_tx(full, bytes);
         __syncwarp();
-        if (row >= 0) tma_box(dst + st * S::kTileBytes, kV ? &maps.v : &maps.k, half * 64, x.kvh, row, full);
+        if (row >= 0) tma_box(dst + st * S::kHalfBytes, kV ? &maps.v : &maps.k, half_dims * 64, x.kvh, row, full);
         row = next;
       }
-      b += b1 - b0;
+      b += nb;
     }
     return n;
   }
@@ -501,7 +502,7 @@ struct Dense {
   __device__ __forceinline__ void issue(int g) {
     constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)HD >> 3) << 17) | ((128u >> 4) << 24);
-    const uint64_t kd0 = desc_k_major(base + S::kOffK), vd0 = desc_n_major(base + S::kOffV, 16384u);
+    const uint64_t kd0 = desc_k_major(base + S::kOffK), vd0 = desc_n_major(base + S::kOffV, 8192u);
     const uint32_t sd = tmem + (uint32_t)g * 128u, od = tmem + 256u + (uint32_t)g * 128u;
     unsigned n = 0, segs = 0, p_par = 0;                     // (p_par: parity of the next P, both halves)
     for (int b = lo; b < hi;) {
@@ -512,12 +513,13 @@ struct Dense {
       const uint64_t qd = desc_k_major(base + S::kOffQ + (dual ? 0 : g) * S::kTileBytes);
       const int step = dual ? 2 : 1;
       auto score = [&](int st, int half) {
-        const uint64_t kd = kd0 + (uint32_t)(st * (S::kTileBytes >> 4) + half * (8192 >> 4));
+        const uint64_t kd = kd0 + (uint32_t)(st * (S::kHalfBytes >> 4));
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t off = (uint32_t)((k >> 2) * (16384 >> 4) + (k & 3) * (32 >> 4));
-          if (k == 0) mma_ss(sd + 64u * half, qd + off, kd + off, kIdescS, 0u);
-          else mma_ss(sd + 64u * half, qd + off, kd + off, kIdescS, 1u);
+          const uint32_t q_off = (uint32_t)((k >> 2) * (16384 >> 4) + (k & 3) * (32 >> 4));
+          const uint32_t k_off = (uint32_t)((k >> 2) * (8192 >> 4) + (k & 3) * (32 >> 4));
+          if (k == 0) mma_ss(sd + 64u * half, qd + q_off, kd + k_off, kIdescS, 0u);
+          else mma_ss(sd + 64u * half, qd + q_off, kd + k_off, kIdescS, 1u);
         }
         mma_commit_to(s_full(g, half));
       };
@@ -529,67 +531,63 @@ struct Dense {
       if (blk < nb) {
         if (!wait_bar(q_full(g), segs & 1u, ctl)) return;
         ++segs;
-        unsigned m = n + (unsigned)blk;
-        int st = (int)(m % S::kStages);
-        if (!wait_bar(k_full(st), (m / S::kStages) & 1u, ctl)) return;
-        tmem_fence_after_sync();
-        score(st, 0);
-        score(st, 1);
-        release(k_empty(st));
+        // halves are numbered n, n + 1, ...: those of block blk are m and m + 1
+        unsigned m = n + 2u * (unsigned)blk;
+        auto score_when_there = [&](unsigned i, int half) {
+          const int st = (int)(i % S::kStages);
+          if (!wait_bar(k_full(st), (i / S::kStages) & 1u, ctl)) return false;
+          tmem_fence_after_sync();
+          score(st, half);
+          release(k_empty(st));
+          return true;
+        };
+        if (!score_when_there(m, 0) || !score_when_there(m + 1, 1)) return;
         uint32_t more = 0;                                   // 0 for the first products of the segment: O is overwritten
         for (; blk < nb; blk += step) {
-          const uint64_t vd = vd0 + (uint32_t)(st * (S::kTileBytes >> 4));
-          const int valid = valid_keys(x, b0 + blk);
           const bool next = blk + step < nb;
-          const unsigned mn = m + (unsigned)step;
-          const int stn = (int)(mn % S::kStages);
-          if (!wait_bar(v_full(st), (m / S::kStages) & 1u, ctl)) return;
+          const unsigned mn = m + 2u * (unsigned)step;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
+            const int st = (int)((m + half) % S::kStages), valid = valid_keys(x, b0 + blk, half);
+            const uint64_t vd = vd0 + (uint32_t)(st * (S::kHalfBytes >> 4));
+            if (!wait_bar(v_full(st), ((m + half) / S::kStages) & 1u, ctl)) return;
             if (!wait_bar(p_full(g, half), p_par, ctl)) return;
             tmem_fence_after_sync();
-            const int mine = valid - 64 * half;              // visible keys of this half
-            if (mine >= 64) {
-              mma_ts(od, sd + 64u * half, vd + (uint32_t)(half * (8192 >> 4)), kIdescO, more);
+            if (valid == 64) {
+              mma_ts(od, sd + 64u * half, vd, kIdescO, more);
 #pragma unroll
-              for (int k = 1; k < 4; ++k)
-                mma_ts(od, sd + 64u * half + 8u * k, vd + (uint32_t)(half * (8192 >> 4) + k * (2048 >> 4)), kIdescO, 1u);
+              for (int k = 1; k < 4; ++k) mma_ts(od, sd + 64u * half + 8u * k, vd + (uint32_t)(k * (2048 >> 4)), kIdescO, 1u);
               more = 1u;
             } else {
 #pragma unroll 1
-              for (int k = 0; 16 * k < mine; ++k) {
-                mma_ts(od, sd + 64u * half + 8u * k, vd + (uint32_t)(half * (8192 >> 4) + k * (2048 >> 4)), kIdescO, more);
+              for (int k = 0; 16 * k < valid; ++k) {
+                mma_ts(od, sd + 64u * half + 8u * k, vd + (uint32_t)(k * (2048 >> 4)), kIdescO, more);
                 more = 1u;
               }
             }
-            if (half == 1) release(v_empty(st));
+            release(v_empty(st));
             if (next) {
-              if (half == 0) {
-                if (!wait_bar(k_full(stn), (mn / S::kStages) & 1u, ctl)) return;
-              }
-              score(stn, half);
-              if (half == 1) release(k_empty(stn));
+              if (!score_when_there(mn + half, half)) return;
             } else {
               mma_commit_to(o_full(g, half));
             }
           }
           p_par ^= 1u;
           m = mn;
-          st = stn;
         }
       }
-      n += (unsigned)nb;
+      n += 2u * (unsigned)nb;
       b += nb;
     }
   }
 
-  // Rows of V behind the last visible key of a block: cleared, so that 0 * V is 0 whatever the page holds there.  (One warp,
+  // Rows of V behind the last visible key of a half: cleared, so that 0 * V is 0 whatever the page holds there.  (One warp,
   // before its P is handed over; rows from the next multiple of 16 on are not read.)
   __device__ __forceinline__ void clear_rows(int st, int valid) {
     const int rows = 16 - (valid & 15);
     for (int i = lane; i < rows * 8 * S::kHalves; i += 32) {
       const int r = valid + i / (8 * S::kHalves), c = i % (8 * S::kHalves);
-      *reinterpret_cast<uint4*>(smem + S::kOffV + st * S::kTileBytes + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) =
+      *reinterpret_cast<uint4*>(smem + S::kOffV + st * S::kHalfBytes + (c >> 3) * 8192 + r * 128 + (c & 7) * 16) =
           make_uint4(0, 0, 0, 0);
     }
     fence_async_shared();
@@ -722,10 +720,10 @@ struct Dense {
           tmem_st32(sh, pk);
           tmem_wait_st();
         }
-        if (half == 0 && (warp & 3) == 0) {
-          const int blk = block_of(j, dual, g), valid = valid_keys(x, b0 + blk);
+        if ((warp & 3) == 0) {
+          const int blk = block_of(j, dual, g), valid = valid_keys(x, b0 + blk, half);
           if (valid % 16 != 0) {
-            const unsigned at = n + (unsigned)blk;
+            const unsigned at = n + 2u * (unsigned)blk + (unsigned)half;
             const int st = (int)(at % S::kStages);
             if (dual || g == 0) {
               ok = wait_bar(v_full(st), (at / S::kStages) & 1u, ctl);
@@ -822,7 +820,7 @@ struct Dense {
           }
         }
       }
-      n += (unsigned)nb;
+      n += 2u * (unsigned)nb;
       b += nb;
     }
   }

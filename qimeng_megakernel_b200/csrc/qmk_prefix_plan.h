@@ -140,16 +140,19 @@ struct Plan {
   Deal dense, strips;               // all blocks to CTAs, all pieces to warps
 };
 
-// Microseconds that a call takes when `ctas` CTAs have the blocks, the longer of the two kinds (measured on B200; a piece at a CTA's share
-// of the memory bandwidth, a block of one tile at its keys' or its steps' time, one of two tiles at its steps').
+// Microseconds that a call takes when `ctas` CTAs have the blocks, the longer of the two kinds.  Measured on B200, per CTA: a block
+// of one tile 0.95 us at head size 64 and 1.75 us at 128, of two tiles 1.65 and 2.2 us; a piece 0.09 and 0.22 us, or its share of
+// 5.5 TB/s; 6 us to the first block's result and out again, 4 us for a strip.
 QMKP_HD float plan_time(const PlanDims& d, const Totals& t, int ctas) {
   const int short_units = d.prefix_len > 0 ? (t.short_tokens + d.unit_tokens - 1) / d.unit_tokens : 0;
   const bool small = t.short_tokens * d.G <= kLongRows, wide = d.head_dim == 128;
-  const float one = wide ? 1.4f : 0.85f, two = wide ? 2.0f : 1.6f, piece = wide ? 0.37f : 0.19f;
+  const float one = wide ? 1.75f : 0.95f, two = wide ? 2.2f : 1.65f;
   const float blocks = ((float)t.long_blocks * two + (float)(short_units * d.prefix_blocks) * (small ? one : two)) * (float)d.NKV;
-  const float dense = blocks > 0.f ? 3.5f + (ctas > 0 ? blocks / (float)ctas : 1e30f) : 0.f;
+  const float dense = blocks > 0.f ? 6.f + (ctas > 0 ? blocks / (float)ctas : 1e30f) : 0.f;
   const int rest = d.ctas - ctas;
-  const float few = t.pieces > 0 ? 2.5f + (rest > 0 ? (float)t.pieces * (float)d.NKV * piece / (float)rest : 1e30f) : 0.f;
+  const float pieces = (float)t.pieces * (float)d.NKV, stream = pieces * (wide ? 0.003f : 0.0015f);
+  const float work = rest > 0 ? pieces * (wide ? 0.22f : 0.09f) / (float)rest : 1e30f;
+  const float few = t.pieces > 0 ? 4.f + (work > stream ? work : stream) : 0.f;
   return dense > few ? dense : few;
 }
 // The numbers of CTAs that are weighed: i of kPlanChoices.
