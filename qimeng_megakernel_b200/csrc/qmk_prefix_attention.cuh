@@ -328,17 +328,18 @@ __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc,
   }
   if (warp == 0) {                                           // each lane weighs one division of the CTAs
     const Totals t{base.x, base.y, base.z, base.w};
-    int ctas = plan_choice(p.d, t, lane);
-    float time = plan_time(p.d, t, ctas);
+    Choice c = plan_choice(p.d, t, lane);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const float ot = __shfl_xor_sync(kFullMask, time, o);
-      const int oc = __shfl_xor_sync(kFullMask, ctas, o);
-      if (ot < time || (ot == time && oc < ctas)) { time = ot; ctas = oc; }
+      Choice x;
+      x.time = __shfl_xor_sync(kFullMask, c.time, o);
+      x.ctas = __shfl_xor_sync(kFullMask, c.ctas, o);
+      x.each = __shfl_xor_sync(kFullMask, c.each, o);
+      if (x.time < c.time || (x.time == c.time && (x.ctas < c.ctas || (x.ctas == c.ctas && x.each > c.each)))) c = x;
     }
     if (lane == 0) {
       out->t = t;
-      out->plan = make_plan(p.d, t, ctas);
+      out->plan = make_plan(p.d, t, c);
     }
   }
   __syncthreads();
@@ -813,7 +814,7 @@ struct Dense {
           }
           // whoever starts the unit says where its rows' parts are
           if (b0 == 0 && p.d.by_G.mod(tile_row) == 0) {
-            const int parts = whole ? 0 : plan.dense.owner(b + x.blocks - 1) - cta + 1;
+            const int parts = whole ? 0 : plan.dense_owner(b + x.blocks - 1) - cta + 1;
             p.dense_desc[(size_t)token * p.d.NKV + x.kvh] = make_int2(rec, parts | (tile_row << 16));
             if (x.s >= 0)
               for (int i = 0; i < p.d.G; ++i) p.strip_desc[(size_t)token * p.NH + head + i] = make_int2(0, 0);

@@ -60,6 +60,7 @@ struct PlanDims {
   int tokens, seqs, G, NKV, prefix_len, ctas, head_dim;
   int room;                         // positions a request can have: max(prefix_len, max_pages * page_size)
   int unit_tokens;                  // tokens of a unit
+  Divider by_unit;
   int prefix_blocks;
   Divider by_G, by_NKV;
 };
@@ -69,6 +70,7 @@ inline PlanDims make_dims(int tokens, int seqs, int G, int NKV, int head_dim, in
   d.room = room > prefix_len ? room : prefix_len;
   d.unit_tokens = kUnitRows / G;
   d.prefix_blocks = (prefix_len + kBlockKeys - 1) / kBlockKeys;
+  d.by_unit = make_divider(d.unit_tokens);
   d.by_G = make_divider(G);
   d.by_NKV = make_divider(NKV);
   return d;
@@ -95,7 +97,7 @@ QMKP_HD int limit_of(const PlanDims& d, const Req& r, int i) {
 QMKP_HD bool is_long(const PlanDims& d, const Req& r) { return (long long)r.n * d.G >= kLongRows; }
 
 // long requests
-QMKP_HD int units_of(const PlanDims& d, const Req& r) { return (r.n + d.unit_tokens - 1) / d.unit_tokens; }
+QMKP_HD int units_of(const PlanDims& d, const Req& r) { return d.by_unit.div(r.n + d.unit_tokens - 1); }
 QMKP_HD int unit_limit(const PlanDims& d, const Req& r, int u) {
   return limit_of(d, r, imin((u + 1) * d.unit_tokens, r.n) - 1);
 }
@@ -106,6 +108,17 @@ QMKP_HD int unit_blocks(const PlanDims& d, const Req& r, int u) {
 QMKP_HD int own_keys(const PlanDims& d, const Req& r) { return r.n > 0 ? imax(0, limit_of(d, r, r.n - 1) - d.prefix_len) : 0; }
 QMKP_HD int strips_of(const PlanDims& d, const Req& r) { return (r.n * d.G + kStripRows - 1) / kStripRows; }   // of a KV head
 QMKP_HD int pieces_of(const PlanDims& d, const Req& r) { return kStripCost + (own_keys(d, r) + kPieceKeys - 1) / kPieceKeys; }
+
+// Quotients where the exact one takes too long: of small whole numbers (a < 2^21, exact: half a unit is far above the error of the
+// reciprocal), and for estimates.
+QMKP_HD float about(float a, float b) {
+#if defined(__CUDA_ARCH__)
+  return __fdividef(a, b);
+#else
+  return a / b;
+#endif
+}
+QMKP_HD int small_div(int a, int b) { return (int)about((float)a + 0.5f, (float)b); }
 
 // `total` things dealt to n takers as contiguous ranges that differ by one at most (with fewer things than takers the first
 // ones get one each, so owners of neighbouring things are always neighbours).
@@ -137,48 +150,81 @@ struct Plan {
   int unit_total;                   // units per KV head
   int blocks;                       // per KV head
   int dense_ctas;                   // CTAs with blocks; the others have pieces
-  Deal dense, strips;               // all blocks to CTAs, all pieces to warps
+  int span;                         // the blocks are dealt span by span: one unit of a KV head, or all there are
+  Deal dense, strips;               // a span's blocks to CTAs, all pieces to warps
+  QMKP_HD int dense_first(int c) const {
+    const int s = small_div(c, dense.n);
+    return s * span + dense.first(c - s * dense.n);
+  }
+  QMKP_HD int dense_owner(int b) const {
+    const int s = b / span;
+    return s * dense.n + dense.owner(b - s * span);
+  }
 };
 
-// Microseconds that a call takes when `ctas` CTAs have the blocks, the longer of the two kinds.  Measured on B200, per CTA: a block
-// of one tile 0.95 us at head size 64 and 1.75 us at 128, of two tiles 1.65 and 2.2 us; a piece 0.09 and 0.22 us, or its share of
-// 5.5 TB/s; 6 us to the first block's result and out again, 4 us for a strip.
-QMKP_HD float plan_time(const PlanDims& d, const Totals& t, int ctas) {
-  const int short_units = d.prefix_len > 0 ? (t.short_tokens + d.unit_tokens - 1) / d.unit_tokens : 0;
+// A way to divide the CTAs: `ctas` of them have the blocks, with `each` > 0 as many to every unit and each of them blocks of one
+// unit only.
+struct Choice {
+  int ctas, each;
+  float time;
+};
+// Estimated microseconds of a call, the longer of blocks and strips.  Measured on B200, per CTA: a block of one tile 0.95 us at head
+// size 64 and 2.2 us at 128, of two tiles 1.65 and 2.2 us; a piece 0.105 and 0.22 us, or its share of 5.5 TB/s; 6 us to the first
+// block's result and out again, 5 us for every unit more; 4 us for a strip.
+QMKP_HD int short_units_of(const PlanDims& d, const Totals& t) {
+  return d.prefix_len > 0 ? d.by_unit.div(t.short_tokens + d.unit_tokens - 1) : 0;
+}
+QMKP_HD float choice_time(const PlanDims& d, const Totals& t, int short_units, int ctas, int each) {
   const bool small = t.short_tokens * d.G <= kLongRows, wide = d.head_dim == 128;
-  const float one = wide ? 1.75f : 0.95f, two = wide ? 2.2f : 1.65f;
-  const float blocks = ((float)t.long_blocks * two + (float)(short_units * d.prefix_blocks) * (small ? one : two)) * (float)d.NKV;
-  const float dense = blocks > 0.f ? 6.f + (ctas > 0 ? blocks / (float)ctas : 1e30f) : 0.f;
-  const int rest = d.ctas - ctas;
+  const float one = wide ? 2.2f : 0.95f, two = wide ? 2.2f : 1.65f, block = small ? one : two;
+  const int units = (t.long_units + short_units) * d.NKV, rest = d.ctas - ctas;
+  float dense = 0.f;
+  if (units > 0 && ctas == 0) dense = 1e30f;
+  else if (units > 0 && each > 0) dense = 6.f + (about((float)d.prefix_blocks, (float)each) + 0.5f) * block;
+  else if (units > 0) {
+    const float more = about((float)units, (float)ctas) + 1.f, most = (float)(units - 1);
+    dense = 6.f + 5.f * (more < most ? more : most) +
+            about(((float)t.long_blocks * two + (float)(short_units * d.prefix_blocks) * block) * (float)d.NKV, (float)ctas);
+  }
   const float pieces = (float)t.pieces * (float)d.NKV, stream = pieces * (wide ? 0.003f : 0.0015f);
-  const float work = rest > 0 ? pieces * (wide ? 0.22f : 0.09f) / (float)rest : 1e30f;
+  const float work = rest > 0 ? about(pieces * (wide ? 0.22f : 0.105f), (float)rest) : 1e30f;
   const float few = t.pieces > 0 ? 4.f + (work > stream ? work : stream) : 0.f;
   return dense > few ? dense : few;
 }
-// The numbers of CTAs that are weighed: i of kPlanChoices.
+// The divisions that are weighed: i of kPlanChoices.
 constexpr int kPlanChoices = 32;
-QMKP_HD int plan_choice(const PlanDims& d, const Totals& t, int i) {
-  const int all = (t.long_blocks + (d.prefix_len > 0 ? (t.short_tokens + d.unit_tokens - 1) / d.unit_tokens * d.prefix_blocks : 0)) * d.NKV;
-  int ctas = t.pieces == 0 ? d.ctas : (i + 1) * (d.ctas - 1) / kPlanChoices;
-  ctas = imax(ctas, 1);
-  return imin(ctas, all);                // (no blocks: none)
+QMKP_HD Choice plan_choice(const PlanDims& d, const Totals& t, int i) {
+  const int short_units = short_units_of(d, t), units = short_units * d.NKV;
+  const int blocks = (t.long_blocks + short_units * d.prefix_blocks) * d.NKV;
+  Choice c;
+  c.ctas = t.pieces == 0 ? d.ctas : (i + 1) * (d.ctas - 1) / kPlanChoices;
+  c.ctas = imin(imax(c.ctas, 1), blocks);   // (no blocks: none)
+  c.each = 0;
+  c.time = choice_time(d, t, short_units, c.ctas, 0);
+  if (t.long_units == 0 && units > 0 && c.ctas >= units) {
+    const int each = imin(small_div(c.ctas, units), d.prefix_blocks);
+    const float time = choice_time(d, t, short_units, units * each, each);
+    if (time <= c.time) { c.ctas = units * each; c.each = each; c.time = time; }
+  }
+  return c;
 }
-QMKP_HD Plan make_plan(const PlanDims& d, const Totals& t, int ctas) {
+QMKP_HD Plan make_plan(const PlanDims& d, const Totals& t, const Choice& c) {
   Plan p;
-  const int short_units = d.prefix_len > 0 ? (t.short_tokens + d.unit_tokens - 1) / d.unit_tokens : 0;
+  const int short_units = short_units_of(d, t);
   p.unit_total = t.long_units + short_units;
   p.blocks = t.long_blocks + short_units * d.prefix_blocks;
-  p.dense_ctas = ctas;
-  p.dense = deal(p.blocks * d.NKV, ctas);
-  p.strips = deal(t.pieces * d.NKV, (d.ctas - ctas) * kStripWarps);
+  p.dense_ctas = c.ctas;
+  p.span = c.each ? d.prefix_blocks : p.blocks * d.NKV;
+  p.dense = deal(p.span, c.each ? c.each : c.ctas);
+  p.strips = deal(t.pieces * d.NKV, (d.ctas - c.ctas) * kStripWarps);
   return p;
 }
 // Blocks [lo, hi) of CTA c.
 QMKP_HD void dense_range(const Plan& p, int c, int& lo, int& hi) {
   lo = hi = 0;
   if (c >= p.dense_ctas) return;
-  lo = p.dense.first(c);
-  hi = p.dense.first(c + 1);
+  lo = p.dense_first(c);
+  hi = p.dense_first(c + 1);
 }
 // Pieces [lo, hi) of a warp of CTA c and the warp's number among those that have any (neighbours sit in neighbouring CTAs).
 QMKP_HD int piece_range(const PlanDims& d, const Plan& p, int c, int warp, int& lo, int& hi) {

@@ -18,6 +18,7 @@ using namespace qmkp;
     }                                                                 \
   } while (0)
 static int g_case;
+static int aligned;
 
 struct Walk { std::vector<std::vector<int>> seen; };   // [row of the step * NKV + kvh][key] -> times
 
@@ -65,11 +66,13 @@ int main() {
       stk.push_back(t.short_tokens);
       pc.push_back((int)t.pieces);
     }
-    int choice = plan_choice(d, t, 0);
+    Choice choice = plan_choice(d, t, 0);
     for (int i = 1; i < kPlanChoices; ++i) {
-      const int other = plan_choice(d, t, i);
-      if (plan_time(d, t, other) < plan_time(d, t, choice)) choice = other;
+      const Choice other = plan_choice(d, t, i);
+      if (other.time < choice.time) choice = other;
     }
+    if (g_case % 3 == 0) choice = plan_choice(d, t, pick(0, kPlanChoices - 1));   // (any of them has to do)
+    aligned += choice.each > 0;
     const Plan p = make_plan(d, t, choice);
     const int pieces = t.pieces * d.NKV, all_blocks = p.blocks * d.NKV;
     CHECK(p.unit_total <= max_units(d));
@@ -129,8 +132,8 @@ int main() {
         const int rec = c + kvh * p.unit_total + index;
         CHECK(rec < max_dense_records(d) && !record[rec]);
         record[rec] = 1;
-        const int parts = p.dense.owner(b - b0 + blocks - 1) - p.dense.owner(b - b0) + 1;
-        CHECK(p.dense.owner(b) == c && p.dense.owner(b + (b1 - b0) - 1) == c);
+        const int parts = p.dense_owner(b - b0 + blocks - 1) - p.dense_owner(b - b0) + 1;
+        CHECK(p.dense_owner(b) == c && p.dense_owner(b + (b1 - b0) - 1) == c);
         for (int i = 0; i < d.unit_tokens; ++i) {
           int tok, lim;
           if (s >= 0) {
@@ -214,6 +217,7 @@ int main() {
         for (int k = 0; k < named[i].n; ++k) CHECK(written[i][k] == named[i].rec + k);
       }
   }
+  CHECK(aligned > 100);
   std::printf("prefix plan ok\n");
   return 0;
 }
