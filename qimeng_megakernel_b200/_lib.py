@@ -54,6 +54,7 @@ class Status(C.Structure):
                 ("seen", C.c_uint32), ("expected", C.c_uint32), ("detail", C.c_int32), ("reserved", C.c_int32)]
 
 
+# The argument structures of the paged-cache entry points, which take their bytes (paged.py packs them directly).
 class BlockTablesArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("lengths", "free_pages", "prefix_table", "tables", "used")] + \
                [(n, C.c_int32) for n in ("seqs", "num_free", "prefix_pages", "page_size", "max_pages")]
@@ -104,10 +105,10 @@ SYMBOLS = [
     ("qmk_static_set_wait_first_dependency", C.c_int, [C.c_int, C.c_int32]),
     ("qmk_generate_device", C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]),
     ("qmk_static_last_cuda_error", C.c_char_p, []),
-    ("qmk_build_block_tables", C.c_int, [C.POINTER(BlockTablesArgs), C.c_int, C.c_void_p]),
-    ("qmk_build_slot_map", C.c_int, [C.POINTER(SlotMapArgs), C.c_int, C.c_void_p]),
+    ("qmk_build_block_tables", C.c_int, [C.c_char_p, C.c_int, C.c_void_p]),
+    ("qmk_build_slot_map", C.c_int, [C.c_char_p, C.c_int, C.c_void_p]),
     ("qmk_prefix_attention_workspace", C.c_int64, [C.c_int32] * 6 + [C.c_int]),
-    ("qmk_prefix_attention", C.c_int, [C.POINTER(PrefixAttentionArgs), C.c_int, C.c_void_p]),
+    ("qmk_prefix_attention", C.c_int, [C.c_char_p, C.c_int, C.c_void_p]),
     ("qmk_paged_last_cuda_error", C.c_char_p, []),
     ("qmk_destroy", None, [C.c_void_p]),
     ("qmk_strerror", C.c_char_p, [C.c_int]),

@@ -19,8 +19,9 @@ multi_batch/decode_schedule/globs.py:27-28); this module has no counterpart ther
 """
 from __future__ import annotations
 
-import ctypes as C
+import functools
 import math
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -60,6 +61,23 @@ class SlotMap:
                    torch.empty(tokens, dtype=torch.uint8, device=device), i32(seqs + 1), i32(seqs))
 
 
+# The library's argument structures, packed in one call (the ctypes structures of _lib take several times as long to fill).
+_TABLES = struct.Struct("@5P5i0P")
+_SLOTS = struct.Struct("@9P4i0P")
+_ATTENTION = struct.Struct("@9P2q9ifPq0P")
+
+
+def _flat(n: int | None, *tensors) -> bool:
+    """Contiguous int32 vectors (of n entries) all of them: the quick form of _check, which says what is wrong."""
+    try:
+        for t in tensors:
+            if t.dtype is not torch.int32 or t.ndim != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+                return False
+    except AttributeError:
+        return False
+    return True
+
+
 def _check(name: str, t, dtype: torch.dtype, dim: int) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
@@ -71,13 +89,13 @@ def _check(name: str, t, dtype: torch.dtype, dim: int) -> None:
         raise ValueError(f"{name} must be contiguous")
 
 
-def _on(device: torch.device, **tensors) -> None:
-    """Every tensor of the call is on one CUDA device (the last check: what it says is about a call that is right otherwise)."""
-    if device.type != "cuda":
-        raise ValueError(f"the tensors must be CUDA tensors (there is no CPU path), got {device}")
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+def _on(index: int, names: str, *tensors) -> None:
+    """Every tensor of the call is on CUDA device `index` (the last check: what it says is about a call that is right otherwise)."""
+    if index < 0:
+        raise ValueError("the tensors must be CUDA tensors (there is no CPU path)")
+    for i, t in enumerate(tensors):
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{names.split()[i]} is on {t.device}, expected cuda:{index}")
 
 
 def _page_size(page_size: int) -> int:
@@ -86,8 +104,12 @@ def _page_size(page_size: int) -> int:
     return int(page_size)
 
 
-def _call(fn, args, device: torch.device) -> None:
-    code = fn(C.byref(args), device.index, torch.cuda.current_stream(device).cuda_stream)
+# (the raw handle: building a torch.cuda.Stream takes longer than the rest of a call's preparation)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _call(fn, args: bytes, index: int) -> None:
+    code = fn(args, index, _stream(index))
     if code != 0:
         raise _lib.QmkError(code, _lib.load().qmk_paged_last_cuda_error().decode() if code == -3 else "")
 
@@ -100,9 +122,9 @@ def build_block_tables(lengths: torch.Tensor, free_pages: torch.Tensor, *, page_
     `free_pages` (int32) in order, behind those of the rows before it; the rest of the row is -1.  `used` holds the
     pages taken from `free_pages` (more than there are when it ran out: the entries it could not give are -1) and the
     number of rows cut off at `max_pages`."""
-    _check("lengths", lengths, torch.int32, 1)
-    device = lengths.device
-    _check("free_pages", free_pages, torch.int32, 1)
+    if not _flat(None, lengths, free_pages):
+        _check("lengths", lengths, torch.int32, 1)
+        _check("free_pages", free_pages, torch.int32, 1)
     seqs, max_pages, shared, page_size = lengths.shape[0], int(max_pages), 0, _page_size(page_size)
     if prefix_table is not None:
         _check("prefix_table", prefix_table, torch.int32, 1)
@@ -114,18 +136,18 @@ def build_block_tables(lengths: torch.Tensor, free_pages: torch.Tensor, *, page_
     if shared > max_pages:
         raise ValueError(f"prefix_table has {shared} pages, more than max_pages = {max_pages}")
     if out is None:
-        out = BlockTables.empty(seqs, max_pages, device)
+        out = BlockTables.empty(seqs, max_pages, lengths.device)
     else:
         _check("out.tables", out.tables, torch.int32, 2)
         _check("out.used", out.used, torch.int32, 1)
         if out.tables.shape != (seqs, max_pages) or out.used.shape != (2,):
             raise ValueError(f"out: expected tables {(seqs, max_pages)} and used (2,), got {tuple(out.tables.shape)} "
                              f"and {tuple(out.used.shape)}")
-    _on(device, free_pages=free_pages, prefix_table=prefix_table, out=out.tables, used=out.used)
-    args = _lib.BlockTablesArgs(lengths.data_ptr(), free_pages.data_ptr(),
-                                prefix_table.data_ptr() if shared else None, out.tables.data_ptr(), out.used.data_ptr(),
-                                seqs, free_pages.shape[0], shared, page_size, max_pages)
-    _call(_lib.load().qmk_build_block_tables, args, device)
+    index = lengths.get_device()
+    _on(index, "free_pages prefix_table out.tables out.used", free_pages, prefix_table, out.tables, out.used)
+    args = _TABLES.pack(lengths.data_ptr(), free_pages.data_ptr(), prefix_table.data_ptr() if shared else 0,
+                        out.tables.data_ptr(), out.used.data_ptr(), seqs, free_pages.shape[0], shared, page_size, max_pages)
+    _call(_lib.load().qmk_build_block_tables, args, index)
     return out
 
 
@@ -136,10 +158,10 @@ def build_slot_map(block_tables: torch.Tensor, kv_lengths: torch.Tensor, new_len
     outputs: what does not fit is cut off (the request that straddles it appends fewer), what is left over is filled
     with slot -1, position 0, request -1, inactive.  `out.kv_lengths` may not be `kv_lengths` itself."""
     _check("block_tables", block_tables, torch.int32, 2)
-    device = block_tables.device
-    _check("kv_lengths", kv_lengths, torch.int32, 1)
-    _check("new_lengths", new_lengths, torch.int32, 1)
     seqs, max_pages = block_tables.shape
+    if not _flat(seqs, kv_lengths, new_lengths):
+        _check("kv_lengths", kv_lengths, torch.int32, 1)
+        _check("new_lengths", new_lengths, torch.int32, 1)
     tokens, page_size = int(tokens), _page_size(page_size)
     if seqs < 1 or max_pages < 1:
         raise ValueError(f"block_tables: empty shape {tuple(block_tables.shape)}")
@@ -149,8 +171,10 @@ def build_slot_map(block_tables: torch.Tensor, kv_lengths: torch.Tensor, new_len
     if not 1 <= tokens < 2 ** 31:
         raise ValueError(f"tokens {tokens}: expected at least 1")
     if out is None:
-        out = SlotMap.empty(seqs, tokens, device)
-    else:
+        out = SlotMap.empty(seqs, tokens, block_tables.device)
+    elif not (_flat(tokens, out.positions, out.seq_ids) and _flat(seqs, out.kv_lengths) and _flat(seqs + 1, out.cu_tokens)
+              and out.slots.dtype is torch.int64 and out.slots.shape == (tokens,) and out.slots.is_contiguous()
+              and out.active.dtype is torch.uint8 and out.active.shape == (tokens,) and out.active.is_contiguous()):
         for name, dtype, n in (("slots", torch.int64, tokens), ("positions", torch.int32, tokens),
                                ("seq_ids", torch.int32, tokens), ("active", torch.uint8, tokens),
                                ("cu_tokens", torch.int32, seqs + 1), ("kv_lengths", torch.int32, seqs)):
@@ -158,14 +182,15 @@ def build_slot_map(block_tables: torch.Tensor, kv_lengths: torch.Tensor, new_len
             _check(f"out.{name}", t, dtype, 1)
             if t.shape[0] != n:
                 raise ValueError(f"out.{name}: expected {n} entries, got {t.shape[0]}")
-        if out.kv_lengths.data_ptr() == kv_lengths.data_ptr():
-            raise ValueError("out.kv_lengths must not be kv_lengths itself")
-    _on(device, kv_lengths=kv_lengths, new_lengths=new_lengths, slots=out.slots, positions=out.positions,
-        seq_ids=out.seq_ids, active=out.active, cu_tokens=out.cu_tokens, out=out.kv_lengths)
-    args = _lib.SlotMapArgs(block_tables.data_ptr(), kv_lengths.data_ptr(), new_lengths.data_ptr(), out.slots.data_ptr(),
-                            out.positions.data_ptr(), out.seq_ids.data_ptr(), out.active.data_ptr(),
-                            out.cu_tokens.data_ptr(), out.kv_lengths.data_ptr(), seqs, tokens, page_size, max_pages)
-    _call(_lib.load().qmk_build_slot_map, args, device)
+    if out.kv_lengths.data_ptr() == kv_lengths.data_ptr():
+        raise ValueError("out.kv_lengths must not be kv_lengths itself")
+    index = block_tables.get_device()
+    _on(index, "kv_lengths new_lengths out.slots out.positions out.seq_ids out.active out.cu_tokens out.kv_lengths", kv_lengths,
+        new_lengths, out.slots, out.positions, out.seq_ids, out.active, out.cu_tokens, out.kv_lengths)
+    args = _SLOTS.pack(block_tables.data_ptr(), kv_lengths.data_ptr(), new_lengths.data_ptr(), out.slots.data_ptr(),
+                       out.positions.data_ptr(), out.seq_ids.data_ptr(), out.active.data_ptr(), out.cu_tokens.data_ptr(),
+                       out.kv_lengths.data_ptr(), seqs, tokens, page_size, max_pages)
+    _call(_lib.load().qmk_build_slot_map, args, index)
     return out
 
 
@@ -185,13 +210,19 @@ def _rows(name: str, t) -> None:
                          f"data 16-byte aligned; got strides {stride}")
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(tokens: int, seqs: int, heads: int, kv_heads: int, size: int, prefix_len: int, index: int) -> int:
+    n = _lib.load().qmk_prefix_attention_workspace(tokens, seqs, heads, kv_heads, size, prefix_len, index)
+    if n < 0:
+        raise _lib.QmkError(int(n))
+    return int(n)
+
+
 def attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, seqs: int, *, prefix_len: int = 0) -> torch.Tensor:
     """The workspace of `prefix_attention` for calls with these shapes: a program that keeps it saves the allocation.  Calls
     that may run at the same time (two streams, two captured graphs) need one each."""
-    n = _lib.load().qmk_prefix_attention_workspace(q.shape[0], seqs, q.shape[1], k_pages.shape[2], q.shape[2], prefix_len,
-                                                   q.device.index)
-    if n < 0:
-        raise _lib.QmkError(int(n))
+    _on(q.get_device(), "k_pages", k_pages)
+    n = _workspace_bytes(q.shape[0], int(seqs), q.shape[1], k_pages.shape[2], q.shape[2], int(prefix_len), q.get_device())
     return torch.empty(n, dtype=torch.uint8, device=q.device)
 
 
@@ -212,12 +243,12 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     scale: 1 / sqrt(HD) by default.  lse: optional float32 [tokens, NH], receives the natural logarithm of the sum of
     exponentials.  Sums are held in 32 bits; probabilities are rounded to bf16 before they meet V.  Inference only."""
     _rows("q", q)
-    device = q.device
     _check("k_pages", k_pages, torch.bfloat16, 4)
     _check("v_pages", v_pages, torch.bfloat16, 4)
     _check("block_tables", block_tables, torch.int32, 2)
-    _check("kv_lengths", kv_lengths, torch.int32, 1)
-    _check("cu_tokens", cu_tokens, torch.int32, 1)
+    if not _flat(None, kv_lengths, cu_tokens):
+        _check("kv_lengths", kv_lengths, torch.int32, 1)
+        _check("cu_tokens", cu_tokens, torch.int32, 1)
     tokens, heads, size = q.shape
     num_pages, page_size, kv_heads, kv_size = k_pages.shape
     seqs, max_pages = block_tables.shape
@@ -250,7 +281,7 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     if q.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("prefix_attention has no gradient: call it under torch.inference_mode() or torch.no_grad()")
     if out is None:
-        out = torch.zeros(tokens, heads, size, dtype=torch.bfloat16, device=device)
+        out = torch.zeros(tokens, heads, size, dtype=torch.bfloat16, device=q.device)
     else:
         _rows("out", out)
         if out.shape != q.shape:
@@ -261,24 +292,21 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         _check("lse", lse, torch.float32, 2)
         if lse.shape != (tokens, heads):
             raise ValueError(f"lse: expected shape {(tokens, heads)}, got {tuple(lse.shape)}")
-    _on(device, k_pages=k_pages, v_pages=v_pages, block_tables=block_tables, kv_lengths=kv_lengths, cu_tokens=cu_tokens,
-        prefix_table=prefix_table if prefix_len else None, out=out, lse=lse, workspace=workspace)
+    index = q.get_device()
+    _on(index, "k_pages v_pages block_tables kv_lengths cu_tokens prefix_table out lse workspace", k_pages, v_pages, block_tables,
+        kv_lengths, cu_tokens, prefix_table if prefix_len else None, out, lse, workspace)
     if tokens == 0:
         return out
-    lib = _lib.load()
-    need = lib.qmk_prefix_attention_workspace(tokens, seqs, heads, kv_heads, size, prefix_len, device.index)
-    if need < 0:
-        raise _lib.QmkError(int(need))
+    need = _workspace_bytes(tokens, seqs, heads, kv_heads, size, prefix_len, index)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    else:
-        if workspace.shape[0] < need:
-            raise ValueError(f"workspace has {workspace.shape[0]} bytes, the call needs {need}")
-    args = _lib.PrefixAttentionArgs(q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
-                                    k_pages.data_ptr(), v_pages.data_ptr(), block_tables.data_ptr(), kv_lengths.data_ptr(),
-                                    cu_tokens.data_ptr(), prefix_table.data_ptr() if prefix_len else None,
-                                    q.stride(0) if tokens > 1 else heads * size, out.stride(0) if tokens > 1 else heads * size,
-                                    tokens, seqs, heads, kv_heads, size, page_size, num_pages, max_pages, prefix_len, scale,
-                                    workspace.data_ptr(), workspace.shape[0])
-    _call(lib.qmk_prefix_attention, args, device)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.shape[0] < need:
+        raise ValueError(f"workspace has {workspace.shape[0]} bytes, the call needs {need}")
+    one = tokens == 1                        # (the stride of a single token means nothing)
+    args = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), k_pages.data_ptr(),
+                           v_pages.data_ptr(), block_tables.data_ptr(), kv_lengths.data_ptr(), cu_tokens.data_ptr(),
+                           prefix_table.data_ptr() if prefix_len else 0, heads * size if one else q.stride(0),
+                           heads * size if one else out.stride(0), tokens, seqs, heads, kv_heads, size, page_size,
+                           num_pages, max_pages, prefix_len, scale, workspace.data_ptr(), workspace.shape[0])
+    _call(_lib.load().qmk_prefix_attention, args, index)
     return out

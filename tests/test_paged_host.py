@@ -98,6 +98,15 @@ def test_attention_refusals(paged):
     refused(ValueError, "no CPU path", f)
 
 
+def test_packed_arguments_match_the_structures(paged):
+    from qimeng_megakernel_b200 import _lib
+    for packed, structure in ((paged._TABLES, _lib.BlockTablesArgs), (paged._SLOTS, _lib.SlotMapArgs),
+                              (paged._ATTENTION, _lib.PrefixAttentionArgs)):
+        assert packed.size == C.sizeof(structure)
+        values = [i + 1 for i in range(len(structure._fields_))]
+        assert packed.pack(*values) == bytes(structure(*values))
+
+
 def test_plan_walks_every_key_once(tmp_path):
     """The division of an attention call's work (tests/prefix_plan_sim.cpp includes the header the kernel is compiled with)."""
     exe = tmp_path / "prefix_plan_sim"
@@ -119,7 +128,7 @@ def test_c_entries_refuse_before_they_launch(paged):
         a = dict(lengths=P, free_pages=P, prefix_table=P, tables=P, used=P, seqs=2, num_free=3, prefix_pages=1, page_size=16,
                  max_pages=4)
         a.update(kw)
-        return lib.qmk_build_block_tables(C.byref(_lib.BlockTablesArgs(**a)), 0, None)
+        return lib.qmk_build_block_tables(bytes(_lib.BlockTablesArgs(**a)), 0, None)
 
     for kw in (dict(lengths=None), dict(tables=None), dict(used=None), dict(free_pages=None), dict(prefix_table=None),
                dict(seqs=0), dict(num_free=-1), dict(prefix_pages=-1), dict(page_size=0), dict(page_size=512),
@@ -130,7 +139,7 @@ def test_c_entries_refuse_before_they_launch(paged):
         a = dict(block_tables=P, kv_lengths=P, new_lengths=P, slots=P, positions=P, seq_ids=P, active=P, cu_tokens=P,
                  kv_lengths_out=2 * P, seqs=2, tokens=3, page_size=16, max_pages=4)
         a.update(kw)
-        return lib.qmk_build_slot_map(C.byref(_lib.SlotMapArgs(**a)), 0, None)
+        return lib.qmk_build_slot_map(bytes(_lib.SlotMapArgs(**a)), 0, None)
 
     for name in ("block_tables", "kv_lengths", "new_lengths", "slots", "positions", "seq_ids", "active", "cu_tokens",
                  "kv_lengths_out"):
@@ -146,7 +155,7 @@ def test_c_entries_refuse_before_they_launch(paged):
                  page_size=16, num_pages=6, max_pages=4, prefix_len=32, scale=0.125, workspace=P,
                  workspace_bytes=max(need, 1 << 30))
         a.update(kw)
-        return lib.qmk_prefix_attention(C.byref(_lib.PrefixAttentionArgs(**a)), 0, None)
+        return lib.qmk_prefix_attention(bytes(_lib.PrefixAttentionArgs(**a)), 0, None)
 
     for name in ("q", "out", "k_pages", "v_pages", "block_tables", "kv_lengths", "cu_tokens", "prefix_table"):
         assert attn(**{name: None}) == -1, name
