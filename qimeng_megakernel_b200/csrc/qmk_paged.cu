@@ -58,9 +58,9 @@ extern "C" int qmk_build_block_tables(const qmk_block_tables_args* a, int device
   p.lengths = a->lengths; p.free_pages = a->free_pages; p.prefix_table = a->prefix_table;
   p.tables = a->tables; p.used = a->used;
   p.seqs = a->seqs; p.num_free = a->num_free; p.prefix_pages = a->prefix_pages; p.page_shift = shift; p.max_pages = a->max_pages;
-  int rows = (a->seqs + 295) / 296;
-  if (rows < 8) rows = 8;
-  if (rows > kTableThreads) rows = kTableThreads;
+  // a row per warp while the CTAs fit the machine at once (eight a multiprocessor), more beyond
+  int rows = kTableThreads / 32;
+  while ((long long)rows * 8 * 148 < a->seqs && rows < kTableThreads) rows *= 2;
   p.rows_per_cta = rows;
   block_tables_kernel<<<(unsigned)((a->seqs + rows - 1) / rows), kTableThreads, 0, (cudaStream_t)cuda_stream>>>(p);
   const cudaError_t e = cudaGetLastError();
