@@ -407,7 +407,25 @@ int64_t qmk_prefix_attention_workspace(int32_t tokens, int32_t seqs, int32_t num
                                        int32_t head_dim, int32_t prefix_len, int device);
 int qmk_prefix_attention(const qmk_prefix_attention_args* args, int device, void* cuda_stream);
 
-/* Text behind the last QMK_ERR_CUDA that one of these three returned to the calling thread. */
+/* One decode step on a paged cache whose sequences share a prefix: the launches of qmk_decode_step cut at every layer's attention,
+ * which is qmk_prefix_attention.  The state is bound with k_cache / v_cache = the pools of all layers, [L, num_pages, page_size,
+ * NKV, HD] (kv_batch = num_pages, kv_seq_len = page_size), position_ids, active_mask and kv_slots (the rows' requests; not read
+ * here), all of them `batch` rows as qmk_build_slot_map leaves them; `slots` says where each row's K and V go.  An active row whose
+ * position or slot is out of range is switched off and reported (qmk_poll_status).  Batched kernel, any batch; no model
+ * parallelism.  A refused call launches nothing.  Asynchronous; a step can be captured into a CUDA graph. */
+typedef struct qmk_paged_step_args {
+  const int32_t* block_tables;  /* [seqs, max_pages] */
+  const int32_t* kv_lengths;    /* [seqs]: the step's tokens included */
+  const int32_t* cu_tokens;     /* [seqs + 1] */
+  const int64_t* slots;         /* [batch] */
+  const int32_t* prefix_table;  /* [prefix_len / page_size] (may be NULL when prefix_len is 0) */
+  int32_t seqs, max_pages, prefix_len;
+  void* workspace;              /* of qmk_prefix_attention for `batch` tokens */
+  int64_t workspace_bytes;
+} qmk_paged_step_args;
+int qmk_decode_step_paged(qmk_handle* h, const qmk_paged_step_args* args, void* cuda_stream);
+
+/* Text behind the last QMK_ERR_CUDA that one of the first three returned to the calling thread. */
 const char* qmk_paged_last_cuda_error(void);
 
 void qmk_destroy(qmk_handle* h);

@@ -18,6 +18,6 @@ __all__ = ["Globals", "ModelConfig", "LlamaConfig", "STATIC_MEGAKERNEL", "HARDWA
 
 def __getattr__(name: str):
     import importlib
-    if name in ("mk_kernel", "decode", "synthetic", "rope", "prefill", "registry"):
+    if name in ("mk_kernel", "decode", "synthetic", "rope", "prefill", "registry", "paged"):
         return importlib.import_module(f".{name}", __name__)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -75,6 +75,12 @@ class PrefixAttentionArgs(C.Structure):
                [("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
+class PagedStepArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("block_tables", "kv_lengths", "cu_tokens", "slots", "prefix_table")] + \
+               [(n, C.c_int32) for n in ("seqs", "max_pages", "prefix_len")] + \
+               [("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 # Every symbol include/qmk_b200.h declares: (name, restype, argtypes).
 SYMBOLS = [
     ("qmk_create", C.c_int, [C.POINTER(ModelDesc), C.POINTER(WeightPtrs), C.c_int, C.POINTER(C.c_void_p)]),
@@ -109,6 +115,7 @@ SYMBOLS = [
     ("qmk_build_slot_map", C.c_int, [C.c_char_p, C.c_int, C.c_void_p]),
     ("qmk_prefix_attention_workspace", C.c_int64, [C.c_int32] * 6 + [C.c_int]),
     ("qmk_prefix_attention", C.c_int, [C.c_char_p, C.c_int, C.c_void_p]),
+    ("qmk_decode_step_paged", C.c_int, [C.c_void_p, C.POINTER(PagedStepArgs), C.c_void_p]),
     ("qmk_paged_last_cuda_error", C.c_char_p, []),
     ("qmk_destroy", None, [C.c_void_p]),
     ("qmk_strerror", C.c_char_p, [C.c_int]),

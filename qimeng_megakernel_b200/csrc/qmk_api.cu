@@ -12,6 +12,7 @@
 
 #include "../../include/qmk_b200.h"
 #include "qmk_batch_host.h"
+#include "qmk_paged_host.h"
 #include "qmk_megakernel.cuh"
 
 using namespace qmk;
@@ -220,7 +221,8 @@ extern "C" int qmk_bind_state(qmk_handle* h, const qmk_state_ptrs* s) {
   return QMK_OK;
 }
 
-static int batched_launch(qmk_handle* h, int pos, int phase_begin, int phase_end, int wait_first, cudaStream_t stream) {
+static int batched_launch(qmk_handle* h, int pos, int phase_begin, int phase_end, int wait_first, cudaStream_t stream,
+                          const int64_t* kv_rows = nullptr) {
   int rc = ensure_bctx(h);
   if (rc) return rc;
   qmkb_launch_args a;
@@ -231,6 +233,7 @@ static int batched_launch(qmk_handle* h, int pos, int phase_begin, int phase_end
   a.cooperative = h->cooperative;
   a.timeout_cycles = h->timeout_cycles;
   a.trace = h->trace;
+  a.kv_rows = kv_rows;
   rc = qmkb_launch(h->bctx, &h->st, &a, stream, h->cuda_err, sizeof(h->cuda_err));
   if (rc) return rc;
   h->launches++;
@@ -525,6 +528,61 @@ extern "C" int qmk_set_wait_first_dependency(qmk_handle* h, int32_t on) {
   if (!h) return QMK_ERR_INVALID_ARG;
   h->wait_first = on ? 1 : 0;
   return QMK_OK;
+}
+
+extern "C" int qmk_decode_step_paged(qmk_handle* h, const qmk_paged_step_args* a, void* cuda_stream) {
+  if (!h || !a) return QMK_ERR_INVALID_ARG;
+  if (!h->bound) return QMK_ERR_NOT_BOUND;
+  const qmk_model_desc& d = h->desc;
+  const qmk_state_ptrs& st = h->st;
+  if (d.ep_world > 1 || d.tp_world > 1) return QMK_ERR_UNSUPPORTED_MODEL;
+  if (!st.position_ids || !st.active_mask || !st.kv_slots || st.kv_batch < 1 || !a->slots || d.num_layers < 1) return QMK_ERR_INVALID_ARG;
+  // every layer's attention on the layer's part of the pool
+  qmk_prefix_attention_args t;
+  memset(&t, 0, sizeof(t));
+  t.q = st.q_post_rope;
+  t.out = st.attn_out;
+  t.k_pages = st.k_cache;
+  t.v_pages = st.v_cache;
+  t.block_tables = a->block_tables;
+  t.kv_lengths = a->kv_lengths;
+  t.cu_tokens = a->cu_tokens;
+  t.prefix_table = a->prefix_table;
+  t.q_token_stride = t.out_token_stride = (int64_t)d.num_attention_heads * d.head_dim;
+  t.tokens = st.batch;
+  t.seqs = a->seqs;
+  t.num_heads = d.num_attention_heads;
+  t.num_kv_heads = d.num_key_value_heads;
+  t.head_dim = d.head_dim;
+  t.page_size = st.kv_seq_len;
+  t.num_pages = st.kv_batch;
+  t.max_pages = a->max_pages;
+  t.prefix_len = a->prefix_len;
+  t.scale = d.attn_scale;
+  t.workspace = a->workspace;
+  t.workspace_bytes = a->workspace_bytes;
+  int rc = qmk_prefix_attention_check(&t, h->device);
+  if (rc) return rc;
+  QMK_CUDA(h, cudaSetDevice(h->device));
+  cudaStream_t stream = (cudaStream_t)cuda_stream;
+  const int phases = qmkb_num_phases(&d), per_layer = (phases - 1) / d.num_layers;
+  const size_t layer_bytes = (size_t)st.kv_batch * st.kv_seq_len * d.num_key_value_heads * d.head_dim * 2;
+  int from = 0;
+  for (int l = 0; l < d.num_layers; ++l) {
+    // what is left of the layer before, and this layer's Q, K and V (K and V into the pool)
+    rc = batched_launch(h, 0, from, l * per_layer + 1, 0, stream, a->slots);
+    if (rc) return rc;
+    t.k_pages = (const unsigned char*)st.k_cache + l * layer_bytes;
+    t.v_pages = (const unsigned char*)st.v_cache + l * layer_bytes;
+    rc = qmk_prefix_attention(&t, h->device, cuda_stream);
+    if (rc) {
+      snprintf(h->cuda_err, sizeof(h->cuda_err), "%s", qmk_paged_last_cuda_error());
+      return rc;
+    }
+    h->launches += 2;
+    from = l * per_layer + 2;
+  }
+  return batched_launch(h, 0, from, phases, 0, stream, a->slots);
 }
 
 extern "C" int64_t qmk_step_bytes(const qmk_handle* h, int32_t pos_id) {

@@ -316,6 +316,8 @@ int qmkb_launch(qmk_batch_ctx* c, const qmk_state_ptrs* st, const qmkb_launch_ar
   p.kv_slots = st->kv_slots;
   p.kv_batch = st->kv_batch > 0 ? st->kv_batch : st->batch;
   p.kv_layer_stride = (long long)p.kv_batch * p.kv_batch_stride;
+  p.kv_rows = (const long long*)a->kv_rows;
+  p.kv_row_limit = (long long)p.kv_batch * st->kv_seq_len;
   p.ws = c->ws;
   p.tile_tickets = c->tile_tickets;
   p.ss = c->ss;
@@ -382,7 +384,8 @@ int qmkb_launch(qmk_batch_ctx* c, const qmk_state_ptrs* st, const qmkb_launch_ar
   p.off_stages = plan.off_stages;
   p.exch_stride = plan.exch_stride;
   p.pos = a->pos;
-  p.pos_limit = st->kv_seq_len < d.rope_rows ? st->kv_seq_len : d.rope_rows;
+  // (paged cache: a sequence is as long as its table, and kv_seq_len is a page's size)
+  p.pos_limit = a->kv_rows || d.rope_rows < st->kv_seq_len ? d.rope_rows : st->kv_seq_len;
   p.phase_begin = a->phase_begin;
   p.phase_end = a->phase_end;
   p.wait_first = a->wait_first;

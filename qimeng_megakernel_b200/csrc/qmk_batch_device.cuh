@@ -733,8 +733,9 @@ __device__ __forceinline__ void epilogue_tile(const Ctx& c, int ph, int kind, in
         } else {
           const int col = is_k ? row - p.QDIM : row - p.QDIM - kdim;
           uint16_t* cache = is_k ? p.k_cache : p.v_cache;
-          *reinterpret_cast<uint4*>(cache + (size_t)layer * p.kv_layer_stride + (size_t)slot_s[b] * p.kv_batch_stride +
-                                    (size_t)pos * p.kv_seq_stride + col) = o4;
+          const size_t at = p.kv_rows ? (size_t)p.kv_rows[b] * p.kv_seq_stride
+                                      : (size_t)slot_s[b] * p.kv_batch_stride + (size_t)pos * p.kv_seq_stride;
+          *reinterpret_cast<uint4*>(cache + (size_t)layer * p.kv_layer_stride + at + col) = o4;
         }
       }
       break;
@@ -1645,8 +1646,10 @@ qmk_batch_kernel(const __grid_constant__ BParams p, const __grid_constant__ Tens
     // An active row whose position lies outside the KV cache or the RoPE table would read and write out of bounds:
     // it is switched off (no KV write, zero projections, like a finished row) and the launch reports it.
     // (the same goes for a row that names a sequence the KV cache does not have)
-    int slot = b < p.B ? (p.kv_slots ? p.kv_slots[b] : b) : 0;
-    if (act != 0 && (pos < 0 || pos >= p.pos_limit || slot < 0 || slot >= p.kv_batch)) {
+    // (or a row of the paged pool that is not there)
+    int slot = b < p.B && !p.kv_rows ? (p.kv_slots ? p.kv_slots[b] : b) : 0;
+    const long long kv_row = b < p.B && p.kv_rows ? p.kv_rows[b] : 0;
+    if (act != 0 && (pos < 0 || pos >= p.pos_limit || slot < 0 || slot >= p.kv_batch || kv_row < 0 || kv_row >= p.kv_row_limit)) {
       if (blockIdx.x == 0) report(p, kErrRowPosition, 0, p.phase_begin, (unsigned)pos, (unsigned)p.pos_limit, b);
       act = 0;
       pos = -1;

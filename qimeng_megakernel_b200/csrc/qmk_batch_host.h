@@ -25,6 +25,7 @@ struct qmkb_launch_args {
   int cooperative;
   long long timeout_cycles;
   unsigned long long* trace;   // optional timeline buffer (qmk_set_trace), or null
+  const int64_t* kv_rows;      // paged cache: pool row of every row's K and V (then without the attention phase), or null
 };
 // One launch of phases [phase_begin, phase_end) (plus the memset of the arrival counters before it).
 int qmkb_launch(qmk_batch_ctx* c, const qmk_state_ptrs* st, const qmkb_launch_args* a, cudaStream_t stream, char* err,

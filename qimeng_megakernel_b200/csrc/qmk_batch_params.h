@@ -45,6 +45,9 @@ struct BParams {
   const unsigned char* active_mask;   // [B] or null (then every row is active)
   const int* kv_slots;           // [B] or null: the sequence of the KV cache row b reads and appends to (null: sequence b)
   int kv_batch;                  // sequences in the KV cache
+  const long long* kv_rows;      // [B] or null: the row of the KV pool that row b's K and V go to (paged cache; the attention phase is
+                                 // not part of such a launch)
+  long long kv_row_limit;        // rows of the pool
   long long kv_layer_stride, kv_batch_stride, kv_seq_stride;   // elements
   // ---- library-owned scratch ----
   long long* ws;                 // [CTAs, Bpad, 128] fixed-point accumulators of split tiles (zero between uses)

@@ -9,6 +9,7 @@
 #include <atomic>
 
 #include "../../include/qmk_b200.h"
+#include "qmk_paged_host.h"
 #include "qmk_paged_tables.cuh"
 #include "qmk_prefix_attention.cuh"
 
@@ -216,20 +217,29 @@ static int launch_attention(const qmk_prefix_attention_args* a, const AttnParams
   return e == cudaSuccess ? QMK_OK : paged_fail(e, "merge_kernel");
 }
 
-extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int device, void* cuda_stream) {
+static PlanDims call_dims(const qmk_prefix_attention_args* a, int ctas) {
+  return make_dims(a->tokens, a->seqs, a->num_heads / a->num_kv_heads, a->num_kv_heads, a->head_dim, a->prefix_len,
+                   a->max_pages * a->page_size, ctas);
+}
+
+int qmk_prefix_attention_check(const qmk_prefix_attention_args* a, int device) {
   const int rc = attention_args(a);
+  if (rc) return rc;
+  const int ctas = sm_count(device);
+  if (ctas < 2) return QMK_ERR_DEVICE;
+  const PlanDims d = call_dims(a, ctas);
+  return counts_fit(d) && a->workspace_bytes >= workspace_layout(d, a->head_dim).total ? QMK_OK : QMK_ERR_INVALID_ARG;
+}
+
+extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int device, void* cuda_stream) {
+  const int rc = qmk_prefix_attention_check(a, device);
   if (rc) return rc;
   DeviceScope scope(device);
   if (scope.err != cudaSuccess) return paged_fail(scope.err, "cudaSetDevice");
-  const int ctas = sm_count(device);
-  if (ctas < 1) return QMK_ERR_DEVICE;
   AttnParams p;
   memset(&p, 0, sizeof(p));
-  p.d = make_dims(a->tokens, a->seqs, a->num_heads / a->num_kv_heads, a->num_kv_heads, a->head_dim, a->prefix_len,
-                  a->max_pages * a->page_size, ctas);
-  if (!counts_fit(p.d)) return QMK_ERR_INVALID_ARG;
+  p.d = call_dims(a, sm_count(device));
   const WorkspaceLayout w = workspace_layout(p.d, a->head_dim);
-  if (a->workspace_bytes < w.total) return QMK_ERR_INVALID_ARG;
   p.q = (const uint16_t*)a->q; p.out = (uint16_t*)a->out; p.lse = a->lse;
   p.tables = a->block_tables; p.kv_lengths = a->kv_lengths; p.cu_tokens = a->cu_tokens; p.prefix_table = a->prefix_table;
   p.q_stride = a->q_token_stride; p.out_stride = a->out_token_stride;

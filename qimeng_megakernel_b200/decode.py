@@ -56,11 +56,13 @@ def decode(model_name: str, *, prefill: PrefillOutput, max_new_tokens: int, deco
     globs = prefill.globs
     if globs is None:
         raise ValueError("prefill.globs is required (run_prefill_synthetic builds it)")
-    if int(globs.k_cache.shape[2]) < prompt_len + max_new_tokens:
+    # On a paged cache (run_prefill_synthetic(shared_prefix=n)) the step's slot map gives positions and cache rows.
+    paged = getattr(globs, "paged", None)
+    if (paged.capacity if paged is not None else int(globs.k_cache.shape[2])) < prompt_len + max_new_tokens:
         raise ValueError("KV cache shorter than prompt_len + max_new_tokens")
     # Per-row positions (the reference's multi-batch state): the kernel reads them instead of position_id, so they are
     # advanced on the stream after every step as the reference's loop does (decode.py:1398-1400).
-    pids = getattr(globs, "position_ids", None)
+    pids = getattr(globs, "position_ids", None) if paged is None else None
     if pids is not None and int(pids.max()) + max_new_tokens > int(globs.k_cache.shape[2]):
         raise ValueError("KV cache shorter than the largest row position + max_new_tokens")
     setup_t0 = time.perf_counter()
@@ -100,6 +102,8 @@ def decode(model_name: str, *, prefill: PrefillOutput, max_new_tokens: int, deco
             globs.position_id = pos
             if events:
                 events[i][0].record()
+            if paged is not None:
+                paged.advance()
             schedule.call_mk(globs, mk)
             if events:
                 events[i][1].record()
@@ -125,6 +129,8 @@ def decode(model_name: str, *, prefill: PrefillOutput, max_new_tokens: int, deco
             globs.position_id = pos
             if events:
                 events[i][0].record()
+            if paged is not None:
+                paged.advance()
             schedule.call_mk(globs, mk)
             if events:
                 events[i][1].record()
@@ -141,6 +147,8 @@ def decode(model_name: str, *, prefill: PrefillOutput, max_new_tokens: int, deco
             globs.position_id = prompt_len + i
             if events:
                 events[i][0].record()
+            if paged is not None:
+                paged.advance()
             schedule.call_mk(globs, mk)
             if events:
                 events[i][1].record()
@@ -183,6 +191,9 @@ def decode(model_name: str, *, prefill: PrefillOutput, max_new_tokens: int, deco
         effective = int(per_row.sum())
         window = max(effective - batch_size, 0)
         step_bytes = sum(mk.step_bytes(prompt_len + i) for i in range(ntok)) / ntok if ntok > 0 else 0.0
+        if paged is not None:   # (the shared positions are read once, not once per sequence)
+            L, _, _, kv_heads, size = globs.k_cache.shape
+            step_bytes -= (batch_size - 1) * paged.prefix_len * L * kv_heads * size * 4
         timing = {
             "instruction_setup_wall_s": instruction_setup_wall_s, "queue_build_wall_s": 0.0, "tensorize_wall_s": 0.0,
             "decode_wall_s": decode_wall_s, "decode_gpu_s": decode_gpu_s, "mk_kernel_gpu_s": mk_kernel_gpu_s,

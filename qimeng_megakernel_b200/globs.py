@@ -51,6 +51,9 @@ class Globals:
     # B200 addition: the KV-cache sequence every row of the step belongs to (int32 [rows]); with it the rows may be
     # consecutive positions of one sequence (prefill) and the state tensors have `rows` rows while the cache has B sequences
     kv_slots: Optional[torch.Tensor] = None
+    # B200 addition: a paged KV cache whose sequences share a prefix (paged.PagedState); k_cache / v_cache are then the pools
+    # [L, num_pages, page_size, NKV, HD], and position_ids, active_mask and kv_slots are the buffers of the state's steps
+    paged: Optional[object] = None
     # Qwen3 (qwen3__0_6b/A100/single_batch/decode_schedule/globs.py): per-head Q/K norm gains, interleaved order
     q_norm_weights: Optional[torch.Tensor] = None        # [L, HD]
     k_norm_weights: Optional[torch.Tensor] = None        # [L, HD]

@@ -40,6 +40,9 @@ def _parse_args() -> argparse.Namespace:
     p.add_argument("--warmup-iters", type=int, default=2)
     p.add_argument("--bench-iters", type=int, default=5)
     p.add_argument("--host-loop", action="store_true", help="use the reference's host token loop instead of the device loop")
+    p.add_argument("--shared-prefix", type=int, default=None, metavar="N",
+                   help="paged KV cache; the prompts of a batch share their first N tokens (N < --prompt-len)")
+    p.add_argument("--page-size", type=int, default=64, help="positions per page of the paged cache")
     p.add_argument("--peak-gbs", type=float, default=HBM_PEAK_GBS)
     return p.parse_args()
 
@@ -47,7 +50,10 @@ def _parse_args() -> argparse.Namespace:
 def _run_once(args, cfg, weights, mk, prompt, batch_size: int, output_len: int) -> dict:
     prompts = prompt.view(1, -1) if batch_size == 1 else synthetic.make_prompts(
         cfg["vocab_size"], batch_size, args.prompt_len, args.prompt_seed)   # row 0 is the single-sequence prompt
-    prefill = run_prefill_synthetic(cfg, weights, prompts, output_len, device=args.device, mk=mk)
+    if args.shared_prefix is not None and batch_size > 1:
+        prompts[1:, :args.shared_prefix] = prompts[0, :args.shared_prefix]
+    prefill = run_prefill_synthetic(cfg, weights, prompts, output_len, device=args.device, mk=mk,
+                                    shared_prefix=args.shared_prefix, page_size=args.page_size)
     wall_t0 = time.perf_counter()
     out = llm_decode(args.model, prefill=prefill, max_new_tokens=output_len, decode_route="mk",
                      hardware=args.hardware, decode_time=True, ignore_eos=True, host_loop=args.host_loop)
@@ -102,7 +108,7 @@ def main() -> int:
     out = {"backend": "mk", "model_path": f"synthetic:{args.model}", "prompt_token_count": args.prompt_len,
            "prompt_mode": "token ids", "eos_policy": "forced_continuation", "decode_strategy": "greedy",
            "hardware": args.hardware, "torch_dtype": "bfloat16", "batch_sizes": batch_sizes,
-           "output_lengths": output_lengths, "warmup_iters": args.warmup_iters, "bench_iters": args.bench_iters,
+           "output_lengths": output_lengths, "shared_prefix": args.shared_prefix, "warmup_iters": args.warmup_iters, "bench_iters": args.bench_iters,
            "hbm_peak_gbs": args.peak_gbs, "results": results}
     if args.out:
         path = Path(args.out).expanduser().resolve()

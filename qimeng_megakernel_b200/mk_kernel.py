@@ -134,6 +134,16 @@ class MegaKernel:
             _check_tensor("out_tokens", g.out_tokens, torch.int64, (n,) if (B == 1 and g.out_tokens.dim() == 1) else (B, n))
         if getattr(g, "position_ids", None) is not None:
             _check_tensor("position_ids", g.position_ids, torch.int32, (B,))
+        if getattr(g, "paged", None) is not None:
+            step = g.paged.step
+            if S != g.paged.page_size or g.paged.rows != B:
+                raise ValueError(f"globs.paged: pages of {g.paged.page_size} and {g.paged.rows} rows, k_cache has {S} and kv_slots {B}")
+            for name, t in (("position_ids", step.positions), ("active_mask", step.active), ("kv_slots", step.seq_ids)):
+                mine = getattr(g, name, None)
+                if mine is None or mine.data_ptr() != t.data_ptr():
+                    raise ValueError(f"globs.{name} must be the buffer of globs.paged.step")
+            if g.paged.block_tables.device != g.k_cache.device:
+                raise ValueError(f"globs.paged is on {g.paged.block_tables.device}, the cache on {g.k_cache.device}")
         if getattr(g, "active_mask", None) is not None:
             if g.active_mask.dtype not in (torch.uint8, torch.bool):
                 raise TypeError("globs.active_mask must be uint8 or bool")
@@ -196,8 +206,18 @@ class MegaKernel:
     def _stream(self) -> int:
         return torch.cuda.current_stream(self._device).cuda_stream
 
+    def _paged_step(self, g: Globals) -> None:
+        cfg = LlamaConfig
+        args = g.paged.step_args(cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim)
+        _lib.check(self._lib.qmk_decode_step_paged(self._handle, C.byref(args), self._stream()), self._handle)
+
     def __call__(self, g: Globals, pos_id: int | None = None) -> None:
         self._ensure(g)
+        if getattr(g, "paged", None) is not None:
+            if pos_id is not None:
+                raise ValueError("the positions of a paged step come from its slot map")
+            self._paged_step(g)
+            return
         pos = int(g.position_id if pos_id is None else pos_id) if (g.position_id is not None or pos_id is not None) else 0
         _lib.check(self._lib.qmk_decode_step(self._handle, pos, self._stream()), self._handle)
 

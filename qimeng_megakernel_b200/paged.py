@@ -310,3 +310,51 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
                            num_pages, max_pages, prefix_len, scale, workspace.data_ptr(), workspace.shape[0])
     _call(_lib.load().qmk_prefix_attention, args, index)
     return out
+
+
+class PagedState:
+    """The paged cache of a decode request: tables, lengths and the rows of the current step.
+
+    `advance(new_lengths)` makes the slot map of a step that appends new_lengths[s] tokens to sequence s; the kernel call
+    on the Globals that carry the state (`mk(globs)`) then runs that step.  The step's buffers (slots, positions, active,
+    seq_ids, cu_tokens) stay where they are from step to step, so the kernel's binding and captured graphs hold; the
+    lengths alternate between two."""
+
+    def __init__(self, block_tables: torch.Tensor, lengths: torch.Tensor, rows: int, page_size: int,
+                 prefix_table: torch.Tensor | None, prefix_len: int):
+        device = block_tables.device
+        seqs = block_tables.shape[0]
+        self.block_tables, self.page_size, self.rows = block_tables, _page_size(page_size), int(rows)
+        self.prefix_table, self.prefix_len = prefix_table, int(prefix_len)
+        self.step = SlotMap.empty(seqs, self.rows, device)
+        for t in (self.step.positions, self.step.active, self.step.seq_ids, self.step.cu_tokens):
+            t.zero_()
+        self.step.slots.fill_(-1)
+        self.step.kv_lengths.copy_(lengths)
+        self._other = torch.empty_like(self.step.kv_lengths)
+        self.ones = torch.ones(seqs, dtype=torch.int32, device=device)
+        self.workspace: torch.Tensor | None = None
+
+    @property
+    def capacity(self) -> int:
+        """Positions a sequence's table has room for."""
+        return self.block_tables.shape[1] * self.page_size
+
+    def advance(self, new_lengths: torch.Tensor | None = None) -> SlotMap:
+        """The step in which sequence s appends new_lengths[s] tokens (one each by default)."""
+        lengths, self.step.kv_lengths = self.step.kv_lengths, self._other
+        self._other = lengths
+        return build_slot_map(self.block_tables, lengths, self.ones if new_lengths is None else new_lengths,
+                              page_size=self.page_size, tokens=self.rows, out=self.step)
+
+    def step_args(self, heads: int, kv_heads: int, size: int) -> _lib.PagedStepArgs:
+        """The step's arguments for the library; makes the workspace on the first call."""
+        device = self.block_tables.device
+        if self.workspace is None:
+            self.workspace = torch.empty(_workspace_bytes(self.rows, self.block_tables.shape[0], heads, kv_heads, size,
+                                                          self.prefix_len, device.index), dtype=torch.uint8, device=device)
+        s = self.step
+        return _lib.PagedStepArgs(self.block_tables.data_ptr(), s.kv_lengths.data_ptr(), s.cu_tokens.data_ptr(),
+                                  s.slots.data_ptr(), self.prefix_table.data_ptr() if self.prefix_len else None,
+                                  self.block_tables.shape[0], self.block_tables.shape[1], self.prefix_len,
+                                  self.workspace.data_ptr(), self.workspace.shape[0])

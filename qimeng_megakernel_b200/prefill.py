@@ -17,7 +17,7 @@ from typing import Any
 
 import torch
 
-from . import _lib, mk_kernel, synthetic
+from . import _lib, mk_kernel, paged, synthetic
 from .globs import Globals
 
 
@@ -46,6 +46,70 @@ def prefill_plan(batch: int, prompt_len: int, rows: int = _lib.MAX_BATCH) -> lis
     return plan
 
 
+def paged_prefill_plan(batch: int, first: int, prompt_len: int, rows: int = _lib.MAX_BATCH) -> list[tuple[int, int, list[int]]]:
+    """The launches of a prefill on the paged cache: (first sequence, last sequence + 1, tokens) -- every sequence of the range
+    appends the same number of tokens, at most `rows` in all; a sequence's tokens come in order from `first` on."""
+    own = prompt_len - first
+    per_seq = min(own, rows)
+    seqs_per_launch = max(1, rows // per_seq)
+    plan = []
+    for p0 in range(0, own, per_seq):
+        n = min(per_seq, own - p0)
+        for s0 in range(0, batch, seqs_per_launch):
+            plan.append((s0, min(batch, s0 + seqs_per_launch), list(range(first + p0, first + p0 + n))))
+    return plan
+
+
+def _paged_rows(g: Globals, config: dict, state) -> Globals:
+    """_prefill_state for a PagedState of its own over the same pool."""
+    gp = _prefill_state(g, config, state.rows)
+    return dataclasses.replace(gp, paged=state, position_ids=state.step.positions, active_mask=state.step.active,
+                               kv_slots=state.step.seq_ids)
+
+
+def _prefill_paged(g: Globals, config: dict, ids: torch.Tensor, mk: Any) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """The shared prefix once, as a sequence of its own, then what the prompts have behind it.  Returns the first generated
+    tokens [B], the logits of the last prompt positions [B, V] and the number of steps."""
+    state, dev = g.paged, g.k_cache.device
+    B, prompt_len = ids.shape
+    P, page, launches = state.prefix_len, state.page_size, 0
+    rows = _lib.MAX_BATCH
+    if P:
+        alone = paged.PagedState(state.prefix_table.view(1, -1), torch.zeros(1, dtype=torch.int32, device=dev), min(rows, P), page,
+                                 None, 0)
+        gp = _paged_rows(g, config, alone)
+        for p0 in range(0, P, alone.rows):
+            n = min(alone.rows, P - p0)
+            gp.token_in.zero_()
+            gp.token_in[:n].copy_(ids[0, p0:p0 + n])
+            alone.advance(torch.tensor([n], dtype=torch.int32, device=dev))
+            mk(gp)
+            launches += 1
+        mk.check_status()
+    plan = paged_prefill_plan(B, P, prompt_len, rows)
+    own = paged.PagedState(state.block_tables, state.step.kv_lengths, max((s1 - s0) * len(pos) for s0, s1, pos in plan), page,
+                           state.prefix_table, P)
+    gp = _paged_rows(g, config, own)
+    first = torch.zeros(B, dtype=torch.int64, device=dev)
+    logits = torch.zeros(B, config["vocab_size"], dtype=torch.bfloat16, device=dev)
+    for s0, s1, pos in plan:
+        n = len(pos)
+        new = torch.zeros(B, dtype=torch.int32)
+        new[s0:s1] = n
+        gp.token_in.zero_()
+        gp.token_in[:(s1 - s0) * n].copy_(ids[s0:s1, pos[0]:pos[0] + n].reshape(-1))
+        own.advance(new.to(dev))
+        mk(gp)
+        launches += 1
+        if pos[-1] == prompt_len - 1:
+            last = torch.arange(s1 - s0, device=dev) * n + n - 1
+            first[s0:s1] = gp.next_token[last]
+            logits[s0:s1] = gp.logits[last]
+    state.step.kv_lengths.copy_(own.step.kv_lengths)
+    mk.check_status()
+    return first, logits, launches
+
+
 def _prefill_state(g: Globals, config: dict, rows: int) -> Globals:
     """State tensors with `rows` rows around the weights and the KV cache of the decode state `g`."""
     dev, bf = g.k_cache.device, torch.bfloat16
@@ -60,14 +124,28 @@ def _prefill_state(g: Globals, config: dict, rows: int) -> Globals:
 
 @torch.inference_mode()
 def run_prefill_synthetic(config: dict, weights: dict, prompt_ids: torch.Tensor, max_new_tokens: int,
-                          device: str | torch.device = "cuda:0", mk: Any = None, fused: bool = True) -> PrefillOutput:
+                          device: str | torch.device = "cuda:0", mk: Any = None, fused: bool = True,
+                          shared_prefix: int | None = None, page_size: int = 64) -> PrefillOutput:
     """prompt_ids: [B, prompt_len] (or [prompt_len]) int64 token ids; B > 1 gives [B, ...] decode state (all prompts of
-    one length, like the reference's fused prefill for a padded batch)."""
+    one length, like the reference's fused prefill for a padded batch).
+
+    shared_prefix = n: the decode state is on a paged cache (paged.PagedState).  The prompts must agree in their first n
+    tokens; the whole pages of those are computed and stored once, and every decode step reads them once for the batch
+    (qmk_decode_step_paged).  0 gives a paged cache that shares nothing."""
     ids = (prompt_ids.view(1, -1) if prompt_ids.dim() == 1 else prompt_ids).to(torch.int64)
     B, prompt_len = int(ids.shape[0]), int(ids.shape[1])
     if prompt_len < 1:
         raise ValueError("empty prompt")
     dev = torch.device(device)
+    if shared_prefix is not None:
+        if not 0 <= shared_prefix < prompt_len:
+            raise ValueError(f"shared_prefix {shared_prefix}: a prompt of {prompt_len} tokens keeps at least its last one to itself")
+        if not bool((ids[:, :shared_prefix] == ids[:1, :shared_prefix]).all()):
+            raise ValueError(f"the prompts differ within their first {shared_prefix} tokens")
+        g = synthetic.make_paged_globals(config, weights, prompt_len, max_new_tokens, int(shared_prefix), B, page_size, dev)
+        mk = mk if mk is not None else mk_kernel.get_mk()
+        first, logits, launches = _prefill_paged(g, config, ids.to(dev), mk)
+        return PrefillOutput(input_ids=ids.to(dev), first_gen_token=first.view(B, 1), logits=logits, globs=g, mk=mk, launches=launches)
     g = synthetic.make_globals(config, weights, kv_seq_len=prompt_len + max(0, max_new_tokens), device=dev,
                                batch=B if B > 1 else None)
     mk = mk if mk is not None else mk_kernel.get_mk()

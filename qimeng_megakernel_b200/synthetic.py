@@ -108,6 +108,33 @@ def random_kv_rows(config: dict, rows: int, seed: int, batch: int = 1, std: floa
     return k, v
 
 
+def make_paged_globals(config: dict, weights: dict, prompt_len: int, max_new_tokens: int, shared_prefix: int, batch: int,
+                       page_size: int = 64, device: str | torch.device = "cuda") -> Globals:
+    """Decode state of `batch` sequences on a paged cache: the whole pages of the first `shared_prefix` positions are stored
+    once, every sequence gets pages of its own for the rest of prompt_len + max_new_tokens.  Nothing is in the cache yet."""
+    from . import paged
+    if page_size not in paged.PAGE_SIZES:
+        raise ValueError(f"page_size {page_size}: expected one of {paged.PAGE_SIZES}")
+    if not 0 <= shared_prefix < prompt_len:
+        raise ValueError(f"shared_prefix {shared_prefix}: a prompt of {prompt_len} tokens keeps at least its last one to itself")
+    total = prompt_len + max(0, max_new_tokens)
+    shared, pages = shared_prefix // page_size, -(-total // page_size)
+    own = pages - shared
+    g = make_globals(config, weights, kv_seq_len=page_size, device=device, batch=batch)
+    dev, bf = g.k_cache.device, torch.bfloat16
+    pool = shared + batch * own
+    shape = (config["num_hidden_layers"], pool, page_size, config["num_key_value_heads"], config["head_dim"])
+    g.k_cache, g.v_cache = torch.zeros(shape, dtype=bf, device=dev), torch.zeros(shape, dtype=bf, device=dev)
+    ids = torch.arange(pool, dtype=torch.int32, device=dev)
+    prefix = ids[:shared].contiguous() if shared else None
+    lengths = torch.full((batch,), total, dtype=torch.int32, device=dev)
+    tables = paged.build_block_tables(lengths, ids[shared:].contiguous(), page_size=page_size, max_pages=pages, prefix_table=prefix)
+    start = torch.full((batch,), shared * page_size, dtype=torch.int32, device=dev)
+    g.paged = paged.PagedState(tables.tables, start, batch, page_size, prefix, shared * page_size)
+    g.position_ids, g.active_mask, g.kv_slots = g.paged.step.positions, g.paged.step.active, g.paged.step.seq_ids
+    return g
+
+
 def make_globals(config: dict, weights: dict, kv_seq_len: int, device: str | torch.device = "cuda",
                  batch: int | None = None) -> Globals:
     """Allocate the buffers the reference's fused prefill allocates

@@ -1,0 +1,195 @@
+"""Decode steps on the paged cache with a shared prefix against the contiguous cache: prefill, steps, the token loops, refusals.
+
+Tolerances are those of the prefill tests of the batched kernel: the two routes round the attention's probabilities
+differently (bf16 here, tf32 there), everything else is the same kernel."""
+import pytest
+import torch
+
+from tests import _util as U
+
+pytestmark = pytest.mark.gpu
+
+
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def _config(name):
+    from qimeng_megakernel_b200.model_config import LLAMA_3_2_1B, OLMOE_1B_7B, QWEN3_0_6B
+    base = {"llama": LLAMA_3_2_1B, "qwen3": QWEN3_0_6B, "olmoe": OLMOE_1B_7B}[name]
+    return dict(base, num_hidden_layers=2, vocab_size=2048, max_position_embeddings=512)
+
+
+def _prompts(cfg, batch, length, shared, seed):
+    from qimeng_megakernel_b200 import synthetic
+    prompts = synthetic.make_prompts(cfg["vocab_size"], batch, length, seed=seed)
+    prompts[1:, :shared] = prompts[0, :shared]
+    return prompts
+
+
+def _dense_cache(g, name, layer, seq, length):
+    """A sequence's rows of the pool, in order."""
+    pages = g.paged.block_tables[seq].long()
+    return getattr(g, name)[layer][pages].flatten(0, 1)[:length]
+
+
+def _close(model, got, want, bound):
+    """Rows (positions or sequences) within `bound`.  A token whose k-th and (k + 1)-th expert nearly tie may be routed to either:
+    one of eight expert terms of about equal weight, all of independent random direction, is exchanged.  The expert sum
+    (variance 8 t^2 of eight terms t) then moves by sqrt(2) t, half of itself, and the residual stream by that share of what the
+    experts add to it; the mixture-of-experts tests bound such rows by 6e-2, and so does this one, for less than half of them."""
+    got, want = got.float().flatten(1), want.float().flatten(1)
+    err = (got - want).norm(dim=1) / want.norm(dim=1)
+    if model == "olmoe":
+        assert float(err.median()) <= bound and float(err.max()) <= 6e-2, err.tolist()
+    else:
+        assert float(err.max()) <= bound, err.tolist()
+
+
+@pytest.mark.parametrize("model,batch,length,shared,page", [
+    ("llama", 3, 70, 40, 16), ("llama", 1, 20, 16, 16), ("qwen3", 5, 100, 64, 32), ("olmoe", 4, 40, 17, 16),
+    ("llama", 4, 30, 0, 64), ("qwen3", 2, 150, 128, 128)])
+def test_paged_prefill_and_steps_match_the_contiguous_cache(model, batch, length, shared, page):
+    _need_gpu()
+    from qimeng_megakernel_b200 import synthetic
+    from qimeng_megakernel_b200.prefill import run_prefill_synthetic
+    cfg = _config(model)
+    weights = synthetic.make_weights(cfg, seed=11, device="cuda:0")
+    prompts = _prompts(cfg, batch, length, shared, seed=40 + batch)
+    steps = 5
+    a = run_prefill_synthetic(cfg, weights, prompts, steps, shared_prefix=shared, page_size=page)
+    b = run_prefill_synthetic(cfg, weights, prompts if batch > 1 else prompts[0], steps)
+    assert a.globs.paged.prefix_len == shared // page * page
+    for layer in range(2):
+        for name in ("k_cache", "v_cache"):
+            for s in range(batch):
+                _close(model, _dense_cache(a.globs, name, layer, s, length), getattr(b.globs, name)[layer, s, :length], 1e-2)
+    _close(model, a.logits, b.logits, 2e-2)
+    # the same tokens through both, row by row the same logits
+    ga, gb = a.globs, b.globs
+    gen = torch.Generator().manual_seed(1)
+    ga.token_in = torch.zeros(batch, dtype=torch.int64, device="cuda:0")
+    gb.token_in = torch.zeros(batch, dtype=torch.int64, device="cuda:0")
+    for i in range(steps):
+        tok = torch.randint(0, cfg["vocab_size"], (batch,), generator=gen)
+        ga.token_in.copy_(tok)
+        gb.token_in.copy_(tok)
+        ga.paged.advance()
+        a.mk(ga)
+        gb.position_id = length + i
+        b.mk(gb)
+        torch.cuda.synchronize()
+        _close(model, ga.logits.view(batch, -1), gb.logits.view(batch, -1), 2e-2)
+        la = ga.logits.view(batch, -1).float()
+        assert ga.next_token.tolist() == la.argmax(-1).tolist()
+        assert ga.paged.step.positions.tolist() == [length + i] * batch
+    a.mk.check_status()
+    b.mk.check_status()
+    for x in (a, b):
+        x.mk.close()
+
+
+def test_token_loops_agree_on_the_paged_cache():
+    """decode(): device loop, host loop and sampling with one candidate give the same tokens, and again the same."""
+    _need_gpu()
+    from qimeng_megakernel_b200 import synthetic
+    from qimeng_megakernel_b200.decode import decode
+    from qimeng_megakernel_b200.prefill import run_prefill_synthetic
+    cfg = _config("llama")
+    weights = synthetic.make_weights(cfg, seed=3, device="cuda:0")
+    prompts = _prompts(cfg, 4, 40, 33, seed=9)
+    out = []
+    for kw in (dict(), dict(decode_time=True), dict(host_loop=True), dict(temperature=1.0, top_k=1, seed=5)):
+        pre = run_prefill_synthetic(cfg, weights, prompts, 12, shared_prefix=33, page_size=16)
+        got = decode("llama-3.2-1b", prefill=pre, max_new_tokens=12, ignore_eos=True, **kw)
+        out.append(got["new_tokens"].tolist())
+        assert len(out[-1][0]) == 12 and pre.globs.paged.step.kv_lengths.tolist() == [40 + 11] * 4
+        pre.mk.close()
+    assert out[0] == out[1] == out[2]
+    pre = run_prefill_synthetic(cfg, weights, prompts, 3, shared_prefix=33, page_size=16)
+    with pytest.raises(ValueError, match="KV cache shorter"):
+        decode("llama-3.2-1b", prefill=pre, max_new_tokens=30, ignore_eos=True)
+    pre.mk.close()
+
+
+@torch.inference_mode()
+def test_finished_sequences_and_a_captured_step():
+    """A step in which some sequences append nothing leaves their rows' places to the others; a captured step replays."""
+    _need_gpu()
+    from qimeng_megakernel_b200 import synthetic
+    from qimeng_megakernel_b200.prefill import run_prefill_synthetic
+    cfg = _config("qwen3")
+    weights = synthetic.make_weights(cfg, seed=5, device="cuda:0")
+    prompts = _prompts(cfg, 4, 50, 32, seed=21)
+    pre = run_prefill_synthetic(cfg, weights, prompts, 8, shared_prefix=32, page_size=16)
+    g, mk = pre.globs, pre.mk
+    new = torch.tensor([1, 0, 1, 0], dtype=torch.int32, device="cuda:0")
+    g.token_in = torch.tensor([5, 6, 0, 0], dtype=torch.int64, device="cuda:0")      # sequences 0 and 2
+    lengths = g.paged.step.kv_lengths.clone()
+    g.paged.advance(new)
+    mk(g)
+    mk.check_status()
+    assert g.active_mask.tolist() == [1, 1, 0, 0] and g.kv_slots.tolist() == [0, 2, -1, -1]
+    assert g.paged.step.kv_lengths.tolist() == [51, 50, 51, 50]
+    pair = g.logits[:2].clone()
+    assert (g.logits[2:].float() < -1e8).all()
+    # the same step of all four, sequences 0 and 2 with the same tokens, from the same lengths
+    g.paged.step.kv_lengths.copy_(lengths)
+    g.token_in.copy_(torch.tensor([5, 9, 6, 9]))
+    g.paged.advance()
+    mk(g)
+    torch.cuda.synchronize()
+    full = g.logits.clone()
+    assert U.rel_l2(full[[0, 2]], pair) <= 2e-2
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        g.paged.step.kv_lengths.copy_(lengths)
+        kept = g.paged.step.kv_lengths.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            g.paged.step.kv_lengths.copy_(kept)
+            g.paged.advance()
+            mk(g)
+        g.logits.zero_()
+        for _ in range(2):
+            graph.replay()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(g.logits, full)
+    mk.check_status()
+    mk.close()
+
+
+@torch.inference_mode()
+def test_rows_without_a_place_are_reported_and_calls_refused():
+    _need_gpu()
+    from qimeng_megakernel_b200 import _lib, mk_kernel, synthetic
+    from qimeng_megakernel_b200.prefill import run_prefill_synthetic
+    cfg = _config("llama")
+    weights = synthetic.make_weights(cfg, seed=6, device="cuda:0")
+    prompts = _prompts(cfg, 2, 20, 16, seed=2)
+    pre = run_prefill_synthetic(cfg, weights, prompts, 4, shared_prefix=16, page_size=16)
+    g, mk = pre.globs, pre.mk
+    g.token_in = torch.zeros(2, dtype=torch.int64, device="cuda:0")
+    g.paged.advance()
+    before = g.k_cache.clone()
+    g.paged.step.slots[1] = 1 << 40                      # behind the pool: switched off, reported, nothing stored
+    mk(g)
+    with pytest.raises(_lib.QmkError):
+        mk.check_status()
+    assert (g.k_cache[:, 1:] != before[:, 1:]).any() and torch.isfinite(g.logits[0].float()).all()
+    with pytest.raises(ValueError, match="slot map"):
+        mk(g, 3)
+    g.active_mask = g.active_mask.clone()
+    with pytest.raises(ValueError, match="active_mask must be the buffer"):
+        mk(g)
+    mk.close()
+    with pytest.raises(ValueError, match="differ within"):
+        run_prefill_synthetic(cfg, weights, synthetic.make_prompts(cfg["vocab_size"], 2, 20, seed=2), 4, shared_prefix=16, page_size=16)
+    with pytest.raises(ValueError, match="keeps at least"):
+        run_prefill_synthetic(cfg, weights, prompts, 4, shared_prefix=20, page_size=16)
+    with pytest.raises(ValueError, match="page_size 24"):
+        run_prefill_synthetic(cfg, weights, prompts, 4, shared_prefix=16, page_size=24)
+    mk_kernel.LlamaConfig.update_from_dict(cfg)

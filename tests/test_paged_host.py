@@ -165,3 +165,35 @@ def test_c_entries_refuse_before_they_launch(paged):
                dict(max_pages=(1 << 26) + 1), dict(workspace=None), dict(workspace=P + 128), dict(page_size=48), dict(num_pages=0), dict(max_pages=0),
                dict(prefix_len=33), dict(prefix_len=-16), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf"))):
         assert attn(**kw) == -1, kw
+
+
+def test_paged_step_refuses_without_a_handle(paged):
+    from qimeng_megakernel_b200 import _lib
+    lib = _lib.load()
+    args = _lib.PagedStepArgs()
+    assert lib.qmk_decode_step_paged(None, C.byref(args), None) == -1
+    assert lib.qmk_paged_last_cuda_error() is not None
+
+
+@pytest.mark.parametrize("batch,first,length,rows", [(3, 32, 70, 64), (1, 16, 20, 64), (40, 0, 30, 64), (2, 128, 150, 64),
+                                                     (5, 64, 400, 64), (64, 0, 1, 64), (7, 5, 6, 8)])
+def test_paged_prefill_plan(batch, first, length, rows):
+    """Every sequence appends its tokens in order, no launch more than its rows."""
+    from qimeng_megakernel_b200.prefill import paged_prefill_plan
+    at = [first] * batch
+    for s0, s1, positions in paged_prefill_plan(batch, first, length, rows):
+        assert 0 < (s1 - s0) * len(positions) <= rows
+        for s in range(s0, s1):
+            assert positions == list(range(at[s], at[s] + len(positions)))
+            at[s] += len(positions)
+    assert at == [length] * batch
+
+
+def test_paged_state_refusals(small_config, small_weights):
+    from qimeng_megakernel_b200 import synthetic
+    f = lambda **kw: synthetic.make_paged_globals(small_config, small_weights, **{**dict(prompt_len=20, max_new_tokens=4,
+                                                  shared_prefix=16, batch=2, page_size=16, device="cpu"), **kw})
+    refused(ValueError, "page_size 24", f, page_size=24)
+    refused(ValueError, "keeps at least", f, shared_prefix=20)
+    refused(ValueError, "keeps at least", f, shared_prefix=-1)
+    refused(ValueError, "no CPU path", f)
