@@ -205,8 +205,8 @@ static int launch_attention(const qmk_prefix_attention_args* a, const AttnParams
   if (e != cudaSuccess) return paged_fail(e, "prefix_attention_kernel");
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)(((long long)a->tokens * a->num_heads + 3) / 4));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3((unsigned)((a->tokens * p.d.G + 31) / 32), (unsigned)p.d.NKV, HD / 4 / (kMergeThreads / 32));
+  cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // (the kernel waits for its predecessor itself)
@@ -246,7 +246,7 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
   p.NH = a->num_heads; p.page_shift = page_shift_of(a->page_size); p.num_pages = a->num_pages; p.max_pages = a->max_pages;
   p.scale_log2e = a->scale * 1.4426950408889634f;
   unsigned char* ws = (unsigned char*)a->workspace;
-  p.dense_ml = (float2*)(ws + w.dense_ml); p.dense_o = (float*)(ws + w.dense_o);
+  p.dense_ml = (float2*)(ws + w.dense_ml); p.dense_o = (float4*)(ws + w.dense_o);
   p.strip_ml = (float2*)(ws + w.strip_ml); p.strip_o = (float*)(ws + w.strip_o);
   p.dense_desc = (int2*)(ws + w.dense_desc); p.strip_desc = (int2*)(ws + w.strip_desc);
   encode_fn enc = tensor_map_encoder();

@@ -48,7 +48,7 @@ struct AttnParams {
   int NH, page_shift, num_pages, max_pages;
   float scale_log2e;
   // workspace
-  float* dense_o;              // [records, 256, HD]
+  float4* dense_o;             // [records, HD / 4, 256]   four dimensions of every row side by side
   float2* dense_ml;            // [records, 256]   (m in log2 units, l)
   float* strip_o;              // [records, 8, HD]
   float2* strip_ml;            // [records, 8]
@@ -295,8 +295,8 @@ __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc,
         }
       }
       x = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
+#pragma unroll 1
+      for (int o = 1; o < 32; o <<= 1) {                     // (rolled, like what else runs once: its code comes from afar)
         const int a = __shfl_up_sync(kFullMask, x.x, o), b = __shfl_up_sync(kFullMask, x.y, o);
         const int c = __shfl_up_sync(kFullMask, x.z, o), d = __shfl_up_sync(kFullMask, x.w, o);
         if (lane >= o) { x.x += a; x.y += b; x.z += c; x.w += d; }
@@ -329,14 +329,10 @@ __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc,
   if (warp == 0) {                                           // each lane weighs one division of the CTAs
     const Totals t{base.x, base.y, base.z, base.w};
     Choice c = plan_choice(p.d, t, lane);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      Choice x;
-      x.time = __shfl_xor_sync(kFullMask, c.time, o);
-      x.ctas = __shfl_xor_sync(kFullMask, c.ctas, o);
-      x.each = __shfl_xor_sync(kFullMask, c.each, o);
-      if (x.time < c.time || (x.time == c.time && (x.ctas < c.ctas || (x.ctas == c.ctas && x.each > c.each)))) c = x;
-    }
+    // (times are positive: their bits order like them; the lane's number takes the last five, and breaks ties)
+    const int best = (int)(__reduce_min_sync(kFullMask, (__float_as_uint(c.time) & ~31u) | (unsigned)lane) & 31u);
+    c.ctas = __shfl_sync(kFullMask, c.ctas, best);
+    c.each = __shfl_sync(kFullMask, c.each, best);
     if (lane == 0) {
       out->t = t;
       out->plan = make_plan(p.d, t, c);
@@ -772,7 +768,7 @@ struct Dense {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const uint32_t other_col = tmem + 256 + (g ^ 1) * 128 + lane_base;
         uint16_t* out = p.out + (size_t)max(token, 0) * p.out_stride + (size_t)head * HD;
-        float* part = p.dense_o + ((size_t)rec * kUnitRows + tile_row) * HD;
+        float4* part = p.dense_o + (size_t)rec * (HD / 4) * kUnitRows + tile_row;
         const int c0 = dual ? g * (HD / 32) : 0, c1 = dual ? c0 + HD / 32 : HD / 16;
 #pragma unroll 1
         for (int c = c0; c < c1; ++c) {
@@ -802,7 +798,8 @@ struct Dense {
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                reinterpret_cast<uint4*>(part + 16 * c)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                part[(4 * c + i) * kUnitRows] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                            __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
             }
           }
         }
@@ -1075,7 +1072,6 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
   extern __shared__ __align__(1024) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile unsigned* ctl = reinterpret_cast<volatile unsigned*>(smem + S::kOffCtl);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Scans sc;
   sc.long_blocks = reinterpret_cast<int*>(smem + S::kOffScan);
   sc.long_units = sc.long_blocks + p.d.seqs + 1;
@@ -1100,18 +1096,21 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
     if (lane == 0) ctl[0] = 0u;
     fence_barrier_init();
   }
-  build_plan(p, sc, reinterpret_cast<int4*>(smem + S::kOffRed), work);
-  if ((int)blockIdx.x >= work->plan.dense_ctas) {
-    if (warp < kStripWarps) walk_strips<HD>(p, maps, smem, ctl, sc, work->plan, warp, lane);
-    return;
-  }
-  dense_range(work->plan, (int)blockIdx.x, w.lo, w.hi);
-  if (warp == kIssueWarp) {
+  if (warp == kIssueWarp) {                                  // (before it is known whether the CTA has blocks: it takes a while)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(w.base + S::kOffCtl + 4) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     tmem_fence_before_sync();
   }
-  __syncthreads();
+  build_plan(p, sc, reinterpret_cast<int4*>(smem + S::kOffRed), work);
+  if ((int)blockIdx.x >= work->plan.dense_ctas) {
+    if (warp == kIssueWarp) {
+      tmem_fence_after_sync();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(ctl[1]) : "memory");
+    }
+    if (warp < kStripWarps) walk_strips<HD>(p, maps, smem, ctl, sc, work->plan, warp, lane);
+    return;
+  }
+  dense_range(work->plan, (int)blockIdx.x, w.lo, w.hi);
   tmem_fence_after_sync();
   w.tmem = ctl[1];
   if (warp < kSoftmaxWarps) {
@@ -1136,81 +1135,68 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
   }
 }
 
-// Adds a row's parts: one warp per (token, query head).  With M = max m_r and w_r = 2^(m_r - M):
-//   o = sum_r w_r O_r / sum_r w_r l_r
-// Lane r reads the statistics of part r; then all parts' values are on their way at once (a part of weight zero may hold
-// anything and is left out by a selection).
+// Adds a row's parts.  With M = max m_r and w_r = 2^(m_r - M):   o = sum_r w_r O_r / sum_r w_r l_r
+// A thread takes four dimensions of a (row, KV head); neighbours take neighbouring rows, which is how the blocks' parts lie.  The
+// statistics and values of eight parts are on their way at once, M is the running maximum (a part of weight zero may hold
+// anything and is left out).  Launched as a programmatic dependent without an early trigger: blocks that wait on the SMs while
+// the attention still runs cost it more (32 rows over 2048 shared keys: 24.6 us) than the plain order of launches (18.5 us);
+// this takes 18.0 us, of which about 4 us are the adding.
+constexpr int kMergeThreads = 128, kMergeParts = 8;
 template <int HD>
-__global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int row = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 5);   // (at most 2^20 tokens of 2^10 heads)
-  const int token = row / p.NH, head = row - token * p.NH;
+  const int row = (int)blockIdx.x * 32 + (int)(threadIdx.x & 31), kvh = (int)blockIdx.y;
+  const int c4 = (int)blockIdx.z * (kMergeThreads / 32) + (int)(threadIdx.x >> 5);       // dimensions 4 c4 ..
+  const int token = p.d.by_G.div(row), g = row - token * p.d.G, head = kvh * p.d.G + g;
   if (token >= p.d.tokens) return;
   const int rows = p.cu_tokens[p.d.seqs];
-  const int kvh = p.d.by_G.div(head), g = p.d.by_G.mod(head);
   const int2 dd = p.dense_desc[(size_t)token * p.d.NKV + kvh], sd = p.strip_desc[(size_t)token * p.NH + head];
-  const int nd = dd.y & 0xffff, parts = nd + (sd.y & 0xffff);
-  if (parts == 0 || token >= rows) return;
-  // row of part r: dense parts are 256 rows apart, strips 8
+  const int nd = dd.y & 0xffff, ns = sd.y & 0xffff;
+  if (nd + ns == 0 || token >= rows) return;
   const size_t drow = (size_t)dd.x * kUnitRows + ((unsigned)dd.y >> 16) + g, srow = (size_t)sd.x * kStripRows + ((unsigned)sd.y >> 16);
-  auto dense_row = [&](int r) { return drow + (size_t)r * kUnitRows; };
-  auto strip_row = [&](int r) { return srow + (size_t)(r - nd) * kStripRows; };
-  constexpr int LPR = HD / 4, PER = 32 / LPR;              // lanes per row, parts per pass
+  const float4* dense = p.dense_o + ((size_t)dd.x * (HD / 4) + c4) * kUnitRows + ((unsigned)dd.y >> 16) + g;
+  const float* strip = p.strip_o + srow * HD + 4 * c4;
+  const int parts = nd + ns;
   float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int r0 = 0; r0 < parts; r0 += 32) {
-    const int mine = r0 + lane;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (mine < parts) ml = mine < nd ? p.dense_ml[dense_row(mine)] : p.strip_ml[strip_row(mine)];
-    float top = ml.x;
+#pragma unroll 1
+  for (int r0 = 0; r0 < parts; r0 += kMergeParts) {
+    float2 ml[kMergeParts];
+    float4 v[kMergeParts];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
-    const float Mn = fmaxf(M, top);
-    const float f = Mn == -INFINITY ? 1.f : ex2(M - Mn);
-    M = Mn;
-    float wgt = Mn == -INFINITY ? 0.f : ex2(ml.x - Mn);
-    if (ml.x != ml.x) wgt = ml.x;
-    L = L * f + warp_sum(wgt * ml.y);
+    for (int i = 0; i < kMergeParts; ++i) {
+      const int r = min(r0 + i, parts - 1);
+      const bool d = r < nd;
+      ml[i] = __ldcg(d ? p.dense_ml + drow + (size_t)r * kUnitRows : p.strip_ml + srow + (size_t)(r - nd) * kStripRows);
+      v[i] = __ldcg(d ? dense + (size_t)r * (HD / 4) * kUnitRows : reinterpret_cast<const float4*>(strip + (size_t)(r - nd) * kStripRows * HD));
+    }
+    float top = M;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < kMergeParts; ++i) {
+      if (r0 + i >= parts) ml[i].x = -INFINITY;
+      top = fmaxf(top, ml[i].x);
+      nan |= ml[i].x != ml[i].x;
+    }
+    const float f = M == -INFINITY ? 0.f : ex2(M - top);
+    M = top;
+    L = nan ? __int_as_float(0x7fffffff) : L * f;
     acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-    const int n = min(32, parts - r0);
-    constexpr int BATCH = 8;
-    for (int b = 0; b < n; b += BATCH * PER) {
-      float4 v[BATCH];
-      float w[BATCH];
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const int r = b + i * PER + lane / LPR;
-        const int at = min(r, n - 1) + r0;
-        w[i] = __shfl_sync(kFullMask, wgt, r & 31);
-        if (r >= n) w[i] = 0.f;
-        const float* src = at < nd ? p.dense_o + dense_row(at) * HD : p.strip_o + strip_row(at) * HD;
-        v[i] = __ldcg(reinterpret_cast<const float4*>(src) + lane % LPR);
-      }
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        acc.x += w[i] != 0.f ? w[i] * v[i].x : 0.f;
-        acc.y += w[i] != 0.f ? w[i] * v[i].y : 0.f;
-        acc.z += w[i] != 0.f ? w[i] * v[i].z : 0.f;
-        acc.w += w[i] != 0.f ? w[i] * v[i].w : 0.f;
+    for (int i = 0; i < kMergeParts; ++i) {
+      const float w = M == -INFINITY ? 0.f : ex2(ml[i].x - M);
+      if (w != 0.f) {
+        L += w * ml[i].y;
+        acc.x += w * v[i].x; acc.y += w * v[i].y; acc.z += w * v[i].z; acc.w += w * v[i].w;
       }
     }
   }
-#pragma unroll
-  for (int d = LPR; d < 32; d <<= 1) {
-    acc.x += __shfl_xor_sync(kFullMask, acc.x, d);
-    acc.y += __shfl_xor_sync(kFullMask, acc.y, d);
-    acc.z += __shfl_xor_sync(kFullMask, acc.z, d);
-    acc.w += __shfl_xor_sync(kFullMask, acc.w, d);
-  }
   const bool none = L == 0.f;
   const float inv = none ? 0.f : 1.f / L;
-  if (lane < LPR) {
-    uint2 w = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
-    if (none) w = make_uint2(0u, 0u);
-    *reinterpret_cast<uint2*>(p.out + (size_t)token * p.out_stride + (size_t)head * HD + 4 * lane) = w;
-  }
-  if (p.lse && lane == 0) p.lse[(size_t)token * p.NH + head] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+  uint2 w = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
+  if (none) w = make_uint2(0u, 0u);
+  *reinterpret_cast<uint2*>(p.out + (size_t)token * p.out_stride + (size_t)head * HD + 4 * c4) = w;
+  if (p.lse && c4 == 0) p.lse[(size_t)token * p.NH + head] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 }  // namespace qmkp
