@@ -348,7 +348,7 @@ const char* qmk_static_last_cuda_error(void);
 /* Block tables of a batch from the lengths its requests have to have room for (prefix included).  Row s gets
  * n_s = min(ceil(lengths[s] / page_size), max_pages) entries: the first prefix_pages are prefix_table's, the others come
  * from free_pages, in order, behind those of the rows before; entries from n_s on, and entries for which free_pages has run
- * out, are -1.  A length of zero or less is an empty row. */
+ * out, are -1.  A length of zero or less is an empty row.  At most 2^20 requests and 2^30 entries a row. */
 typedef struct qmk_block_tables_args {
   const int32_t* lengths;      /* [seqs]                                                                     */
   const int32_t* free_pages;   /* [num_free] (may be NULL when num_free is 0)                                */
@@ -363,7 +363,8 @@ int qmk_build_block_tables(const qmk_block_tables_args* args, int device, void* 
 /* Where the K and V rows of a step's new tokens go.  Request s holds kv_lengths[s] tokens and appends new_lengths[s]
  * (values below zero count as zero); the tokens of the step are numbered request by request, cut off at `tokens`.  Token t
  * of request s: position = kv_lengths[s] + (t - cu_tokens[s]), slot = page * page_size + position % page_size, or -1 where
- * the table has no page.  Entries behind the last token: slot -1, position 0, seq_id -1, active 0. */
+ * the table has no page.  Entries behind the last token: slot -1, position 0, seq_id -1, active 0.  At most 2^20 requests and
+ * 2^24 tokens. */
 typedef struct qmk_slot_map_args {
   const int32_t* block_tables;   /* [seqs, max_pages]                                  */
   const int32_t* kv_lengths;     /* [seqs]                                             */
@@ -373,7 +374,7 @@ typedef struct qmk_slot_map_args {
   int32_t* seq_ids;              /* out [tokens]                                       */
   uint8_t* active;               /* out [tokens]: 1 where slots[t] >= 0                */
   int32_t* cu_tokens;            /* out [seqs + 1]: first token of every request       */
-  int32_t* kv_lengths_out;       /* out [seqs]: tokens in the cache after the step; not kv_lengths itself */
+  int32_t* kv_lengths_out;       /* out [seqs]: tokens in the cache after the step; not an input itself */
   int32_t seqs, tokens, page_size, max_pages;
 } qmk_slot_map_args;
 int qmk_build_slot_map(const qmk_slot_map_args* args, int device, void* cuda_stream);
@@ -384,7 +385,10 @@ int qmk_build_slot_map(const qmk_slot_map_args* args, int device, void* cuda_str
  * prefix_len through prefix_table, the others through its block table (whose entries below prefix_len are not read).
  * A row that sees nothing gets zeros and an lse of minus infinity; rows from cu_tokens[seqs] on are left as they were.
  * A page index outside the pool reads as keys and values of zero.  What lies behind a request's last token in its last
- * page is never used, whatever it holds.  bf16, fp32 accumulation; head_dim 64 or 128, 1..16 query heads per KV head. */
+ * page is never used, whatever it holds.  cu_tokens must ascend from 0 to at most `tokens`, as qmk_build_slot_map leaves it: the
+ * kernel looks, and a call where it does not sets all its rows to NaN.  out may be q itself.  bf16, fp32 accumulation; head_dim 64
+ * or 128, 1..16 query heads per KV head, at most 1024 query heads, 1536 requests, 2^20 tokens, 2^30 positions (prefix_len, and
+ * max_pages * page_size) and 2^31 - 1024 rows in the pool. */
 typedef struct qmk_prefix_attention_args {
   const void* q;               /* [tokens, num_heads, head_dim], q_token_stride elements from token to token */
   void* out;                   /* the same, out_token_stride (strides: multiples of 8; 16-byte aligned)      */

@@ -48,7 +48,9 @@ static int page_shift_of(int page_size) {
 static bool aligned_to(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1u)) == 0; }
 
 extern "C" int qmk_build_block_tables(const qmk_block_tables_args* a, int device, void* cuda_stream) {
-  if (!a || a->seqs < 1 || a->max_pages < 1 || a->num_free < 0 || a->prefix_pages < 0) return QMK_ERR_INVALID_ARG;
+  if (!a || a->seqs < 1 || a->seqs > kMaxTableSeqs || a->max_pages < 1 || a->max_pages > kMaxTablePages || a->num_free < 0 ||
+      a->prefix_pages < 0)
+    return QMK_ERR_INVALID_ARG;
   const int shift = page_shift_of(a->page_size);
   if (shift < 0 || !a->lengths || !a->tables || !a->used || (a->num_free > 0 && !a->free_pages) ||
       (a->prefix_pages > 0 && !a->prefix_table) || a->prefix_pages > a->max_pages)
@@ -69,12 +71,15 @@ extern "C" int qmk_build_block_tables(const qmk_block_tables_args* a, int device
 }
 
 extern "C" int qmk_build_slot_map(const qmk_slot_map_args* a, int device, void* cuda_stream) {
-  if (!a || a->seqs < 1 || a->tokens < 1 || a->max_pages < 1) return QMK_ERR_INVALID_ARG;
+  if (!a || a->seqs < 1 || a->seqs > kMaxTableSeqs || a->tokens < 1 || a->tokens > kMaxTableTokens || a->max_pages < 1 ||
+      a->max_pages > kMaxTablePages)
+    return QMK_ERR_INVALID_ARG;
   const int shift = page_shift_of(a->page_size);
   if (shift < 0 || !a->block_tables || !a->kv_lengths || !a->new_lengths || !a->slots || !a->positions || !a->seq_ids ||
       !a->active || !a->cu_tokens || !a->kv_lengths_out)
     return QMK_ERR_INVALID_ARG;
-  if (a->kv_lengths_out == a->kv_lengths) return QMK_ERR_INVALID_ARG;   // other CTAs still read the lengths
+  // other CTAs still read the lengths
+  if (a->kv_lengths_out == a->kv_lengths || a->kv_lengths_out == a->new_lengths) return QMK_ERR_INVALID_ARG;
   DeviceScope scope(device);
   if (scope.err != cudaSuccess) return paged_fail(scope.err, "cudaSetDevice");
   SlotParams p;
@@ -103,12 +108,13 @@ static int sm_count(int device) {
 }
 
 // Regions of the workspace; every one starts on a 256-byte boundary.
-struct WorkspaceLayout { long long dense_ml, dense_o, strip_ml, strip_o, dense_desc, strip_desc, total; };
+struct WorkspaceLayout { long long refused, dense_ml, dense_o, strip_ml, strip_o, dense_desc, strip_desc, total; };
 static WorkspaceLayout workspace_layout(const PlanDims& d, int head_dim) {
   WorkspaceLayout w;
   long long at = 0;
   auto take = [&](long long bytes) { const long long here = at; at += (bytes + 255) / 256 * 256; return here; };
   const long long records = max_dense_records(d), strips = max_strip_records(d);
+  w.refused = take(4);
   w.dense_ml = take(records * kUnitRows * 8);
   w.strip_ml = take(strips * kStripRows * 8);
   w.dense_desc = take((long long)d.tokens * d.NKV * 8);
@@ -246,6 +252,7 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
   p.NH = a->num_heads; p.page_shift = page_shift_of(a->page_size); p.num_pages = a->num_pages; p.max_pages = a->max_pages;
   p.scale_log2e = a->scale * 1.4426950408889634f;
   unsigned char* ws = (unsigned char*)a->workspace;
+  p.refused = (int*)(ws + w.refused);
   p.dense_ml = (float2*)(ws + w.dense_ml); p.dense_o = (float4*)(ws + w.dense_o);
   p.strip_ml = (float2*)(ws + w.strip_ml); p.strip_o = (float*)(ws + w.strip_o);
   p.dense_desc = (int2*)(ws + w.dense_desc); p.strip_desc = (int2*)(ws + w.strip_desc);

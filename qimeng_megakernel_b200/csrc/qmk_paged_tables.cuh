@@ -11,6 +11,9 @@
 namespace qmkp {
 
 constexpr int kTableThreads = 256;
+// A CTA reads the lengths of the requests before its own: a million of them keep a call within milliseconds.  Entries and tokens are
+// counted in 32 bits with room for a pass's step.
+constexpr int kMaxTableSeqs = 1 << 20, kMaxTablePages = 1 << 30, kMaxTableTokens = 1 << 24;
 
 // Sum of v over the CTA, in every thread.  `red` has one word per warp.
 __device__ __forceinline__ long long block_sum(long long v, long long* red) {

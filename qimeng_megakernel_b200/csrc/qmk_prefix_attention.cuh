@@ -54,6 +54,7 @@ struct AttnParams {
   float2* strip_ml;            // [records, 8]
   int2* dense_desc;            // [tokens, NKV]    {first record, records | row << 16}; records 0: none
   int2* strip_desc;            // [tokens, NH]     {first record, records | row << 16}
+  int* refused;                // 1: cu_tokens does not ascend from 0 to at most `tokens`, nothing was computed
 };
 struct AttnMaps {
   CUtensorMap k, v;            // {HD, NKV, slots}, box {64, 1, min(page, 64)}
@@ -274,17 +275,21 @@ struct Work {                  // in shared memory
   Plan plan;
 };
 // Prefix sums of the requests' numbers and the plan.  One pass takes as many requests as the CTA has threads; only warps that
-// have some take part in the sums.
-__device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc, int4* red, Work* out) {
+// have some take part in the sums.  False: cu_tokens does not ascend from 0 to at most `tokens`, so rows would belong to several
+// requests or to none, and what they leave would not fit the workspace.
+__device__ __forceinline__ bool build_plan(const AttnParams& p, const Scans& sc, int4* red, Work* out) {
   const int seqs = p.d.seqs, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int4 base = make_int4(0, 0, 0, 0);
+  bool bad = false;
   for (int s0 = 0; s0 < seqs; s0 += kAttnThreads) {
     const int s = s0 + (int)threadIdx.x;
     const int warps = (min(seqs - s0, kAttnThreads) + 31) / 32;
     int4 v = make_int4(0, 0, 0, 0), x;
     if (warp < warps) {
       if (s < seqs) {
-        const Req r = load_request(p, s);
+        const int c0 = p.cu_tokens[s], c1 = p.cu_tokens[s + 1];
+        bad |= c0 > c1 || c1 > p.d.tokens || (s == 0 && c0 != 0);
+        const Req r = request(p.d, c0, c1, p.kv_lengths[s]);
         if (is_long(p.d, r)) {
           const int n = units_of(p.d, r);
           for (int u = 0; u < n; ++u) v.x += unit_blocks(p.d, r, u);
@@ -338,7 +343,7 @@ __device__ __forceinline__ void build_plan(const AttnParams& p, const Scans& sc,
       out->plan = make_plan(p.d, t, c);
     }
   }
-  __syncthreads();
+  return !__syncthreads_or(bad);
 }
 
 // A unit of one KV head.
@@ -1101,13 +1106,14 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     tmem_fence_before_sync();
   }
-  build_plan(p, sc, reinterpret_cast<int4*>(smem + S::kOffRed), work);
-  if ((int)blockIdx.x >= work->plan.dense_ctas) {
+  const bool ok = build_plan(p, sc, reinterpret_cast<int4*>(smem + S::kOffRed), work);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.refused = !ok;
+  if (!ok || (int)blockIdx.x >= work->plan.dense_ctas) {
     if (warp == kIssueWarp) {
       tmem_fence_after_sync();
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(ctl[1]) : "memory");
     }
-    if (warp < kStripWarps) walk_strips<HD>(p, maps, smem, ctl, sc, work->plan, warp, lane);
+    if (ok && warp < kStripWarps) walk_strips<HD>(p, maps, smem, ctl, sc, work->plan, warp, lane);
     return;
   }
   dense_range(work->plan, (int)blockIdx.x, w.lo, w.hi);
@@ -1138,7 +1144,7 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
 // Adds a row's parts.  With M = max m_r and w_r = 2^(m_r - M):   o = sum_r w_r O_r / sum_r w_r l_r
 // A thread takes four dimensions of a (row, KV head); neighbours take neighbouring rows, which is how the blocks' parts lie.  The
 // statistics and values of eight parts are on their way at once, M is the running maximum (a part of weight zero may hold
-// anything and is left out).  Launched as a programmatic dependent without an early trigger: blocks that wait on the SMs while
+// anything and is left out).  A refused call's rows are NaN, all of them.  Launched as a programmatic dependent without an early trigger: blocks that wait on the SMs while
 // the attention still runs cost it more (32 rows over 2048 shared keys: 24.6 us) than the plain order of launches (18.5 us);
 // this takes 18.0 us, of which about 4 us are the adding.
 constexpr int kMergeThreads = 128, kMergeParts = 8;
@@ -1149,10 +1155,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   const int c4 = (int)blockIdx.z * (kMergeThreads / 32) + (int)(threadIdx.x >> 5);       // dimensions 4 c4 ..
   const int token = p.d.by_G.div(row), g = row - token * p.d.G, head = kvh * p.d.G + g;
   if (token >= p.d.tokens) return;
-  const int rows = p.cu_tokens[p.d.seqs];
+  const int rows = p.cu_tokens[p.d.seqs], refused = *p.refused;
   const int2 dd = p.dense_desc[(size_t)token * p.d.NKV + kvh], sd = p.strip_desc[(size_t)token * p.NH + head];
-  const int nd = dd.y & 0xffff, ns = sd.y & 0xffff;
-  if (nd + ns == 0 || token >= rows) return;
+  const int nd = refused ? 0 : dd.y & 0xffff, ns = refused ? 0 : sd.y & 0xffff;
+  if (!refused && (nd + ns == 0 || token >= rows)) return;
   const size_t drow = (size_t)dd.x * kUnitRows + ((unsigned)dd.y >> 16) + g, srow = (size_t)sd.x * kStripRows + ((unsigned)sd.y >> 16);
   const float4* dense = p.dense_o + ((size_t)dd.x * (HD / 4) + c4) * kUnitRows + ((unsigned)dd.y >> 16) + g;
   const float* strip = p.strip_o + srow * HD + 4 * c4;
@@ -1191,6 +1197,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       }
     }
   }
+  if (refused) L = __int_as_float(0x7fffffff);
   const bool none = L == 0.f;
   const float inv = none ? 0.f : 1.f / L;
   uint2 w = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));

@@ -32,6 +32,10 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
 MAX_GROUP = 16            # query heads per KV head
 MAX_SEQS = 1536           # requests of one attention call
+MAX_TOKENS = 1 << 20      # rows of one attention call
+MAX_LENGTH = 1 << 30      # positions of a sequence
+# block tables and slot maps
+MAX_TABLE_SEQS, MAX_TABLE_PAGES, MAX_TABLE_TOKENS = 1 << 20, 1 << 30, 1 << 24
 
 
 @dataclass
@@ -131,8 +135,10 @@ def build_block_tables(lengths: torch.Tensor, free_pages: torch.Tensor, *, page_
         shared = prefix_table.shape[0]
     if seqs < 1:
         raise ValueError("lengths: no requests")
-    if not 1 <= max_pages < 2 ** 31:
-        raise ValueError(f"max_pages {max_pages}: expected at least 1")
+    if seqs > MAX_TABLE_SEQS:
+        raise ValueError(f"lengths: {seqs} requests, expected at most {MAX_TABLE_SEQS}")
+    if not 1 <= max_pages <= MAX_TABLE_PAGES:
+        raise ValueError(f"max_pages {max_pages}: expected 1..{MAX_TABLE_PAGES}")
     if shared > max_pages:
         raise ValueError(f"prefix_table has {shared} pages, more than max_pages = {max_pages}")
     if out is None:
@@ -156,7 +162,7 @@ def build_slot_map(block_tables: torch.Tensor, kv_lengths: torch.Tensor, new_len
     """Where the K and V rows of a step's new tokens go: request s holds `kv_lengths[s]` tokens and appends
     `new_lengths[s]` (both int32 [seqs]).  The step's tokens are numbered request by request; `tokens` is the room of the
     outputs: what does not fit is cut off (the request that straddles it appends fewer), what is left over is filled
-    with slot -1, position 0, request -1, inactive.  `out.kv_lengths` may not be `kv_lengths` itself."""
+    with slot -1, position 0, request -1, inactive.  `out.kv_lengths` may not be `kv_lengths` or `new_lengths` itself."""
     _check("block_tables", block_tables, torch.int32, 2)
     seqs, max_pages = block_tables.shape
     if not _flat(seqs, kv_lengths, new_lengths):
@@ -165,11 +171,14 @@ def build_slot_map(block_tables: torch.Tensor, kv_lengths: torch.Tensor, new_len
     tokens, page_size = int(tokens), _page_size(page_size)
     if seqs < 1 or max_pages < 1:
         raise ValueError(f"block_tables: empty shape {tuple(block_tables.shape)}")
+    if seqs > MAX_TABLE_SEQS or max_pages > MAX_TABLE_PAGES:
+        raise ValueError(f"block_tables: shape {tuple(block_tables.shape)}, expected at most {MAX_TABLE_SEQS} requests with "
+                         f"{MAX_TABLE_PAGES} pages")
     if kv_lengths.shape[0] != seqs or new_lengths.shape[0] != seqs:
         raise ValueError(f"kv_lengths and new_lengths: expected {seqs} requests, got {kv_lengths.shape[0]} and "
                          f"{new_lengths.shape[0]}")
-    if not 1 <= tokens < 2 ** 31:
-        raise ValueError(f"tokens {tokens}: expected at least 1")
+    if not 1 <= tokens <= MAX_TABLE_TOKENS:
+        raise ValueError(f"tokens {tokens}: expected 1..{MAX_TABLE_TOKENS}")
     if out is None:
         out = SlotMap.empty(seqs, tokens, block_tables.device)
     elif not (_flat(tokens, out.positions, out.seq_ids) and _flat(seqs, out.kv_lengths) and _flat(seqs + 1, out.cu_tokens)
@@ -184,6 +193,8 @@ def build_slot_map(block_tables: torch.Tensor, kv_lengths: torch.Tensor, new_len
                 raise ValueError(f"out.{name}: expected {n} entries, got {t.shape[0]}")
     if out.kv_lengths.data_ptr() == kv_lengths.data_ptr():
         raise ValueError("out.kv_lengths must not be kv_lengths itself")
+    if out.kv_lengths.data_ptr() == new_lengths.data_ptr():
+        raise ValueError("out.kv_lengths must not be new_lengths itself")
     index = block_tables.get_device()
     _on(index, "kv_lengths new_lengths out.slots out.positions out.seq_ids out.active out.cu_tokens out.kv_lengths", kv_lengths,
         new_lengths, out.slots, out.positions, out.seq_ids, out.active, out.cu_tokens, out.kv_lengths)
@@ -236,7 +247,8 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     included; its row i sees the positions below kv_lengths[s] - rows + i + 1.  Positions below `prefix_len` (a multiple
     of the page size) are read through `prefix_table`, once for all requests; the others through `block_tables`, whose
     entries below prefix_len are not read.  A row that sees nothing gets zeros (lse: minus infinity).  Rows from
-    cu_tokens[seqs] on are left as they were in `out` and `lse` (a new `out` holds zeros there).  A page index outside the
+    cu_tokens[seqs] on are left as they were in `out` and `lse` (a new `out` holds zeros there).  cu_tokens must ascend from 0 to
+    at most `tokens`, as build_slot_map makes it: where it does not, all rows become NaN.  `out` may be `q` itself.  A page index outside the
     pool reads as zeros.  What the last page holds behind a request's last token is never used; a non-finite V row
     inside a request may reach every row of its step.
 
@@ -257,6 +269,8 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} differ")
     if size not in HEAD_DIMS or kv_size != size:
         raise ValueError(f"head_dim {size} (cache {kv_size}): expected one of {HEAD_DIMS}")
+    if tokens > MAX_TOKENS:
+        raise ValueError(f"{tokens} rows: expected at most {MAX_TOKENS}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads != 0 or heads // kv_heads > MAX_GROUP:
         raise ValueError(f"{heads} query heads over {kv_heads} KV heads: expected 1..{MAX_GROUP} per KV head")
     if max_pages < 1 or num_pages < 1:
@@ -266,8 +280,10 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     if kv_lengths.shape[0] != seqs or cu_tokens.shape[0] != seqs + 1:
         raise ValueError(f"expected kv_lengths [{seqs}] and cu_tokens [{seqs + 1}], got {kv_lengths.shape[0]} and "
                          f"{cu_tokens.shape[0]}")
-    if prefix_len < 0 or prefix_len % _page_size(page_size) != 0:
-        raise ValueError(f"prefix_len {prefix_len}: expected whole pages of {page_size}")
+    if not 0 <= prefix_len <= MAX_LENGTH or prefix_len % _page_size(page_size) != 0:
+        raise ValueError(f"prefix_len {prefix_len}: expected whole pages of {page_size}, at most {MAX_LENGTH} positions")
+    if max_pages * page_size > MAX_LENGTH:
+        raise ValueError(f"block_tables: {max_pages} pages of {page_size}, expected at most {MAX_LENGTH} positions")
     if prefix_len:
         if prefix_table is None:
             raise ValueError("prefix_len needs a prefix_table")
@@ -278,7 +294,7 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         scale = 1.0 / math.sqrt(size)
     elif not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"scale {scale}: expected a positive number")
-    if q.requires_grad and torch.is_grad_enabled():
+    if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("prefix_attention has no gradient: call it under torch.inference_mode() or torch.no_grad()")
     if out is None:
         out = torch.zeros(tokens, heads, size, dtype=torch.bfloat16, device=q.device)

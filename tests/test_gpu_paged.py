@@ -331,6 +331,79 @@ def test_same_bits_twice_on_another_stream_and_in_a_graph(paged):
     compare(c, a)
 
 
+def test_offsets_that_do_not_ascend_are_refused_on_the_device(paged):
+    """cu_tokens that give a row to two requests or to none: every row becomes NaN, nothing outside the outputs is touched, and the
+    next call on the same workspace is right."""
+    for heads in ("32/8x64", "16/8x128"):
+        c = make_case(heads, 16, 64, [40, 30, 9, 17], [1, 20, 2, 1], seed=14, pad=2)
+        rows, H, D = c["q"].shape
+        ws = paged.attention_workspace(c["q"], c["k"], 4, prefix_len=64)
+        wide = torch.full((rows, H + 1, D), 5.0, dtype=torch.bfloat16, device="cuda:0")
+        for cu in ([0, rows, 0, rows, 0], [0, 1, 21, 23, rows + 1], [1, 2, 21, 23, 24], [0, 21, 1, 23, 24], [-1, 1, 21, 23, 24],
+                   [0, 1 << 30, 1 << 30, 1 << 30, (1 << 31) - 1]):
+            lse = torch.zeros(rows, H, device="cuda:0")
+            out = call(paged, dict(c, cu=ints(cu)), out=wide[:, :H], lse=lse, workspace=ws)
+            assert torch.isnan(out.float()).all() and torch.isnan(lse).all(), cu
+            assert (wide[:, H:] == 5.0).all()
+        out = call(paged, c, workspace=ws)
+        compare(c, out)
+        assert (out[-2:] == 0).all()
+
+
+def test_output_in_place_of_the_queries(paged):
+    c = make_case("32/8x64", 16, 256, [40, 3, 200, 7, 150], [5, 3, 1, 7, 70], seed=15)
+    want = call(paged, c)
+    assert call(paged, c, out=c["q"]) is c["q"] and torch.equal(c["q"], want)
+
+
+def test_two_calls_at_once_with_a_workspace_each(paged):
+    a = make_case("16/8x128", 16, 1024, [70, 1, 300, 20] * 4, [1, 1, 3, 20] * 4, seed=9)
+    b = make_case("32/8x64", 64, 2048, [33] * 24, [1] * 24, seed=16)
+    want = [call(paged, c) for c in (a, b)]
+    kept = [paged.attention_workspace(c["q"], c["k"], c["tables"].shape[0], prefix_len=c["prefix"]) for c in (a, b)]
+    outs = [[torch.empty_like(c["q"]) for _ in range(8)] for c in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(8):
+        for c, stream, ws, out in zip((a, b), streams, kept, outs):
+            with torch.cuda.stream(stream):
+                call(paged, c, out=out[i], workspace=ws)
+    torch.cuda.synchronize()
+    for w, out in zip(want, outs):
+        assert all(torch.equal(w, o) for o in out)
+
+
+def test_the_most_requests_and_no_rows(paged):
+    # 1536 requests of one row each, some without any; a page named by several tables and twice in the prefix
+    own = [1 + i % 23 for i in range(1536)]
+    c = make_case("6/2x64", 16, 32, own, [0 if i % 7 == 3 else 1 for i in range(1536)], seed=17)
+    c["prefix_table"] = ints([c["pool"][0]] * 2)
+    t = c["tables"].tolist()
+    for s in range(0, 1536, 5):
+        t[s][2] = t[1][2]
+        c["own"][s] = min(own[s], own[1])
+    c["tables"], c["kv"] = ints(t), ints([32 + n for n in c["own"]])
+    compare(c, call(paged, c))
+    none = call(paged, dict(c, q=c["q"][:0]))
+    assert none.shape == (0, 6, 64)
+
+
+def test_pool_past_32_bit_offsets(paged):
+    """Pages whose elements lie beyond 2^32 (and rows beyond 2^31 bytes) in a pool of 9 GB each for K and V."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    c = make_case("16/16x128", 64, 128, [130, 40], [1, 3], seed=18)
+    n = c["k"].shape[0]
+    big = (1 << 32) // (64 * 16 * 128) + 100
+    for name in ("k", "v"):
+        pool = torch.empty(big, 64, 16, 128, dtype=torch.bfloat16, device="cuda:0")
+        pool[big - n:] = c[name]
+        c[name] = pool
+    c["tables"] = c["tables"] + (big - n) * ((c["tables"] >= 0) & (c["tables"] < n)).int()
+    c["prefix_table"] = c["prefix_table"] + (big - n)
+    compare(c, call(paged, c))
+
+
 def test_tables_slots_and_attention_together(paged):
     """Admission, a step of prompt pieces and two decode steps as a server runs them, K and V rows stored through the slot map."""
     page, H, HK, D = 32, 16, 8, 128

@@ -37,6 +37,8 @@ def test_block_tables_refusals(paged):
     refused(ValueError, "no requests", f, i32(0), i32(3), **ok)
     refused(ValueError, "page_size 24", f, i32(3), i32(3), page_size=24, max_pages=4)
     refused(ValueError, "max_pages 0", f, i32(3), i32(3), page_size=16, max_pages=0)
+    refused(ValueError, "max_pages 1073741825", f, i32(3), i32(3), page_size=16, max_pages=2 ** 30 + 1)
+    refused(ValueError, "1048577 requests", f, i32(2 ** 20 + 1), i32(3), **ok)
     refused(ValueError, "more than max_pages", f, i32(3), i32(3), prefix_table=i32(5), **ok)
     refused(ValueError, "out: expected", f, i32(3), i32(3), out=paged.BlockTables(i32(3, 5), i32(2)), **ok)
     refused(TypeError, "out.tables", f, i32(3), i32(3), out=paged.BlockTables(i32(3, 4).long(), i32(2)), **ok)
@@ -51,10 +53,13 @@ def test_slot_map_refusals(paged):
     refused(ValueError, "expected 3 requests", f, i32(3, 2), i32(2), i32(3), **ok)
     refused(ValueError, "expected 3 requests", f, i32(3, 2), i32(3), i32(4), **ok)
     refused(ValueError, "tokens 0", f, i32(3, 2), i32(3), i32(3), page_size=16, tokens=0)
+    refused(ValueError, "tokens 16777217", f, i32(3, 2), i32(3), i32(3), page_size=16, tokens=2 ** 24 + 1)
+    refused(ValueError, "1048577, 1", f, i32(2 ** 20 + 1, 1), i32(3), i32(3), **ok)
     refused(ValueError, "page_size 8", f, i32(3, 2), i32(3), i32(3), page_size=8, tokens=4)
     out = paged.SlotMap.empty(3, 4, "cpu")
     refused(ValueError, "out.slots: expected 5", f, i32(3, 2), i32(3), i32(3), page_size=16, tokens=5, out=out)
     refused(ValueError, "not be kv_lengths itself", f, i32(3, 2), out.kv_lengths, i32(3), out=out, **ok)
+    refused(ValueError, "not be new_lengths itself", f, i32(3, 2), i32(3), out.kv_lengths, out=out, **ok)
     refused(ValueError, "no CPU path", f, i32(3, 2), i32(3), i32(3), out=out, **ok)
 
 
@@ -82,6 +87,9 @@ def test_attention_refusals(paged):
     refused(ValueError, "page_size 48", f, page=48, prefix=48)
     refused(ValueError, "whole pages", f, prefix=24)
     refused(ValueError, "whole pages", f, prefix=-16)
+    refused(ValueError, "at most 1073741824 positions", f, prefix_len=2 ** 31, prefix_table=i32(1))
+    refused(ValueError, "67108865 pages of 16", f, tables=i32(1, 2 ** 26 + 1), kv=i32(1), cu=i32(2))
+    refused(ValueError, "1048577 rows", f, q=bf(2 ** 20 + 1, 1, 64), k=bf(6, 16, 1, 64), v=bf(6, 16, 1, 64))
     refused(ValueError, "prefix_table has 1 pages", f, prefix_table=i32(1))
     refused(ValueError, "needs a prefix_table", f, prefix_table=None)
     refused(ValueError, "expected 1..1536 requests", f, seqs=1537)
@@ -95,6 +103,7 @@ def test_attention_refusals(paged):
     refused(TypeError, "lse: expected torch.float32", f, lse=bf(3, 8))
     refused(TypeError, "workspace: expected torch.uint8", f, workspace=torch.zeros(3))
     refused(RuntimeError, "no gradient", f, q=bf(3, 8, 64).requires_grad_())
+    refused(RuntimeError, "no gradient", f, v=bf(6, 16, 2, 64).requires_grad_())
     refused(ValueError, "no CPU path", f)
 
 
@@ -132,7 +141,7 @@ def test_c_entries_refuse_before_they_launch(paged):
 
     for kw in (dict(lengths=None), dict(tables=None), dict(used=None), dict(free_pages=None), dict(prefix_table=None),
                dict(seqs=0), dict(num_free=-1), dict(prefix_pages=-1), dict(page_size=0), dict(page_size=512),
-               dict(page_size=17), dict(max_pages=0), dict(prefix_pages=5)):
+               dict(page_size=17), dict(max_pages=0), dict(prefix_pages=5), dict(seqs=(1 << 20) + 1), dict(max_pages=(1 << 30) + 1)):
         assert tables(**kw) == -1, kw
 
     def slots(**kw):
@@ -144,7 +153,8 @@ def test_c_entries_refuse_before_they_launch(paged):
     for name in ("block_tables", "kv_lengths", "new_lengths", "slots", "positions", "seq_ids", "active", "cu_tokens",
                  "kv_lengths_out"):
         assert slots(**{name: None}) == -1, name
-    for kw in (dict(seqs=0), dict(tokens=0), dict(page_size=1), dict(max_pages=0), dict(kv_lengths_out=P)):
+    for kw in (dict(seqs=0), dict(tokens=0), dict(page_size=1), dict(max_pages=0), dict(kv_lengths=2 * P), dict(new_lengths=2 * P),
+               dict(seqs=(1 << 20) + 1), dict(tokens=(1 << 24) + 1), dict(max_pages=(1 << 30) + 1)):
         assert slots(**kw) == -1, kw
 
     need = lib.qmk_prefix_attention_workspace(3, 2, 8, 2, 64, 32, 0)
