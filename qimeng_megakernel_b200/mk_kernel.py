@@ -59,6 +59,15 @@ def _sig(t):
     return (t.data_ptr(), tuple(t.shape), t.dtype)
 
 
+def _paged_sig(state) -> tuple:
+    """Identity of a PagedState as far as a bound state depends on it (its lengths alternate from step to step)."""
+    if state is None:
+        return ()
+    step = state.step
+    return (step.positions.data_ptr(), step.active.data_ptr(), step.seq_ids.data_ptr(), step.slots.data_ptr(), state.rows,
+            state.page_size, _sig(state.block_tables))
+
+
 class MegaKernel:
     """Callable returned by get_mk(): owns one native handle per set of weights."""
 
@@ -68,6 +77,7 @@ class MegaKernel:
         self._weights_key = None
         self._state_key = None
         self._device = None
+        self._paged = False
         self._variant = 0
         self._timeout_cycles = int(os.environ.get("QMK_TIMEOUT_CYCLES", "0"))   # device wait budget override (0 = default)
 
@@ -153,7 +163,7 @@ class MegaKernel:
     def _ensure(self, g: Globals) -> None:
         wkey = tuple(_ptr(getattr(g, f, None)) for _, f in _WEIGHT_FIELDS) + tuple(
             LlamaConfig.as_dict().items())
-        skey = tuple(_sig(getattr(g, f, None)) for f in _STATE_FIELDS)
+        skey = tuple(_sig(getattr(g, f, None)) for f in _STATE_FIELDS) + _paged_sig(getattr(g, "paged", None))
         if wkey == self._weights_key and skey == self._state_key:
             return
         rows, S, B, Bc = self._validate(g)
@@ -189,6 +199,7 @@ class MegaKernel:
             st.kv_batch = Bc
             _lib.check(self._lib.qmk_bind_state(self._handle, C.byref(st)), self._handle)
             self._state_key = skey
+            self._paged = getattr(g, "paged", None) is not None
 
     def close(self) -> None:
         if self._handle is not None:
@@ -205,6 +216,10 @@ class MegaKernel:
     # -- launches ----------------------------------------------------------------------------
     def _stream(self) -> int:
         return torch.cuda.current_stream(self._device).cuda_stream
+
+    def _contiguous_only(self, what: str) -> None:
+        if self._paged:
+            raise ValueError(f"{what}: the state is on a paged cache, whose steps are mk(globs) after globs.paged.advance()")
 
     def _paged_step(self, g: Globals) -> None:
         cfg = LlamaConfig
@@ -224,6 +239,7 @@ class MegaKernel:
     def run_phases(self, g: Globals, phase_begin: int, phase_end: int, mode: int = 0) -> None:
         """Run a sub-range of phases (per-op verification), see qmk_run_phases."""
         self._ensure(g)
+        self._contiguous_only("run_phases")
         pos = int(g.position_id or 0)
         _lib.check(self._lib.qmk_run_phases(self._handle, pos, phase_begin, phase_end, mode, self._stream()),
                    self._handle)
@@ -232,6 +248,7 @@ class MegaKernel:
                       teacher_forced: bool = False, host_argmax: torch.Tensor | None = None) -> None:
         """Greedy decode with host token buffers (int64 CPU tensors, ideally pinned)."""
         self._ensure(g)
+        self._contiguous_only("generate_host")
         if host_tokens.dtype != torch.int64 or host_tokens.is_cuda or not host_tokens.is_contiguous():
             raise TypeError("host_tokens must be a contiguous int64 CPU tensor")
         ha = host_argmax.data_ptr() if host_argmax is not None else None
@@ -243,6 +260,7 @@ class MegaKernel:
         """n_steps greedy steps from first_pos with the token loop on the device (g.token_in feeds the first step, every
         later one takes the arg-max of the step before): one persistent launch on the batch-1 kernel."""
         self._ensure(g)
+        self._contiguous_only("generate_device")
         _lib.check(self._lib.qmk_generate_device(self._handle, int(first_pos), int(n_steps), self._stream()), self._handle)
 
     def poll_status(self) -> dict:
@@ -289,6 +307,7 @@ class MegaKernel:
         re-validation: the form a device-resident token loop and the benchmark's timed loops use)."""
         if self._handle is None:
             raise RuntimeError("decode_step needs a bound state: call mk(globs) once first")
+        self._contiguous_only("decode_step")
         _lib.check(self._lib.qmk_decode_step(self._handle, int(pos), self._stream()), self._handle)
 
     def run_phases_bound(self, pos: int, phase_begin: int, phase_end: int, mode: int = 0) -> None:
@@ -296,6 +315,7 @@ class MegaKernel:
         re-validation (a profiling loop that launches single phases back to back)."""
         if self._handle is None:
             raise RuntimeError("run_phases_bound needs a bound state: call run_phases(globs, ...) once first")
+        self._contiguous_only("run_phases_bound")
         _lib.check(self._lib.qmk_run_phases(self._handle, int(pos), int(phase_begin), int(phase_end), int(mode),
                                             self._stream()), self._handle)
 

@@ -193,3 +193,33 @@ def test_rows_without_a_place_are_reported_and_calls_refused():
     with pytest.raises(ValueError, match="page_size 24"):
         run_prefill_synthetic(cfg, weights, prompts, 4, shared_prefix=16, page_size=24)
     mk_kernel.LlamaConfig.update_from_dict(cfg)
+
+
+@torch.inference_mode()
+def test_another_state_on_the_same_rows_and_the_contiguous_forms():
+    """A PagedState put in the place of another one is looked over again; launches that know nothing of pages are refused."""
+    _need_gpu()
+    from qimeng_megakernel_b200 import paged, synthetic
+    from qimeng_megakernel_b200.prefill import run_prefill_synthetic
+    cfg = _config("llama")
+    weights = synthetic.make_weights(cfg, seed=6, device="cuda:0")
+    pre = run_prefill_synthetic(cfg, weights, _prompts(cfg, 2, 20, 16, seed=2), 4, shared_prefix=16, page_size=16)
+    g, mk = pre.globs, pre.mk
+    g.token_in = torch.zeros(2, dtype=torch.int64, device="cuda:0")
+    g.paged.advance()
+    mk(g)
+    host = torch.zeros(8, dtype=torch.int64)
+    for call in (lambda: mk.generate_device(g, 20, 1), lambda: mk.generate_host(g, host, 0, 1), lambda: mk.run_phases(g, 0, 1),
+                 lambda: mk.decode_step(20), lambda: mk.run_phases_bound(20, 0, 1)):
+        with pytest.raises(ValueError, match="paged cache"):
+            call()
+    held = g.paged
+    for rows in (1, 2):                                  # fewer rows than the step has; other buffers than the step reads
+        g.paged = paged.PagedState(held.block_tables, held.step.kv_lengths, rows, 16, held.prefix_table, held.prefix_len)
+        with pytest.raises(ValueError, match="1 rows" if rows == 1 else "must be the buffer"):
+            mk(g)
+    g.paged = held
+    g.paged.advance()
+    mk(g)
+    mk.check_status()
+    mk.close()
