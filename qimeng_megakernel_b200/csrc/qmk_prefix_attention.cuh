@@ -150,6 +150,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* u) {
       "r"(u[31])
       : "memory");
 }
+// Waits for loads; the 32 values are of use behind it only, whatever order the compiler gives the rest.
+__device__ __forceinline__ void tmem_wait_ld_of(float* r) {
+#define F4(i) "+f"(r[i]), "+f"(r[i + 1]), "+f"(r[i + 2]), "+f"(r[i + 3])
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : F4(0), F4(4), F4(8), F4(12), F4(16), F4(20), F4(24), F4(28)::"memory");
+#undef F4
+}
 __device__ __forceinline__ float ex2(float x) {   // 2^x, 2 ulp; results below 2^-126 are zero
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -631,31 +637,37 @@ struct Dense {
       float m = -INFINITY, l = 0.f;
       bool seen = false;                              // every row of the warp has an m
       const int steps = steps_of(nb, dual, g);
+      // the step of the half in which the keys end inside 16 of them: its V is cleared behind them, by a warp of the group
+      int clear_step = -1;
+      if ((warp & 3) == 0 && (x.limit & 15) != 0) {
+        const int blk = x.limit / kBlockKeys - b0;
+        if (blk >= 0 && blk < nb && (!dual || (blk & 1) == g)) clear_step = (dual ? blk - g : 2 * blk) + ((x.limit >> 6) & 1);
+      }
       bool ok = true;
       for (int j = 0; j < steps; ++j) {
         const int half = j & 1;
+        const uint32_t sh = s_col + 64 * half;
         ok = wait_bar(s_full(g, half), s_par, ctl);
         if (!ok) break;
         tmem_fence_after_sync();
         if (warp_works) {
-          const uint32_t sh = s_col + 64 * half;
           float s[64];
           tmem_ld32(s, sh);
+          tmem_wait_ld_of(s);
           tmem_ld32(s + 32, sh + 32);
-          tmem_wait_ld();
           const int k0 = (b0 + block_of(j, dual, g)) * kBlockKeys + 64 * half;
           const f32x2 scale2 = pair(p.scale_log2e, p.scale_log2e);
-          float sum, most;
+          float sum = 0.f, most = -INFINITY;
           uint32_t pk[32];
           // 2^(scale s - m) of the row, packed, and their sum.  One pair in kPolyEvery goes to the multiply-add pipe; the
           // largest exponent of those is noted, the others say themselves when they are too large.
-          auto exps = [&](auto with_poly) {
+          auto exps = [&](auto with_poly, int first) {       // of the 32 from `first` on
             const float off = m == -INFINITY ? 0.f : m;
             const f32x2 off2 = pair(-off, -off);
             f32x2 sum2[2] = {0ull, 0ull};
-            most = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
+            for (int u = 0; u < 16; ++u) {
+              const int i = first / 2 + u;
               const f32x2 e = fma2(pair(s[2 * i], s[2 * i + 1]), scale2, off2);
               float a, d;
               unpair(e, a, d);
@@ -671,15 +683,22 @@ struct Dense {
             }
             float a, d;
             unpair(add2(sum2[0], sum2[1]), a, d);
-            sum = a + d;
+            sum += a + d;
           };
           bool done = false;
           const bool plain = k0 + 64 <= warp_lim;
           if (plain && seen) {
-            exps(Yes{});
+            exps(Yes{}, 0);
+            tmem_wait_ld_of(s + 32);
+            exps(Yes{}, 32);
             done = __all_sync(kFullMask, sum <= 1099511627776.f && most <= 40.f);
           }
           if (!done) {                                  // the first step, hidden keys, a score far above m, or a NaN
+            tmem_wait_ld_of(s + 32);
+            tmem_ld32(s, sh);                           // (read again: they need not be kept for this)
+            tmem_ld32(s + 32, sh + 32);
+            tmem_wait_ld_of(s);
+            tmem_wait_ld_of(s + 32);
             if (!plain) {
               const int vis = lim - k0;
 #pragma unroll
@@ -716,27 +735,26 @@ struct Dense {
               m = m_new;
               seen = __all_sync(kFullMask, m != -INFINITY);
             }
-            exps(No{});
+            sum = 0.f;
+            exps(No{}, 0);
+            exps(No{}, 32);
           }
           l += sum;
           tmem_st32(sh, pk);
           tmem_wait_st();
         }
-        if ((warp & 3) == 0) {
-          const int blk = block_of(j, dual, g), valid = valid_keys(x, b0 + blk, half);
-          if (valid % 16 != 0) {
-            const unsigned at = n + 2u * (unsigned)blk + (unsigned)half;
-            const int st = (int)(at % S::kStages);
-            if (dual || g == 0) {
-              ok = wait_bar(v_full(st), (at / S::kStages) & 1u, ctl);
-              if (!ok) break;
-              clear_rows(st, valid);
-              if (!dual && lane == 0) mbar_arrive(v_clear());
-            } else {                                         // (the block of both groups is cleared by the first)
-              ok = wait_bar(v_clear(), clears & 1u, ctl);
-              if (!ok) break;
-              ++clears;
-            }
+        if (j == clear_step) {
+          const unsigned at = n + 2u * (unsigned)block_of(j, dual, g) + (unsigned)half;
+          const int st = (int)(at % S::kStages);
+          if (dual || g == 0) {
+            ok = wait_bar(v_full(st), (at / S::kStages) & 1u, ctl);
+            if (!ok) break;
+            clear_rows(st, x.limit & 63);
+            if (!dual && lane == 0) mbar_arrive(v_clear());
+          } else {                                           // (the block of both groups is cleared by the first)
+            ok = wait_bar(v_clear(), clears & 1u, ctl);
+            if (!ok) break;
+            ++clears;
           }
         }
         tmem_fence_before_sync();
