@@ -1167,17 +1167,17 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
 }
 
 // Adds a row's parts.  With M = max m_r and w_r = 2^(m_r - M):   o = sum_r w_r O_r / sum_r w_r l_r
-// A thread takes four dimensions of a (row, KV head); neighbours take neighbouring rows, which is how the blocks' parts lie.  The
-// statistics and values of eight parts are on their way at once, M is the running maximum (a part of weight zero may hold
-// anything and is left out).  A refused call's rows are NaN, all of them.  Launched as a programmatic dependent without an early trigger: blocks that wait on the SMs while
-// the attention still runs cost it more (32 rows over 2048 shared keys: 24.6 us) than the plain order of launches (18.5 us);
-// this takes 18.0 us, of which about 4 us are the adding.
+// A thread takes four dimensions of a (row, KV head) at a time; neighbours take neighbouring rows, which is how the blocks' parts
+// lie.  The statistics and values of eight parts are on their way at once, M is the running maximum (a part of weight zero may
+// hold anything and is left out).  A refused call's rows are NaN, all of them.  Launched as a programmatic dependent without an
+// early trigger: blocks that wait on the SMs while the attention still runs cost it more (32 rows over 2048 shared keys: 24.6 us)
+// than the plain order of launches (18.5 us); this takes 17.8 us, of which about 4 us are the adding.
 constexpr int kMergeThreads = 128, kMergeParts = 8;
+constexpr long long kMergeBlocks = 4 * 148 * 6;              // four waves of the blocks that fit the machine
 template <int HD>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int row = (int)blockIdx.x * 32 + (int)(threadIdx.x & 31), kvh = (int)blockIdx.y;
-  const int c4 = (int)blockIdx.z * (kMergeThreads / 32) + (int)(threadIdx.x >> 5);       // dimensions 4 c4 ..
   const int token = p.d.by_G.div(row), g = row - token * p.d.G, head = kvh * p.d.G + g;
   if (token >= p.d.tokens) return;
   const int rows = p.cu_tokens[p.d.seqs], refused = *p.refused;
@@ -1185,50 +1185,58 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   const int nd = refused ? 0 : dd.y & 0xffff, ns = refused ? 0 : sd.y & 0xffff;
   if (!refused && (nd + ns == 0 || token >= rows)) return;
   const size_t drow = (size_t)dd.x * kUnitRows + ((unsigned)dd.y >> 16) + g, srow = (size_t)sd.x * kStripRows + ((unsigned)sd.y >> 16);
-  const float4* dense = p.dense_o + ((size_t)dd.x * (HD / 4) + c4) * kUnitRows + ((unsigned)dd.y >> 16) + g;
-  const float* strip = p.strip_o + srow * HD + 4 * c4;
   const int parts = nd + ns;
-  float M = -INFINITY, L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float2 ml[kMergeParts];
 #pragma unroll 1
-  for (int r0 = 0; r0 < parts; r0 += kMergeParts) {
-    float2 ml[kMergeParts];
-    float4 v[kMergeParts];
+  for (int c4 = (int)blockIdx.z * (kMergeThreads / 32) + (int)(threadIdx.x >> 5), first = 1; c4 < HD / 4;      // dimensions 4 c4 ..
+       c4 += (int)gridDim.z * (kMergeThreads / 32), first = 0) {
+    const float4* dense = p.dense_o + ((size_t)dd.x * (HD / 4) + c4) * kUnitRows + ((unsigned)dd.y >> 16) + g;
+    const float* strip = p.strip_o + srow * HD + 4 * c4;
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int r0 = 0; r0 < parts; r0 += kMergeParts) {
+      float4 v[kMergeParts];
 #pragma unroll
-    for (int i = 0; i < kMergeParts; ++i) {
-      const int r = min(r0 + i, parts - 1);
-      const bool d = r < nd;
-      ml[i] = __ldcg(d ? p.dense_ml + drow + (size_t)r * kUnitRows : p.strip_ml + srow + (size_t)(r - nd) * kStripRows);
-      v[i] = __ldcg(d ? dense + (size_t)r * (HD / 4) * kUnitRows : reinterpret_cast<const float4*>(strip + (size_t)(r - nd) * kStripRows * HD));
-    }
-    float top = M;
-    bool nan = false;
+      for (int i = 0; i < kMergeParts; ++i) {
+        const int r = r0 + i;
+        if (first || parts > kMergeParts) {
+          ml[i] = make_float2(-INFINITY, 0.f);
+          if (r < parts) ml[i] = __ldcg(r < nd ? p.dense_ml + drow + (size_t)r * kUnitRows : p.strip_ml + srow + (size_t)(r - nd) * kStripRows);
+        }
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < parts)
+          v[i] = __ldcg(r < nd ? dense + (size_t)r * (HD / 4) * kUnitRows
+                               : reinterpret_cast<const float4*>(strip + (size_t)(r - nd) * kStripRows * HD));
+      }
+      float top = M;
+      bool nan = false;
 #pragma unroll
-    for (int i = 0; i < kMergeParts; ++i) {
-      if (r0 + i >= parts) ml[i].x = -INFINITY;
-      top = fmaxf(top, ml[i].x);
-      nan |= ml[i].x != ml[i].x;
-    }
-    const float f = M == -INFINITY ? 0.f : ex2(M - top);
-    M = top;
-    L = nan ? __int_as_float(0x7fffffff) : L * f;
-    acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+      for (int i = 0; i < kMergeParts; ++i) {
+        top = fmaxf(top, ml[i].x);
+        nan |= ml[i].x != ml[i].x;
+      }
+      const float f = M == -INFINITY ? 0.f : ex2(M - top);
+      M = top;
+      L = nan ? __int_as_float(0x7fffffff) : L * f;
+      acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
 #pragma unroll
-    for (int i = 0; i < kMergeParts; ++i) {
-      const float w = M == -INFINITY ? 0.f : ex2(ml[i].x - M);
-      if (w != 0.f) {
-        L += w * ml[i].y;
-        acc.x += w * v[i].x; acc.y += w * v[i].y; acc.z += w * v[i].z; acc.w += w * v[i].w;
+      for (int i = 0; i < kMergeParts; ++i) {
+        const float w = M == -INFINITY ? 0.f : ex2(ml[i].x - M);
+        if (w != 0.f) {
+          L += w * ml[i].y;
+          acc.x += w * v[i].x; acc.y += w * v[i].y; acc.z += w * v[i].z; acc.w += w * v[i].w;
+        }
       }
     }
+    if (refused) L = __int_as_float(0x7fffffff);
+    const bool none = L == 0.f;
+    const float inv = none ? 0.f : 1.f / L;
+    uint2 w = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
+    if (none) w = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2*>(p.out + (size_t)token * p.out_stride + (size_t)head * HD + 4 * c4) = w;
+    if (p.lse && c4 == 0) p.lse[(size_t)token * p.NH + head] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
   }
-  if (refused) L = __int_as_float(0x7fffffff);
-  const bool none = L == 0.f;
-  const float inv = none ? 0.f : 1.f / L;
-  uint2 w = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
-  if (none) w = make_uint2(0u, 0u);
-  *reinterpret_cast<uint2*>(p.out + (size_t)token * p.out_stride + (size_t)head * HD + 4 * c4) = w;
-  if (p.lse && c4 == 0) p.lse[(size_t)token * p.NH + head] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 }  // namespace qmkp
