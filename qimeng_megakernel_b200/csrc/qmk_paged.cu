@@ -195,8 +195,8 @@ static bool pool_map(encode_fn enc, CUtensorMap* m, const void* base, const qmk_
 }
 
 // 32 rows of a KV head a block, and the fewer dimensions to a thread the fewer rows there are: all blocks of a small call run at
-// once, a thread of a large one weighs the parts once for several quads.  4400 tokens at 16/8 heads x 128: 342 us with a quad to a
-// thread, 332 with eight; 32 rows at 32/8 x 64: 18.0 with one, 24.9 with four.
+// once, a thread of a large one weighs the parts once for several quads.  9 pieces behind 8192 keys at 16/8 heads x 128: 342 us with
+// a quad to a thread, 324 with eight, four of them read together; 32 rows at 32/8 x 64: 18.0 with one, 24.9 with four.
 template <int HD>
 static dim3 merge_grid(const PlanDims& d) {
   const long long blocks = (long long)((d.tokens * d.G + 31) / 32) * d.NKV;
@@ -230,7 +230,8 @@ static int launch_attention(const qmk_prefix_attention_args* a, const AttnParams
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, merge_kernel<HD>, p);
+  e = cfg.gridDim.z < HD / 4 / (kMergeThreads / 32) ? cudaLaunchKernelEx(&cfg, merge_kernel<HD, true>, p)
+                                                    : cudaLaunchKernelEx(&cfg, merge_kernel<HD, false>, p);
   return e == cudaSuccess ? QMK_OK : paged_fail(e, "merge_kernel");
 }
 

@@ -1174,7 +1174,7 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
 // than the plain order of launches (18.5 us); this takes 17.8 us, of which about 4 us are the adding.
 constexpr int kMergeThreads = 128, kMergeParts = 8;
 constexpr long long kMergeBlocks = 4 * 148 * 6;              // four waves of the blocks that fit the machine
-template <int HD>
+template <int HD, bool kMany>                                // kMany: a large call
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int row = (int)blockIdx.x * 32 + (int)(threadIdx.x & 31), kvh = (int)blockIdx.y;
@@ -1185,11 +1185,46 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   const int nd = refused ? 0 : dd.y & 0xffff, ns = refused ? 0 : sd.y & 0xffff;
   if (!refused && (nd + ns == 0 || token >= rows)) return;
   const size_t drow = (size_t)dd.x * kUnitRows + ((unsigned)dd.y >> 16) + g, srow = (size_t)sd.x * kStripRows + ((unsigned)sd.y >> 16);
-  const int parts = nd + ns;
+  const int parts = nd + ns, from = (int)blockIdx.z * (kMergeThreads / 32) + (int)(threadIdx.x >> 5);
+  const int step = (int)gridDim.z * (kMergeThreads / 32);
+  uint16_t* out = p.out + (size_t)token * p.out_stride + (size_t)head * HD;
+  if (kMany && parts <= 2) {                                 // four quads on their way at once
+    auto stat = [&](int r) { return __ldcg(r < nd ? p.dense_ml + drow + (size_t)r * kUnitRows : p.strip_ml + srow + (size_t)(r - nd) * kStripRows); };
+    const float2 a = parts > 0 ? stat(0) : make_float2(-INFINITY, 0.f), b = parts > 1 ? stat(1) : make_float2(-INFINITY, 0.f);
+    const float M = fmaxf(a.x, b.x);
+    const float wa = M == -INFINITY ? 0.f : ex2(a.x - M), wb = M == -INFINITY ? 0.f : ex2(b.x - M);
+    float L = (wa != 0.f ? wa * a.y : 0.f) + (wb != 0.f ? wb * b.y : 0.f);
+    if (refused || a.x != a.x || b.x != b.x) L = __int_as_float(0x7fffffff);
+    const bool none = L == 0.f;
+    const float inv = none ? 0.f : 1.f / L;
+#pragma unroll 1
+    for (int c0 = from; c0 < HD / 4; c0 += 4 * step) {
+      float4 va[4], vb[4];
+      auto value = [&](int r, int c4) {
+        return __ldcg(r < nd ? p.dense_o + (((size_t)dd.x + r) * (HD / 4) + c4) * kUnitRows + ((unsigned)dd.y >> 16) + g
+                             : reinterpret_cast<const float4*>(p.strip_o + (srow + (size_t)(r - nd) * kStripRows) * HD + 4 * c4));
+      };
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool there = c0 + i * step < HD / 4;
+        va[i] = vb[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (there && wa != 0.f) va[i] = value(0, c0 + i * step);
+        if (there && wb != 0.f) vb[i] = value(1, c0 + i * step);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = (wa * va[i].x + wb * vb[i].x) * inv, y = (wa * va[i].y + wb * vb[i].y) * inv;
+        const float z = (wa * va[i].z + wb * vb[i].z) * inv, t = (wa * va[i].w + wb * vb[i].w) * inv;
+        const uint2 w = none ? make_uint2(0u, 0u) : make_uint2(pack2(x, y), pack2(z, t));
+        if (c0 + i * step < HD / 4) *reinterpret_cast<uint2*>(out + 4 * (c0 + i * step)) = w;
+      }
+    }
+    if (p.lse && from == 0) p.lse[(size_t)token * p.NH + head] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    return;
+  }
   float2 ml[kMergeParts];
 #pragma unroll 1
-  for (int c4 = (int)blockIdx.z * (kMergeThreads / 32) + (int)(threadIdx.x >> 5), first = 1; c4 < HD / 4;      // dimensions 4 c4 ..
-       c4 += (int)gridDim.z * (kMergeThreads / 32), first = 0) {
+  for (int c4 = from, first = 1; c4 < HD / 4; c4 += step, first = 0) {      // dimensions 4 c4 ..
     const float4* dense = p.dense_o + ((size_t)dd.x * (HD / 4) + c4) * kUnitRows + ((unsigned)dd.y >> 16) + g;
     const float* strip = p.strip_o + srow * HD + 4 * c4;
     float M = -INFINITY, L = 0.f;
@@ -1234,7 +1269,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
     const float inv = none ? 0.f : 1.f / L;
     uint2 w = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
     if (none) w = make_uint2(0u, 0u);
-    *reinterpret_cast<uint2*>(p.out + (size_t)token * p.out_stride + (size_t)head * HD + 4 * c4) = w;
+    *reinterpret_cast<uint2*>(out + 4 * c4) = w;
     if (p.lse && c4 == 0) p.lse[(size_t)token * p.NH + head] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
   }
 }

@@ -331,6 +331,26 @@ def test_same_bits_twice_on_another_stream_and_in_a_graph(paged):
     compare(c, a)
 
 
+@pytest.mark.parametrize("heads,own,new", [("16/16x128", [400, 1, 610, 77], [400, 1, 610, 77]), ("32/8x64", [900, 40, 410], [900, 3, 400]),
+                                           ("16/8x128", [700, 650, 5], [700, 640, 5])])
+def test_large_calls(paged, heads, own, new):
+    """Calls whose rows' parts are added by fewer threads than the others': rows with one part, two, several and none."""
+    c = make_case(heads, 32, 512, own, new, seed=19, pad=5)
+    rows, H, D = c["q"].shape
+    lse = torch.full((rows, H), 7.0, device="cuda:0")
+    out = torch.full_like(c["q"], 3.0)
+    call(paged, c, out=out, lse=lse)
+    compare(c, out, lse)
+    assert (out[-5:] == 3.0).all() and (lse[-5:] == 7.0).all()
+    c["kv"] = ints([0, *c["kv"].tolist()[1:]])                     # the first request's rows see nothing
+    call(paged, c, out=out, lse=lse)
+    assert (out[:new[0]] == 0).all() and torch.isinf(lse[:new[0]]).all()
+    c["own"] = [-512, *own[1:]]
+    compare(c, out, lse)
+    call(paged, dict(c, cu=ints([0, rows, 0, rows] + [0] * (len(own) - 3))), out=out, lse=lse)
+    assert torch.isnan(out.float()).all() and torch.isnan(lse).all()
+
+
 def test_offsets_that_do_not_ascend_are_refused_on_the_device(paged):
     """cu_tokens that give a row to two requests or to none: every row becomes NaN, nothing outside the outputs is touched, and the
     next call on the same workspace is right."""
