@@ -23,9 +23,9 @@
 // What bounds it (B200, whole calls).  Many rows: the softmax warps' instructions.  A step of 64 keys for both groups (256 rows)
 // takes about 1450 clocks, 1070 of them the exponentials of the two warps that share a scheduler's issue slots (65 % of them
 // used), the rest reading S, writing P and the barriers; the products take 630 clocks of the tensor pipe at head size 64.
-// 4 pieces of 500..1100 tokens behind 32768 shared keys at 32/8 heads x 64: 1075 us, 745 TFLOP/s; 9 pieces behind 8192 at
-// 16/8 x 128, where a step has twice the products: 346 us, 1000 TFLOP/s.  Few rows: the latency of plan, first loads, last
-// block and merge, about 11 us in all (2 rows), and the bytes: 64 rows behind 12288 keys at 16/8 x 128 46 us, 4.2 TB/s.
+// 4 pieces of 500..1100 tokens behind 32768 shared keys at 32/8 heads x 64: 1050 us, 760 TFLOP/s; 9 pieces behind 8192 at
+// 16/8 x 128, where a step has twice the products: 324 us, 1066 TFLOP/s.  Few rows: the latency of plan, first loads, last
+// block and merge, about 11 us in all (2 rows), and the bytes: 64 rows behind 12288 keys at 16/8 x 128 45 us, 4.2 TB/s.
 //
 // Both parts leave partial results (m, l, unnormalised O, all in 32 bits) unless a row is complete; merge_kernel adds them
 // up in a fixed order, so a call gives the same bits every time.  Nothing is kept between calls.
