@@ -24,8 +24,8 @@
 // takes about 1450 clocks, 1070 of them the exponentials of the two warps that share a scheduler's issue slots (65 % of them
 // used), the rest reading S, writing P and the barriers; the products take 630 clocks of the tensor pipe at head size 64.
 // 4 pieces of 500..1100 tokens behind 32768 shared keys at 32/8 heads x 64: 1050 us, 760 TFLOP/s; 9 pieces behind 8192 at
-// 16/8 x 128, where a step has twice the products: 324 us, 1066 TFLOP/s.  Few rows: the latency of plan, first loads, last
-// block and merge, about 11 us in all (2 rows), and the bytes: 64 rows behind 12288 keys at 16/8 x 128 45 us, 4.2 TB/s.
+// 16/8 x 128, where a step has twice the products: 322 us, 1075 TFLOP/s.  Few rows: the latency of plan, first loads, last
+// block and merge, about 12 us in all (2 rows), and the bytes: 64 rows behind 12288 keys at 16/8 x 128 45 us, 4.2 TB/s.
 //
 // Both parts leave partial results (m, l, unnormalised O, all in 32 bits) unless a row is complete; merge_kernel adds them
 // up in a fixed order, so a call gives the same bits every time.  Nothing is kept between calls.
@@ -1171,7 +1171,7 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
 // lie.  The statistics and values of eight parts are on their way at once, M is the running maximum (a part of weight zero may
 // hold anything and is left out).  A refused call's rows are NaN, all of them.  Launched as a programmatic dependent without an
 // early trigger: blocks that wait on the SMs while the attention still runs cost it more (32 rows over 2048 shared keys: 24.6 us)
-// than the plain order of launches (18.5 us); this takes 17.8 us, of which about 4 us are the adding.
+// than the plain order of launches (18.5 us); this takes 17.8 us (all before the present division of the CTAs), of which about 4 us are the adding.
 constexpr int kMergeThreads = 128, kMergeParts = 8;
 constexpr long long kMergeBlocks = 4 * 148 * 6;              // four waves of the blocks that fit the machine
 template <int HD, bool kMany>                                // kMany: a large call

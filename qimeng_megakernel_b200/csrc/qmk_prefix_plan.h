@@ -27,7 +27,8 @@ constexpr int kLongRows = 128;      // a request with fewer rows shares its unit
 constexpr int kStripRows = 8;       // rows of a strip (the short side of an mma.sync tile)
 constexpr int kMaxGroup = 16;       // query heads of a KV head
 constexpr int kPieceKeys = 32;      // keys of a piece
-constexpr int kStripCost = 2;       // pieces without keys at the head of a strip: what it costs to take one up
+constexpr int kStripCost = 3;       // pieces without keys at the head of a strip: what it costs to take one up (2 is 1 %
+                                    // slower over 14 calls, 1 and 4 are 6 and 2 % over six)
 constexpr int kStripWarps = 8;      // warps of a CTA that walk strips
 constexpr int kMaxSeqs = 1536;      // requests of a call (their prefix sums are kept in shared memory)
 
