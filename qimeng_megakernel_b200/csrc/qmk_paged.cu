@@ -127,7 +127,7 @@ static WorkspaceLayout workspace_layout(const PlanDims& d, int head_dim) {
 
 // The device counts blocks, pieces and records in 32 bits.
 static bool counts_fit(const PlanDims& d) {
-  const long long most = 0x7fffffffll, strips = max_strips(d), by_request = (long long)d.seqs * (kLongRows / kStripRows) * d.NKV;
+  const long long most = 0x7fffffffll, strips = max_strips(d), by_request = (long long)d.seqs * (kMostShort / kStripRows) * d.NKV;
   return max_units(d) * d.NKV * (d.room / kBlockKeys + 1) <= most && max_strip_records(d) <= most &&
          (strips < by_request ? strips : by_request) * (d.room / kPieceKeys + 1 + kStripCost) <= most;
 }

@@ -2,9 +2,9 @@
 // and by a host test that replays it.
 //
 // Rows of a KV head are the step's (token, query head of the group) pairs.  Requests come in two kinds:
-//   long   (n * G >= kLongRows rows)  cut into units of up to 256 rows of ONE request; a unit walks all its keys, prefix
+//   long   (is_long: pieces of prompts)  cut into units of up to 256 rows of ONE request; a unit walks all its keys, prefix
 //          included, causal limits applied
-//   short  (fewer rows: decoding, verification)  their tokens are strung together and cut into units of 256 rows, which
+//   short  (few rows: decoding, verification, short pieces behind a long prefix)  their tokens are strung together and cut into units of 256 rows, which
 //          walk the shared prefix; what each request holds behind the prefix is walked by single warps, 8 rows at a time: a
 //          STRIP is (request, 8 of its rows, KV head), cut into pieces of 32 keys
 // The 128-key blocks of all (KV head, unit) pairs, in that order, are dealt to the first CTAs as equal contiguous ranges, the
@@ -24,6 +24,7 @@ namespace qmkp {
 constexpr int kUnitRows = 256;      // two tensor-core tiles of 128 rows
 constexpr int kBlockKeys = 128;     // keys of a block
 constexpr int kLongRows = 128;      // a request with fewer rows shares its units
+constexpr int kMostShort = 512;     // one with as many or more does not
 constexpr int kStripRows = 8;       // rows of a strip (the short side of an mma.sync tile)
 constexpr int kMaxGroup = 16;       // query heads of a KV head
 constexpr int kPieceKeys = 32;      // keys of a piece
@@ -95,8 +96,6 @@ QMKP_HD int limit_of(const PlanDims& d, const Req& r, int i) {
   const long long l = (long long)r.base + i + 1;
   return l < 0 ? 0 : (l > d.room ? d.room : (int)l);
 }
-QMKP_HD bool is_long(const PlanDims& d, const Req& r) { return (long long)r.n * d.G >= kLongRows; }
-
 // long requests
 QMKP_HD int units_of(const PlanDims& d, const Req& r) { return d.by_unit.div(r.n + d.unit_tokens - 1); }
 QMKP_HD int unit_limit(const PlanDims& d, const Req& r, int u) {
@@ -107,6 +106,16 @@ QMKP_HD int unit_blocks(const PlanDims& d, const Req& r, int u) {
 }
 // short requests
 QMKP_HD int own_keys(const PlanDims& d, const Req& r) { return r.n > 0 ? imax(0, limit_of(d, r, r.n - 1) - d.prefix_len) : 0; }
+// Between kLongRows and kMostShort rows the cheaper way: units of its own are padded to whole ones and walk all keys so, shared ones
+// are not, but a row and key of a strip cost 8 (head size 64; 13 at 128) of a block's.  Weighed with about twice that, as the blocks
+// lack the strips' CTAs: 10 pieces of 64..90 tokens behind 28160 keys at 16/8 x 128 take 189 us against 243 us in units of their
+// own, 5 of 70..120 behind 16384 at 32/8 x 64 115 against 127; 16 of 33..100 behind 2048 61 either way (64 weighed with once that).
+QMKP_HD bool is_long(const PlanDims& d, const Req& r) {
+  const long long rows = (long long)r.n * d.G;
+  if (rows < kLongRows || rows >= kMostShort) return rows >= kLongRows;
+  const int pad = rows == kLongRows ? 0 : units_of(d, r) * kUnitRows - (int)rows;
+  return (long long)pad * limit_of(d, r, r.n - 1) <= (d.head_dim == 128 ? 26 : 14) * rows * (own_keys(d, r) + kStripCost * kPieceKeys);
+}
 QMKP_HD int strips_of(const PlanDims& d, const Req& r) { return (r.n * d.G + kStripRows - 1) / kStripRows; }   // of a KV head
 QMKP_HD int pieces_of(const PlanDims& d, const Req& r) { return kStripCost + (own_keys(d, r) + kPieceKeys - 1) / kPieceKeys; }
 

@@ -18,7 +18,7 @@ using namespace qmkp;
     }                                                                 \
   } while (0)
 static int g_case;
-static int aligned;
+static int aligned, middle;                            // middle: requests of some hundred rows that share their units
 
 struct Walk { std::vector<std::vector<int>> seen; };   // [row of the step * NKV + kvh][key] -> times
 
@@ -34,14 +34,18 @@ int main() {
   }
   for (g_case = 0; g_case < 1500; ++g_case) {
     const int G = pick(1, 16), ctas = pick(0, 1) ? 148 : pick(2, 30), page = 16;
-    const int prefix_len = pick(0, 3) ? 16 * pick(0, 60) : 0, max_pages = prefix_len / page + pick(1, 40);
-    PlanDims d = make_dims(1, pick(1, pick(0, 3) ? 6 : 40), G, pick(1, 4), pick(0, 1) ? 64 : 128, prefix_len, max_pages * page, ctas);
+    const bool far = g_case % 25 == 24;                      // short pieces behind a long prefix
+    const int prefix_len = far ? 16 * pick(200, 400) : (pick(0, 3) ? 16 * pick(0, 60) : 0);
+    const int max_pages = prefix_len / page + pick(1, 40);
+    PlanDims d = make_dims(1, far ? pick(1, 3) : pick(1, pick(0, 3) ? 6 : 40), G, far ? 1 : pick(1, 4), pick(0, 1) ? 64 : 128, prefix_len,
+                           max_pages * page, ctas);
     std::vector<int> cu(1, 0), kv;
     const int kind = pick(0, 3);
     for (int s = 0; s < d.seqs; ++s) {
-      const int n = kind == 0 ? 1 : (kind == 1 ? pick(0, 5) : (kind == 2 ? pick(0, 400 / d.G) : pick(0, 2) * pick(0, 600)));
+      const int n = far ? pick(128, 511) / d.G : kind == 0 ? 1 : (kind == 1 ? pick(0, 5) : (kind == 2 ? pick(0, 400 / d.G) : pick(0, 2) * pick(0, 600)));
       cu.push_back(cu.back() + n);
-      kv.push_back(pick(0, 9) ? d.prefix_len + pick(0, max_pages * page - d.prefix_len + 5) : pick(-3, d.prefix_len + n));
+      if (far) kv.push_back(d.prefix_len + n + pick(0, 30));
+      else kv.push_back(pick(0, 9) ? d.prefix_len + pick(0, max_pages * page - d.prefix_len + 5) : pick(-3, d.prefix_len + n));
     }
     d.tokens = cu.back() + pick(-3, 5);
     if (d.tokens < 1) d.tokens = 1;
@@ -58,6 +62,7 @@ int main() {
         t.long_blocks += blocks;
         t.long_units += units_of(d, r);
       } else {
+        middle += r.n * d.G >= kLongRows;
         t.short_tokens += r.n;
         t.pieces += (long long)strips_of(d, r) * pieces_of(d, r);
       }
@@ -218,6 +223,7 @@ int main() {
       }
   }
   CHECK(aligned > 100);
+  CHECK(middle > 30);
   std::printf("prefix plan ok\n");
   return 0;
 }

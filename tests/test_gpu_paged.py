@@ -351,6 +351,16 @@ def test_large_calls(paged, heads, own, new):
     assert torch.isnan(out.float()).all() and torch.isnan(lse).all()
 
 
+@pytest.mark.parametrize("heads,prefix,own,new", [("32/8x64", 4096, [40, 60, 33, 90, 300], [40, 60, 33, 85, 1]),
+                                                  ("16/8x128", 8192, [70, 100, 64, 20], [70, 90, 64, 3]),
+                                                  ("5/1x128", 8192, [30, 75, 102], [30, 75, 102])])
+def test_short_pieces_behind_a_long_prefix(paged, heads, prefix, own, new):
+    """Requests of 128..511 rows, most of whose keys are the prefix: they share units and have strips of their own."""
+    c = make_case(heads, 64, prefix, own, new, seed=21, pad=2)
+    lse = torch.empty(c["q"].shape[0], c["q"].shape[1], device="cuda:0")
+    compare(c, call(paged, c, lse=lse), lse)
+
+
 def test_offsets_that_do_not_ascend_are_refused_on_the_device(paged):
     """cu_tokens that give a row to two requests or to none: every row becomes NaN, nothing outside the outputs is touched, and the
     next call on the same workspace is right."""
