@@ -65,7 +65,7 @@ def _paged_sig(state) -> tuple:
         return ()
     step = state.step
     return (step.positions.data_ptr(), step.active.data_ptr(), step.seq_ids.data_ptr(), step.slots.data_ptr(), state.rows,
-            state.page_size, _sig(state.block_tables))
+            state.page_size, _sig(state.block_tables), _sig(state.prefix_table), state.prefix_len)
 
 
 class MegaKernel:
@@ -145,6 +145,7 @@ class MegaKernel:
         if getattr(g, "position_ids", None) is not None:
             _check_tensor("position_ids", g.position_ids, torch.int32, (B,))
         if getattr(g, "paged", None) is not None:
+            g.paged.check()
             step = g.paged.step
             if S != g.paged.page_size or g.paged.rows != B:
                 raise ValueError(f"globs.paged: pages of {g.paged.page_size} and {g.paged.rows} rows, k_cache has {S} and kv_slots {B}")

@@ -338,10 +338,13 @@ class PagedState:
 
     def __init__(self, block_tables: torch.Tensor, lengths: torch.Tensor, rows: int, page_size: int,
                  prefix_table: torch.Tensor | None, prefix_len: int):
-        device = block_tables.device
-        seqs = block_tables.shape[0]
         self.block_tables, self.page_size, self.rows = block_tables, _page_size(page_size), int(rows)
         self.prefix_table, self.prefix_len = prefix_table, int(prefix_len)
+        self.step: SlotMap | None = None
+        self.check()
+        device, seqs = block_tables.device, block_tables.shape[0]
+        if not isinstance(lengths, torch.Tensor) or lengths.shape != (seqs,):
+            raise ValueError(f"lengths: expected one for each of {seqs} requests")
         self.step = SlotMap.empty(seqs, self.rows, device)
         for t in (self.step.positions, self.step.active, self.step.seq_ids, self.step.cu_tokens):
             t.zero_()
@@ -350,6 +353,40 @@ class PagedState:
         self._other = torch.empty_like(self.step.kv_lengths)
         self.ones = torch.ones(seqs, dtype=torch.int32, device=device)
         self.workspace: torch.Tensor | None = None
+
+    def check(self) -> None:
+        """Everything that the library takes as a bare address is what its kernels read.  (At construction, and again by the
+        kernel call when a tensor has been put in another's place.)"""
+        _check("block_tables", self.block_tables, torch.int32, 2)
+        seqs, max_pages = self.block_tables.shape
+        if seqs < 1 or max_pages < 1:
+            raise ValueError(f"block_tables: empty shape {tuple(self.block_tables.shape)}")
+        if seqs > MAX_SEQS:
+            raise ValueError(f"{seqs} requests: expected 1..{MAX_SEQS} requests")
+        if self.rows < 1:
+            raise ValueError(f"rows {self.rows}: expected at least one")
+        if not 0 <= self.prefix_len <= MAX_LENGTH or self.prefix_len % self.page_size != 0:
+            raise ValueError(f"prefix_len {self.prefix_len}: expected whole pages of {self.page_size}, at most {MAX_LENGTH} positions")
+        tensors = []
+        if self.prefix_len:
+            if self.prefix_table is None:
+                raise ValueError("prefix_len needs a prefix_table")
+            _check("prefix_table", self.prefix_table, torch.int32, 1)
+            if self.prefix_table.shape[0] * self.page_size < self.prefix_len:
+                raise ValueError(f"prefix_table has {self.prefix_table.shape[0]} pages, prefix_len needs {self.prefix_len // self.page_size}")
+            tensors.append(("prefix_table", self.prefix_table))
+        if self.step is not None:
+            for name, dtype, n in (("slots", torch.int64, self.rows), ("positions", torch.int32, self.rows),
+                                   ("seq_ids", torch.int32, self.rows), ("active", torch.uint8, self.rows),
+                                   ("cu_tokens", torch.int32, seqs + 1), ("kv_lengths", torch.int32, seqs)):
+                t = getattr(self.step, name)
+                _check(f"step.{name}", t, dtype, 1)
+                if t.shape[0] != n:
+                    raise ValueError(f"step.{name}: expected {n} entries, got {t.shape[0]}")
+                tensors.append((f"step.{name}", t))
+        for name, t in tensors:
+            if t.device != self.block_tables.device:
+                raise ValueError(f"{name} is on {t.device}, expected {self.block_tables.device}")
 
     @property
     def capacity(self) -> int:

@@ -207,3 +207,45 @@ def test_paged_state_refusals(small_config, small_weights):
     refused(ValueError, "keeps at least", f, shared_prefix=20)
     refused(ValueError, "keeps at least", f, shared_prefix=-1)
     refused(ValueError, "no CPU path", f)
+
+
+def state(paged, seqs=2, room=4, rows=2, page=16, lengths=None, prefix_table=None, prefix_len=0, tables=None):
+    return paged.PagedState(i32(seqs, room) if tables is None else tables, i32(seqs) if lengths is None else lengths, rows, page,
+                            prefix_table, prefix_len)
+
+
+def test_paged_state_looks_at_its_tables(paged):
+    """What a state hands to the library as bare pointers has to be what the kernels read (int32, contiguous, long enough)."""
+    f = lambda **kw: state(paged, **kw)
+    refused(TypeError, "prefix_table: expected torch.int32", f, prefix_table=i32(2).long(), prefix_len=32)
+    refused(ValueError, "prefix_table must be contiguous", f, prefix_table=i32(4)[::2], prefix_len=32)
+    refused(ValueError, "prefix_table: expected 1 dim", f, prefix_table=i32(2, 1), prefix_len=32)
+    refused(ValueError, "prefix_table has 1 pages", f, prefix_table=i32(1), prefix_len=32)
+    refused(ValueError, "needs a prefix_table", f, prefix_len=16)
+    refused(ValueError, "prefix_table is on meta", f, prefix_table=i32(2).to("meta"), prefix_len=32)
+    refused(ValueError, "whole pages", f, prefix_table=i32(2), prefix_len=24)
+    refused(ValueError, "whole pages", f, prefix_table=i32(2), prefix_len=-16)
+    refused(TypeError, "block_tables: expected torch.int32", f, tables=i32(2, 4).long())
+    refused(ValueError, "block_tables must be contiguous", f, tables=i32(4, 2).t())
+    refused(ValueError, "block_tables: empty", f, tables=i32(0, 4), lengths=i32(0))
+    refused(ValueError, "expected 1..1536 requests", f, seqs=1537)
+    refused(ValueError, "lengths: expected", f, lengths=i32(1))
+    refused(ValueError, "rows 0", f, rows=0)
+    f(prefix_table=i32(3), prefix_len=32)
+
+
+def test_a_replaced_table_is_looked_at_again(paged):
+    """The kernel call's binding depends on every table of the state; what was put in one's place is checked again."""
+    from qimeng_megakernel_b200 import mk_kernel
+    s = state(paged, prefix_table=i32(2), prefix_len=32)
+    s.check()
+    for name, value in (("prefix_table", i32(3)), ("prefix_len", 16), ("block_tables", i32(2, 5))):
+        before = mk_kernel._paged_sig(s)
+        setattr(s, name, value)
+        assert mk_kernel._paged_sig(s) != before, name
+    s.check()
+    s.prefix_table = i32(2).long()
+    refused(TypeError, "prefix_table: expected torch.int32", s.check)
+    s.prefix_table = i32(2)
+    s.step.slots = i32(2)
+    refused(TypeError, "step.slots: expected torch.int64", s.check)
