@@ -178,6 +178,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {   // NaN if any of them is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 // Two floats in a register pair.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair(float lo, float hi) {
@@ -196,7 +201,8 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
   return v;
 }
-// 2^x of a pair on the fused multiply-add pipe, for x <= 127; below -126 the result is about 2^-126.  x = n + f with n the
+// 2^x of a pair on the fused multiply-add pipe, for x <= 127; below -126, and for a NaN, the result is about 2^-126 (whoever calls
+// this looks for NaN himself).  x = n + f with n the
 // nearest whole number (an addition of 1.5 * 2^23 rounds to it and leaves it in the low bits), 2^f on [-1/2, 1/2] by the
 // polynomial of degree 4 with the smallest largest relative error (2.6e-6, found by Remez exchange), n into the exponent.
 __device__ __forceinline__ void ex2_pair(f32x2 x, float& lo, float& hi) {
@@ -667,7 +673,7 @@ struct Dense {
           float sum = 0.f, most = -INFINITY;
           uint32_t pk[32];
           // 2^(scale s - m) of the row, packed, and their sum.  One pair in kPolyEvery goes to the multiply-add pipe; the
-          // largest exponent of those is noted, the others say themselves when they are too large.
+          // largest exponent of those is noted (a NaN before all), the others say themselves when they are too large or NaN.
           auto exps = [&](auto with_poly, int first) {       // of the 32 from `first` on
             const float off = m == -INFINITY ? 0.f : m;
             const f32x2 off2 = pair(-off, -off);
@@ -679,7 +685,7 @@ struct Dense {
               float a, d;
               unpair(e, a, d);
               if (decltype(with_poly)::value && i % kPolyEvery == kPolyEvery - 1) {
-                most = max3(most, a, d);
+                most = max3_nan(most, a, d);
                 ex2_pair(e, a, d);
               } else {
                 a = ex2(a);

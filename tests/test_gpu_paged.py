@@ -475,3 +475,76 @@ def test_tables_slots_and_attention_together(paged):
             at += n
         kv = step.kv_lengths
         assert (out[at:] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ NaN and infinity in sight
+def compare_nonfinite(c, out, lse):
+    """A row is NaN where the definition is, and only there; the others are within the derived tolerance."""
+    o, want_lse, A, r = definition(c)
+    real = c["cu_list"][-1]
+    o, want_lse, A, r, out, lse = (x[:real] for x in (o, want_lse, A, r, out, lse))
+    none = torch.isnan(o)
+    assert torch.equal(torch.isnan(out), none), "rows that are NaN differ from the definition's"
+    row = none[..., 0]
+    assert torch.equal(torch.isnan(lse), row)
+    err, tol = (out.double() - o).abs(), 2.0 ** -8 * o.abs() + (2.0 ** -8 + r) * (1 + 2.0 ** -6) * A
+    assert (err <= tol)[~none].all()
+    gap, slack = (lse.double() - want_lse).abs(), r[..., 0] + 2.0 ** -22 * want_lse.abs()
+    assert (gap <= slack)[~row & ~torch.isinf(want_lse)].all()
+    return row
+
+
+def put_key(c, s, key, head, value):
+    """K row of position `key` as request s sees it (None: any), in KV head `head`."""
+    page = c["page"]
+    ids = c["prefix_table"] if key < c["prefix"] else c["tables"][s]
+    c["k"][int(ids[key // page]), key % page, head] = value
+
+
+@pytest.mark.parametrize("heads", ["32/8x64", "16/8x128"])
+@pytest.mark.parametrize("at", [0, 72, 1024 + 64, 1024 + 104, 2048 - 64, 2048 - 8])
+def test_nan_key_in_the_prefix(paged, heads, at):
+    """A NaN in K of KV head h at the place h modulo 8 of a step of the shared prefix (the first step of a run of blocks and later
+    ones): every row is NaN, whichever place it was."""
+    few = make_case(heads, 16, 2048, [20, 5], [1, 3], seed=30)
+    many = make_case(heads, 16, 2048, [9] * 60, [5] * 60, seed=31)       # two tiles a unit
+    for c in (few, many):
+        for head in range(8):
+            put_key(c, None, at + head, head, float("nan"))
+        lse = torch.empty(c["q"].shape[:2], device="cuda:0")
+        row = compare_nonfinite(c, call(paged, c, lse=lse), lse)
+        assert row.all()
+
+
+@pytest.mark.parametrize("heads", ["32/8x64", "16/8x128"])
+@pytest.mark.parametrize("at", [8, 64 + 16, 256 + 24, 256 + 600])
+def test_nan_key_in_a_long_piece(paged, heads, at):
+    """The same in a piece of rows that are causal among themselves: rows before the key do not see it."""
+    for prefix in (0, 256):
+        c = make_case(heads, 32, prefix, [900, 3], [900, 1], seed=32)
+        for head in range(8):
+            put_key(c, 0, prefix + at + head, head, float("nan"))
+        lse = torch.empty(c["q"].shape[:2], device="cuda:0")
+        row = compare_nonfinite(c, call(paged, c, lse=lse), lse)
+        assert row.any() and not row.all()
+
+
+@pytest.mark.parametrize("heads", ["32/8x64", "16/8x128"])
+def test_infinite_scores_in_sight(paged, heads):
+    """Keys with an infinity in one dimension: a score of plus infinity makes the row NaN, one of minus infinity counts as absent."""
+    c = make_case(heads, 32, 512, [300, 40, 7], [1, 40, 300 // 60], seed=33)
+    for head in range(8):
+        for s, key in ((None, 200 + head), (None, 64 * 3 + 8 + head), (0, 512 + 33 + head), (1, 512 + 20)):
+            put_key(c, s, key, head, 0.0)
+            page = c["page"]
+            ids = c["prefix_table"] if key < c["prefix"] else c["tables"][s]
+            c["k"][int(ids[key // page]), key % page, head, head] = float("inf") if key % 2 else float("-inf")
+    lse = torch.empty(c["q"].shape[:2], device="cuda:0")
+    o, want, A, r = definition(c)
+    out = call(paged, c, lse=lse)
+    real = c["cu_list"][-1]
+    none = torch.isnan(o)
+    assert torch.equal(torch.isnan(out)[:real], none[:real]) and none[:real].any() and not none[:real].all()
+    err, tol = (out.double() - o).abs(), 2.0 ** -8 * o.abs() + (2.0 ** -8 + r) * (1 + 2.0 ** -6) * A
+    assert (err <= tol)[:real][~none[:real]].all()
+    assert torch.equal(torch.isnan(lse)[:real], none[:real, :, 0])
