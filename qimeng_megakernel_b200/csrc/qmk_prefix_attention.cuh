@@ -1083,7 +1083,8 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
           dst[16 * j] = o[j][h];
           dst[16 * j + 8] = o[j][2 + h];
         }
-        if (g == 0) p.strip_ml[(size_t)rec * kStripRows + row] = make_float2(m, l);
+        // (a NaN is told from m: scores that are all NaN leave no maximum, and the merge would give such a part no weight)
+        if (g == 0) p.strip_ml[(size_t)rec * kStripRows + row] = make_float2(l == l ? m : l, l);
       }
       if (c0 == 0 && g == 0) {                              // whoever starts the strip says where its rows' parts are
         const int parts = whole ? 0 : plan.strips.owner(f + per - 1) - number + 1;
@@ -1175,7 +1176,7 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
 // Adds a row's parts.  With M = max m_r and w_r = 2^(m_r - M):   o = sum_r w_r O_r / sum_r w_r l_r
 // A thread takes four dimensions of a (row, KV head) at a time; neighbours take neighbouring rows, which is how the blocks' parts
 // lie.  The statistics and values of eight parts are on their way at once, M is the running maximum (a part of weight zero may
-// hold anything and is left out).  A refused call's rows are NaN, all of them.  Launched as a programmatic dependent without an
+// hold anything and is left out; one whose scores had a NaN has m = NaN and makes the row NaN).  A refused call's rows are NaN, all of them.  Launched as a programmatic dependent without an
 // early trigger: blocks that wait on the SMs while the attention still runs cost it more (32 rows over 2048 shared keys: 24.6 us)
 // than the plain order of launches (18.5 us); this takes 17.8 us (all before the present division of the CTAs), of which about 4 us are the adding.
 constexpr int kMergeThreads = 128, kMergeParts = 8;

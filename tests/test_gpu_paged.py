@@ -548,3 +548,32 @@ def test_infinite_scores_in_sight(paged, heads):
     err, tol = (out.double() - o).abs(), 2.0 ** -8 * o.abs() + (2.0 ** -8 + r) * (1 + 2.0 ** -6) * A
     assert (err <= tol)[:real][~none[:real]].all()
     assert torch.equal(torch.isnan(lse)[:real], none[:real, :, 0])
+
+
+@pytest.mark.parametrize("heads", ["32/8x64", "16/8x128", "6/2x64", "5/1x128"])
+@pytest.mark.parametrize("prefix", [0, 256])
+def test_nan_key_behind_the_prefix(paged, heads, prefix):
+    """A NaN in K of what a request holds behind the prefix: its only key, the only one of a piece, one among others.  The rows of
+    the request that see it are NaN in that KV head, and no others are."""
+    HK = HEADS[heads][1]
+    for own, new, s, key in (([1], [1], 0, 0), ([1, 7], [1, 1], 0, 0), ([33, 2], [1, 1], 0, 32), ([65, 40], [3, 1], 0, 64),
+                             ([40, 100], [1, 5], 1, 96), ([40, 100], [1, 5], 1, 17), ([20] * 30, [2] * 30, 11, 5)):
+        for head in {0, HK - 1}:
+            c = make_case(heads, 16, prefix, own, new, seed=34)
+            put_key(c, s, prefix + key, head, float("nan"))
+            lse = torch.empty(c["q"].shape[:2], device="cuda:0")
+            row = compare_nonfinite(c, call(paged, c, lse=lse), lse)
+            assert row.any()
+
+
+@pytest.mark.parametrize("heads", ["32/8x64", "16/16x128"])
+@pytest.mark.parametrize("prefix", [0, 512])
+def test_nan_key_behind_the_prefix_in_a_large_call(paged, heads, prefix):
+    """The same where the parts are added by fewer threads (more than 888 rows)."""
+    own, new = [920, 1, 40, 33, 2], [920, 1, 3, 1, 2]
+    for s, key in ((1, 0), (2, 39), (3, 32), (4, 1)):
+        c = make_case(heads, 32, prefix, own, new, seed=35)
+        put_key(c, s, prefix + key, 3 if heads == "32/8x64" else 0, float("nan"))
+        lse = torch.empty(c["q"].shape[:2], device="cuda:0")
+        row = compare_nonfinite(c, call(paged, c, lse=lse), lse)
+        assert row.any() and not row[:920].any()
