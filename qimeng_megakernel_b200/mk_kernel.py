@@ -60,12 +60,13 @@ def _sig(t):
 
 
 def _paged_sig(state) -> tuple:
-    """Identity of a PagedState as far as a bound state depends on it (its lengths alternate from step to step)."""
+    """Identity of a PagedState as far as a bound state depends on it."""
     if state is None:
         return ()
     step = state.step
-    return (step.positions.data_ptr(), step.active.data_ptr(), step.seq_ids.data_ptr(), step.slots.data_ptr(), state.rows,
-            state.page_size, _sig(state.block_tables), _sig(state.prefix_table), state.prefix_len)
+    return (step.positions.data_ptr(), step.active.data_ptr(), step.seq_ids.data_ptr(), step.slots.data_ptr(),
+            step.cu_tokens.data_ptr(), step.kv_lengths.data_ptr(), state.rows, state.page_size, _sig(state.block_tables),
+            _sig(state.prefix_table), state.prefix_len)
 
 
 class MegaKernel:

@@ -332,9 +332,10 @@ class PagedState:
     """The paged cache of a decode request: tables, lengths and the rows of the current step.
 
     `advance(new_lengths)` makes the slot map of a step that appends new_lengths[s] tokens to sequence s; the kernel call
-    on the Globals that carry the state (`mk(globs)`) then runs that step.  The step's buffers (slots, positions, active,
-    seq_ids, cu_tokens) stay where they are from step to step, so the kernel's binding and captured graphs hold; the
-    lengths alternate between two."""
+    on the Globals that carry the state (`mk(globs)`) then runs that step.  All buffers of the step stay where they are from
+    step to step, so the kernel's binding holds, and a graph that captured advance() and the kernel call is one more step
+    every time it is replayed.  `step.kv_lengths` is what the cache holds with the last step's tokens; who writes other
+    lengths there goes on from them."""
 
     def __init__(self, block_tables: torch.Tensor, lengths: torch.Tensor, rows: int, page_size: int,
                  prefix_table: torch.Tensor | None, prefix_len: int):
@@ -350,7 +351,6 @@ class PagedState:
             t.zero_()
         self.step.slots.fill_(-1)
         self.step.kv_lengths.copy_(lengths)
-        self._other = torch.empty_like(self.step.kv_lengths)
         self.ones = torch.ones(seqs, dtype=torch.int32, device=device)
         self.workspace: torch.Tensor | None = None
 
@@ -394,10 +394,9 @@ class PagedState:
         return self.block_tables.shape[1] * self.page_size
 
     def advance(self, new_lengths: torch.Tensor | None = None) -> SlotMap:
-        """The step in which sequence s appends new_lengths[s] tokens (one each by default)."""
-        lengths, self.step.kv_lengths = self.step.kv_lengths, self._other
-        self._other = lengths
-        return build_slot_map(self.block_tables, lengths, self.ones if new_lengths is None else new_lengths,
+        """The step in which sequence s appends new_lengths[s] tokens (one each by default).  A refused call changes nothing."""
+        # (a copy on the stream, in a captured graph too: the map's CTAs read the lengths while it writes the new ones)
+        return build_slot_map(self.block_tables, self.step.kv_lengths.clone(), self.ones if new_lengths is None else new_lengths,
                               page_size=self.page_size, tokens=self.rows, out=self.step)
 
     def step_args(self, heads: int, kv_heads: int, size: int) -> _lib.PagedStepArgs:

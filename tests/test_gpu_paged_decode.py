@@ -223,3 +223,50 @@ def test_another_state_on_the_same_rows_and_the_contiguous_forms():
     mk(g)
     mk.check_status()
     mk.close()
+
+
+@torch.inference_mode()
+def test_replays_of_a_captured_step_go_forward():
+    """advance() and the kernel call captured once: every replay is the next step, as the same number of eager ones."""
+    _need_gpu()
+    from qimeng_megakernel_b200 import synthetic
+    from qimeng_megakernel_b200.prefill import run_prefill_synthetic
+    cfg = _config("llama")
+    weights = synthetic.make_weights(cfg, seed=5, device="cuda:0")
+    prompts = _prompts(cfg, 3, 50, 32, seed=23)
+    steps, seen = 7, []
+    for captured in (False, True):
+        pre = run_prefill_synthetic(cfg, weights, prompts, steps + 1, shared_prefix=32, page_size=16)
+        g, mk = pre.globs, pre.mk
+        g.token_in = pre.first_gen_token.view(-1).clone()
+        g.next_token = g.token_in                        # the token a step picks is the next one's
+        first = g.paged.step.kv_lengths
+        g.paged.advance()                                # (an eager step before the capture)
+        mk(g)
+        rows = [[g.paged.step.positions.tolist(), g.paged.step.kv_lengths.tolist(), g.token_in.tolist()]]
+        logits = [g.logits.clone()]
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                g.paged.advance()
+                mk(g)
+            assert g.paged.step.kv_lengths.tolist() == [51] * 3      # nothing has run
+        for i in range(1, steps):
+            if captured and i != 4:
+                graph.replay()
+            else:                                        # (eager steps in between go on where the replays were)
+                g.paged.advance()
+                mk(g)
+            rows.append([g.paged.step.positions.tolist(), g.paged.step.kv_lengths.tolist(), g.token_in.tolist()])
+            logits.append(g.logits.clone())
+        mk.check_status()
+        assert [r[0] for r in rows] == [[50 + i] * 3 for i in range(steps)]
+        assert [r[1] for r in rows] == [[51 + i] * 3 for i in range(steps)]
+        assert not captured or g.paged.step.kv_lengths.data_ptr() == first.data_ptr()
+        seen.append((rows, logits))
+        if captured:
+            del graph
+        mk.close()
+    assert seen[0][0] == seen[1][0]
+    assert all(torch.equal(a, b) for a, b in zip(seen[0][1], seen[1][1]))

@@ -249,3 +249,11 @@ def test_a_replaced_table_is_looked_at_again(paged):
     s.prefix_table = i32(2)
     s.step.slots = i32(2)
     refused(TypeError, "step.slots: expected torch.int64", s.check)
+
+
+def test_a_refused_step_leaves_the_state_as_it_was(paged):
+    s = state(paged, lengths=torch.tensor([5, 9], dtype=torch.int32))
+    for bad in (i32(3), i32(2).long(), i32(2), [1, 1]):                # (the third: no CPU path)
+        with pytest.raises((TypeError, ValueError)):
+            s.advance(bad)
+        assert s.step.kv_lengths.tolist() == [5, 9]
