@@ -60,6 +60,12 @@ def decode(model_name: str, *, prefill: PrefillOutput, max_new_tokens: int, deco
     paged = getattr(globs, "paged", None)
     if (paged.capacity if paged is not None else int(globs.k_cache.shape[2])) < prompt_len + max_new_tokens:
         raise ValueError("KV cache shorter than prompt_len + max_new_tokens")
+    if paged is not None:
+        # Every sequence starts behind its prompt, as position_id does on the contiguous cache, whatever an earlier run appended.
+        held = paged.step.kv_lengths
+        if int(held.min()) < prompt_len:
+            raise ValueError(f"the paged cache holds fewer tokens than the prompt's {prompt_len}: {held.tolist()}")
+        held.fill_(prompt_len)
     # Per-row positions (the reference's multi-batch state): the kernel reads them instead of position_id, so they are
     # advanced on the stream after every step as the reference's loop does (decode.py:1398-1400).
     pids = getattr(globs, "position_ids", None) if paged is None else None

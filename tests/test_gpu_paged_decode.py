@@ -270,3 +270,26 @@ def test_replays_of_a_captured_step_go_forward():
         mk.close()
     assert seen[0][0] == seen[1][0]
     assert all(torch.equal(a, b) for a, b in zip(seen[0][1], seen[1][1]))
+
+
+def test_decode_starts_behind_the_prompt_every_time():
+    """Several decode() calls on one prefill: each starts behind the prompt, as on the contiguous cache, whatever ran before."""
+    _need_gpu()
+    from qimeng_megakernel_b200 import synthetic
+    from qimeng_megakernel_b200.decode import decode
+    from qimeng_megakernel_b200.prefill import run_prefill_synthetic
+    cfg = _config("llama")
+    weights = synthetic.make_weights(cfg, seed=3, device="cuda:0")
+    prompts = _prompts(cfg, 4, 40, 33, seed=9)
+    pre = run_prefill_synthetic(cfg, weights, prompts, 12, shared_prefix=33, page_size=16)
+    run = lambda n, **kw: decode("llama-3.2-1b", prefill=pre, max_new_tokens=n, ignore_eos=True, **kw)["new_tokens"].tolist()
+    first = run(12)
+    assert run(12) == first and run(12, host_loop=True) == first
+    assert [row[:5] for row in first] == run(5)
+    pre.globs.paged.advance()
+    assert run(12) == first and pre.globs.paged.step.kv_lengths.tolist() == [40 + 11] * 4
+    with torch.inference_mode():
+        pre.globs.paged.step.kv_lengths.copy_(torch.tensor([40, 39, 40, 40]))
+    with pytest.raises(ValueError, match="fewer tokens than the prompt"):
+        run(12)
+    pre.mk.close()
