@@ -179,7 +179,8 @@ typedef struct qmk_status {
   int32_t code;      /* 0 = healthy; 1 = dependency wait expired; 2 = weight-copy wait expired;
                         3 = activation-staging wait expired; 4 = (batched kernel) an active row's position was
                         outside the KV cache or the RoPE table: that row was treated as inactive, `seen` is the
-                        position, `expected` the limit, `detail` the row; qmk_poll_status returns QMK_ERR_POSITION */
+                        position, `expected` the limit, `detail` the row; qmk_poll_status returns QMK_ERR_POSITION.
+                        (qmk_decode_step_paged: or its slot was outside the pool, or the block table had no page for it) */
   int32_t sm;        /* CTA (one per SM) that reported */
   int32_t warp;
   int32_t phase;     /* global phase index: layer*5 + {0 qkv,1 attn,2 oproj,3 upgate,4 down}; 5*L = lm head */
@@ -413,10 +414,11 @@ int qmk_prefix_attention(const qmk_prefix_attention_args* args, int device, void
 
 /* One decode step on a paged cache whose sequences share a prefix: the launches of qmk_decode_step cut at every layer's attention,
  * which is qmk_prefix_attention.  The state is bound with k_cache / v_cache = the pools of all layers, [L, num_pages, page_size,
- * NKV, HD] (kv_batch = num_pages, kv_seq_len = page_size), position_ids, active_mask and kv_slots (the rows' requests; not read
- * here), all of them `batch` rows as qmk_build_slot_map leaves them; `slots` says where each row's K and V go.  An active row whose
- * position or slot is out of range is switched off and reported (qmk_poll_status).  Batched kernel, any batch; no model
- * parallelism.  A refused call launches nothing.  Asynchronous; a step can be captured into a CUDA graph. */
+ * NKV, HD] (kv_batch = num_pages, kv_seq_len = page_size), position_ids, active_mask and kv_slots (the rows' requests), all of
+ * them `batch` rows as qmk_build_slot_map leaves them; `slots` says where each row's K and V go.  An active row whose position or
+ * slot is out of range is switched off and reported (qmk_poll_status); so is a request's token without a page (request >= 0, slot
+ * -1, active 0).  Batched kernel, any batch; no model parallelism.  A refused call launches nothing.  Asynchronous; a step can be
+ * captured into a CUDA graph. */
 typedef struct qmk_paged_step_args {
   const int32_t* block_tables;  /* [seqs, max_pages] */
   const int32_t* kv_lengths;    /* [seqs]: the step's tokens included */

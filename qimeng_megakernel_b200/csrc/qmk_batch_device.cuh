@@ -1646,10 +1646,12 @@ qmk_batch_kernel(const __grid_constant__ BParams p, const __grid_constant__ Tens
     // An active row whose position lies outside the KV cache or the RoPE table would read and write out of bounds:
     // it is switched off (no KV write, zero projections, like a finished row) and the launch reports it.
     // (the same goes for a row that names a sequence the KV cache does not have)
-    // (or a row of the paged pool that is not there)
+    // (or a row of the paged pool that is not there; there the slot map itself switches off a request's token that got no
+    // page, which is reported too)
     int slot = b < p.B && !p.kv_rows ? (p.kv_slots ? p.kv_slots[b] : b) : 0;
     const long long kv_row = b < p.B && p.kv_rows ? p.kv_rows[b] : 0;
-    if (act != 0 && (pos < 0 || pos >= p.pos_limit || slot < 0 || slot >= p.kv_batch || kv_row < 0 || kv_row >= p.kv_row_limit)) {
+    const bool no_page = act == 0 && kv_row < 0 && p.kv_slots[b] >= 0;
+    if (no_page || (act != 0 && (pos < 0 || pos >= p.pos_limit || slot < 0 || slot >= p.kv_batch || kv_row < 0 || kv_row >= p.kv_row_limit))) {
       if (blockIdx.x == 0) report(p, kErrRowPosition, 0, p.phase_begin, (unsigned)pos, (unsigned)p.pos_limit, b);
       act = 0;
       pos = -1;

@@ -293,3 +293,52 @@ def test_decode_starts_behind_the_prompt_every_time():
     with pytest.raises(ValueError, match="fewer tokens than the prompt"):
         run(12)
     pre.mk.close()
+
+
+@torch.inference_mode()
+def test_a_token_without_a_page_is_reported():
+    """A row whose token has no page (behind the table, or an entry of -1) is switched off, and the status says so; one that was
+    switched off by hand is not reported."""
+    _need_gpu()
+    from qimeng_megakernel_b200 import _lib, synthetic
+    from qimeng_megakernel_b200.prefill import run_prefill_synthetic
+    cfg = _config("llama")
+    weights = synthetic.make_weights(cfg, seed=6, device="cuda:0")
+    pre = run_prefill_synthetic(cfg, weights, _prompts(cfg, 2, 20, 16, seed=2), 4, shared_prefix=16, page_size=16)
+    g, mk = pre.globs, pre.mk
+    g.token_in = torch.tensor([3, 4], dtype=torch.int64, device="cuda:0")
+    lengths = g.paged.step.kv_lengths.clone()
+    g.paged.advance()
+    mk(g)
+    mk.check_status()
+    good = g.logits.clone()
+    # sequence 1 has no page for position 20
+    g.paged.step.kv_lengths.copy_(lengths)
+    page = g.paged.block_tables[1, 1].clone()
+    g.paged.block_tables[1, 1] = -1
+    g.paged.advance()
+    mk(g)
+    status = mk.poll_status()
+    assert status["rc"] == -6 and status["code"] == 4 and status["detail"] == 1, status
+    assert torch.equal(g.logits[0], good[0])
+    mk.check_status()
+    g.paged.block_tables[1, 1] = page
+    # behind the table
+    g.paged.step.kv_lengths.copy_(torch.tensor([20, 32]))
+    g.paged.advance()
+    mk(g)
+    with pytest.raises(_lib.QmkError):
+        mk.check_status()
+    assert torch.equal(g.logits[0], good[0])
+    # a sequence without a new token, and a row that the caller switched off, are nothing to report
+    g.paged.step.kv_lengths.copy_(lengths)
+    g.paged.advance(torch.tensor([1, 0], dtype=torch.int32, device="cuda:0"))
+    mk(g)
+    mk.check_status()
+    g.paged.step.kv_lengths.copy_(lengths)
+    g.paged.advance()
+    g.active_mask[1] = 0
+    mk(g)
+    mk.check_status()
+    assert torch.equal(g.logits[0], good[0])
+    mk.close()
