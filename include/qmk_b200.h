@@ -180,7 +180,10 @@ typedef struct qmk_status {
                         3 = activation-staging wait expired; 4 = (batched kernel) an active row's position was
                         outside the KV cache or the RoPE table: that row was treated as inactive, `seen` is the
                         position, `expected` the limit, `detail` the row; qmk_poll_status returns QMK_ERR_POSITION.
-                        (qmk_decode_step_paged: or its slot was outside the pool, or the block table had no page for it) */
+                        (qmk_decode_step_paged: or its slot was outside the pool, or the block table had no page for it);
+                        5 = (qmk_decode_step_paged) cu_tokens do not ascend from 0 to at most `batch`: the attention's rows are
+                        NaN, `seen` is the last offset, `expected` the rows; qmk_poll_status returns QMK_ERR_POSITION.  A wait
+                        that expires inside a paged step's attention is code 2 with that phase; its rows are NaN */
   int32_t sm;        /* CTA (one per SM) that reported */
   int32_t warp;
   int32_t phase;     /* global phase index: layer*5 + {0 qkv,1 attn,2 oproj,3 upgate,4 down}; 5*L = lm head */
@@ -252,7 +255,8 @@ int qmk_set_timeout_cycles(qmk_handle* h, int64_t cycles);
 int qmk_set_cooperative_launch(qmk_handle* h, int32_t on);
 
 /* Debug knob used by the failure-detection test: when set, qmk_run_phases(mode 1) also waits for the
- * dependency of its first phase, which nothing publishes, so the bounded wait must expire. */
+ * dependency of its first phase, which nothing publishes, so the bounded wait must expire; so does the attention of
+ * qmk_decode_step_paged. */
 int qmk_set_wait_first_dependency(qmk_handle* h, int32_t on);
 
 /* Which kernel serves the handle.  0 (default): the batch-1 kernel when the descriptor has its compiled

@@ -472,8 +472,9 @@ extern "C" int qmk_poll_status(qmk_handle* h, qmk_status* out) {
   out->expected = words[kStExpected];
   out->detail = (int32_t)words[kStDetail];
   out->reserved = 0;
-  if (out->code == kErrRowPosition) {
-    // no wait expired: a row's position was out of range, the row was switched off and the step completed
+  if (out->code == kErrRowPosition || out->code == kErrRowOffsets) {
+    // no wait expired: a row's position was out of range and the row was switched off, or the rows' offsets were no division of the
+    // rows and their attention is NaN; the step completed
     QMK_CUDA(h, cudaMemsetAsync(status, 0, 32, h->last_stream));
     QMK_CUDA(h, cudaStreamSynchronize(h->last_stream));
     return QMK_ERR_POSITION;
@@ -574,7 +575,9 @@ extern "C" int qmk_decode_step_paged(qmk_handle* h, const qmk_paged_step_args* a
     if (rc) return rc;
     t.k_pages = (const unsigned char*)st.k_cache + l * layer_bytes;
     t.v_pages = (const unsigned char*)st.v_cache + l * layer_bytes;
-    rc = qmk_prefix_attention(&t, h->device, cuda_stream);
+    // (twice the budget of a dependency wait, as the copies of the other phases)
+    const qmk_attention_watch watch = {qmkb_status_ptr(h->bctx), l * per_layer + 1, 2 * h->timeout_cycles, h->wait_first};
+    rc = qmk_prefix_attention_launch(&t, &watch, h->device, cuda_stream);
     if (rc) {
       snprintf(h->cuda_err, sizeof(h->cuda_err), "%s", qmk_paged_last_cuda_error());
       return rc;

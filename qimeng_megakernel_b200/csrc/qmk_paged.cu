@@ -108,13 +108,14 @@ static int sm_count(int device) {
 }
 
 // Regions of the workspace; every one starts on a 256-byte boundary.
-struct WorkspaceLayout { long long refused, dense_ml, dense_o, strip_ml, strip_o, dense_desc, strip_desc, total; };
+struct WorkspaceLayout { long long refused, aborted, dense_ml, dense_o, strip_ml, strip_o, dense_desc, strip_desc, total; };
 static WorkspaceLayout workspace_layout(const PlanDims& d, int head_dim) {
   WorkspaceLayout w;
   long long at = 0;
   auto take = [&](long long bytes) { const long long here = at; at += (bytes + 255) / 256 * 256; return here; };
   const long long records = max_dense_records(d), strips = max_strip_records(d);
   w.refused = take(4);
+  w.aborted = take((long long)d.ctas * kStripWarps * 4);
   w.dense_ml = take(records * kUnitRows * 8);
   w.strip_ml = take(strips * kStripRows * 8);
   w.dense_desc = take((long long)d.tokens * d.NKV * 8);
@@ -250,6 +251,11 @@ int qmk_prefix_attention_check(const qmk_prefix_attention_args* a, int device) {
 }
 
 extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int device, void* cuda_stream) {
+  const qmk_attention_watch nobody = {nullptr, 0, 4000000000ll, 0};   // (waits of about two seconds)
+  return qmk_prefix_attention_launch(a, &nobody, device, cuda_stream);
+}
+
+int qmk_prefix_attention_launch(const qmk_prefix_attention_args* a, const qmk_attention_watch* watch, int device, void* cuda_stream) {
   const int rc = qmk_prefix_attention_check(a, device);
   if (rc) return rc;
   DeviceScope scope(device);
@@ -263,8 +269,11 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
   p.q_stride = a->q_token_stride; p.out_stride = a->out_token_stride;
   p.NH = a->num_heads; p.page_shift = page_shift_of(a->page_size); p.num_pages = a->num_pages; p.max_pages = a->max_pages;
   p.scale_log2e = a->scale * 1.4426950408889634f;
+  p.status = watch->status; p.phase = watch->phase; p.wait_first = watch->wait_first;
+  const long long budget = (watch->wait_cycles + 1023) / 1024;
+  p.wait_budget = (unsigned)(budget < 1 ? 1 : (budget > 0xffffffffll ? 0xffffffffll : budget));
   unsigned char* ws = (unsigned char*)a->workspace;
-  p.refused = (int*)(ws + w.refused);
+  p.refused = (int*)(ws + w.refused); p.aborted = (unsigned*)(ws + w.aborted);
   p.dense_ml = (float2*)(ws + w.dense_ml); p.dense_o = (float4*)(ws + w.dense_o);
   p.strip_ml = (float2*)(ws + w.strip_ml); p.strip_o = (float*)(ws + w.strip_o);
   p.dense_desc = (int2*)(ws + w.dense_desc); p.strip_desc = (int2*)(ws + w.strip_desc);

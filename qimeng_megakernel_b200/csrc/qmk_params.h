@@ -12,7 +12,8 @@ enum StatusWord : int { kStCode = 0, kStSm = 1, kStWarp = 2, kStPhase = 3, kStSe
 // 1: a producer's tagged words never arrived; 2: a weight copy never completed; 3: another warp of the CTA never staged its part;
 // 4: (batched kernel) an active row's position lies outside the KV cache or the RoPE table: the row was treated as inactive
 //    (paged cache: or its slot outside the pool, or it is a request's token for which the block table has no page)
-enum StatusCode : int { kOkCode = 0, kErrCounterWait = 1, kErrCopyWait = 2, kErrStageWait = 3, kErrRowPosition = 4 };
+// 5: (paged cache) the step's cu_tokens do not ascend from 0 to at most its rows: the attention computed nothing
+enum StatusCode : int { kOkCode = 0, kErrCounterWait = 1, kErrCopyWait = 2, kErrStageWait = 3, kErrRowPosition = 4, kErrRowOffsets = 5 };
 
 struct Params {
   // ---- weights (bf16 as raw 16-bit words) ----

@@ -30,12 +30,14 @@
 // Both parts leave partial results (m, l, unnormalised O, all in 32 bits) unless a row is complete; merge_kernel adds them
 // up in a fixed order, so a call gives the same bits every time.  Nothing is kept between calls.
 //
-// Every wait is bounded: one that expires raises the CTA's abort word, all waits then return, and the CTA's rows are NaN.
+// Every wait is bounded: one that expires raises the CTA's abort word, all waits then return, the CTA's rows are NaN, and the
+// caller's status record, if there is one, says so.
 #pragma once
 #include <cuda.h>
 #include <stdint.h>
 
 #include "qmk_device.cuh"
+#include "qmk_params.h"
 #include "qmk_prefix_plan.h"
 
 namespace qmkp {
@@ -62,6 +64,12 @@ struct AttnParams {
   int2* dense_desc;            // [tokens, NKV]    {first record, records | row << 16}; records 0: none
   int2* strip_desc;            // [tokens, NH]     {first record, records | row << 16}
   int* refused;                // 1: cu_tokens does not ascend from 0 to at most `tokens`, nothing was computed
+  unsigned* aborted;           // [CTAs, 8]  not 0: a wait expired there (one word for each warp with strips; blocks write all)
+  // failures: the merge, which runs behind all CTAs, reports them
+  unsigned* status;            // record of StatusWord, or null
+  int phase;                   // of the step, for the record
+  unsigned wait_budget;        // of every wait, in units of 1024 clocks
+  int wait_first;              // failure test: every CTA waits for an arrival that nothing makes
 };
 struct AttnMaps {
   CUtensorMap k, v;            // {HD, NKV, slots}, box {64, 1, min(page, 64)}
@@ -73,7 +81,6 @@ constexpr int kSoftmaxWarps = 8, kKeyWarp = 8, kIssueWarp = 9, kValueWarp = 11; 
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 constexpr int kPolyEvery = 4;                        // one pair of exponentials in so many goes to the multiply-add pipe
-constexpr long long kWaitCycles = 4000000000ll;      // about two seconds
 
 template <int HD>
 struct AttnSmem {
@@ -257,12 +264,12 @@ __device__ __forceinline__ uint32_t mbar_try_wait_parked(uint32_t bar, uint32_t 
       : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000000u) : "memory");
   return ok;
 }
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile unsigned* ctl) {
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile unsigned* ctl, const AttnParams& p) {
   if (mbar_try_wait_parked(bar, parity)) return true;
   const long long t0 = clock64();
   while (!mbar_try_wait_parked(bar, parity)) {
     if (ctl[0] != 0u) return false;
-    if (clock64() - t0 > kWaitCycles) {
+    if (clock64() - t0 > (long long)p.wait_budget * 1024) {
       ctl[0] = 1u;
       return false;
     }
@@ -477,6 +484,7 @@ struct Dense {
     const int oob = p.num_pages << p.page_shift;             // behind the last row: reads as zeros
     const uint32_t dst = base + (kV ? S::kOffV : S::kOffK) + (uint32_t)(half_dims * 8192 + key_of_lane * 128);
     unsigned n = 0;
+    if (!kV && p.wait_first && !wait_bar(v_clear(), 0u, ctl, p)) return n;   // (V is cleared behind the first scores only)
     for (int b = lo; b < hi;) {
       int b0;
       const Unit x = unit_at(p, sc, t, plan, b, b0);
@@ -495,7 +503,7 @@ struct Dense {
         const unsigned issue = __ballot_sync(kFullMask, row >= 0);
         const uint32_t bytes = (uint32_t)__popc(issue) * (uint32_t)(box_rows * 128);
         const int next = part + 1 < end ? row_of(part + 1) : -1;
-        if (!wait_bar(empty, ((n / S::kStages) & 1u) ^ 1u, ctl)) return n;
+        if (!wait_bar(empty, ((n / S::kStages) & 1u) ^ 1u, ctl, p)) return n;
         if (lane == 0) mbar_expect_tx(full, bytes);
         __syncwarp();
         if (row >= 0) tma_box(dst + st * S::kHalfBytes, kV ? &maps.v : &maps.k, half_dims * 64, x.kvh, row, full);
@@ -550,13 +558,13 @@ struct Dense {
       };
       int blk = dual ? g : 0;
       if (blk < nb) {
-        if (!wait_bar(q_full(g), segs & 1u, ctl)) return;
+        if (!wait_bar(q_full(g), segs & 1u, ctl, p)) return;
         ++segs;
         // halves are numbered n, n + 1, ...: those of block blk are m and m + 1
         unsigned m = n + 2u * (unsigned)blk;
         auto score_when_there = [&](unsigned i, int half) {
           const int st = (int)(i % S::kStages);
-          if (!wait_bar(k_full(st), (i / S::kStages) & 1u, ctl)) return false;
+          if (!wait_bar(k_full(st), (i / S::kStages) & 1u, ctl, p)) return false;
           tmem_fence_after_sync();
           score(st, half);
           release(k_empty(st));
@@ -571,8 +579,8 @@ struct Dense {
           for (int half = 0; half < 2; ++half) {
             const int st = (int)((m + half) % S::kStages), valid = valid_keys(x, b0 + blk, half);
             const uint64_t vd = vd0 + (uint32_t)(st * (S::kHalfBytes >> 4));
-            if (!wait_bar(v_full(st), ((m + half) / S::kStages) & 1u, ctl)) return;
-            if (!wait_bar(p_full(g, half), p_par, ctl)) return;
+            if (!wait_bar(v_full(st), ((m + half) / S::kStages) & 1u, ctl, p)) return;
+            if (!wait_bar(p_full(g, half), p_par, ctl, p)) return;
             tmem_fence_after_sync();
             if (valid == 64) {
               mma_ts(od, sd + 64u * half, vd, kIdescO, more);
@@ -660,7 +668,7 @@ struct Dense {
       for (int j = 0; j < steps; ++j) {
         const int half = j & 1;
         const uint32_t sh = s_col + 64 * half;
-        ok = wait_bar(s_full(g, half), s_par, ctl);
+        ok = wait_bar(s_full(g, half), s_par, ctl, p);
         if (!ok) break;
         tmem_fence_after_sync();
         if (warp_works) {
@@ -730,7 +738,7 @@ struct Dense {
               const float m_new = fmaxf(m, top);
               if (j > 0) {
                 // O may be touched once P V of step j - 1 is through: the scores of step j + 1 were issued behind it
-                ok = j + 1 < steps ? wait_bar(s_full(g, half ^ 1), half ? s_par ^ 1u : s_par, ctl) : wait_bar(o_full(g, 0), o_par, ctl);
+                ok = j + 1 < steps ? wait_bar(s_full(g, half ^ 1), half ? s_par ^ 1u : s_par, ctl, p) : wait_bar(o_full(g, 0), o_par, ctl, p);
                 if (!ok) break;
                 tmem_fence_after_sync();
                 const float f = m_new == -INFINITY ? 1.f : ex2(m - m_new);
@@ -760,12 +768,12 @@ struct Dense {
           const unsigned at = n + 2u * (unsigned)block_of(j, dual, g) + (unsigned)half;
           const int st = (int)(at % S::kStages);
           if (dual || g == 0) {
-            ok = wait_bar(v_full(st), (at / S::kStages) & 1u, ctl);
+            ok = wait_bar(v_full(st), (at / S::kStages) & 1u, ctl, p);
             if (!ok) break;
             clear_rows(st, x.limit & 63);
             if (!dual && lane == 0) mbar_arrive(v_clear());
           } else {                                           // (the block of both groups is cleared by the first)
-            ok = wait_bar(v_clear(), clears & 1u, ctl);
+            ok = wait_bar(v_clear(), clears & 1u, ctl, p);
             if (!ok) break;
             ++clears;
           }
@@ -774,7 +782,7 @@ struct Dense {
         mbar_arrive(p_full(g, half));
         s_par ^= (unsigned)half;
       }
-      if (ok && steps > 0) ok = wait_bar(o_full(g, 1), o_par, ctl);
+      if (ok && steps > 0) ok = wait_bar(o_full(g, 1), o_par, ctl, p);
       if (steps > 0) o_par ^= 1u;
       tmem_fence_after_sync();
       // ---- the unit's rows: complete, or a record.  With one tile both groups have a part of every row (in the same lanes
@@ -947,6 +955,7 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
   };
   for (int i = 0; i < S::kStripStages; ++i) send();
   bool ok = true;
+  if (p.wait_first) ok = wait_bar(smem_u32(smem) + S::kOffBars + (S::kDenseBars - 1) * 8, 0u, ctl, p);   // (a barrier of the blocks')
   for (int f = lo; f < hi;) {
     const StripRun x = strip_at(p, sc, f, hi, KS);
     const Req& r = x.r;
@@ -971,7 +980,7 @@ __device__ __forceinline__ void walk_strips(const AttnParams& p, const AttnMaps&
     for (int j = 0; j < HD / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     for (int i = 0; i < stages; ++i) {
       const int st = (int)(used % S::kStripStages);
-      ok = ok && wait_bar(bars + st * 8, (used / S::kStripStages) & 1u, ctl);
+      ok = ok && wait_bar(bars + st * 8, (used / S::kStripStages) & 1u, ctl, p);
       if (!ok) break;
       ++used;
       const uint32_t kb = ring + st * S::kStripStageBytes, vb = kb + KBYTES;
@@ -1145,7 +1154,10 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
       tmem_fence_after_sync();
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(ctl[1]) : "memory");
     }
-    if (ok && warp < kStripWarps) walk_strips<HD>(p, maps, smem, ctl, sc, work->plan, warp, lane);
+    if (ok && warp < kStripWarps) {
+      walk_strips<HD>(p, maps, smem, ctl, sc, work->plan, warp, lane);
+      if (lane == 0) p.aborted[blockIdx.x * kStripWarps + warp] = ctl[0];
+    }
     return;
   }
   dense_range(work->plan, (int)blockIdx.x, w.lo, w.hi);
@@ -1170,6 +1182,7 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
   if (warp == kIssueWarp) {
     tmem_fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(w.tmem) : "memory");
+    if (lane < kStripWarps) p.aborted[blockIdx.x * kStripWarps + lane] = ctl[0];
   }
 }
 
@@ -1181,9 +1194,26 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
 // than the plain order of launches (18.5 us); this takes 17.8 us (all before the present division of the CTAs), of which about 4 us are the adding.
 constexpr int kMergeThreads = 128, kMergeParts = 8;
 constexpr long long kMergeBlocks = 4 * 148 * 6;              // four waves of the blocks that fit the machine
+// What failed goes to the status record, whose first entry stays.
+static __device__ __noinline__ void report_failures(const int* refused, const unsigned* aborted, int ctas, unsigned* status, int phase,
+                                                    int last, int tokens) {
+  const bool offsets = *refused != 0;                        // (then no CTA has waited for anything)
+  for (int i = (int)threadIdx.x; i < (offsets ? 1 : ctas * kStripWarps); i += kMergeThreads) {
+    if (!offsets && aborted[i] == 0u) continue;
+    if (atomicCAS(&status[kStCode], 0u, (unsigned)(offsets ? kErrRowOffsets : kErrCopyWait)) != 0u) continue;
+    status[kStSm] = i / kStripWarps;
+    status[kStWarp] = i % kStripWarps;
+    status[kStPhase] = phase;
+    status[kStSeen] = offsets ? last : 0;
+    status[kStExpected] = offsets ? tokens : 0;
+    status[kStDetail] = 0;
+  }
+}
 template <int HD, bool kMany>                                // kMany: a large call
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.status != nullptr && blockIdx.x + blockIdx.y + blockIdx.z == 0)
+    report_failures(p.refused, p.aborted, p.d.ctas, p.status, p.phase, p.cu_tokens[p.d.seqs], p.d.tokens);
   const int row = (int)blockIdx.x * 32 + (int)(threadIdx.x & 31), kvh = (int)blockIdx.y;
   const int token = p.d.by_G.div(row), g = row - token * p.d.G, head = kvh * p.d.G + g;
   if (token >= p.d.tokens) return;

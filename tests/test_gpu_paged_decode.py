@@ -342,3 +342,50 @@ def test_a_token_without_a_page_is_reported():
     mk.check_status()
     assert torch.equal(g.logits[0], good[0])
     mk.close()
+
+
+@torch.inference_mode()
+def test_attention_failures_reach_the_status():
+    """Offsets that do not ascend and a wait that runs out inside a step's attention: the rows are NaN, the status names it, and the
+    next step is right."""
+    _need_gpu()
+    from qimeng_megakernel_b200 import _lib, synthetic
+    from qimeng_megakernel_b200.prefill import run_prefill_synthetic
+    cfg = _config("llama")
+    weights = synthetic.make_weights(cfg, seed=6, device="cuda:0")
+    # (a prefix: blocks and strips; none and short requests: strips alone)
+    for shared in (32, 0):
+        pre = run_prefill_synthetic(cfg, weights, _prompts(cfg, 3, 50, shared, seed=2), 6, shared_prefix=shared, page_size=16)
+        g, mk = pre.globs, pre.mk
+        g.token_in = torch.tensor([3, 4, 5], dtype=torch.int64, device="cuda:0")
+        lengths = g.paged.step.kv_lengths.clone()
+        g.paged.advance()
+        mk(g)
+        mk.check_status()
+        good = g.logits.clone()
+        g.paged.step.cu_tokens.copy_(torch.tensor([0, 2, 1, 3]))
+        mk(g)
+        status = mk.poll_status()
+        assert status["rc"] == -6 and status["code"] == 5, status
+        assert torch.isnan(g.attn_out.float()).all()
+        g.paged.step.kv_lengths.copy_(lengths)
+        g.paged.advance()
+        mk(g)
+        mk.check_status()
+        assert torch.equal(g.logits, good)
+        mk.set_timeout_cycles(20_000_000)                # about 10 ms
+        mk.set_wait_first_dependency(True)               # the attention waits for a copy that nothing starts
+        g.paged.step.kv_lengths.copy_(lengths)
+        g.paged.advance()
+        mk(g)
+        status = mk.poll_status()
+        mk.set_wait_first_dependency(False)
+        mk.set_timeout_cycles(2_000_000_000)
+        assert status["rc"] == _lib.ERR_DEVICE_TIMEOUT and status["code"] == 2 and status["phase"] == 1, status
+        assert torch.isnan(g.attn_out.float()).all()
+        g.paged.step.kv_lengths.copy_(lengths)
+        g.paged.advance()
+        mk(g)
+        mk.check_status()
+        assert torch.equal(g.logits, good)
+        mk.close()
