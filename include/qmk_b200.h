@@ -353,7 +353,8 @@ const char* qmk_static_last_cuda_error(void);
 /* Block tables of a batch from the lengths its requests have to have room for (prefix included).  Row s gets
  * n_s = min(ceil(lengths[s] / page_size), max_pages) entries: the first prefix_pages are prefix_table's, the others come
  * from free_pages, in order, behind those of the rows before; entries from n_s on, and entries for which free_pages has run
- * out, are -1.  A length of zero or less is an empty row.  At most 2^20 requests and 2^30 entries a row. */
+ * out, are -1.  A length of zero or less is an empty row.  At most 2^20 requests and 2^30 entries a row.  No output may overlap an
+ * input or another output. */
 typedef struct qmk_block_tables_args {
   const int32_t* lengths;      /* [seqs]                                                                     */
   const int32_t* free_pages;   /* [num_free] (may be NULL when num_free is 0)                                */
@@ -369,7 +370,7 @@ int qmk_build_block_tables(const qmk_block_tables_args* args, int device, void* 
  * (values below zero count as zero); the tokens of the step are numbered request by request, cut off at `tokens`.  Token t
  * of request s: position = kv_lengths[s] + (t - cu_tokens[s]), slot = page * page_size + position % page_size, or -1 where
  * the table has no page.  Entries behind the last token: slot -1, position 0, seq_id -1, active 0.  At most 2^20 requests and
- * 2^24 tokens. */
+ * 2^24 tokens.  No output may overlap an input or another output. */
 typedef struct qmk_slot_map_args {
   const int32_t* block_tables;   /* [seqs, max_pages]                                  */
   const int32_t* kv_lengths;     /* [seqs]                                             */
@@ -379,7 +380,7 @@ typedef struct qmk_slot_map_args {
   int32_t* seq_ids;              /* out [tokens]                                       */
   uint8_t* active;               /* out [tokens]: 1 where slots[t] >= 0                */
   int32_t* cu_tokens;            /* out [seqs + 1]: first token of every request       */
-  int32_t* kv_lengths_out;       /* out [seqs]: tokens in the cache after the step; not an input itself */
+  int32_t* kv_lengths_out;       /* out [seqs]: tokens in the cache after the step */
   int32_t seqs, tokens, page_size, max_pages;
 } qmk_slot_map_args;
 int qmk_build_slot_map(const qmk_slot_map_args* args, int device, void* cuda_stream);
@@ -435,7 +436,8 @@ typedef struct qmk_paged_step_args {
 } qmk_paged_step_args;
 int qmk_decode_step_paged(qmk_handle* h, const qmk_paged_step_args* args, void* cuda_stream);
 
-/* Text behind the last QMK_ERR_CUDA that one of the first three returned to the calling thread. */
+/* Text behind the last error that one of the first three returned to the calling thread: the failed call behind QMK_ERR_CUDA, the
+ * reason behind a QMK_ERR_INVALID_ARG that the arguments alone do not show (else empty). */
 const char* qmk_paged_last_cuda_error(void);
 
 void qmk_destroy(qmk_handle* h);

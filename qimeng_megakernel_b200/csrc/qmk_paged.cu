@@ -19,6 +19,28 @@ static thread_local char g_paged_err[256];
 
 extern "C" const char* qmk_paged_last_cuda_error(void) { return g_paged_err; }
 
+// An operand's bytes.  Outputs may not cover any of an input or of one another: other CTAs still read, or write too.
+struct Bytes {
+  const char* name;
+  const void* at;
+  long long n;
+};
+static bool apart(const Bytes* out, int outs, const Bytes* in, int ins) {
+  const auto meet = [](const Bytes& a, const Bytes& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    if (a.n <= 0 || b.n <= 0 || x + (uintptr_t)a.n <= y || y + (uintptr_t)b.n <= x) return false;
+    snprintf(g_paged_err, sizeof(g_paged_err), "%s overlaps %s", a.name, b.name);
+    return true;
+  };
+  for (int i = 0; i < outs; ++i) {
+    for (int j = 0; j < ins; ++j)
+      if (meet(out[i], in[j])) return false;
+    for (int j = 0; j < i; ++j)
+      if (meet(out[i], out[j])) return false;
+  }
+  return true;
+}
+
 static int paged_fail(cudaError_t e, const char* what) {
   snprintf(g_paged_err, sizeof(g_paged_err), "%s: %s", what, cudaGetErrorString(e));
   return QMK_ERR_CUDA;
@@ -48,6 +70,7 @@ static int page_shift_of(int page_size) {
 static bool aligned_to(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1u)) == 0; }
 
 extern "C" int qmk_build_block_tables(const qmk_block_tables_args* a, int device, void* cuda_stream) {
+  g_paged_err[0] = 0;
   if (!a || a->seqs < 1 || a->seqs > kMaxTableSeqs || a->max_pages < 1 || a->max_pages > kMaxTablePages || a->num_free < 0 ||
       a->prefix_pages < 0)
     return QMK_ERR_INVALID_ARG;
@@ -55,6 +78,10 @@ extern "C" int qmk_build_block_tables(const qmk_block_tables_args* a, int device
   if (shift < 0 || !a->lengths || !a->tables || !a->used || (a->num_free > 0 && !a->free_pages) ||
       (a->prefix_pages > 0 && !a->prefix_table) || a->prefix_pages > a->max_pages)
     return QMK_ERR_INVALID_ARG;
+  const Bytes in[] = {{"lengths", a->lengths, 4ll * a->seqs}, {"free_pages", a->free_pages, 4ll * a->num_free},
+                      {"prefix_table", a->prefix_table, 4ll * a->prefix_pages}};
+  const Bytes out[] = {{"tables", a->tables, 4ll * a->seqs * a->max_pages}, {"used", a->used, 8}};
+  if (!apart(out, 2, in, 3)) return QMK_ERR_INVALID_ARG;
   DeviceScope scope(device);
   if (scope.err != cudaSuccess) return paged_fail(scope.err, "cudaSetDevice");
   TableParams p;
@@ -71,6 +98,7 @@ extern "C" int qmk_build_block_tables(const qmk_block_tables_args* a, int device
 }
 
 extern "C" int qmk_build_slot_map(const qmk_slot_map_args* a, int device, void* cuda_stream) {
+  g_paged_err[0] = 0;
   if (!a || a->seqs < 1 || a->seqs > kMaxTableSeqs || a->tokens < 1 || a->tokens > kMaxTableTokens || a->max_pages < 1 ||
       a->max_pages > kMaxTablePages)
     return QMK_ERR_INVALID_ARG;
@@ -78,8 +106,12 @@ extern "C" int qmk_build_slot_map(const qmk_slot_map_args* a, int device, void* 
   if (shift < 0 || !a->block_tables || !a->kv_lengths || !a->new_lengths || !a->slots || !a->positions || !a->seq_ids ||
       !a->active || !a->cu_tokens || !a->kv_lengths_out)
     return QMK_ERR_INVALID_ARG;
-  // other CTAs still read the lengths
-  if (a->kv_lengths_out == a->kv_lengths || a->kv_lengths_out == a->new_lengths) return QMK_ERR_INVALID_ARG;
+  const Bytes in[] = {{"block_tables", a->block_tables, 4ll * a->seqs * a->max_pages}, {"kv_lengths", a->kv_lengths, 4ll * a->seqs},
+                      {"new_lengths", a->new_lengths, 4ll * a->seqs}};
+  const Bytes out[] = {{"slots", a->slots, 8ll * a->tokens}, {"positions", a->positions, 4ll * a->tokens},
+                       {"seq_ids", a->seq_ids, 4ll * a->tokens}, {"active", a->active, a->tokens},
+                       {"cu_tokens", a->cu_tokens, 4ll * (a->seqs + 1)}, {"kv_lengths_out", a->kv_lengths_out, 4ll * a->seqs}};
+  if (!apart(out, 6, in, 3)) return QMK_ERR_INVALID_ARG;
   DeviceScope scope(device);
   if (scope.err != cudaSuccess) return paged_fail(scope.err, "cudaSetDevice");
   SlotParams p;
@@ -256,6 +288,7 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
 }
 
 int qmk_prefix_attention_launch(const qmk_prefix_attention_args* a, const qmk_attention_watch* watch, int device, void* cuda_stream) {
+  g_paged_err[0] = 0;
   const int rc = qmk_prefix_attention_check(a, device);
   if (rc) return rc;
   DeviceScope scope(device);

@@ -115,7 +115,7 @@ _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: tor
 def _call(fn, args: bytes, index: int) -> None:
     code = fn(args, index, _stream(index))
     if code != 0:
-        raise _lib.QmkError(code, _lib.load().qmk_paged_last_cuda_error().decode() if code == -3 else "")
+        raise _lib.QmkError(code, _lib.load().qmk_paged_last_cuda_error().decode())
 
 
 def build_block_tables(lengths: torch.Tensor, free_pages: torch.Tensor, *, page_size: int, max_pages: int,
@@ -125,7 +125,7 @@ def build_block_tables(lengths: torch.Tensor, free_pages: torch.Tensor, *, page_
     Row s gets min(ceil(lengths[s] / page_size), max_pages) pages: first those of `prefix_table` (int32), then pages of
     `free_pages` (int32) in order, behind those of the rows before it; the rest of the row is -1.  `used` holds the
     pages taken from `free_pages` (more than there are when it ran out: the entries it could not give are -1) and the
-    number of rows cut off at `max_pages`."""
+    number of rows cut off at `max_pages`.  No tensor of `out` may cover part of another one of the call."""
     if not _flat(None, lengths, free_pages):
         _check("lengths", lengths, torch.int32, 1)
         _check("free_pages", free_pages, torch.int32, 1)
@@ -162,7 +162,7 @@ def build_slot_map(block_tables: torch.Tensor, kv_lengths: torch.Tensor, new_len
     """Where the K and V rows of a step's new tokens go: request s holds `kv_lengths[s]` tokens and appends
     `new_lengths[s]` (both int32 [seqs]).  The step's tokens are numbered request by request; `tokens` is the room of the
     outputs: what does not fit is cut off (the request that straddles it appends fewer), what is left over is filled
-    with slot -1, position 0, request -1, inactive.  `out.kv_lengths` may not be `kv_lengths` or `new_lengths` itself."""
+    with slot -1, position 0, request -1, inactive.  No tensor of `out` may cover part of another one of the call."""
     _check("block_tables", block_tables, torch.int32, 2)
     seqs, max_pages = block_tables.shape
     if not _flat(seqs, kv_lengths, new_lengths):

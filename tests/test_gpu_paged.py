@@ -577,3 +577,28 @@ def test_nan_key_behind_the_prefix_in_a_large_call(paged, heads, prefix):
         lse = torch.empty(c["q"].shape[:2], device="cuda:0")
         row = compare_nonfinite(c, call(paged, c, lse=lse), lse)
         assert row.any() and not row[:920].any()
+
+
+def test_outputs_beside_the_inputs_and_over_them(paged):
+    """Outputs that lie right beside their inputs are taken, those that cover part of one are refused and nothing is written."""
+    from qimeng_megakernel_b200 import _lib
+    want = paged.build_slot_map(ints([[3, 4]] * 3), ints([1, 20, 5]), ints([2, 1, 1]), page_size=16, tokens=5)
+    buf = torch.full((16,), -5, dtype=torch.int32, device="cuda:0")
+    kv, new = buf[3:6], buf[6:9]
+    kv.copy_(ints([1, 20, 5]))
+    new.copy_(ints([2, 1, 1]))
+    out = paged.SlotMap.empty(3, 5, "cuda:0")
+    out.kv_lengths, out.cu_tokens = buf[:3], buf[9:13]
+    paged.build_slot_map(ints([[3, 4]] * 3), kv, new, page_size=16, tokens=5, out=out)
+    for name in ("slots", "positions", "seq_ids", "active", "cu_tokens", "kv_lengths"):
+        assert torch.equal(getattr(out, name), getattr(want, name)), name
+    before = buf.clone()
+    for name, t in (("kv_lengths", buf[1:4]), ("kv_lengths", buf[7:10]), ("cu_tokens", buf[5:9])):
+        bad = paged.SlotMap.empty(3, 5, "cuda:0")
+        setattr(bad, name, t)
+        with pytest.raises(_lib.QmkError, match="overlaps"):
+            paged.build_slot_map(ints([[3, 4]] * 3), kv, new, page_size=16, tokens=5, out=bad)
+    tables = paged.BlockTables(buf[:6].view(3, 2), buf[14:])
+    with pytest.raises(_lib.QmkError, match="tables overlaps lengths"):
+        paged.build_block_tables(kv, new, page_size=16, max_pages=2, out=tables)
+    assert torch.equal(buf, before)

@@ -257,3 +257,36 @@ def test_a_refused_step_leaves_the_state_as_it_was(paged):
         with pytest.raises((TypeError, ValueError)):
             s.advance(bad)
         assert s.step.kv_lengths.tolist() == [5, 9]
+
+
+def test_outputs_that_overlap_are_refused(paged):
+    """Other CTAs still read what an output would write: an output that covers part of an input, or of another output, is refused."""
+    from qimeng_megakernel_b200 import _lib
+    lib = _lib.load()
+    text = lambda: lib.qmk_paged_last_cuda_error().decode()
+
+    def slots(**kw):                                               # 3 requests x 4 pages, 5 tokens, 4 KB apart
+        a = {n: (i + 1) * 4096 for i, n in enumerate(("block_tables", "kv_lengths", "new_lengths", "slots", "positions", "seq_ids",
+                                                      "active", "cu_tokens", "kv_lengths_out"))}
+        a.update(seqs=3, tokens=5, page_size=16, max_pages=4)
+        a.update({k: a[v[0]] + v[1] for k, v in kw.items()})
+        return lib.qmk_build_slot_map(bytes(_lib.SlotMapArgs(**a)), 0, None)
+
+    for kw in (dict(kv_lengths_out=("kv_lengths", 8)), dict(kv_lengths_out=("kv_lengths", -8)), dict(cu_tokens=("new_lengths", 0)),
+               dict(cu_tokens=("kv_lengths", -12)), dict(kv_lengths_out=("new_lengths", 4)), dict(slots=("block_tables", 40)),
+               dict(positions=("block_tables", -4)), dict(seq_ids=("positions", 16)), dict(active=("slots", 39)),
+               dict(kv_lengths_out=("cu_tokens", 12)), dict(positions=("kv_lengths", 0))):
+        assert slots(**kw) == -1, kw
+        assert "overlap" in text(), kw
+
+    def tables(**kw):                                              # 3 requests x 4 pages
+        a = {n: (i + 1) * 4096 for i, n in enumerate(("lengths", "free_pages", "prefix_table", "tables", "used"))}
+        a.update(seqs=3, num_free=6, prefix_pages=2, page_size=16, max_pages=4)
+        a.update({k: a[v[0]] + v[1] for k, v in kw.items()})
+        return lib.qmk_build_block_tables(bytes(_lib.BlockTablesArgs(**a)), 0, None)
+
+    for kw in (dict(tables=("lengths", 8)), dict(used=("lengths", 8)), dict(tables=("free_pages", -44)), dict(prefix_table=("tables", 0)),
+               dict(used=("tables", 44)), dict(used=("free_pages", 20))):
+        assert tables(**kw) == -1, kw
+        assert "overlap" in text(), kw
+    assert lib.qmk_build_slot_map(None, 0, None) == -1 and text() == ""
