@@ -25,6 +25,7 @@ import struct
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -296,6 +297,8 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         raise ValueError(f"scale {scale}: expected a positive number")
     if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("prefix_attention has no gradient: call it under torch.inference_mode() or torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k_pages, v_pages)):
+        raise RuntimeError("prefix_attention has no gradient: a tangent of its inputs would be lost")
     if out is None:
         out = torch.zeros(tokens, heads, size, dtype=torch.bfloat16, device=q.device)
     else:

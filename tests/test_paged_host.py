@@ -290,3 +290,15 @@ def test_outputs_that_overlap_are_refused(paged):
         assert tables(**kw) == -1, kw
         assert "overlap" in text(), kw
     assert lib.qmk_build_slot_map(None, 0, None) == -1 and text() == ""
+
+
+def test_forward_mode_tangents_are_refused(paged):
+    """A dual tensor's tangent would be dropped without a word."""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        for name, shape in (("q", (3, 8, 64)), ("k", (6, 16, 2, 64)), ("v", (6, 16, 2, 64))):
+            dual = forward_ad.make_dual(bf(*shape), bf(*shape))
+            refused(RuntimeError, "no gradient", lambda: attention(paged, **{name: dual}))
+            with torch.no_grad():                                  # (which does not stop forward mode)
+                refused(RuntimeError, "no gradient", lambda: attention(paged, **{name: dual}))
+        refused(ValueError, "no CPU path", lambda: attention(paged))
