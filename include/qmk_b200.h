@@ -394,7 +394,11 @@ int qmk_build_slot_map(const qmk_slot_map_args* args, int device, void* cuda_str
  * page is never used, whatever it holds.  cu_tokens must ascend from 0 to at most `tokens`, as qmk_build_slot_map leaves it: the
  * kernel looks, and a call where it does not sets all its rows to NaN.  out may be q itself.  bf16, fp32 accumulation; head_dim 64
  * or 128, 1..16 query heads per KV head, at most 1024 query heads, 1536 requests, 2^20 tokens, 2^30 positions (prefix_len, and
- * max_pages * page_size) and 2^31 - 1024 rows in the pool. */
+ * max_pages * page_size) and 2^31 - 1024 rows in the pool.  Beyond these, the device counts its work in 32 bits: with room = the
+ * larger of prefix_len and max_pages * page_size, calls are refused whose (rows * query heads / 256) * (room / 128) blocks or
+ * ((rows * query heads per KV head / 8 + seqs) * num_kv_heads) * (room / 32) pieces of short requests, about, pass 2^31 (1536 short
+ * requests of 16384 rows at 32/8 heads: room above 880,000 positions).  A NaN among a row's scores, or one of plus infinity, makes the
+ * row and its lse NaN; keys of minus infinity count as absent. */
 typedef struct qmk_prefix_attention_args {
   const void* q;               /* [tokens, num_heads, head_dim], q_token_stride elements from token to token */
   void* out;                   /* the same, out_token_stride (strides: multiples of 8; 16-byte aligned)      */

@@ -19,6 +19,11 @@ static thread_local char g_paged_err[256];
 
 extern "C" const char* qmk_paged_last_cuda_error(void) { return g_paged_err; }
 
+static int refuse(const char* why) {
+  snprintf(g_paged_err, sizeof(g_paged_err), "%s", why);
+  return QMK_ERR_INVALID_ARG;
+}
+
 // An operand's bytes.  Outputs may not cover any of an input or of one another: other CTAs still read, or write too.
 struct Bytes {
   const char* name;
@@ -181,23 +186,25 @@ extern "C" int64_t qmk_prefix_attention_workspace(int32_t tokens, int32_t seqs, 
 
 static int attention_args(const qmk_prefix_attention_args* a) {
   if (!a) return QMK_ERR_INVALID_ARG;
+  if (a->num_heads > 1024) return refuse("more than 1024 query heads");
   if (!attention_sizes_ok(a->tokens, a->seqs, a->num_heads, a->num_kv_heads, a->head_dim, a->prefix_len)) return QMK_ERR_INVALID_ARG;
   if (a->max_pages < 1 || a->num_pages < 1) return QMK_ERR_INVALID_ARG;
   if (page_shift_of(a->page_size) < 0 || a->prefix_len % a->page_size != 0) return QMK_ERR_INVALID_ARG;
   // positions and rows of the pool are 32-bit coordinates
   if ((long long)a->max_pages * a->page_size > (1ll << 30) || a->prefix_len > (1 << 30) ||
       (long long)a->num_pages * a->page_size > (1ll << 31) - 1024)
-    return QMK_ERR_INVALID_ARG;
+    return refuse("more than 2^30 positions, or more than 2^31 - 1024 rows in the pool");
   if (a->prefix_len > 0 && !a->prefix_table) return QMK_ERR_INVALID_ARG;
   if (!a->block_tables || !a->kv_lengths || !a->cu_tokens || !a->q || !a->out || !a->k_pages || !a->v_pages || !a->workspace)
     return QMK_ERR_INVALID_ARG;
   const long long row = (long long)a->num_heads * a->head_dim;
   if (a->q_token_stride < row || a->out_token_stride < row || a->q_token_stride % 8 != 0 || a->out_token_stride % 8 != 0)
     return QMK_ERR_INVALID_ARG;
-  if (!aligned_to(a->q, 16) || !aligned_to(a->out, 16) || !aligned_to(a->k_pages, 16) || !aligned_to(a->v_pages, 16) ||
-      !aligned_to(a->workspace, 256))
-    return QMK_ERR_INVALID_ARG;
-  if (!(a->scale > 0.f) || isinf(a->scale)) return QMK_ERR_INVALID_ARG;
+  if (!aligned_to(a->q, 16) || !aligned_to(a->out, 16)) return refuse("q and out must be 16-byte aligned");
+  if (!aligned_to(a->k_pages, 16) || !aligned_to(a->v_pages, 16)) return refuse("the pages must be 16-byte aligned");
+  if (!aligned_to(a->workspace, 256)) return refuse("the workspace must be 256-byte aligned");
+  // (log2(e) * scale is what the kernel multiplies by)
+  if (!(a->scale > 0.f) || isinf(a->scale * 1.4426950408889634f)) return refuse("the scale is not a positive number in 32 bits");
   return QMK_OK;
 }
 
@@ -274,12 +281,17 @@ static PlanDims call_dims(const qmk_prefix_attention_args* a, int ctas) {
 }
 
 int qmk_prefix_attention_check(const qmk_prefix_attention_args* a, int device) {
+  g_paged_err[0] = 0;
   const int rc = attention_args(a);
   if (rc) return rc;
   const int ctas = sm_count(device);
   if (ctas < 2) return QMK_ERR_DEVICE;
   const PlanDims d = call_dims(a, ctas);
-  return counts_fit(d) && a->workspace_bytes >= workspace_layout(d, a->head_dim).total ? QMK_OK : QMK_ERR_INVALID_ARG;
+  if (!counts_fit(d))
+    return refuse("rows and the room of prefix and tables: their units of 256 rows x 128 keys, or strips of 8 rows x 32 keys, do not count in "
+                  "32 bits");
+  if (a->workspace_bytes < workspace_layout(d, a->head_dim).total) return refuse("the workspace is too small");
+  return QMK_OK;
 }
 
 extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int device, void* cuda_stream) {
@@ -288,7 +300,6 @@ extern "C" int qmk_prefix_attention(const qmk_prefix_attention_args* a, int devi
 }
 
 int qmk_prefix_attention_launch(const qmk_prefix_attention_args* a, const qmk_attention_watch* watch, int device, void* cuda_stream) {
-  g_paged_err[0] = 0;
   const int rc = qmk_prefix_attention_check(a, device);
   if (rc) return rc;
   DeviceScope scope(device);

@@ -32,6 +32,7 @@ from . import _lib
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
 MAX_GROUP = 16            # query heads per KV head
+MAX_HEADS = 1024          # query heads
 MAX_SEQS = 1536           # requests of one attention call
 MAX_TOKENS = 1 << 20      # rows of one attention call
 MAX_LENGTH = 1 << 30      # positions of a sequence
@@ -253,6 +254,11 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     pool reads as zeros.  What the last page holds behind a request's last token is never used; a non-finite V row
     inside a request may reach every row of its step.
 
+    A NaN among a row's scores, or one of plus infinity, makes the row and its lse NaN; keys of minus infinity count as absent.
+    At most 1024 query heads; the room of the prefix and the tables (max_pages * page size, whatever the lengths are) times the rows
+    is limited by what the device counts in 32 bits: 1536 short requests of 16384 rows at 32/8 heads may have room for 880,000 positions
+    each, 64 rows of 64 requests for 89 million; a call beyond that is refused.
+
     scale: 1 / sqrt(HD) by default.  lse: optional float32 [tokens, NH], receives the natural logarithm of the sum of
     exponentials.  Sums are held in 32 bits; probabilities are rounded to bf16 before they meet V.  Inference only."""
     _rows("q", q)
@@ -274,6 +280,8 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         raise ValueError(f"{tokens} rows: expected at most {MAX_TOKENS}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads != 0 or heads // kv_heads > MAX_GROUP:
         raise ValueError(f"{heads} query heads over {kv_heads} KV heads: expected 1..{MAX_GROUP} per KV head")
+    if heads > MAX_HEADS:
+        raise ValueError(f"{heads} query heads: expected at most {MAX_HEADS} query heads")
     if max_pages < 1 or num_pages < 1:
         raise ValueError("block_tables and pages must not be empty")
     if not 1 <= seqs <= MAX_SEQS:
@@ -293,7 +301,7 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
             raise ValueError(f"prefix_table has {prefix_table.shape[0]} pages, prefix_len needs {prefix_len // page_size}")
     if scale is None:
         scale = 1.0 / math.sqrt(size)
-    elif not (scale > 0.0 and math.isfinite(scale)):
+    elif not (2.0 ** -149 <= scale and scale * 1.4426950408889634 < 3.4028235e38):     # (log2(e) * scale, in 32 bits)
         raise ValueError(f"scale {scale}: expected a positive number")
     if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("prefix_attention has no gradient: call it under torch.inference_mode() or torch.no_grad()")

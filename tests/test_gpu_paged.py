@@ -602,3 +602,24 @@ def test_outputs_beside_the_inputs_and_over_them(paged):
     with pytest.raises(_lib.QmkError, match="tables overlaps lengths"):
         paged.build_block_tables(kv, new, page_size=16, max_pages=2, out=tables)
     assert torch.equal(buf, before)
+
+
+def test_refusals_say_why(paged):
+    """Calls inside the limits of every single argument that are refused all the same name the reason."""
+    from qimeng_megakernel_b200 import _lib
+    z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t, device="cuda:0")
+    pool = z(2, 256, 8, 64)
+    q, tables = z(16384, 32, 64), z(1536, 4096, t=torch.int32)
+    args = (q, pool, pool, tables, z(1536, t=torch.int32), z(1537, t=torch.int32))
+    with pytest.raises(_lib.QmkError, match="32 bits"):
+        paged.prefix_attention(*args)
+    paged.prefix_attention(*args[:3], tables[:, :3400].contiguous(), *args[4:])
+    few = (z(2, 32, 64), pool, pool, z(1, 4, t=torch.int32), z(1, t=torch.int32), z(2, t=torch.int32))
+    ws = paged.attention_workspace(few[0], pool, 1)
+    with pytest.raises(_lib.QmkError, match="workspace"):
+        paged.prefix_attention(*few, workspace=torch.empty(ws.numel() + 16, dtype=torch.uint8, device="cuda:0")[16:])
+    odd = z(pool.numel() + 4)[4:].view(pool.shape)
+    with pytest.raises(_lib.QmkError, match="pages"):
+        paged.prefix_attention(few[0], odd, odd, *few[3:])
+    with pytest.raises(ValueError, match="1024 query heads"):
+        paged.prefix_attention(z(2, 1040, 64), z(2, 16, 65, 64), z(2, 16, 65, 64), *few[3:])

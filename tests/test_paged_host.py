@@ -302,3 +302,17 @@ def test_forward_mode_tangents_are_refused(paged):
             with torch.no_grad():                                  # (which does not stop forward mode)
                 refused(RuntimeError, "no gradient", lambda: attention(paged, **{name: dual}))
         refused(ValueError, "no CPU path", lambda: attention(paged))
+
+
+def test_scales_outside_32_bits_are_refused(paged):
+    """The kernel multiplies by log2(e) * scale in 32 bits: a scale for which that is zero or infinite has no answer."""
+    for scale in (1e39, 3e38, 1e-50):
+        refused(ValueError, "scale .*: expected a positive number", lambda: attention(paged, scale=scale))
+    for scale in (2e38, 1e-40, 1):
+        refused(ValueError, "no CPU path", lambda: attention(paged, scale=scale))
+    from qimeng_megakernel_b200 import _lib
+    P = 4096
+    a = dict(q=P, out=P, lse=None, k_pages=P, v_pages=P, block_tables=P, kv_lengths=P, cu_tokens=P, prefix_table=P, q_token_stride=512,
+             out_token_stride=512, tokens=3, seqs=2, num_heads=8, num_kv_heads=2, head_dim=64, page_size=16, num_pages=6, max_pages=4,
+             prefix_len=32, scale=3e38, workspace=P, workspace_bytes=1 << 30)
+    assert _lib.load().qmk_prefix_attention(bytes(_lib.PrefixAttentionArgs(**a)), 0, None) == -1
