@@ -260,8 +260,10 @@ QMKP_HD long long max_units(const PlanDims& d) {
   return a < b ? a : b;
 }
 QMKP_HD long long max_dense_records(const PlanDims& d) { return d.ctas + max_units(d) * d.NKV; }
+// (A short request has fewer than kMostShort rows.  With T short tokens in all, floor(before * G / 8) + strip <= floor(T * G / 8).)
 QMKP_HD long long max_strips(const PlanDims& d) {
-  return ((long long)d.tokens * d.G / kStripRows + d.seqs) * d.NKV;
+  const long long by_request = (long long)d.seqs * ((kMostShort - 1) / d.G);
+  return ((by_request < d.tokens ? by_request : d.tokens) * d.G / kStripRows + d.seqs) * d.NKV;
 }
 QMKP_HD long long max_strip_records(const PlanDims& d) { return (long long)d.ctas * kStripWarps + max_strips(d); }
 

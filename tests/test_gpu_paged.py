@@ -623,3 +623,10 @@ def test_refusals_say_why(paged):
         paged.prefix_attention(few[0], odd, odd, *few[3:])
     with pytest.raises(ValueError, match="1024 query heads"):
         paged.prefix_attention(z(2, 1040, 64), z(2, 16, 65, 64), z(2, 16, 65, 64), *few[3:])
+
+
+@pytest.mark.parametrize("rows,seqs,most", [(8192, 1, 110e6), (8192, 4, 125e6), (64, 64, 60e6)])
+def test_workspace_has_room_for_short_requests_only_as_far_as_there_can_be_any(paged, rows, seqs, most):
+    """A request of 512 (token, head) rows and more has no strips: one piece of 8192 rows needs records for 511 short ones at most."""
+    q = torch.empty(rows, 16, 128, dtype=torch.bfloat16, device="cuda:0")
+    assert paged.attention_workspace(q, torch.empty(1, 16, 16, 128, dtype=torch.bfloat16, device="cuda:0"), seqs).numel() < most
