@@ -139,6 +139,8 @@ def build_block_tables(lengths: torch.Tensor, free_pages: torch.Tensor, *, page_
         raise ValueError("lengths: no requests")
     if seqs > MAX_TABLE_SEQS:
         raise ValueError(f"lengths: {seqs} requests, expected at most {MAX_TABLE_SEQS}")
+    if free_pages.shape[0] >= 1 << 31:
+        raise ValueError(f"free_pages: {free_pages.shape[0]} pages, expected fewer than {1 << 31}")
     if not 1 <= max_pages <= MAX_TABLE_PAGES:
         raise ValueError(f"max_pages {max_pages}: expected 1..{MAX_TABLE_PAGES}")
     if shared > max_pages:

@@ -316,3 +316,8 @@ def test_scales_outside_32_bits_are_refused(paged):
              out_token_stride=512, tokens=3, seqs=2, num_heads=8, num_kv_heads=2, head_dim=64, page_size=16, num_pages=6, max_pages=4,
              prefix_len=32, scale=3e38, workspace=P, workspace_bytes=1 << 30)
     assert _lib.load().qmk_prefix_attention(bytes(_lib.PrefixAttentionArgs(**a)), 0, None) == -1
+
+
+def test_a_free_list_past_32_bits_is_refused(paged):
+    free = torch.empty(1 << 31, dtype=torch.int32, device="meta")
+    refused(ValueError, "free_pages: 2147483648 pages", paged.build_block_tables, i32(3), free, page_size=16, max_pages=4)
