@@ -263,6 +263,7 @@ static int launch_attention(const qmk_prefix_attention_args* a, const AttnParams
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = merge_grid<HD>(p.d);
+  if (p.status) cfg.gridDim.x += 1;                                  // (the block that reports)
   cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -64,7 +64,8 @@ struct AttnParams {
   int2* dense_desc;            // [tokens, NKV]    {first record, records | row << 16}; records 0: none
   int2* strip_desc;            // [tokens, NH]     {first record, records | row << 16}
   int* refused;                // 1: cu_tokens does not ascend from 0 to at most `tokens`, nothing was computed
-  unsigned* aborted;           // [CTAs, 8]  not 0: a wait expired there (one word for each warp with strips; blocks write all)
+  unsigned* aborted;           // [CTAs, 8]  not 0: a wait expired there (one word for each warp with strips; blocks set all).  Zeroed at
+                               // the CTA's start and set on failure only: a store at its end would make every call longer (0.2 us)
   // failures: the merge, which runs behind all CTAs, reports them
   unsigned* status;            // record of StatusWord, or null
   int phase;                   // of the step, for the record
@@ -268,11 +269,8 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
   if (mbar_try_wait_parked(bar, parity)) return true;
   const long long t0 = clock64();
   while (!mbar_try_wait_parked(bar, parity)) {
+    if (clock64() - t0 > (long long)p.wait_budget * 1024) ctl[0] = 1u;
     if (ctl[0] != 0u) return false;
-    if (clock64() - t0 > (long long)p.wait_budget * 1024) {
-      ctl[0] = 1u;
-      return false;
-    }
   }
   return true;
 }
@@ -1140,6 +1138,7 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
       mbar_init(w.bar(i), count);
     }
     if (lane == 0) ctl[0] = 0u;
+    if (lane < kStripWarps) p.aborted[blockIdx.x * kStripWarps + lane] = 0u;
     fence_barrier_init();
   }
   if (warp == kIssueWarp) {                                  // (before it is known whether the CTA has blocks: it takes a while)
@@ -1156,7 +1155,7 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
     }
     if (ok && warp < kStripWarps) {
       walk_strips<HD>(p, maps, smem, ctl, sc, work->plan, warp, lane);
-      if (lane == 0) p.aborted[blockIdx.x * kStripWarps + warp] = ctl[0];
+      if (lane == 0 && ctl[0] != 0u) p.aborted[blockIdx.x * kStripWarps + warp] = 1u;
     }
     return;
   }
@@ -1179,10 +1178,10 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
   __syncwarp();
   tmem_fence_before_sync();
   __syncthreads();
+  if (threadIdx.x < kStripWarps && ctl[0] != 0u) p.aborted[blockIdx.x * kStripWarps + threadIdx.x] = 1u;
   if (warp == kIssueWarp) {
     tmem_fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(w.tmem) : "memory");
-    if (lane < kStripWarps) p.aborted[blockIdx.x * kStripWarps + lane] = ctl[0];
   }
 }
 
@@ -1194,10 +1193,11 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
 // than the plain order of launches (18.5 us); this takes 17.8 us (all before the present division of the CTAs), of which about 4 us are the adding.
 constexpr int kMergeThreads = 128, kMergeParts = 8;
 constexpr long long kMergeBlocks = 4 * 148 * 6;              // four waves of the blocks that fit the machine
-// What failed goes to the status record, whose first entry stays.
+// What failed goes to the status record, whose first entry stays.  A block beside those that merge does it, where there is a record.
 static __device__ __noinline__ void report_failures(const int* refused, const unsigned* aborted, int ctas, unsigned* status, int phase,
                                                     int last, int tokens) {
   const bool offsets = *refused != 0;                        // (then no CTA has waited for anything)
+#pragma unroll 4
   for (int i = (int)threadIdx.x; i < (offsets ? 1 : ctas * kStripWarps); i += kMergeThreads) {
     if (!offsets && aborted[i] == 0u) continue;
     if (atomicCAS(&status[kStCode], 0u, (unsigned)(offsets ? kErrRowOffsets : kErrCopyWait)) != 0u) continue;
@@ -1212,8 +1212,11 @@ static __device__ __noinline__ void report_failures(const int* refused, const un
 template <int HD, bool kMany>                                // kMany: a large call
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (p.status != nullptr && blockIdx.x + blockIdx.y + blockIdx.z == 0)
-    report_failures(p.refused, p.aborted, p.d.ctas, p.status, p.phase, p.cu_tokens[p.d.seqs], p.d.tokens);
+  if (p.status != nullptr && blockIdx.x == gridDim.x - 1) {
+    if (blockIdx.y + blockIdx.z == 0)
+      report_failures(p.refused, p.aborted, p.d.ctas, p.status, p.phase, p.cu_tokens[p.d.seqs], p.d.tokens);
+    return;
+  }
   const int row = (int)blockIdx.x * 32 + (int)(threadIdx.x & 31), kvh = (int)blockIdx.y;
   const int token = p.d.by_G.div(row), g = row - token * p.d.G, head = kvh * p.d.G + g;
   if (token >= p.d.tokens) return;
