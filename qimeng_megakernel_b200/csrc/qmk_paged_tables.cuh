@@ -65,7 +65,7 @@ __device__ __forceinline__ int pages_own(const TableParams& p, int length) {
 // Row s of the table:  n_s = min(ceil(len_s / page), max_pages) entries, the first prefix_pages of them the shared
 // ones, the others taken from the free list behind those of the rows before:  first_s = sum_{t < s} own_t.
 // Bound by the 4 * seqs * max_pages bytes written, or by the launch for a small batch.  A warp takes a row and a CTA eight: measured
-// at 4096 requests x 512 entries 6.7 us, half of it the launch.
+// at 4096 requests x 512 entries 6.1 us by graph replay, 2.5 of it the launch.
 __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const TableParams p) {
   __shared__ long long red[kTableThreads / 32];
   __shared__ long long first_s[kTableThreads];
@@ -156,8 +156,9 @@ constexpr int kSlotChunk = kTableThreads * kSlotItems;       // requests per pas
 
 // One thread per token.  Every CTA walks the requests in passes of kSlotChunk until it has met its own tokens:
 //   cu_s = min(sum_{t < s} new_t, tokens)   position = kv_s + (token - cu_s)   slot = table[s][position / page] * page + position % page
-// Pass c's cu_tokens and lengths are written by CTA c mod grid.  Bound by the launch and one pass's latency: 3.5 us for 64 requests of
-// a token, 4.3 us for 16411 tokens of 777 (kv_lengths kept beside cu in shared memory: 4.1 and 4.3).
+// Pass c's cu_tokens and lengths are written by CTA c mod grid.  Bound by the launch and one pass's latency: 2.9 us for 64 requests of
+// a token, 3.8 us for 16411 tokens of 777 by graph replay (where these took 3.5 and 4.3, kv_lengths kept beside cu in shared memory
+// took 4.1 and 4.3).
 __global__ void __launch_bounds__(kTableThreads) slot_map_kernel(const SlotParams p) {
   __shared__ long long red[kTableThreads / 32];
   __shared__ int cu_s[kSlotChunk + 1];

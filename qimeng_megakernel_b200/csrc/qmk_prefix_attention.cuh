@@ -20,12 +20,16 @@
 // Strips.  What a short request holds behind the prefix: 8 rows x a run of 32-key pieces per warp, on mma.sync with the keys
 // (for P V the dimensions) as the long side of the tile, K and V through a ring of the warp's own in shared memory.
 //
-// What bounds it (B200, whole calls).  Many rows: the softmax warps' instructions.  A step of 64 keys for both groups (256 rows)
-// takes about 1450 clocks, 1070 of them the exponentials of the two warps that share a scheduler's issue slots (65 % of them
-// used), the rest reading S, writing P and the barriers; the products take 630 clocks of the tensor pipe at head size 64.
-// 4 pieces of 500..1100 tokens behind 32768 shared keys at 32/8 heads x 64: 1050 us, 760 TFLOP/s; 9 pieces behind 8192 at
-// 16/8 x 128, where a step has twice the products: 322 us, 1075 TFLOP/s.  Few rows: the latency of plan, first loads, last
-// block and merge, about 12 us in all (2 rows), and the bytes: 64 rows behind 12288 keys at 16/8 x 128 45 us, 4.2 TB/s.
+// P is rounded to bf16 because the instruction takes one 16-bit type for both operands: 2^-8 of a probability at most, 0.0015 of the
+// output in the root mean square (its own rounding is 0.0017); the sum l is over the unrounded values.
+//
+// What bounds it (B200, whole calls at 1965 MHz).  Many rows: the softmax warps' steps.  One of 64 keys for both groups (256 rows)
+// takes about 1450 clocks, 1070 of them the exponentials of the two warps that share a scheduler (768 of the exponential unit), the
+// rest reading S, writing P and the barriers, which nothing of the same warp runs beside; the products take 630 clocks of the tensor
+// pipe at head size 64.  4 pieces of 500..1100 tokens behind 32768 shared keys at 32/8 heads x 64: 1079 us, 740 TFLOP/s; 9 pieces
+// behind 8192 at 16/8 x 128, where a step has twice the products: 324 us, 1065 TFLOP/s (372 us at the 1660 MHz that the power limit
+// leaves when it runs on).  Few rows: the latency of plan, first loads, last block and merge, about 11.4 us in all (2 rows), and
+// the bytes: 64 rows behind 12288 keys at 16/8 x 128 44 us, 4.3 TB/s.
 //
 // Both parts leave partial results (m, l, unnormalised O, all in 32 bits) unless a row is complete; merge_kernel adds them
 // up in a fixed order, so a call gives the same bits every time.  Nothing is kept between calls.
@@ -1185,12 +1189,6 @@ prefix_attention_kernel(const __grid_constant__ AttnParams p, const __grid_const
   }
 }
 
-// Adds a row's parts.  With M = max m_r and w_r = 2^(m_r - M):   o = sum_r w_r O_r / sum_r w_r l_r
-// A thread takes four dimensions of a (row, KV head) at a time; neighbours take neighbouring rows, which is how the blocks' parts
-// lie.  The statistics and values of eight parts are on their way at once, M is the running maximum (a part of weight zero may
-// hold anything and is left out; one whose scores had a NaN has m = NaN and makes the row NaN).  A refused call's rows are NaN, all of them.  Launched as a programmatic dependent without an
-// early trigger: blocks that wait on the SMs while the attention still runs cost it more (32 rows over 2048 shared keys: 24.6 us)
-// than the plain order of launches (18.5 us); this takes 17.8 us (all before the present division of the CTAs), of which about 4 us are the adding.
 constexpr int kMergeThreads = 128, kMergeParts = 8;
 constexpr long long kMergeBlocks = 4 * 148 * 6;              // four waves of the blocks that fit the machine
 // What failed goes to the status record, whose first entry stays.  A block beside those that merge does it, where there is a record.
@@ -1209,6 +1207,14 @@ static __device__ __noinline__ void report_failures(const int* refused, const un
     status[kStDetail] = 0;
   }
 }
+
+// Adds a row's parts.  With M = max m_r and w_r = 2^(m_r - M):   o = sum_r w_r O_r / sum_r w_r l_r
+// A thread takes four dimensions of a (row, KV head) at a time; neighbours take neighbouring rows, which is how the blocks' parts
+// lie.  The statistics and values of eight parts are on their way at once, M is the running maximum (a part of weight zero may
+// hold anything and is left out; one whose scores had a NaN has m = NaN and makes the row NaN).  A refused call's rows are NaN, all of
+// them.  Launched as a programmatic dependent without an early trigger: blocks that wait on the SMs while the attention still runs
+// cost it more (32 rows over 2048 shared keys: 24.6 us) than the plain order of launches (18.5 us); this takes 17.8 us (all before
+// the present division of the CTAs, 16.5 us with it), of which about 4 us are the adding.
 template <int HD, bool kMany>                                // kMany: a large call
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -131,7 +131,8 @@ def run_prefill_synthetic(config: dict, weights: dict, prompt_ids: torch.Tensor,
 
     shared_prefix = n: the decode state is on a paged cache (paged.PagedState).  The prompts must agree in their first n
     tokens; the whole pages of those are computed and stored once, and every decode step reads them once for the batch
-    (qmk_decode_step_paged).  0 gives a paged cache that shares nothing."""
+    (qmk_decode_step_paged).  0 gives a paged cache that shares nothing.  Probabilities are rounded to bf16 before they meet V there
+    (the contiguous cache's attention multiplies in tf32), so logits differ by that rounding.  The prefill is always the fused one."""
     ids = (prompt_ids.view(1, -1) if prompt_ids.dim() == 1 else prompt_ids).to(torch.int64)
     B, prompt_len = int(ids.shape[0]), int(ids.shape[1])
     if prompt_len < 1:
