@@ -398,7 +398,7 @@ int qmk_build_slot_map(const qmk_slot_map_args* args, int device, void* cuda_str
  * larger of prefix_len and max_pages * page_size, calls are refused whose (rows * query heads / 256) * (room / 128) blocks or
  * ((rows * query heads per KV head / 8 + seqs) * num_kv_heads) * (room / 32) pieces of short requests, about, pass 2^31 (1536 short
  * requests of 16384 rows at 32/8 heads: room above 880,000 positions).  A NaN among a row's scores, or one of plus infinity, makes the
- * row and its lse NaN; keys of minus infinity count as absent. */
+ * row and its lse NaN; keys of minus infinity count as absent (a row that has no others sees nothing). */
 typedef struct qmk_prefix_attention_args {
   const void* q;               /* [tokens, num_heads, head_dim], q_token_stride elements from token to token */
   void* out;                   /* the same, out_token_stride (strides: multiples of 8; 16-byte aligned)      */

@@ -256,7 +256,8 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     pool reads as zeros.  What the last page holds behind a request's last token is never used; a non-finite V row
     inside a request may reach every row of its step.
 
-    A NaN among a row's scores, or one of plus infinity, makes the row and its lse NaN; keys of minus infinity count as absent.
+    A NaN among a row's scores, or one of plus infinity, makes the row and its lse NaN; keys of minus infinity count as absent (a row
+    that has no others sees nothing).
     At most 1024 query heads; the room of the prefix and the tables (max_pages * page size, whatever the lengths are) times the rows
     is limited by what the device counts in 32 bits: 1536 short requests of 16384 rows at 32/8 heads may have room for 880,000 positions
     each, 64 rows of 64 requests for 89 million; a call beyond that is refused.

@@ -630,3 +630,21 @@ def test_workspace_has_room_for_short_requests_only_as_far_as_there_can_be_any(p
     """A request of 512 (token, head) rows and more has no strips: one piece of 8192 rows needs records for 511 short ones at most."""
     q = torch.empty(rows, 16, 128, dtype=torch.bfloat16, device="cuda:0")
     assert paged.attention_workspace(q, torch.empty(1, 16, 16, 128, dtype=torch.bfloat16, device="cuda:0"), seqs).numel() < most
+
+
+@pytest.mark.parametrize("heads", ["32/8x64", "16/8x128"])
+def test_rows_of_minus_infinity_alone_see_nothing(paged, heads):
+    """Keys of minus infinity count as absent, and a row that has no others gives zeros and an lse of minus infinity: a single own
+    key, a whole short request, the first rows of a long piece."""
+    c = make_case(heads, 16, 0, [1, 40, 300], [1, 3, 300], seed=36)
+    c["q"] = c["q"].abs() + 1
+    for s, keys in ((0, range(1)), (1, range(40)), (2, range(70))):
+        for key in keys:
+            c["k"][int(c["tables"][s, key // 16]), key % 16] = float("-inf")
+    lse = torch.empty(c["q"].shape[:2], device="cuda:0")
+    out = call(paged, c, lse=lse)
+    o, want, A, r = definition(c)
+    assert torch.isinf(want[:74]).all() and not torch.isinf(want[74:]).any()
+    assert (out[:74] == 0).all() and (lse[:74] == float("-inf")).all()
+    err, tol = (out.double() - o).abs(), 2.0 ** -8 * o.abs() + (2.0 ** -8 + r) * (1 + 2.0 ** -6) * A
+    assert (err <= tol)[74:].all()
